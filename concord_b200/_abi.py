@@ -35,6 +35,8 @@ GEMM_CUTLASS = 1
 CONV_FPROP = 0
 CONV_DGRAD = 1
 CONV_WGRAD = 2
+# element types of the training operators (CONCORD_F32 / BF16 / F16)
+F32, BF16, F16 = 0, 1, 2
 PEER_SUM_F32 = 0
 PEER_MAX_I32 = 1
 
@@ -145,6 +147,19 @@ class PeerSync(ctypes.Structure):
     ]
 
 
+class DistillParams(ctypes.Structure):
+    """Mirror of `concord_distill_params` (include/concord_b200.h)."""
+    _fields_ = [
+        ("temperature", ctypes.c_float),
+        ("alpha", ctypes.c_float),
+        ("grad_scale", ctypes.c_float),
+        ("mean", ctypes.c_int32),
+        ("ids64", ctypes.c_int32),
+        ("labels64", ctypes.c_int32),
+        ("ignore_index", ctypes.c_int64),
+    ]
+
+
 _LIB = None
 
 _P = ctypes.c_void_p
@@ -220,6 +235,17 @@ _SIGS = [
     ("concord_conv_fprop_nhwc", ctypes.c_int, [_P, _P, _P] + [_I64] * 11 + [_P, ctypes.c_size_t, _P]),
     ("concord_conv_dgrad_nhwc", ctypes.c_int, [_P, _P, _P] + [_I64] * 11 + [_P, ctypes.c_size_t, _P]),
     ("concord_conv_wgrad_nhwc", ctypes.c_int, [_P, _P, _P] + [_I64] * 11 + [_P, ctypes.c_size_t, _P]),
+    ("concord_layer_norm_fwd", ctypes.c_int, [_P, _I32, _I64, _P, _P, _P, _I32, _P, _P, _I64, _I64, _F, _P]),
+    ("concord_layer_norm_bwd_workspace_bytes", ctypes.c_size_t, [_I64, _I64]),
+    ("concord_layer_norm_bwd", ctypes.c_int,
+     [_P, _I32, _I64, _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, ctypes.c_size_t, _P]),
+    ("concord_distill_workspace_bytes", ctypes.c_size_t, [_I64]),
+    ("concord_distill_loss", ctypes.c_int,
+     [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P,
+      ctypes.c_size_t, _P]),
+    ("concord_distill_grad", ctypes.c_int,
+     [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _I64, _P,
+      ctypes.c_size_t, _P]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

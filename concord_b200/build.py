@@ -44,6 +44,9 @@ def _flags_for(cu):
                        "-I" + os.path.join(root, "include"),
                        "-I" + os.path.join(root, "tools", "util", "include"),
                        "-DNDEBUG", "-Xcompiler", "-Wno-psabi", "-diag-suppress", "20012"]
+    if os.path.basename(cu) in ("norm.cu", "distill.cu", "attention.cu"):
+        # no reference arithmetic to reproduce: a multiply and an add may become one fma
+        return ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
     return NVFLAGS
 
 

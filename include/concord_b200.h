@@ -562,6 +562,60 @@ int concord_conv_wgrad_nhwc(const uint16_t* dy, const uint16_t* x, uint16_t* dw,
                             int64_t C, int64_t O, int64_t kh, int64_t kw, int64_t sh, int64_t sw, int64_t ph,
                             int64_t pw, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- operators around the packed layers in a training step ----
+ * Element types of their tensors: */
+#define CONCORD_F32 0
+#define CONCORD_BF16 1
+#define CONCORD_F16 2
+
+/*
+ * Layer norm over the last dimension of x [N, D] (row stride ldx, columns
+ * contiguous, D <= 16384), y [N, D] contiguous in its own type; w, b fp32 or
+ * NULL (ones, zeros).  mean / rstd [N] (both or neither) are what the backward
+ * takes.  The backward writes dx (x's type, contiguous) and, unless NULL, dw
+ * and db (fp32 [D], sums over the rows in a fixed order).
+ */
+int concord_layer_norm_fwd(const void* x, int32_t x_type, int64_t ldx, const float* w, const float* b, void* y,
+                           int32_t y_type, float* mean, float* rstd, int64_t N, int64_t D, float eps, void* stream);
+size_t concord_layer_norm_bwd_workspace_bytes(int64_t N, int64_t D);
+int concord_layer_norm_bwd(const void* x, int32_t x_type, int64_t ldx, const void* dy, int32_t dy_type, int64_t lddy,
+                           const float* w, const float* mean, const float* rstd, void* dx, float* dw, float* db,
+                           int64_t N, int64_t D, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Distillation from a teacher's top K <= 512 logits per row (ids [N, K] int32
+ * or int64, t [N, K] fp32, both contiguous; an id outside [0, V) or a logit of
+ * -inf is an absent entry), with hard labels [N] (or NULL) beside:
+ *   p = softmax(t / T),  KL = sum p (log p - log softmax(z / T)),
+ *   row loss = alpha T^2 KL + (1 - alpha) (lse(z) - z_label).
+ * A row whose label is ignore_index or outside [0, V) (without labels: a row
+ * with no teacher entry) has loss 0 and gradient 0.  With p->mean, loss and
+ * gradient are divided by the number of the other rows (at least 1).
+ *   concord_distill_loss: loss (one fp32) and / or row_loss [N]; stats [N, 3]
+ *     (NULL: not kept) is what concord_distill_grad takes; with dz != NULL the
+ *     same pass writes the gradient of the loss times p->grad_scale.
+ *   concord_distill_grad: dz = p->grad_scale * grad_out * d(loss)/dz, grad_out
+ *     one value, one per row, or NULL (1).
+ * dz [N, V] is contiguous, of z's type, and not z itself.
+ */
+typedef struct concord_distill_params {
+    float temperature;
+    float alpha;
+    float grad_scale;
+    int32_t mean;
+    int32_t ids64;       /* ids are int64 (else int32)    */
+    int32_t labels64;    /* labels are int64 (else int32) */
+    int64_t ignore_index;
+} concord_distill_params;
+size_t concord_distill_workspace_bytes(int64_t N);
+int concord_distill_loss(const concord_distill_params* p, const void* z, int32_t z_type, int64_t ldz, const void* ids,
+                         const float* t, const void* labels, float* loss, float* row_loss, float* stats, void* dz,
+                         int64_t N, int64_t V, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t z_type, int64_t ldz, const void* ids,
+                         const float* t, const void* labels, const float* stats, const float* grad_out,
+                         int32_t grad_out_per_row, void* dz, int64_t N, int64_t V, int64_t K, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
