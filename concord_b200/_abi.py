@@ -160,6 +160,23 @@ class DistillParams(ctypes.Structure):
     ]
 
 
+class AttentionParams(ctypes.Structure):
+    """Mirror of `concord_attention_params` (include/concord_b200.h)."""
+    _fields_ = [
+        ("cu_q", ctypes.c_void_p),
+        ("cu_k", ctypes.c_void_p),
+        ("seqs", ctypes.c_int64),
+        ("tokens_q", ctypes.c_int64),
+        ("tokens_k", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("type", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _LIB = None
 
 _P = ctypes.c_void_p
@@ -246,6 +263,11 @@ _SIGS = [
     ("concord_distill_grad", ctypes.c_int,
      [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _I64, _P,
       ctypes.c_size_t, _P]),
+    ("concord_attention_fwd", ctypes.c_int,
+     [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P] * 4),
+    ("concord_attention_bwd", ctypes.c_int,
+     [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P, _P, _P, _P, _I64, _I64] + [_P] * 5),
+    ("concord_attention_error", ctypes.c_int, [_I32]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

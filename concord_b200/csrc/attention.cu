@@ -1,0 +1,1111 @@
+// attention.cu — attention over packed sequences of different lengths, with
+// grouped heads, causal or not, forward and backward.
+//
+//   s_ij = scale q_i . k_j           (j <= i + Lk - Lq where causal)
+//   o_i  = sum_j exp(s_ij - m_i) v_j / l_i,  lse_i = m_i + log l_i
+//   p_ij = exp(s_ij - lse_i),  delta_i = do_i . o_i
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+// (sums over i also run over the query heads that share the key head).
+//
+// Every product runs on tcgen05 (bf16 or fp16 operands, fp32 accumulators in
+// tensor memory); tiles are 128 rows of up to 128 columns, loaded by TMA.  A
+// head dimension below 64 or 128 is filled up with zeros by the loads.  p and
+// ds are rounded to the operands' type for their second product, as the tensor
+// cores read 16 bits; maxima, sums, lse and delta stay in fp32.
+//
+// Warp roles: warp 0 loads, warp 1 issues the products (and zeroes the rows of
+// a tile that lie beyond its sequence: they belong to another sequence, or to
+// nobody, and 0 * NaN is NaN), warps 4-11 do the softmax arithmetic, one row
+// of 128 a thread in the forward, half a row in the backward.  Every wait on a
+// barrier is bounded (2 s of GPU time): the role then records an error word
+// and stops, the others run out too, and the block frees its tensor memory and
+// returns.
+//
+// The backward is two kernels without atomics, so gradients are the same bits
+// on every run: one owns 128 rows of q and walks the keys (dq, and delta), the
+// other owns 128 keys and walks the queries of every head that shares them (dk,
+// dv).  Both compute s and do . v, seven products in place of five; the
+// alternative adds dq atomically into an fp32 buffer, which is another order of
+// the sums on every run, and a pass to clear and one to round it.
+#include <cuda.h>
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "common.cuh"
+#include "tc.cuh"
+#include "vec.cuh"
+
+namespace concord {
+int bind_current_context(const char* name);
+
+namespace attn {
+
+using namespace tc;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int THREADS = 384;
+
+struct Params {
+    const int* cuq;       // [B + 1] first rows of the sequences (queries)
+    const int* cuk;       // [B + 1] (keys)
+    int B;
+    int Tq, Tk;
+    int H, G;             // query heads, query heads of one key head
+    int D;
+    int causal;
+    float scale, scale2;  // scale, scale * log2(e)
+    void* o;              // [Tq, H, D]
+    void* rest;           // [Tq, H, D]: what o's rounding left over, for delta (NULL: not kept)
+    float* lse;           // [H, Tq]
+    const void* dout;     // row strides of dout in elements
+    int64_t do_ts, do_hs;
+    float* delta;         // [H, Tq]
+    void *dq, *dk, *dv;
+    int* err;
+};
+
+// a block's work: sequence bounds (clamped to the tensors) and tile
+struct Work {
+    int q0, lq, k0, lk;   // first row and length of the sequence
+    int tile;             // -1: none left; then `spare` of `spares` blocks zero the rows of no sequence
+    int spare, spares;
+    int first, last;      // rows [0, first) and [last, T) belong to no sequence
+};
+
+// The t-th tile of `rows` rows, sequences in order, a sequence's last tile
+// first where `back` (causal queries: the longest first).  Whole warp.
+__device__ __forceinline__ void find_tile(const Params& P, bool keys, int t, int tiles_bound, int rows, bool back,
+                                          Work* w) {
+    const int lane = threadIdx.x & 31;
+    const int* cu = keys ? P.cuk : P.cuq;
+    const int T = keys ? P.Tk : P.Tq;
+    int before = 0;
+    for (int b0 = 0; b0 < P.B; b0 += 32) {
+        const int b = b0 + lane;
+        int n = 0, s = 0, len = 0;
+        if (b < P.B) {
+            s = min(max(cu[b], 0), T);
+            len = min(max(cu[b + 1], s), T) - s;
+            n = (len + rows - 1) / rows;
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const int lo = before + incl - n;
+        const bool mine = t >= lo && t < lo + n;
+        if (mine) {
+            const int* other = keys ? P.cuq : P.cuk;
+            const int To = keys ? P.Tq : P.Tk;
+            const int so = min(max(other[b], 0), To), lo2 = min(max(other[b + 1], so), To) - so;
+            w->q0 = keys ? so : s;
+            w->lq = keys ? lo2 : len;
+            w->k0 = keys ? s : so;
+            w->lk = keys ? len : lo2;
+            w->tile = back ? n - 1 - (t - lo) : t - lo;
+        }
+        if (__any_sync(0xffffffffu, mine)) return;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+        w->tile = -1;
+        w->spare = t - before;
+        w->spares = tiles_bound - before;
+        w->first = min(max(cu[0], 0), T);
+        w->last = min(max(cu[P.B], w->first), T);
+    }
+}
+
+// zero out[row, head, :] for the rows of no sequence (16-byte stores)
+__device__ __forceinline__ void zero_uncovered(void* out, const Work& w, int T, int heads, int head, int D) {
+    const int chunks = D / 8, rows = w.first + (T - w.last);
+    for (int64_t i = (int64_t)w.spare * blockDim.x + threadIdx.x; i < (int64_t)rows * chunks;
+         i += (int64_t)w.spares * blockDim.x) {
+        const int r = (int)(i / chunks), c = (int)(i % chunks);
+        const int64_t row = r < w.first ? r : w.last + (r - w.first);
+        reinterpret_cast<uint4*>(out)[(row * heads + head) * chunks + c] = make_uint4(0, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
+    return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
+}
+
+// COLS columns of this lane's row in tensor memory, times f, to out as elements
+// of T; with REST also what that rounding left over, to rest (unless null)
+template <typename T, int COLS, bool REST = false>
+__device__ __forceinline__ void store_row(uint32_t tm, int col0, float f, T* out, int D, bool live,
+                                          T* rest = nullptr) {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) {
+        uint32_t r[32];
+        ld32(tm + c, r);
+        wait_ld();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[k * 8 + e]) * f;
+            const int at = col0 + c + k * 8;
+            if (live && at < D) {
+                const uint4 o = Pack16<T>::pack(v);
+                *reinterpret_cast<uint4*>(out + at) = o;
+                if (REST && rest) {
+                    float h[8];
+                    Pack16<T>::unpack(o, h);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] -= h[e];
+                    *reinterpret_cast<uint4*>(rest + at) = Pack16<T>::pack(v);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- forward
+// A block owns 256 query rows (two tiles, one softmax warpgroup each) of one
+// head; K and V tiles go through one ring and serve both.  Tensor memory: S_0,
+// S_1 (128 columns each; P_i, as 16-bit pairs, takes the first 64 of S_i once
+// it has been read), O_0, O_1.
+template <int DP> struct Fwd {
+    static constexpr int TILE = 256 * DP;               // bytes of 128 rows
+    static constexpr int ST = DP == 128 ? 5 : 8;        // ring of K and V tiles
+    static constexpr int RING = 2 * TILE;
+    static constexpr int BARS = RING + ST * TILE;
+    static constexpr size_t SMEM = BARS + 512 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1)
+    fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+               const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params P) {
+    using C = Fwd<DP>;
+    constexpr int ST = C::ST, TILE = C::TILE;
+    constexpr int BF = sizeof(T) == 2 && !__is_same(T, __half);
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = align1024(raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 10);
+    Work* work = reinterpret_cast<Work*>(slot + 4);
+    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+    auto q_full = [&](int i) { return bar0 + 8u * (2 * ST + i); };
+    auto s_full = [&](int i) { return bar0 + 8u * (2 * ST + 2 + i); };
+    auto p_full = [&](int i) { return bar0 + 8u * (2 * ST + 4 + i); };
+    auto pv_done = [&](int i) { return bar0 + 8u * (2 * ST + 6 + i); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.x % P.H, t = blockIdx.x / P.H, kvh = head / P.G;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(q_full(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 128); mbar_init(pv_done(i), 1);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        find_tile(P, false, t, gridDim.x / P.H, 256, P.causal, work);
+    }
+    if (warp == 1) tmem_alloc<512>(smem_u32(slot));
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *slot;
+    const Work w = *work;
+    T* out = static_cast<T*>(P.o);
+
+    // key blocks of the two tiles
+    const int off = w.lk - w.lq;
+    int n[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r0 = w.tile * 256 + i * 128;
+        const int last = min(r0 + 127, w.lq - 1);
+        const int keys = w.tile < 0 || r0 >= w.lq ? 0 : P.causal ? min(w.lk, last + off + 1) : w.lk;
+        n[i] = keys > 0 ? (keys + 127) / 128 : 0;
+    }
+    const int nmax = max(n[0], n[1]);
+    const uint32_t ring = base + C::RING;
+
+    if (w.tile < 0) {
+        if (w.first + (P.Tq - w.last) > 0) {
+            zero_uncovered(out, w, P.Tq, P.H, head, P.D);
+            for (int64_t r = (int64_t)w.spare * blockDim.x + threadIdx.x; r < w.first + (P.Tq - w.last);
+                 r += (int64_t)w.spares * blockDim.x)
+                P.lse[(int64_t)head * P.Tq + (r < w.first ? r : w.last + (r - w.first))] = 0.f;
+        }
+    } else if (warp == 0) {
+        // ---- loads ----
+        if (lane == 0 && nmax > 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int h, int row) {
+                mbar_expect(bar, TILE);
+                for (int b = 0; b < DP / 64; ++b) tma_load(dst + b * BOX, m, bar, b * 64, h, row);
+            };
+            auto load_q = [&](int i) {
+                if (n[i] > 0) load(base + i * TILE, &mq, q_full(i), head, w.q0 + w.tile * 256 + i * 128);
+            };
+            load_q(0);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int x = 0; x < 2 * nmax; ++x) {      // K_0, V_0, K_1, V_1, ...
+                if (!mbar_wait(empty(s), ph ^ 1, P.err, 1)) goto done;
+                load(ring + s * TILE, x & 1 ? &mv : &mk, full(s), kvh, w.k0 + (x >> 1) * 128);
+                if (x == 0) load_q(1);
+                if (++s == ST) { s = 0; ph ^= 1; }
+            }
+            // the last use of every slot: nothing arrives on these barriers after the block has left
+            for (int x = 0; x < ST && x < 2 * nmax; ++x) {
+                const int y = 2 * nmax - 1 - x;
+                if (!mbar_wait(empty(y % ST), (y / ST) & 1, P.err, 2)) goto done;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- products ----
+        constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_O = instr_desc(BF, DP, 1);
+        auto mma_s = [&](int i, int s) {
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tmem + i * 128, desc_k(base + i * TILE, kk), desc_k(ring + s * TILE, kk), ID_S, kk != 0);
+                mma_commit(s_full(i));
+            }
+        };
+        if (nmax > 0) {
+            if (!mbar_wait(full(0), 0, P.err, 3)) goto done;
+            for (int i = 0; i < 2; ++i) {
+                if (n[i] == 0) continue;
+                if (!mbar_wait(q_full(i), 0, P.err, 4)) goto done;
+                fence_after();
+                mma_s(i, 0);
+            }
+            if (lane == 0) mma_commit(empty(0));
+        }
+        for (int j = 0; j < nmax; ++j) {
+            const int xv = 2 * j + 1, xk = 2 * j + 2, sv = xv % ST, sk = xk % ST;
+            const bool more = j + 1 < nmax;
+            if (!mbar_wait(full(sv), (xv / ST) & 1, P.err, 5)) goto done;
+            if (w.lk - j * 128 < 128) zero_rows<DP>(smem + C::RING + sv * TILE, w.lk - j * 128);
+            if (more && !mbar_wait(full(sk), (xk / ST) & 1, P.err, 6)) goto done;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (j >= n[i]) continue;
+                if (!mbar_wait(p_full(i), j & 1, P.err, 7)) goto done;
+                fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mma_ts(tmem + 256 + i * DP, tmem + i * 128 + kk * 8, desc_mn(ring + sv * TILE, kk), ID_O,
+                               (j | kk) != 0);
+                    mma_commit(pv_done(i));
+                }
+                if (j + 1 < n[i]) {     // S_i takes P_i's place: only after the product that reads P_i
+                    if (!mbar_wait(pv_done(i), j & 1, P.err, 8)) goto done;
+                    fence_after();
+                    mma_s(i, sk);
+                }
+            }
+            if (lane == 0) {
+                mma_commit(empty(sv));
+                if (more) mma_commit(empty(sk));
+            }
+        }
+    } else if (warp >= 4) {
+        // ---- softmax: one row a thread ----
+        const int i = (warp - 4) >> 2, q = warp & 3;
+        const int ni = i ? n[1] : n[0];
+        const int row = w.tile * 256 + i * 128 + q * 32 + lane;      // in the sequence
+        const bool live = row < w.lq;
+        const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + i * 128;
+        const uint32_t to = tmem + ((uint32_t)(q * 32) << 16) + 256 + i * DP;
+        const float c = P.scale2, slack = 8.0f / c;
+        // keys this row sees; and those every row of the tile sees
+        const int mine = P.causal ? min(w.lk, row + off + 1) : w.lk;
+        const int every = P.causal ? min(w.lk, w.tile * 256 + i * 128 + off + 1) : w.lk;
+        float m = -INFINITY, l = 0.f;
+        for (int j = 0; j < ni; ++j) {
+            if (!mbar_wait(s_full(i), j & 1, P.err, 9)) goto done;
+            fence_after();
+            uint32_t u[128];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ld32(ts + k * 32, u + k * 32);
+            wait_ld();
+            float* s = reinterpret_cast<float*>(u);
+            if ((j + 1) * 128 > every) {
+#pragma unroll
+                for (int k = 0; k < 128; ++k)
+                    if (j * 128 + k >= mine) s[k] = -INFINITY;
+            }
+            float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k < 128; ++k) x[k & 3] = fmaxf(x[k & 3], s[k]);
+            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            // the reference maximum follows only where it has fallen 2^8 behind:
+            // p up to 256 is as exact, and O is rescaled a few times in all
+            const bool up = top > m + slack || (m == -INFINITY && top > m);
+            if (__any_sync(0xffffffffu, up)) {
+                const float to_m = fmaxf(m, top);
+                const float f = m == to_m ? 1.0f : ex2_approx((m - to_m) * c);
+                m = to_m;
+                l *= f;
+                if (j > 0) {            // P_i V of block j - 1 is complete: S_i was issued after it
+#pragma unroll
+                    for (int k = 0; k < DP; k += 32) {
+                        uint32_t o[32];
+                        ld32(to + k, o);
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        st32(to + k, o);
+                    }
+                }
+            }
+            const float mc = m == -INFINITY ? 0.f : -m * c;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 128; k += 2) {
+                const float a = ex2_approx(fmaf(s[k], c, mc)), b = ex2_approx(fmaf(s[k + 1], c, mc));
+                sum[k & 2] += a;
+                sum[(k & 2) + 1] += b;
+                u[k >> 1] = pack2(a, b, T());
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            st32(ts, u);
+            st32(ts + 32, u + 32);
+            wait_st();
+            fence_before();
+            mbar_arrive(p_full(i));
+        }
+        const int64_t trow = (int64_t)w.q0 + row;
+        T* dst = out + (trow * P.H + head) * P.D;
+        T* rest = P.rest ? static_cast<T*>(P.rest) + (trow * P.H + head) * P.D : nullptr;
+        if (ni > 0) {
+            if (!mbar_wait(pv_done(i), (ni - 1) & 1, P.err, 10)) goto done;
+            fence_after();
+            store_row<T, DP, true>(to, 0, l == 0.f ? 0.f : 1.0f / l, dst, P.D, live, rest);
+        } else if (live) {
+            for (int d = 0; d < P.D; d += 8) {
+                *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+                if (rest) *reinterpret_cast<uint4*>(rest + d) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (live) P.lse[(int64_t)head * P.Tq + trow] = l == 0.f ? -INFINITY : fmaf(m, P.scale, logf(l));
+    }
+done:
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<512>(tmem);
+    }
+}
+
+// ---------------------------------------------------------------- backward: dq and delta
+// A block owns 128 query rows of one head.  Tensor memory: S 0, dP 128, dQ
+// 256, dS (16-bit pairs) 384.  S and dP of the next key block are computed as
+// soon as the softmax warps have read the present ones.
+template <int DP> struct BwdQ {
+    static constexpr int TILE = 256 * DP;
+    static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 128 ? 2 : 4;
+    static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + KS * TILE;
+    static constexpr int BARS = V_OFF + VS * TILE;
+    static constexpr int RED = BARS + 512;                     // 256 halves of delta
+    static constexpr size_t SMEM = RED + 1024 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1)
+    bwd_q_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
+                 const __grid_constant__ Params P) {
+    using C = BwdQ<DP>;
+    constexpr int TILE = C::TILE, KS = C::KS, VS = C::VS;
+    constexpr int BF = !__is_same(T, __half);
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = align1024(raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * KS + 2 * VS + 9);
+    Work* work = reinterpret_cast<Work*>(slot + 4);
+    float* red = reinterpret_cast<float*>(smem + C::RED);
+    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
+    auto k_full = [&](int s) { return bar0 + 8u * s; };
+    auto k_empty = [&](int s) { return bar0 + 8u * (KS + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (2 * KS + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (2 * KS + VS + s); };
+    const uint32_t one = bar0 + 8u * (2 * KS + 2 * VS);
+    const uint32_t q_full = one, s_full = one + 8, s_free = one + 16, dp_full = one + 24, dp_free = one + 32,
+                   ds_full = one + 40, ds_free = one + 48;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.x % P.H, t = blockIdx.x / P.H, kvh = head / P.G;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
+            for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
+            mbar_init(q_full, 1);
+            mbar_init(s_full, 1); mbar_init(s_free, 256);
+            mbar_init(dp_full, 1); mbar_init(dp_free, 256);
+            mbar_init(ds_full, 256); mbar_init(ds_free, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        find_tile(P, false, t, gridDim.x / P.H, 128, P.causal, work);
+    }
+    if (warp == 1) tmem_alloc<512>(smem_u32(slot));
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *slot;
+    const Work w = *work;
+    const int off = w.lk - w.lq, r0 = w.tile * 128;
+    int n = 0;
+    if (w.tile >= 0) {
+        const int last = min(r0 + 127, w.lq - 1);
+        const int keys = P.causal ? min(w.lk, last + off + 1) : w.lk;
+        n = keys > 0 ? (keys + 127) / 128 : 0;
+    }
+
+    if (w.tile < 0) {
+        zero_uncovered(P.dq, w, P.Tq, P.H, head, P.D);
+    } else if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int h, int row) {
+                for (int b = 0; b < DP / 64; ++b) tma_load(dst + b * BOX, m, bar, b * 64, h, row);
+            };
+            mbar_expect(q_full, 2 * TILE);
+            load(base, &mq, q_full, head, w.q0 + r0);
+            load(base + TILE, &mdo, q_full, head, w.q0 + r0);
+            for (int j = 0; j < n; ++j) {
+                const int sk = j % KS, sv = j % VS;
+                if (!mbar_wait(k_empty(sk), ((j / KS) & 1) ^ 1, P.err, 21)) goto done;
+                mbar_expect(k_full(sk), TILE);
+                load(base + C::K_OFF + sk * TILE, &mk, k_full(sk), kvh, w.k0 + j * 128);
+                if (!mbar_wait(v_empty(sv), ((j / VS) & 1) ^ 1, P.err, 22)) goto done;
+                mbar_expect(v_full(sv), TILE);
+                load(base + C::V_OFF + sv * TILE, &mv, v_full(sv), kvh, w.k0 + j * 128);
+            }
+            for (int x = 0; x < KS && x < n; ++x)
+                if (!mbar_wait(k_empty((n - 1 - x) % KS), ((n - 1 - x) / KS) & 1, P.err, 23)) goto done;
+            for (int x = 0; x < VS && x < n; ++x)
+                if (!mbar_wait(v_empty((n - 1 - x) % VS), ((n - 1 - x) / VS) & 1, P.err, 24)) goto done;
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_Q = instr_desc(BF, DP, 1);
+        auto dq_product = [&](int j) {        // dQ += dS_j K_j
+            if (lane == 0) {
+                const uint32_t kt = base + C::K_OFF + (j % KS) * TILE;
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ts(tmem + 256, tmem + 384 + kk * 8, desc_mn(kt, kk), ID_Q, (j | kk) != 0);
+                mma_commit(k_empty(j % KS));
+                mma_commit(ds_free);
+            }
+        };
+        if (n > 0 && !mbar_wait(q_full, 0, P.err, 25)) goto done;
+        for (int j = 0; j < n; ++j) {
+            const int sk = j % KS, sv = j % VS;
+            if (!mbar_wait(k_full(sk), (j / KS) & 1, P.err, 26)) goto done;
+            // rows of another sequence: dS is 0 there, and 0 * NaN must not reach dQ
+            if (w.lk - j * 128 < 128) zero_rows<DP>(smem + C::K_OFF + sk * TILE, w.lk - j * 128);
+            if (j > 0 && !mbar_wait(s_free, (j - 1) & 1, P.err, 27)) goto done;
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tmem, desc_k(base, kk), desc_k(base + C::K_OFF + sk * TILE, kk), ID_S, kk != 0);
+                mma_commit(s_full);
+            }
+            if (!mbar_wait(v_full(sv), (j / VS) & 1, P.err, 28)) goto done;
+            if (j > 0 && !mbar_wait(dp_free, (j - 1) & 1, P.err, 29)) goto done;
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tmem + 128, desc_k(base + TILE, kk), desc_k(base + C::V_OFF + sv * TILE, kk), ID_S, kk != 0);
+                mma_commit(dp_full);
+                mma_commit(v_empty(sv));
+            }
+            if (j > 0) {
+                if (!mbar_wait(ds_full, (j - 1) & 1, P.err, 30)) goto done;
+                fence_after();
+                dq_product(j - 1);
+            }
+        }
+        if (n > 0) {
+            if (!mbar_wait(ds_full, (n - 1) & 1, P.err, 31)) goto done;
+            fence_after();
+            dq_product(n - 1);
+        }
+    } else if (warp >= 4) {
+        const int half = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
+        const int row = r0 + r;
+        const bool live = row < w.lq;
+        const int64_t trow = (int64_t)w.q0 + row;
+        // delta = do . o, o with its rest: o rounded to 16 bits alone makes the
+        // error of dq and dk a tenth larger.  The halves take alternate 16
+        // bytes, then add in order.
+        float d = 0.f;
+        if (live) {
+            const T* a = static_cast<const T*>(P.dout) + trow * P.do_ts + head * P.do_hs;
+            const T* b = static_cast<const T*>(P.o) + (trow * P.H + head) * P.D;
+            const T* b2 = static_cast<const T*>(P.rest) + (trow * P.H + head) * P.D;
+            for (int c = half * 8; c < P.D; c += 16) {
+                float x[8], y[8], z[8];
+                load_vec<8>(a + c, x);
+                load_vec<8>(b + c, y);
+                load_vec<8>(b2 + c, z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e] + z[e], d);
+            }
+        }
+        red[half * 128 + r] = d;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        d = red[r] + red[128 + r];
+        float lse = live ? P.lse[(int64_t)head * P.Tq + trow] : 0.f;
+        if (lse == -INFINITY) lse = 0.f;           // no key: everything is masked below
+        if (live && half == 0) P.delta[(int64_t)head * P.Tq + trow] = d;
+        const float c = P.scale2, l2 = -lse * LOG2E;
+        const int mine = (P.causal ? min(w.lk, row + off + 1) : w.lk) - half * 64;
+        const int every = P.causal ? min(w.lk, r0 + off + 1) : w.lk;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        for (int j = 0; j < n; ++j) {
+            float p[64];
+            uint32_t u[64];
+            if (!mbar_wait(s_full, j & 1, P.err, 32)) goto done;
+            fence_after();
+            ld32(tmem + lanes + half * 64, u);
+            ld32(tmem + lanes + half * 64 + 32, u + 32);
+            wait_ld();
+            fence_before();
+            mbar_arrive(s_free);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) p[k] = ex2_approx(fmaf(__uint_as_float(u[k]), c, l2));
+            if (!mbar_wait(dp_full, j & 1, P.err, 33)) goto done;
+            fence_after();
+            ld32(tmem + lanes + 128 + half * 64, u);
+            ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
+            wait_ld();
+            fence_before();
+            mbar_arrive(dp_free);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) p[k] *= __uint_as_float(u[k]) - d;
+            if ((j + 1) * 128 > every) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (j * 128 + k >= mine) p[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) u[k] = pack2(p[2 * k], p[2 * k + 1], T());
+            if (j > 0 && !mbar_wait(ds_free, (j - 1) & 1, P.err, 34)) goto done;
+            st32(tmem + lanes + 384 + half * 32, u);
+            wait_st();
+            fence_before();
+            mbar_arrive(ds_full);
+        }
+        T* dst = static_cast<T*>(P.dq) + (trow * P.H + head) * P.D;
+        if (n > 0) {
+            if (!mbar_wait(ds_free, (n - 1) & 1, P.err, 35)) goto done;
+            fence_after();
+            store_row<T, DP / 2>(tmem + lanes + 256 + half * (DP / 2), half * (DP / 2), P.scale, dst, P.D, live);
+        } else if (live) {
+            for (int x = half * 8; x < P.D; x += 16) *reinterpret_cast<uint4*>(dst + x) = make_uint4(0, 0, 0, 0);
+        }
+    }
+done:
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<512>(tmem);
+    }
+}
+
+// ---------------------------------------------------------------- backward: dk and dv
+// A block owns 128 keys of one key head and walks the query blocks of every
+// head that shares it.  The scores are transposed (a key is a row), so p and
+// ds are the A operands of their products as they come from the softmax.
+// Tensor memory: S 0, dP 128, dV 256, dK 256 + DP.  P takes half of each half
+// of S (columns 0-31 and 64-95), dS the same of dP: each softmax warp writes
+// only where it has read itself.  The order of the products, dV, next S, dK,
+// next dP, lets the exponentials run beside dK and dP, and ds beside dV and S.
+template <int DP> struct BwdK {
+    static constexpr int TILE = 256 * DP;
+    static constexpr int QS = DP == 128 ? 2 : 3, OS = DP == 128 ? 2 : 3;
+    static constexpr int Q_OFF = 2 * TILE, O_OFF = Q_OFF + QS * TILE;
+    static constexpr int BARS = O_OFF + OS * TILE;
+    static constexpr int STAT = BARS + 512;                    // 2 stages of (lse, delta)[128]
+    static constexpr size_t SMEM = STAT + 2 * 1024 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, 1)
+    bwd_k_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
+                 const __grid_constant__ Params P) {
+    using C = BwdK<DP>;
+    constexpr int TILE = C::TILE, QS = C::QS, OS = C::OS;
+    constexpr int BF = !__is_same(T, __half);
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = align1024(raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * QS + 2 * OS + 12);
+    Work* work = reinterpret_cast<Work*>(slot + 4);
+    float* stat = reinterpret_cast<float*>(smem + C::STAT);
+    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
+    auto q_full = [&](int s) { return bar0 + 8u * s; };
+    auto q_empty = [&](int s) { return bar0 + 8u * (QS + s); };
+    auto o_full = [&](int s) { return bar0 + 8u * (2 * QS + s); };
+    auto o_empty = [&](int s) { return bar0 + 8u * (2 * QS + OS + s); };
+    const uint32_t one = bar0 + 8u * (2 * QS + 2 * OS);
+    const uint32_t kv_full = one, s_full = one + 8, p_full = one + 16, dv_done = one + 24, dp_full = one + 32,
+                   ds_full = one + 40, dk_done = one + 48;
+    auto st_full = [&](int s) { return one + 56u + 8u * s; };
+    auto st_empty = [&](int s) { return one + 72u + 8u * s; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int HK = P.H / P.G;
+    const int kvh = blockIdx.x % HK, t = blockIdx.x / HK;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < QS; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
+            for (int s = 0; s < OS; ++s) { mbar_init(o_full(s), 1); mbar_init(o_empty(s), 1); }
+            mbar_init(kv_full, 1);
+            mbar_init(s_full, 1); mbar_init(p_full, 256); mbar_init(dv_done, 1);
+            mbar_init(dp_full, 1); mbar_init(ds_full, 256); mbar_init(dk_done, 1);
+            for (int s = 0; s < 2; ++s) { mbar_init(st_full(s), 64); mbar_init(st_empty(s), 256); }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        find_tile(P, true, t, gridDim.x / HK, 128, false, work);
+    }
+    if (warp == 1) tmem_alloc<512>(smem_u32(slot));
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *slot;
+    const Work w = *work;
+    const int off = w.lk - w.lq, k0 = w.tile * 128;
+    // query blocks [jq, jq + nq) of every head; `n` in all
+    int jq = 0, nq = 0;
+    if (w.tile >= 0) {
+        const int first = P.causal ? max(0, k0 - off) : 0;
+        if (first < w.lq) { jq = first / 128; nq = (w.lq + 127) / 128 - jq; }
+    }
+    const int n = nq * P.G;
+
+    if (w.tile < 0) {
+        zero_uncovered(P.dk, w, P.Tk, HK, kvh, P.D);
+        zero_uncovered(P.dv, w, P.Tk, HK, kvh, P.D);
+    } else if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int h, int row) {
+                for (int b = 0; b < DP / 64; ++b) tma_load(dst + b * BOX, m, bar, b * 64, h, row);
+            };
+            mbar_expect(kv_full, 2 * TILE);
+            load(base, &mk, kv_full, kvh, w.k0 + k0);
+            load(base + TILE, &mv, kv_full, kvh, w.k0 + k0);
+            for (int x = 0; x < n; ++x) {
+                const int sq = x % QS, so = x % OS;
+                const int head = kvh * P.G + x / nq, row = w.q0 + (jq + x % nq) * 128;
+                if (!mbar_wait(q_empty(sq), ((x / QS) & 1) ^ 1, P.err, 41)) goto done;
+                mbar_expect(q_full(sq), TILE);
+                load(base + C::Q_OFF + sq * TILE, &mq, q_full(sq), head, row);
+                if (!mbar_wait(o_empty(so), ((x / OS) & 1) ^ 1, P.err, 42)) goto done;
+                mbar_expect(o_full(so), TILE);
+                load(base + C::O_OFF + so * TILE, &mdo, o_full(so), head, row);
+            }
+            for (int x = 0; x < QS && x < n; ++x)
+                if (!mbar_wait(q_empty((n - 1 - x) % QS), ((n - 1 - x) / QS) & 1, P.err, 43)) goto done;
+            for (int x = 0; x < OS && x < n; ++x)
+                if (!mbar_wait(o_empty((n - 1 - x) % OS), ((n - 1 - x) / OS) & 1, P.err, 44)) goto done;
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_D = instr_desc(BF, DP, 1);
+        const uint32_t qt = base + C::Q_OFF, ot = base + C::O_OFF;
+        // rows of another sequence hold anything: p and ds are 0 there, and 0 * NaN must not reach dk and dv
+        auto short_by = [&](int x) { return w.lq - (jq + x % nq) * 128; };
+        auto s_product = [&](int x) -> bool {
+            const int s = x % QS;
+            if (!mbar_wait(q_full(s), (x / QS) & 1, P.err, 45)) return false;
+            if (short_by(x) < 128) zero_rows<DP>(smem + C::Q_OFF + s * TILE, short_by(x));
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tmem, desc_k(base, kk), desc_k(qt + s * TILE, kk), ID_S, kk != 0);
+                mma_commit(s_full);
+            }
+            return true;
+        };
+        auto dp_product = [&](int x) -> bool {
+            const int s = x % OS;
+            if (!mbar_wait(o_full(s), (x / OS) & 1, P.err, 46)) return false;
+            if (short_by(x) < 128) zero_rows<DP>(smem + C::O_OFF + s * TILE, short_by(x));
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_ss(tmem + 128, desc_k(base + TILE, kk), desc_k(ot + s * TILE, kk), ID_S, kk != 0);
+                mma_commit(dp_full);
+            }
+            return true;
+        };
+        if (n > 0) {
+            if (!mbar_wait(kv_full, 0, P.err, 47)) goto done;
+            if (!s_product(0) || !dp_product(0)) goto done;
+        }
+        for (int x = 0; x < n; ++x) {
+            if (!mbar_wait(p_full, x & 1, P.err, 48)) goto done;
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ts(tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8, desc_mn(ot + (x % OS) * TILE, kk), ID_D,
+                           (x | kk) != 0);
+                mma_commit(dv_done);
+                mma_commit(o_empty(x % OS));
+            }
+            if (!mbar_wait(dv_done, x & 1, P.err, 49)) goto done;      // S takes P's place
+            if (x + 1 < n && !s_product(x + 1)) goto done;
+            if (!mbar_wait(ds_full, x & 1, P.err, 50)) goto done;
+            fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ts(tmem + 256 + DP, tmem + 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_mn(qt + (x % QS) * TILE, kk),
+                           ID_D, (x | kk) != 0);
+                mma_commit(dk_done);
+                mma_commit(q_empty(x % QS));
+            }
+            if (x + 1 < n) {
+                if (!mbar_wait(dk_done, x & 1, P.err, 51)) goto done;  // dP takes dS's place
+                if (!dp_product(x + 1)) goto done;
+            }
+        }
+    } else if (warp < 4) {
+        // ---- lse and delta of the query rows, for the softmax warps ----
+        const int i = threadIdx.x - 64;
+        for (int x = 0; x < n; ++x) {
+            const int s = x & 1, head = kvh * P.G + x / nq, row0 = (jq + x % nq) * 128;
+            if (!mbar_wait(st_empty(s), ((x >> 1) & 1) ^ 1, P.err, 52)) goto done;
+            for (int k = i; k < 128; k += 64) {
+                float l = INFINITY, d = 0.f;       // no such row, or one without keys: p = 0
+                if (row0 + k < w.lq) {
+                    const int64_t at = (int64_t)head * P.Tq + w.q0 + row0 + k;
+                    l = P.lse[at];
+                    l = l == -INFINITY ? INFINITY : l * LOG2E;
+                    d = P.delta[at];
+                }
+                stat[s * 256 + k] = -l;
+                stat[s * 256 + 128 + k] = d;
+            }
+            mbar_arrive(st_full(s));
+        }
+    } else {
+        const int half = (warp - 4) >> 2, q = warp & 3;
+        const int key = k0 + q * 32 + lane;
+        const bool live = key < w.lk;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const float c = P.scale2;
+        for (int x = 0; x < n; ++x) {
+            const int s = x & 1, row0 = (jq + x % nq) * 128 + half * 64;
+            const float4* l4 = reinterpret_cast<const float4*>(stat + s * 256 + half * 64);
+            const float4* d4 = reinterpret_cast<const float4*>(stat + s * 256 + 128 + half * 64);
+            // the first query of this half that sees the key, as a column
+            const int from = P.causal ? key - off - row0 : 0;
+            const bool masked = P.causal && row0 + off < k0 + 127;
+            float p[64];
+            uint32_t u[64], v[32];
+            if (!mbar_wait(st_full(s), (x >> 1) & 1, P.err, 53)) goto done;
+            if (!mbar_wait(s_full, x & 1, P.err, 54)) goto done;
+            fence_after();
+            ld32(tmem + lanes + half * 64, u);
+            ld32(tmem + lanes + half * 64 + 32, u + 32);
+            wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float4 l = l4[k];
+                p[4 * k] = ex2_approx(fmaf(__uint_as_float(u[4 * k]), c, l.x));
+                p[4 * k + 1] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 1]), c, l.y));
+                p[4 * k + 2] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 2]), c, l.z));
+                p[4 * k + 3] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 3]), c, l.w));
+            }
+            if (masked) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (k < from) p[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = pack2(p[2 * k], p[2 * k + 1], T());
+            st32(tmem + lanes + half * 64, v);
+            wait_st();
+            fence_before();
+            mbar_arrive(p_full);
+            if (!mbar_wait(dp_full, x & 1, P.err, 55)) goto done;
+            fence_after();
+            ld32(tmem + lanes + 128 + half * 64, u);
+            ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
+            wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float4 d = d4[k];
+                p[4 * k] *= __uint_as_float(u[4 * k]) - d.x;
+                p[4 * k + 1] *= __uint_as_float(u[4 * k + 1]) - d.y;
+                p[4 * k + 2] *= __uint_as_float(u[4 * k + 2]) - d.z;
+                p[4 * k + 3] *= __uint_as_float(u[4 * k + 3]) - d.w;
+            }
+            mbar_arrive(st_empty(s));
+            if (masked) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (k < from) p[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = pack2(p[2 * k], p[2 * k + 1], T());
+            st32(tmem + lanes + 128 + half * 64, v);
+            wait_st();
+            fence_before();
+            mbar_arrive(ds_full);
+        }
+        const int64_t trow = (int64_t)w.k0 + key;
+        T* dk = static_cast<T*>(P.dk) + (trow * HK + kvh) * P.D;
+        T* dv = static_cast<T*>(P.dv) + (trow * HK + kvh) * P.D;
+        if (n > 0) {
+            if (!mbar_wait(dk_done, (n - 1) & 1, P.err, 56)) goto done;      // and dV before it
+            fence_after();
+            store_row<T, DP / 2>(tmem + lanes + 256 + half * (DP / 2), half * (DP / 2), 1.0f, dv, P.D, live);
+            store_row<T, DP / 2>(tmem + lanes + 256 + DP + half * (DP / 2), half * (DP / 2), P.scale, dk, P.D, live);
+        } else if (live) {
+            for (int d = half * 8; d < P.D; d += 16) {
+                *reinterpret_cast<uint4*>(dk + d) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(dv + d) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+done:
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<512>(tmem);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+
+// [rows, heads, D] with strides in elements; boxes of 128 rows x 64 columns of one head
+bool make_map(CUtensorMap* m, const void* base, int bf16, int64_t rows, int64_t heads, int64_t D, int64_t ts,
+              int64_t hs) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)ts * 2};
+    cuuint32_t box[3] = {64, 1, 128};
+    cuuint32_t step[3] = {1, 1, 1};
+    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+               const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+__device__ int g_err;      // first wait that ran out (0: none), per device
+
+int* error_word() {
+    int* p = nullptr;
+    return cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_err) == cudaSuccess ? p : nullptr;
+}
+
+template <typename T, int DP> bool raise_smem() {
+    return cudaFuncSetAttribute(fwd_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)Fwd<DP>::SMEM) == cudaSuccess &&
+           cudaFuncSetAttribute(bwd_q_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)BwdQ<DP>::SMEM) == cudaSuccess &&
+           cudaFuncSetAttribute(bwd_k_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)BwdK<DP>::SMEM) == cudaSuccess;
+}
+
+// the kernels' shared-memory limits, once per device
+bool device_ready() {
+    constexpr int MAX_DEVICES = 64;
+    static std::atomic<int> ready[MAX_DEVICES];
+    static std::mutex mu;
+    int d = 0;
+    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return false;
+    if (ready[d].load()) return true;
+    std::lock_guard<std::mutex> g(mu);
+    if (!raise_smem<__nv_bfloat16, 64>() || !raise_smem<__nv_bfloat16, 128>() || !raise_smem<__half, 64>() ||
+        !raise_smem<__half, 128>()) {
+        cudaGetLastError();
+        return false;
+    }
+    ready[d].store(1);
+    return true;
+}
+
+// blocks per head: enough for every tile of every sequence, and one more where a row is in none
+int64_t tiles_bound(int64_t T, int64_t B, int rows) { return (T + rows - 1) / rows + B; }
+
+int check(const char* name, const concord_attention_params* p) {
+    const std::string n(name);
+    if (!p) return fail(CONCORD_EINVAL, n + ": null pointer");
+    if (p->type != CONCORD_BF16 && p->type != CONCORD_F16) return fail(CONCORD_EINVAL, n + ": operands must be bf16 or fp16");
+    if (p->tokens_q < 0 || p->tokens_k < 0 || p->seqs < 1 || p->heads < 1 || p->kv_heads < 1 ||
+        p->heads % p->kv_heads || p->tokens_q > INT32_MAX - 256 || p->tokens_k > INT32_MAX - 256)
+        return fail(CONCORD_ESHAPE, n + ": bad extents, or heads not a multiple of the key heads");
+    if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8)
+        return fail(CONCORD_ESHAPE, n + ": head_dim must be a multiple of 8 up to 128");
+    if (!(p->scale > 0.f) || !(p->scale < INFINITY)) return fail(CONCORD_EINVAL, n + ": scale must be positive");
+    if (!p->cu_q || !p->cu_k) return fail(CONCORD_EINVAL, n + ": null pointer");
+    if (tiles_bound(std::max(p->tokens_q, p->tokens_k), p->seqs, 128) * p->heads > INT32_MAX)
+        return fail(CONCORD_ETOOBIG, n + ": too many tiles");
+    return CONCORD_OK;
+}
+
+int check_operand(const char* name, const void* x, int64_t ts, int64_t hs) {
+    if (!x) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
+    if (!aligned(x, 16) || ts % 8 || hs % 8) return fail(CONCORD_EALIGN, std::string(name) + ": rows must start on 16 bytes");
+    if (ts <= 0 || hs <= 0 || ts >= (1ll << 38) || hs >= (1ll << 38))
+        return fail(CONCORD_ESHAPE, std::string(name) + ": strides must be positive");
+    return CONCORD_OK;
+}
+
+Params make_params(const concord_attention_params* p, int* err) {
+    Params P{};
+    P.cuq = p->cu_q; P.cuk = p->cu_k; P.B = (int)p->seqs;
+    P.Tq = (int)p->tokens_q; P.Tk = (int)p->tokens_k;
+    P.H = (int)p->heads; P.G = (int)(p->heads / p->kv_heads); P.D = (int)p->head_dim;
+    P.causal = p->causal; P.scale = p->scale; P.scale2 = p->scale * LOG2E;
+    P.err = err;
+    return P;
+}
+
+template <typename T, int DP>
+void launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& P, cudaStream_t st) {
+    const int grid = (int)(tiles_bound(P.Tq, P.B, 256) * P.H);
+    fwd_kernel<T, DP><<<grid, THREADS, Fwd<DP>::SMEM, st>>>(q, k, v, P);
+}
+
+template <typename T, int DP>
+void launch_bwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& d,
+                const Params& P, cudaStream_t st) {
+    if (P.Tq > 0)
+        bwd_q_kernel<T, DP><<<(int)(tiles_bound(P.Tq, P.B, 128) * P.H), THREADS, BwdQ<DP>::SMEM, st>>>(q, k, v, d, P);
+    bwd_k_kernel<T, DP><<<(int)(tiles_bound(P.Tk, P.B, 128) * (P.H / P.G)), THREADS, BwdK<DP>::SMEM, st>>>(q, k, v, d,
+                                                                                                         P);
+}
+
+}  // namespace attn
+}  // namespace concord
+
+using namespace concord;
+
+extern "C" int concord_attention_fwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs,
+                                     const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
+                                     int64_t v_hs, void* o, void* o_rest, float* lse, void* stream) {
+    const char* name = "concord_attention_fwd";
+    if (int rc = attn::check(name, p)) return rc;
+    if (p->tokens_q == 0) return CONCORD_OK;
+    if (p->tokens_k == 0) return fail(CONCORD_ESHAPE, "concord_attention_fwd: no keys");
+    if (int rc = attn::check_operand(name, q, q_ts, q_hs)) return rc;
+    if (int rc = attn::check_operand(name, k, k_ts, k_hs)) return rc;
+    if (int rc = attn::check_operand(name, v, v_ts, v_hs)) return rc;
+    if (!o || !lse) return fail(CONCORD_EINVAL, "concord_attention_fwd: null pointer");
+    if (!aligned(o, 16) || !aligned(o_rest, 16)) return fail(CONCORD_EALIGN, "concord_attention_fwd: output must be 16-byte aligned");
+    if (int rc = bind_current_context(name)) return rc;
+    CUtensorMap mq, mk, mv;
+    const int bf = p->type == CONCORD_BF16;
+    if (!attn::make_map(&mq, q, bf, p->tokens_q, p->heads, p->head_dim, q_ts, q_hs) ||
+        !attn::make_map(&mk, k, bf, p->tokens_k, p->kv_heads, p->head_dim, k_ts, k_hs) ||
+        !attn::make_map(&mv, v, bf, p->tokens_k, p->kv_heads, p->head_dim, v_ts, v_hs))
+        return fail(CONCORD_ELAUNCH, "concord_attention_fwd: TMA descriptor encoding failed");
+    int* err = attn::error_word();
+    if (!err || !attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_fwd: device set-up failed");
+    attn::Params P = attn::make_params(p, err);
+    P.o = o;
+    P.rest = o_rest;
+    P.lse = lse;
+    cudaStream_t st = as_stream(stream);
+    if (bf) {
+        if (p->head_dim <= 64) attn::launch_fwd<__nv_bfloat16, 64>(mq, mk, mv, P, st);
+        else attn::launch_fwd<__nv_bfloat16, 128>(mq, mk, mv, P, st);
+    } else {
+        if (p->head_dim <= 64) attn::launch_fwd<__half, 64>(mq, mk, mv, P, st);
+        else attn::launch_fwd<__half, 128>(mq, mk, mv, P, st);
+    }
+    return check_launch(name);
+}
+
+extern "C" int concord_attention_bwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs,
+                                     const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
+                                     int64_t v_hs, const void* o, const void* o_rest, const float* lse,
+                                     const void* dout, int64_t do_ts, int64_t do_hs, float* delta, void* dq, void* dk, void* dv, void* stream) {
+    const char* name = "concord_attention_bwd";
+    if (int rc = attn::check(name, p)) return rc;
+    if (p->tokens_q == 0 || p->tokens_k == 0) return fail(CONCORD_ESHAPE, "concord_attention_bwd: no rows");
+    if (int rc = attn::check_operand(name, q, q_ts, q_hs)) return rc;
+    if (int rc = attn::check_operand(name, k, k_ts, k_hs)) return rc;
+    if (int rc = attn::check_operand(name, v, v_ts, v_hs)) return rc;
+    if (int rc = attn::check_operand(name, dout, do_ts, do_hs)) return rc;
+    if (!o || !o_rest || !lse || !delta || !dq || !dk || !dv) return fail(CONCORD_EINVAL, "concord_attention_bwd: null pointer");
+    if (!aligned(o, 16) || !aligned(o_rest, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16))
+        return fail(CONCORD_EALIGN, "concord_attention_bwd: tensors must be 16-byte aligned");
+    if (int rc = bind_current_context(name)) return rc;
+    CUtensorMap mq, mk, mv, md;
+    const int bf = p->type == CONCORD_BF16;
+    if (!attn::make_map(&mq, q, bf, p->tokens_q, p->heads, p->head_dim, q_ts, q_hs) ||
+        !attn::make_map(&mk, k, bf, p->tokens_k, p->kv_heads, p->head_dim, k_ts, k_hs) ||
+        !attn::make_map(&mv, v, bf, p->tokens_k, p->kv_heads, p->head_dim, v_ts, v_hs) ||
+        !attn::make_map(&md, dout, bf, p->tokens_q, p->heads, p->head_dim, do_ts, do_hs))
+        return fail(CONCORD_ELAUNCH, "concord_attention_bwd: TMA descriptor encoding failed");
+    int* err = attn::error_word();
+    if (!err || !attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_bwd: device set-up failed");
+    attn::Params P = attn::make_params(p, err);
+    P.o = const_cast<void*>(o);
+    P.rest = const_cast<void*>(o_rest);
+    P.lse = const_cast<float*>(lse);
+    P.dout = dout;
+    P.do_ts = do_ts;
+    P.do_hs = do_hs;
+    P.delta = delta;
+    P.dq = dq;
+    P.dk = dk;
+    P.dv = dv;
+    cudaStream_t st = as_stream(stream);
+    if (bf) {
+        if (p->head_dim <= 64) attn::launch_bwd<__nv_bfloat16, 64>(mq, mk, mv, md, P, st);
+        else attn::launch_bwd<__nv_bfloat16, 128>(mq, mk, mv, md, P, st);
+    } else {
+        if (p->head_dim <= 64) attn::launch_bwd<__half, 64>(mq, mk, mv, md, P, st);
+        else attn::launch_bwd<__half, 128>(mq, mk, mv, md, P, st);
+    }
+    return check_launch(name);
+}
+
+// the attention kernels' error word on the current device (0: no wait ran out)
+extern "C" int concord_attention_error(int32_t reset) {
+    int* err = attn::error_word();
+    if (!err) return -1;
+    int v = 0;
+    cudaMemcpy(&v, err, sizeof(int), cudaMemcpyDeviceToHost);
+    if (reset) cudaMemset(err, 0, sizeof(int));
+    return v;
+}

@@ -616,6 +616,39 @@ int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t
                          int32_t grad_out_per_row, void* dz, int64_t N, int64_t V, int64_t K, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/*
+ * Attention over packed sequences.  q / o / dout / dq [tokens_q, heads, D], k
+ * / v / dk / dv [tokens_k, kv_heads, D] (bf16 or fp16, D a multiple of 8 up
+ * to 128); query head h reads key head h / (heads / kv_heads).  Sequence b is
+ * rows cu_q[b] .. cu_q[b + 1] of the queries and cu_k[b] .. cu_k[b + 1] of the
+ * keys (int32 [seqs + 1] on the device, clamped to the tensors; they may
+ * differ in length).  causal: query i of Lq sees the keys j <= i + Lk - Lq.  A
+ * query without keys gives o = 0, lse = -inf; a row of no sequence o = 0, lse
+ * = 0 and zero gradients.  Inputs take a token and a head stride (elements,
+ * positive multiples of 8, columns contiguous, 16-byte aligned); o and the
+ * gradients are contiguous; o_rest (o's layout; NULL in the forward where no
+ * backward follows) is what o's rounding left over, from which the backward
+ * has delta = dout . o to fp32; lse and delta are fp32 [heads, tokens_q], delta
+ * being scratch that the backward fills.  concord_attention_error: non-zero
+ * once a barrier wait inside a kernel has run out (2 s of GPU time per wait).
+ */
+typedef struct concord_attention_params {
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    int64_t seqs, tokens_q, tokens_k, heads, kv_heads, head_dim;
+    int32_t type;        /* CONCORD_BF16 or CONCORD_F16 */
+    int32_t causal;
+    float scale;         /* positive */
+} concord_attention_params;
+int concord_attention_fwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                          int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, void* o, void* o_rest,
+                          float* lse, void* stream);
+int concord_attention_bwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                          int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const void* o,
+                          const void* o_rest, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs, float* delta, void* dq,
+                          void* dk, void* dv, void* stream);
+int concord_attention_error(int32_t reset);
+
 #ifdef __cplusplus
 }
 #endif
