@@ -261,8 +261,7 @@ _SIGS = [
      [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P,
       ctypes.c_size_t, _P]),
     ("concord_distill_grad", ctypes.c_int,
-     [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _I64, _P,
-      ctypes.c_size_t, _P]),
+     [ctypes.POINTER(DistillParams), _P, _I32, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _I64, _P]),
     ("concord_attention_fwd", ctypes.c_int,
      [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P] * 4),
     ("concord_attention_bwd", ctypes.c_int,

@@ -35,26 +35,23 @@ def need_type(name, t, types):
         raise TypeError(f"{name} must be one of {[str(x) for x in types]}, got {t.dtype}")
 
 
-def call(name, device, *args):
-    """Call `name` of the C ABI on the tensors' device and its current stream
+_FN = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream(...).cuda_stream without the Stream object
+
+
+def call(name, index, *args):
+    """Call `name` of the C ABI on CUDA device `index` and its current stream
     (appended as the last argument)."""
-    lib = _abi.load()
-    fn = getattr(lib, name)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index is not None and device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            status = fn(*args, stream)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_abi.load(), name)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
     else:
-        status = fn(*args, stream)
+        status = fn(*args, _raw_stream(index))
     if status != 0:
         _abi.check(status, name)
 
 
-def workspace(nbytes, device):
-    """Scratch of one call, from the caching allocator (ordered with the
-    current stream, and part of a captured graph's pool)."""
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
-
-
-def byref(struct):
-    return ctypes.byref(struct)
+byref = ctypes.byref

@@ -38,14 +38,14 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
         q, k, v = _operand(q), _operand(k), _operand(v)
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o = q.new_empty(q.shape)
         rest = torch.empty_like(o) if any(ctx.needs_input_grad[:3]) else None
         lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
         if k.shape[0] == 0:
             o.zero_()
             lse.fill_(float("-inf"))
         elif q.shape[0]:
-            _ops.call("concord_attention_fwd", q.device, _ops.byref(_params(q, k, cu_q, cu_k, causal, scale)),
+            _ops.call("concord_attention_fwd", q.get_device(), _ops.byref(_params(q, k, cu_q, cu_k, causal, scale)),
                       *_arg(q), *_arg(k), *_arg(v), o.data_ptr(), _ops.ptr(rest), lse.data_ptr())
         ctx.save_for_backward(q, k, v, cu_q, cu_k, o, rest, lse)
         ctx.causal, ctx.scale = causal, scale
@@ -56,12 +56,12 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do, _):
         q, k, v, cu_q, cu_k, o, rest, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
         if q.shape[0] == 0 or k.shape[0] == 0:
             return dq.zero_(), dk.zero_(), dv.zero_(), None, None, None, None
         do = _operand(do)
         delta = torch.empty_like(lse)
-        _ops.call("concord_attention_bwd", q.device, _ops.byref(_params(q, k, cu_q, cu_k, ctx.causal, ctx.scale)),
+        _ops.call("concord_attention_bwd", q.get_device(), _ops.byref(_params(q, k, cu_q, cu_k, ctx.causal, ctx.scale)),
                   *_arg(q), *_arg(k), *_arg(v), o.data_ptr(), rest.data_ptr(), lse.data_ptr(), *_arg(do),
                   delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None, None, None

@@ -47,9 +47,11 @@ struct Args {
     const float* gout;      // upstream gradient: one value (gout_stride 0) or one per row (1)
     int gout_stride;
     int mean;               // divide by the number of rows that count
-    const int* counts;      // [COUNT_BLOCKS] partial counts
+    const int* counts;      // [COUNT_BLOCKS] partial counts (value and gradient in one pass)
+    const float* number;    // the number of rows that count, from the forward (gradient alone)
     float* stats;           // [N, 3]: maximum, sum at 1/T, sum at 1
     float* row_loss;        // [N]
+    float* row_counts;      // [N]: 1 where the row counts
     void* dz;
     int squarings;          // log2(T) where T = 2, 4, 8
     int tpr;
@@ -169,7 +171,8 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
     X.c1 = LOG2E;
     X.squarings = A.squarings;
     float number = 1.f;
-    if ((MODE & 2) && A.mean) number = (float)max(1, total_count(A));
+    if (MODE == 3 && A.mean) number = (float)max(1, total_count(A));
+    if (MODE == 2 && A.mean) number = *A.number;
 
     auto sync = [&]() { if (tpr == 32) __syncwarp(); else __syncthreads(); };
     for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < A.N; r0 += (int64_t)gridDim.x * groups) {
@@ -278,6 +281,7 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
                     if (A.labels) loss += (1.f - A.alpha) * (R.m + logf(R.s1) - to_f32(z[y]));
                 }
                 A.row_loss[row] = loss;
+                if (A.row_counts) A.row_counts[row] = counts ? 1.f : 0.f;
                 if (A.stats) { A.stats[row * 3] = R.m; A.stats[row * 3 + 1] = R.s; A.stats[row * 3 + 2] = R.s1; }
             }
         }
@@ -334,19 +338,27 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
 }
 
 // the rows' losses in a fixed order, divided by the number of rows that count
-__global__ void __launch_bounds__(1024) total_kernel(const Args A, float* loss) {
-    __shared__ double red[32];
-    double s = 0.0;
-    for (int64_t r = threadIdx.x; r < A.N; r += 1024) s += (double)A.row_loss[r];
+// (which the gradient reads); 64 bits: a sum of up to 2^24 whole numbers is exact
+__global__ void __launch_bounds__(1024) total_kernel(const Args A, float* loss, float* number) {
+    __shared__ double red[32][2];
+    double s = 0.0, n = 0.0;
+    for (int64_t r = threadIdx.x; r < A.N; r += 1024) {
+        s += (double)A.row_loss[r];
+        n += (double)A.row_counts[r];
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-    const int number = A.mean ? max(1, total_count(A)) : 1;
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5][0] = s; red[threadIdx.x >> 5][1] = n; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = 0.0;
-        for (int i = 0; i < 32; ++i) s += red[i];
-        loss[0] = (float)(s / (double)number);
+        s = n = 0.0;
+        for (int i = 0; i < 32; ++i) { s += red[i][0]; n += red[i][1]; }
+        n = n > 1.0 ? n : 1.0;
+        loss[0] = (float)(A.mean ? s / n : s);
+        if (number) number[0] = (float)n;
     }
 }
 
@@ -403,9 +415,9 @@ Args make_args(const concord_distill_params* p, const void* z, int64_t ldz, cons
 
 using namespace concord;
 
-// workspace: the partial counts and the rows' losses
+// workspace: the partial counts, the rows' losses, which rows count
 extern "C" size_t concord_distill_workspace_bytes(int64_t N) {
-    return distill::COUNT_BLOCKS * sizeof(int) + (N > 0 ? (size_t)N * sizeof(float) : 0);
+    return distill::COUNT_BLOCKS * sizeof(int) + (N > 0 ? (size_t)N * 2 * sizeof(float) : 0);
 }
 
 extern "C" int concord_distill_loss(const concord_distill_params* p, const void* z, int32_t z_type, int64_t ldz,
@@ -424,34 +436,31 @@ extern "C" int concord_distill_loss(const concord_distill_params* p, const void*
         return check_launch(name);
     }
     int* counts = static_cast<int*>(workspace);
+    float* rows = reinterpret_cast<float*>(counts + distill::COUNT_BLOCKS);
     A.counts = counts;
-    A.row_loss = row_loss ? row_loss : reinterpret_cast<float*>(counts + distill::COUNT_BLOCKS);
+    A.row_loss = row_loss ? row_loss : rows;
+    A.row_counts = loss ? rows + N : nullptr;
     A.stats = stats;
     A.dz = dz;
-    if (A.mean) distill::count_kernel<<<distill::COUNT_BLOCKS, 256, 0, st>>>(A, counts);
+    if (A.mean && dz) distill::count_kernel<<<distill::COUNT_BLOCKS, 256, 0, st>>>(A, counts);
     if (int rc = dz ? distill::run<3>(A, z_type, st, name) : distill::run<1>(A, z_type, st, name)) return rc;
-    if (loss) distill::total_kernel<<<1, 1024, 0, st>>>(A, loss);
+    if (loss) distill::total_kernel<<<1, 1024, 0, st>>>(A, loss, stats ? stats + 3 * N : nullptr);
     return check_launch(name);
 }
 
 extern "C" int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t z_type, int64_t ldz,
                                     const void* ids, const float* t, const void* labels, const float* stats,
                                     const float* grad_out, int32_t grad_out_per_row, void* dz, int64_t N, int64_t V,
-                                    int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+                                    int64_t K, void* stream) {
     const char* name = "concord_distill_grad";
     if (!p || (N > 0 && (!stats || !dz))) return fail(CONCORD_EINVAL, "concord_distill_grad: null pointer");
     distill::Args A = distill::make_args(p, z, ldz, ids, t, labels, N, V, K);
     if (int rc = distill::check(name, A, z_type)) return rc;
-    if (!workspace || workspace_bytes < concord_distill_workspace_bytes(0))
-        return fail(CONCORD_EWORKSPACE, "concord_distill_grad: workspace too small");
     if (N == 0) return CONCORD_OK;
-    cudaStream_t st = as_stream(stream);
-    int* counts = static_cast<int*>(workspace);
-    A.counts = counts;
     A.stats = const_cast<float*>(stats);
+    A.number = stats + 3 * N;
     A.gout = grad_out;
     A.gout_stride = grad_out_per_row ? 1 : 0;
     A.dz = dz;
-    if (A.mean) distill::count_kernel<<<distill::COUNT_BLOCKS, 256, 0, st>>>(A, counts);
-    return distill::run<2>(A, z_type, st, name);
+    return distill::run<2>(A, z_type, as_stream(stream), name);
 }

@@ -47,44 +47,43 @@ def _check(logits, top_ids, top_logits, labels, temperature, alpha):
 
 def _flat(logits, top_ids, top_logits, labels):
     V, K = logits.shape[-1], top_ids.shape[-1]
-    z = logits.reshape(-1, V)
-    if z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < V):
+    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if not z.is_contiguous() and (z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < V)):
         z = z.contiguous()
-    return (z, top_ids.reshape(-1, K).contiguous(), top_logits.reshape(-1, K).float().contiguous(),
-            None if labels is None else labels.reshape(-1).contiguous())
+    ids = top_ids if top_ids.dim() == 2 else top_ids.reshape(-1, K)
+    t = top_logits if top_logits.dim() == 2 else top_logits.reshape(-1, K)
+    if labels is not None:
+        labels = (labels if labels.dim() == 1 else labels.reshape(-1)).contiguous()
+    return z, ids.contiguous(), t.float().contiguous(), labels
 
 
 def _params(ids, labels, temperature, alpha, ignore_index, mean, scale=1.0):
-    return _abi.DistillParams(temperature=temperature, alpha=alpha, grad_scale=scale, mean=int(mean),
-                              ids64=int(ids.dtype == torch.int64),
-                              labels64=int(labels is not None and labels.dtype == torch.int64),
-                              ignore_index=int(ignore_index))
+    return _abi.DistillParams(temperature, alpha, scale, mean, ids.dtype == torch.int64,
+                              labels is not None and labels.dtype == torch.int64, ignore_index)
 
 
 def _loss(z, ids, t, labels, params, loss, row_loss, stats, dz):
     N, V = z.shape
-    ws = _ops.workspace(_abi.load().concord_distill_workspace_bytes(N), z.device)
-    _ops.call("concord_distill_loss", z.device, _ops.byref(params), z.data_ptr(), _ops.TYPES[z.dtype],
+    nbytes = 512 + 8 * N          # concord_distill_workspace_bytes(N)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
+    _ops.call("concord_distill_loss", z.get_device(), _ops.byref(params), z.data_ptr(), _ops.TYPES[z.dtype],
               z.stride(0) if N > 1 else V, ids.data_ptr(), t.data_ptr(), _ops.ptr(labels), _ops.ptr(loss),
-              _ops.ptr(row_loss), _ops.ptr(stats), _ops.ptr(dz), N, V, ids.shape[1], ws.data_ptr(), ws.numel())
+              _ops.ptr(row_loss), _ops.ptr(stats), _ops.ptr(dz), N, V, ids.shape[1], ws.data_ptr(), nbytes)
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_ids, top_logits, labels, temperature, alpha, ignore_index, reduction):
         z, ids, t, lab = _flat(logits, top_ids, top_logits, labels)
-        N = z.shape[0]
         params = _params(ids, lab, temperature, alpha, ignore_index, reduction == "mean")
         f32 = dict(dtype=torch.float32, device=z.device)
-        stats = torch.empty(N, 3, **f32) if ctx.needs_input_grad[0] else None
-        if reduction == "none":
-            out = torch.empty(logits.shape[:-1], **f32)
-            _loss(z, ids, t, lab, params, None, out, stats, None)
-        else:
-            out = torch.empty((), **f32)
-            _loss(z, ids, t, lab, params, out, None, stats, None)
-        ctx.save_for_backward(z, ids, t, lab, stats)
-        ctx.params, ctx.shape, ctx.per_row = params, logits.shape, reduction == "none"
+        per_row = reduction == "none"
+        out = torch.empty(logits.shape[:-1] if per_row else (), **f32)
+        stats = torch.empty(3 * z.shape[0] + 1, **f32) if ctx.needs_input_grad[0] else None
+        _loss(z, ids, t, lab, params, None if per_row else out, out if per_row else None, stats, None)
+        if stats is not None:
+            ctx.save_for_backward(z, ids, t, lab, stats)
+            ctx.params, ctx.shape, ctx.per_row = params, logits.shape, per_row
         return out
 
     @staticmethod
@@ -92,13 +91,12 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, grad):
         z, ids, t, lab, stats = ctx.saved_tensors
         N, V = z.shape
-        grad = grad.reshape(-1).float().contiguous()
-        dz = torch.empty(N, V, dtype=z.dtype, device=z.device)
-        ws = _ops.workspace(_abi.load().concord_distill_workspace_bytes(0), z.device)
-        _ops.call("concord_distill_grad", z.device, _ops.byref(ctx.params), z.data_ptr(), _ops.TYPES[z.dtype],
+        grad = grad.contiguous()
+        dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
+        _ops.call("concord_distill_grad", z.get_device(), _ops.byref(ctx.params), z.data_ptr(), _ops.TYPES[z.dtype],
                   z.stride(0) if N > 1 else V, ids.data_ptr(), t.data_ptr(), _ops.ptr(lab), stats.data_ptr(),
-                  grad.data_ptr(), int(ctx.per_row), dz.data_ptr(), N, V, ids.shape[1], ws.data_ptr(), ws.numel())
-        return (dz.view(ctx.shape),) + (None,) * 7
+                  grad.data_ptr(), ctx.per_row, dz.data_ptr(), N, V, ids.shape[1])
+        return dz, None, None, None, None, None, None, None
 
 
 def distill_loss(logits, top_ids, top_logits, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100,

@@ -591,8 +591,9 @@ int concord_layer_norm_bwd(const void* x, int32_t x_type, int64_t ldx, const voi
  * A row whose label is ignore_index or outside [0, V) (without labels: a row
  * with no teacher entry) has loss 0 and gradient 0.  With p->mean, loss and
  * gradient are divided by the number of the other rows (at least 1).
- *   concord_distill_loss: loss (one fp32) and / or row_loss [N]; stats [N, 3]
- *     (NULL: not kept) is what concord_distill_grad takes; with dz != NULL the
+ *   concord_distill_loss: loss (one fp32) and / or row_loss [N]; stats
+ *     (3 N + 1 values; NULL: not kept) is what concord_distill_grad takes
+ *     (with p->mean, only a call that wrote `loss` has filled it); with dz != NULL the
  *     same pass writes the gradient of the loss times p->grad_scale.
  *   concord_distill_grad: dz = p->grad_scale * grad_out * d(loss)/dz, grad_out
  *     one value, one per row, or NULL (1).
@@ -613,8 +614,7 @@ int concord_distill_loss(const concord_distill_params* p, const void* z, int32_t
                          int64_t N, int64_t V, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t z_type, int64_t ldz, const void* ids,
                          const float* t, const void* labels, const float* stats, const float* grad_out,
-                         int32_t grad_out_per_row, void* dz, int64_t N, int64_t V, int64_t K, void* workspace,
-                         size_t workspace_bytes, void* stream);
+                         int32_t grad_out_per_row, void* dz, int64_t N, int64_t V, int64_t K, void* stream);
 
 /*
  * Attention over packed sequences.  q / o / dout / dq [tokens_q, heads, D], k
