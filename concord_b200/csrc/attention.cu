@@ -332,26 +332,43 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < ni; ++j) {
             if (!mbar_wait(s_full(i), j & 1, P.err, 9)) goto done;
             fence_after();
-            uint32_t u[128];
+            // 32 scores at a time: the second half first, for the maximum alone;
+            // the first half stays in registers for the exponentials
+            const bool masked = (j + 1) * 128 > every;
+            uint32_t x[32], y[32];
+            auto load = [&](int at) {
+                ld32(ts + at, x);
+                ld32(ts + at + 32, y);
+                wait_ld();
+                if (masked) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ld32(ts + k * 32, u + k * 32);
-            wait_ld();
-            float* s = reinterpret_cast<float*>(u);
-            if ((j + 1) * 128 > every) {
+                    for (int k = 0; k < 32; ++k) {
+                        if (j * 128 + at + k >= mine) x[k] = 0xff800000u;          // -inf
+                        if (j * 128 + at + 32 + k >= mine) y[k] = 0xff800000u;
+                    }
+                }
+            };
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto largest = [&]() {
 #pragma unroll
-                for (int k = 0; k < 128; ++k)
-                    if (j * 128 + k >= mine) s[k] = -INFINITY;
-            }
-            float x[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int k = 4; k < 128; ++k) x[k & 3] = fmaxf(x[k & 3], s[k]);
-            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                for (int k = 0; k < 32; k += 4) {
+                    tops[0] = max3(tops[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                    tops[1] = max3(tops[1], __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                    tops[2] = max3(tops[2], __uint_as_float(y[k]), __uint_as_float(y[k + 1]));
+                    tops[3] = max3(tops[3], __uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
+                }
+            };
+            load(64);
+            largest();
+            load(0);
+            largest();
+            const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
             // the reference maximum follows only where it has fallen 2^8 behind:
             // p up to 256 is as exact, and O is rescaled a few times in all
             const bool up = top > m + slack || (m == -INFINITY && top > m);
             if (__any_sync(0xffffffffu, up)) {
                 const float to_m = fmaxf(m, top);
-                const float f = m == to_m ? 1.0f : ex2_approx((m - to_m) * c);
+                const float f = m == to_m ? 1.0f : ex2f((m - to_m) * c);
                 m = to_m;
                 l *= f;
                 if (j > 0) {            // P_i V of block j - 1 is complete: S_i was issued after it
@@ -367,17 +384,29 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
             const float mc = m == -INFINITY ? 0.f : -m * c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t c2 = f2(c, c), mc2 = f2(mc, mc);
+            uint64_t sum[2] = {0, 0};
+            auto weigh = [&](const uint32_t* v, int at) {       // P of 32 columns, into columns of S that are done with
+                uint32_t w16[16];
 #pragma unroll
-            for (int k = 0; k < 128; k += 2) {
-                const float a = ex2_approx(fmaf(s[k], c, mc)), b = ex2_approx(fmaf(s[k + 1], c, mc));
-                sum[k & 2] += a;
-                sum[(k & 2) + 1] += b;
-                u[k >> 1] = pack2(a, b, T());
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            st32(ts, u);
-            st32(ts + 32, u + 32);
+                for (int k = 0; k < 32; k += 2) {
+                    float a, b;
+                    unf2(fma2(f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, mc2), a, b);
+                    a = ex2f(a);
+                    b = ex2f(b);
+                    sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], f2(a, b));
+                    w16[k >> 1] = pack2(a, b, T());
+                }
+                st16(ts + at, w16);
+            };
+            weigh(x, 0);
+            weigh(y, 16);
+            load(64);
+            weigh(x, 32);
+            weigh(y, 48);
+            float sa, sb;
+            unf2(add2(sum[0], sum[1]), sa, sb);
+            l += sa + sb;
             wait_st();
             fence_before();
             mbar_arrive(p_full(i));
@@ -569,7 +598,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         float lse = live ? P.lse[(int64_t)head * P.Tq + trow] : 0.f;
         if (lse == -INFINITY) lse = 0.f;           // no key: everything is masked below
         if (live && half == 0) P.delta[(int64_t)head * P.Tq + trow] = d;
-        const float c = P.scale2, l2 = -lse * LOG2E;
+        const float l2 = -lse * LOG2E;
+        const uint64_t c2 = f2(P.scale2, P.scale2), l22 = f2(l2, l2), nd2 = f2(-d, -d);
         const int mine = (P.causal ? min(w.lk, row + off + 1) : w.lk) - half * 64;
         const int every = P.causal ? min(w.lk, r0 + off + 1) : w.lk;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -584,7 +614,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             fence_before();
             mbar_arrive(s_free);
 #pragma unroll
-            for (int k = 0; k < 64; ++k) p[k] = ex2_approx(fmaf(__uint_as_float(u[k]), c, l2));
+            for (int k = 0; k < 64; k += 2) {
+                float a, b;
+                unf2(fma2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, l22), a, b);
+                p[k] = ex2f(a);
+                p[k + 1] = ex2f(b);
+            }
             if (!mbar_wait(dp_full, j & 1, P.err, 33)) goto done;
             fence_after();
             ld32(tmem + lanes + 128 + half * 64, u);
@@ -593,7 +628,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             fence_before();
             mbar_arrive(dp_free);
 #pragma unroll
-            for (int k = 0; k < 64; ++k) p[k] *= __uint_as_float(u[k]) - d;
+            for (int k = 0; k < 64; k += 2)
+                unf2(mul2(f2(p[k], p[k + 1]), add2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), nd2)), p[k],
+                     p[k + 1]);
             if ((j + 1) * 128 > every) {
 #pragma unroll
                 for (int k = 0; k < 64; ++k)
@@ -638,7 +675,7 @@ template <int DP> struct BwdK {
     static constexpr int QS = DP == 128 ? 2 : 3, OS = DP == 128 ? 2 : 3;
     static constexpr int Q_OFF = 2 * TILE, O_OFF = Q_OFF + QS * TILE;
     static constexpr int BARS = O_OFF + OS * TILE;
-    static constexpr int STAT = BARS + 512;                    // 2 stages of (lse, delta)[128]
+    static constexpr int STAT = BARS + 512;                    // 2 stages of (-lse log2(e), -delta)[128]
     static constexpr size_t SMEM = STAT + 2 * 1024 + 1024;
 };
 
@@ -801,7 +838,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     d = P.delta[at];
                 }
                 stat[s * 256 + k] = -l;
-                stat[s * 256 + 128 + k] = d;
+                stat[s * 256 + 128 + k] = -d;
             }
             mbar_arrive(st_full(s));
         }
@@ -810,7 +847,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int key = k0 + q * 32 + lane;
         const bool live = key < w.lk;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const float c = P.scale2;
+        const uint64_t c2 = f2(P.scale2, P.scale2);
         for (int x = 0; x < n; ++x) {
             const int s = x & 1, row0 = (jq + x % nq) * 128 + half * 64;
             const float4* l4 = reinterpret_cast<const float4*>(stat + s * 256 + half * 64);
@@ -829,10 +866,14 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 const float4 l = l4[k];
-                p[4 * k] = ex2_approx(fmaf(__uint_as_float(u[4 * k]), c, l.x));
-                p[4 * k + 1] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 1]), c, l.y));
-                p[4 * k + 2] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 2]), c, l.z));
-                p[4 * k + 3] = ex2_approx(fmaf(__uint_as_float(u[4 * k + 3]), c, l.w));
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    float a, b;
+                    unf2(fma2(f2(__uint_as_float(u[4 * k + e]), __uint_as_float(u[4 * k + e + 1])), c2,
+                              e ? f2(l.z, l.w) : f2(l.x, l.y)), a, b);
+                    p[4 * k + e] = ex2f(a);
+                    p[4 * k + e + 1] = ex2f(b);
+                }
             }
             if (masked) {
 #pragma unroll
@@ -853,10 +894,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 const float4 d = d4[k];
-                p[4 * k] *= __uint_as_float(u[4 * k]) - d.x;
-                p[4 * k + 1] *= __uint_as_float(u[4 * k + 1]) - d.y;
-                p[4 * k + 2] *= __uint_as_float(u[4 * k + 2]) - d.z;
-                p[4 * k + 3] *= __uint_as_float(u[4 * k + 3]) - d.w;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    unf2(mul2(f2(p[4 * k + e], p[4 * k + e + 1]),
+                              add2(f2(__uint_as_float(u[4 * k + e]), __uint_as_float(u[4 * k + e + 1])),
+                                   e ? f2(d.z, d.w) : f2(d.x, d.y))), p[4 * k + e], p[4 * k + e + 1]);
             }
             mbar_arrive(st_empty(s));
             if (masked) {

@@ -110,8 +110,8 @@ struct Run {
 template <bool TWO>
 __device__ __forceinline__ void merge(Run& a, float m, float s, float s1, float c, float c1) {
     const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
-    a.s = a.s * ex2_approx((a.m - ref) * c) + s * ex2_approx((m - ref) * c);
-    if (TWO) a.s1 = a.s1 * ex2_approx((a.m - ref) * c1) + s1 * ex2_approx((m - ref) * c1);
+    a.s = a.s * ex2f((a.m - ref) * c) + s * ex2f((m - ref) * c);
+    if (TWO) a.s1 = a.s1 * ex2f((a.m - ref) * c1) + s1 * ex2f((m - ref) * c1);
     a.m = top;
 }
 
@@ -122,13 +122,13 @@ template <bool TWO> struct Exps {
     // type's lowest value, or of 1e4 and more, lose nothing in a product
     __device__ __forceinline__ void at(float z, float m, float& e, float& e1) const {
         const float d = z - m;
-        e = ex2_approx(d * c);
+        e = ex2f(d * c);
         if (TWO) {
             if (squarings) {
                 e1 = e * e;
                 if (squarings > 1) e1 *= e1;
                 if (squarings > 2) e1 *= e1;
-            } else e1 = ex2_approx(d * c1);
+            } else e1 = ex2f(d * c1);
         }
     }
 };
@@ -140,8 +140,8 @@ __device__ __forceinline__ void take(Run& r, const float* v, const Exps<TWO>& X)
     for (int i = 1; i < NE; ++i) top = fmaxf(top, v[i]);
     if (top > r.m) {
         const float old = r.m;          // -inf at first: exp gives 0
-        r.s *= ex2_approx((old - top) * X.c);
-        if (TWO) r.s1 *= ex2_approx((old - top) * X.c1);
+        r.s *= ex2f((old - top) * X.c);
+        if (TWO) r.s1 *= ex2f((old - top) * X.c1);
         r.m = top;
     }
     const float ref = r.m == -INFINITY ? 0.f : r.m;
