@@ -10,9 +10,14 @@
 // largest width), so the variance is the mean of squared deviations from the
 // finished mean and nothing is read twice.  The grid is one wave of resident
 // blocks that walk the rows; each thread keeps its columns' weight, and in the
-// backward its columns' sums of dy xh and dy, from row to row.  The blocks'
+// backward its columns' sums of dy xh and dy, from row to row.  Rows whose
+// pieces are 16 bytes come through a ring in shared memory, three rows ahead
+// of their use: a thread copies only what it reads itself, so the ring needs no
+// barrier, and the loads in flight do not depend on the registers.  The blocks'
 // sums are added in block order by a second kernel: no atomics, so the
 // gradients are the same bits on every run of one device.
+#include <atomic>
+
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -34,62 +39,193 @@ __device__ __forceinline__ void row_sum(float& a, float& b, int tpr, float2* red
     if (lane == 0) r[warp] = make_float2(a, b);
     __syncthreads();
     const int w0 = warp & ~(nw - 1);
+    if (nw <= 4) {
+        float2 s = r[w0];
+        a = s.x;
+        b = s.y;
+        for (int i = 1; i < nw; ++i) {
+            s = r[w0 + i];
+            a += s.x;
+            if (NB == 2) b += s.y;
+        }
+        return;
+    }
     const float2 s = lane < nw ? r[w0 + lane] : make_float2(0.f, 0.f);
     a = warp_sum(s.x);
     if (NB == 2) b = warp_sum(s.y);
 }
 
-template <typename TX, typename TY, int VEC>
-__global__ void __launch_bounds__(1024)
-    fwd_kernel(const TX* __restrict__ x, int64_t ldx, const float* __restrict__ w, const float* __restrict__ b,
-               TY* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t N, int D, float eps,
-               int tpr) {
-    constexpr int NV = PER / VEC;
-    __shared__ float2 red[64];
-    int turn = 0;
-    const int t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-    const float inv = 1.0f / (float)D;
-    float wv[PER], bv[PER];
+// A thread's elements of a row, in pairs (two columns an instruction): element
+// i * VEC + j is column (i * tpr + t) * VEC + j.
+template <int PER> struct PairsOf {
+    uint64_t v[PER / 2];
+    __device__ __forceinline__ void fill(float a) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * tpr + t) * VEC;
+        for (int e = 0; e < PER / 2; ++e) v[e] = f2(a, a);
+    }
+    __device__ __forceinline__ float sum() const {
+        uint64_t s = v[0];
+        float a, b;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            wv[i * VEC + j] = w && c + j < D ? w[c + j] : 1.0f;
-            bv[i * VEC + j] = b && c + j < D ? b[c + j] : 0.0f;
+        for (int e = 1; e < PER / 2; ++e) s = add2(s, v[e]);
+        unf2(s, a, b);
+        return a + b;
+    }
+    __device__ __forceinline__ float get(int e) const {
+        float a, b;
+        unf2(v[e / 2], a, b);
+        return e & 1 ? b : a;
+    }
+    __device__ __forceinline__ void set(int e, float x) {
+        float a, b;
+        unf2(v[e / 2], a, b);
+        v[e / 2] = e & 1 ? f2(a, x) : f2(x, b);
+    }
+    // VEC columns from / to memory as piece i
+    template <int VEC, typename T> __device__ __forceinline__ void load(int i, const T* p) {
+        if constexpr (VEC == 1) set(i, to_f32(*p));
+        else {
+            float x[8];
+            load_vec<8>(p, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i * 4 + j] = f2(x[2 * j], x[2 * j + 1]);
         }
     }
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < N; r0 += (int64_t)gridDim.x * groups) {
-        const int64_t row = r0 + group;
-        const bool live = row < N;
-        float v[PER];
-        float sum = 0.f, none = 0.f;
+    template <int VEC, typename T> __device__ __forceinline__ void store(int i, T* p) const {
+        if constexpr (VEC == 1) *p = from_f32<T>(get(i));
+        else {
+            float x[8];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * tpr + t) * VEC;
-            if (live && c < D) load_vec<VEC>(x + row * ldx + c, v + i * VEC);
-            else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0.f;
-            }
+            for (int j = 0; j < 4; ++j) unf2(v[i * 4 + j], x[2 * j], x[2 * j + 1]);
+            store_vec<8>(p, x);
         }
+    }
+    template <int VEC> __device__ __forceinline__ void clear(int i) {
+        if constexpr (VEC == 1) set(i, 0.f);
+        else {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) sum += v[i];
-        row_sum<1>(sum, none, tpr, red, turn);
-        const float mu = sum * inv;
-        float sq = 0.f;
+            for (int j = 0; j < 4; ++j) v[i * 4 + j] = 0;
+        }
+    }
+};
+
+using Pairs = PairsOf<PER>;
+
+// rows of a ring: three or two on their way (1024 threads of 4-byte pieces fill 192 KB with three stages)
+template <typename TX, typename TY> constexpr int ring_stages() { return sizeof(TX) + sizeof(TY) > 4 ? 3 : 4; }
+
+// A thread's pieces of rows, STAGES deep: [stage][piece][thread] of 16 bytes.
+// Addresses are 32-bit offsets and pointers that move by a constant a row:
+// computed anew for every piece they were half of all instructions issued.
+// Piece groups (8 elements) of a thread are `gap` bytes apart in memory.
+template <typename T, int STAGES, int EL = PER> struct Ring {
+    static constexpr int HALF = (int)sizeof(T) / 2, GROUPS = EL / 8;      // HALF: pieces of 8 elements
+    static constexpr int BYTES = STAGES * GROUPS * HALF * 16;             // per thread
+    const char* src;         // this thread's part of the next row to fetch
+    int64_t row_bytes;       // from one of its rows to the next
+    uint32_t base, piece, stage_bytes, put, get;
+    __device__ __forceinline__ Ring(uint32_t smem, const T* first, int64_t stride)
+        : src(reinterpret_cast<const char*>(first)), row_bytes(stride * (int64_t)sizeof(T)),
+          base(smem + threadIdx.x * 16), piece(blockDim.x * 16), stage_bytes(GROUPS * HALF * piece), put(0), get(0) {}
+    __device__ __forceinline__ void fetch(bool row, int gap, int here, int D, int cols) {
+        if (row) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if ((i * tpr + t) * VEC < D) {
+            for (int i = 0; i < GROUPS; ++i) {
+                if (here + i * cols < D) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    v[i * VEC + j] -= mu;
-                    sq += v[i * VEC + j] * v[i * VEC + j];
+                    for (int h = 0; h < HALF; ++h)
+                        copy16(base + put + (i * HALF + h) * piece, src + i * gap + h * 16);
                 }
             }
         }
+        copy_commit();
+        src += row_bytes;
+        put += stage_bytes;
+        if (put == STAGES * stage_bytes) put = 0;
+    }
+    __device__ __forceinline__ void read(int i, PairsOf<EL>& p) const {
+        float x[8];
+#pragma unroll
+        for (int h = 0; h < HALF; ++h)
+            Pack16<T>::unpack(read16(base + get + (i * HALF + h) * piece), x + h * Pack16<T>::N);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.v[i * 4 + j] = f2(x[2 * j], x[2 * j + 1]);
+    }
+    __device__ __forceinline__ void next() {
+        get += stage_bytes;
+        if (get == STAGES * stage_bytes) get = 0;
+    }
+};
+
+template <typename TX, int EL> constexpr int fwd_stages() { return EL == 64 || sizeof(TX) == 4 ? 3 : 4; }
+
+// EL elements a thread.  With 64 of them a row of 2048 belongs to one warp: no
+// barrier, and the two sums cost a third of an instruction an element; with 16
+// (four warps a row) the kernel issued 25 an element and took 135 us for 65533
+// x 2048 bf16, above the 82 us of its bytes.
+// ONE: a row is one warp's (the columns' distances are then constants).
+template <typename TX, typename TY, int VEC, int EL, bool ONE>
+__global__ void __launch_bounds__(VEC == 1 ? 1024 : 256)
+    fwd_kernel(const TX* __restrict__ x, int64_t ldx, const float* __restrict__ w, const float* __restrict__ b,
+               TY* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t N, int D, float eps,
+               int threads_per_row) {
+    constexpr int NV = EL / VEC, STAGES = fwd_stages<TX, EL>();
+    extern __shared__ __align__(16) uint8_t dyn_f[];
+    __shared__ float2 red[64];
+    int turn = 0;
+    const int tpr = ONE ? 32 : threads_per_row;
+    const int t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    const float inv = 1.0f / (float)D;
+    const bool whole = D == tpr * EL;            // every piece of every thread is there
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    const int cols = tpr * VEC, here = t * VEC;
+    Ring<TX, STAGES, EL> ring(static_cast<uint32_t>(__cvta_generic_to_shared(dyn_f)), x + row * ldx + here,
+                              step * ldx);
+    TY* dst = y + row * D + here;
+    if constexpr (VEC == 8) {
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; ++k)
+            ring.fetch(row + k * step < N, cols * (int)sizeof(TX), here, D, cols);
+    }
+    for (; row - group < N; row += step) {
+        const bool live = row < N;
+        PairsOf<EL> v;
+        if constexpr (VEC == 8) {
+            ring.fetch(row + (STAGES - 1) * step < N, cols * (int)sizeof(TX), here, D, cols);
+            copy_wait<STAGES - 1>();
+        }
+        if (!whole || !live) v.fill(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (live && here + i * cols < D) {
+                if constexpr (VEC == 8) ring.read(i, v);
+                else v.template load<VEC>(i, x + row * ldx + here + i * cols);
+            }
+        }
+        ring.next();
+        float sum = v.sum(), none = 0.f;
+        row_sum<1>(sum, none, tpr, red, turn);
+        const float mu = sum * inv;
+        const uint64_t mu2 = f2(-mu, -mu);
+#pragma unroll
+        for (int e = 0; e < EL / 2; ++e) v.v[e] = add2(v.v[e], mu2);
+        if (!whole) {                             // deviations of columns that are not there weigh nothing
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (here + i * cols >= D) v.template clear<VEC>(i);
+        }
+        uint64_t sq2 = 0;
+#pragma unroll
+        for (int e = 0; e < EL / 2; ++e) sq2 = fma2(v.v[e], v.v[e], sq2);
+        float sq, sq_b;
+        unf2(sq2, sq, sq_b);
+        sq += sq_b;
         row_sum<1>(sq, none, tpr, red, turn);
-        const float rs = 1.0f / sqrtf(sq * inv + eps);
+        const float rs = rsqrtf(sq * inv + eps);
+        const uint64_t rs2 = f2(rs, rs);
+#pragma unroll
+        for (int e = 0; e < EL / 2; ++e) v.v[e] = mul2(v.v[e], rs2);
         if (live) {
             if (mean && t == 0) {
                 mean[row] = mu;
@@ -97,15 +233,24 @@ __global__ void __launch_bounds__(1024)
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VEC;
-                if (c < D) {
-                    float o[VEC];
+                const int c = here + i * cols;
+                if (c < D) {                          // weight and bias stay in the L1
+                    if constexpr (VEC == 1) {
+                        v.set(i, fmaf(v.get(i), w ? w[c] : 1.0f, b ? b[c] : 0.0f));
+                    } else {
+                        PairsOf<8> wv, bv;
+                        wv.fill(1.0f);
+                        bv.fill(0.0f);
+                        if (w) wv.template load<8>(0, w + here + i * cols);
+                        if (b) bv.template load<8>(0, b + here + i * cols);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) o[j] = v[i * VEC + j] * rs * wv[i * VEC + j] + bv[i * VEC + j];
-                    store_vec<VEC>(y + row * D + c, o);
+                        for (int j = 0; j < 4; ++j) v.v[i * 4 + j] = fma2(v.v[i * 4 + j], wv.v[j], bv.v[j]);
+                    }
+                    v.template store<VEC>(i, dst + i * cols);
                 }
             }
         }
+        dst += step * D;
     }
 }
 
@@ -117,73 +262,126 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 512)
     bwd_kernel(const TX* __restrict__ x, int64_t ldx, const TY* __restrict__ dy, int64_t lddy,
                const float* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd,
                TX* __restrict__ dx, float* __restrict__ part, int64_t N, int D, int tpr) {
-    constexpr int NV = PER / VEC;
-    extern __shared__ float dyn[];               // WIDE: 2 * PER * blockDim sums; else groups * D * 2 at the end
+    constexpr int NV = PER / VEC, STAGES = ring_stages<TX, TY>();
+    // WIDE: 2 * PER * 1024 sums; else the rings, whose place the groups' sums take at the end
+    extern __shared__ __align__(16) uint8_t dyn_b[];
+    float* dyn = reinterpret_cast<float*>(dyn_b);
     __shared__ float2 red[64];
     int turn = 0;
     const int t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const int64_t step = (int64_t)gridDim.x * groups;
     const float inv = 1.0f / (float)D;
-    float aw[WIDE ? 1 : PER], ab[WIDE ? 1 : PER];
+    const bool whole = D == tpr * PER;
+    constexpr bool RING = VEC == 8 && !WIDE;     // WIDE has no room beside its sums
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    const int cols = tpr * VEC, here = t * VEC;
+    const uint32_t smem = static_cast<uint32_t>(__cvta_generic_to_shared(dyn_b));
+    Ring<TX, STAGES> xr(smem, x + row * ldx + here, step * ldx);
+    Ring<TY, STAGES> yr(smem + Ring<TX, STAGES>::BYTES * blockDim.x, dy + row * lddy + here, step * lddy);
+    TX* dst = dx + row * D + here;
+    // (two groups of copies a row)
+    auto fetch = [&](bool there) {
+        xr.fetch(there, cols * (int)sizeof(TX), here, D, cols);
+        yr.fetch(there, cols * (int)sizeof(TY), here, D, cols);
+    };
+    if constexpr (RING) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if constexpr (WIDE) { dyn[i * 1024 + threadIdx.x] = 0.f; dyn[(PER + i) * 1024 + threadIdx.x] = 0.f; }
-        else { aw[i] = 0.f; ab[i] = 0.f; }
+        for (int k = 0; k < STAGES - 1; ++k) fetch(row + k * step < N);
     }
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < N; r0 += (int64_t)gridDim.x * groups) {
-        const int64_t row = r0 + group;
+    Pairs aw, ab;                                 // column sums of dy xh and dy (not WIDE)
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < 2 * PER; ++e) dyn[e * 1024 + threadIdx.x] = 0.f;
+    } else {
+        aw.fill(0.f);
+        ab.fill(0.f);
+    }
+    Pairs wv;
+    wv.fill(1.0f);
+    if (!WIDE && w) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * tpr + t) * VEC;
+            if (c < D) wv.template load<VEC>(i, w + c);
+        }
+    }
+    float mu = 0.f, rs = 0.f;                     // of this row, fetched a row ahead
+    if (row < N) { mu = mean[row]; rs = rstd[row]; }
+    for (; row - group < N; row += step) {
         const bool live = row < N;
-        const float mu = live ? mean[row] : 0.f, rs = live ? rstd[row] : 0.f;
-        float xh[PER], g[PER];
-        float s1 = 0.f, s2 = 0.f;
+        float next_mu = 0.f, next_rs = 0.f;
+        if (row + step < N) { next_mu = mean[row + step]; next_rs = rstd[row + step]; }
+        Pairs xh, g;
+        if constexpr (RING) {
+            fetch(row + (STAGES - 1) * step < N);
+            copy_wait<2 * (STAGES - 1)>();
+        }
+        if (!whole || !live) {                    // g = 0: what is not there weighs nothing
+            xh.fill(0.f);
+            g.fill(0.f);
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * tpr + t) * VEC;
+            const int c = here + i * cols;
             if (live && c < D) {
-                load_vec<VEC>(x + row * ldx + c, xh + i * VEC);
-                load_vec<VEC>(dy + row * lddy + c, g + i * VEC);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) { xh[i * VEC + j] = mu; g[i * VEC + j] = 0.f; }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * tpr + t) * VEC;
-            float wv[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) wv[j] = 1.0f;
-            if (w && c < D) load_vec<VEC>(w + c, wv);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int e = i * VEC + j;
-                xh[e] = (xh[e] - mu) * rs;
-                if constexpr (WIDE) {
-                    dyn[e * 1024 + threadIdx.x] += g[e] * xh[e];
-                    dyn[(PER + e) * 1024 + threadIdx.x] += g[e];
+                if constexpr (RING) {
+                    xr.read(i, xh);
+                    yr.read(i, g);
                 } else {
-                    aw[e] += g[e] * xh[e];
-                    ab[e] += g[e];
+                    xh.template load<VEC>(i, x + row * ldx + c);
+                    g.template load<VEC>(i, dy + row * lddy + c);
                 }
-                g[e] *= wv[j];
-                s1 += g[e];
-                s2 += g[e] * xh[e];
             }
         }
-        row_sum<2>(s1, s2, tpr, red, turn);
-        s1 *= inv;
-        s2 *= inv;
-        if (live) {
+        xr.next();
+        yr.next();
+        const uint64_t rs2 = f2(rs, rs), mr2 = f2(-mu * rs, -mu * rs);
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) {
+            xh.v[e] = fma2(xh.v[e], rs2, mr2);
+            if constexpr (WIDE) {
+                float ga, gb, xa, xb;
+                unf2(g.v[e], ga, gb);
+                unf2(xh.v[e], xa, xb);
+                dyn[(2 * e) * 1024 + threadIdx.x] += ga * xa;
+                dyn[(2 * e + 1) * 1024 + threadIdx.x] += gb * xb;
+                dyn[(PER + 2 * e) * 1024 + threadIdx.x] += ga;
+                dyn[(PER + 2 * e + 1) * 1024 + threadIdx.x] += gb;
+            } else {
+                aw.v[e] = fma2(g.v[e], xh.v[e], aw.v[e]);
+                ab.v[e] = add2(g.v[e], ab.v[e]);
+            }
+        }
+        if (WIDE && w) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * tpr + t) * VEC;
-                if (c < D) {
-                    float o[VEC];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) o[j] = rs * (g[i * VEC + j] - s1 - xh[i * VEC + j] * s2);
-                    store_vec<VEC>(dx + row * D + c, o);
-                }
+                if (c < D) wv.template load<VEC>(i, w + c);
             }
         }
+        uint64_t gx = 0;
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) {
+            g.v[e] = mul2(g.v[e], wv.v[e]);
+            gx = fma2(g.v[e], xh.v[e], gx);
+        }
+        float s1 = g.sum(), s2, s2_b;
+        unf2(gx, s2, s2_b);
+        s2 += s2_b;
+        row_sum<2>(s1, s2, tpr, red, turn);
+        // dx = rs g - rs mean(g) - rs mean(g xh) xh
+        const uint64_t c1 = f2(-rs * (s1 * inv), -rs * (s1 * inv)), c2 = f2(-rs * (s2 * inv), -rs * (s2 * inv));
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) g.v[e] = fma2(xh.v[e], c2, fma2(g.v[e], rs2, c1));
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (here + i * cols < D) g.template store<VEC>(i, dst + i * cols);
+            }
+        }
+        dst += step * D;
+        mu = next_mu;
+        rs = next_rs;
     }
     if (!part) return;
     float* out = part + (int64_t)blockIdx.x * 2 * D;
@@ -195,10 +393,14 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 512)
         }
     } else {
         // the groups' sums meet in shared memory and are added in group order
+        if constexpr (RING) {
+            copy_wait<0>();
+            __syncthreads();
+        }
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int c = ((e / VEC) * tpr + t) * VEC + e % VEC;
-            if (c < D) { dyn[group * 2 * D + c] = aw[e]; dyn[group * 2 * D + D + c] = ab[e]; }
+            if (c < D) { dyn[group * 2 * D + c] = aw.get(e); dyn[group * 2 * D + D + c] = ab.get(e); }
         }
         __syncthreads();
         for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
@@ -243,6 +445,13 @@ int sm_count() {
     return n;
 }
 
+// more than 48 KB of shared memory a block, 1 KB of it static here, has to be asked for (per device; asking again changes nothing)
+template <typename K> int allow_smem(K k, size_t smem, const char* name) {
+    if (smem <= 47 * 1024) return CONCORD_OK;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    return e == cudaSuccess ? CONCORD_OK : fail(CONCORD_ELAUNCH, std::string(name) + ": " + cudaGetErrorString(e));
+}
+
 // blocks of the backward: one wave of 512 threads per SM (1024 where a row takes 1024)
 int bwd_blocks(int64_t N, int64_t D, int* threads) {
     const int tpr = threads_per_row(D);
@@ -252,17 +461,38 @@ int bwd_blocks(int64_t N, int64_t D, int* threads) {
     return (int)(need < wave ? need : wave);
 }
 
+template <typename TX, typename TY, int VEC, int EL>
+int launch_fwd(const void* x, int64_t ldx, const float* w, const float* b, void* y, float* mean, float* rstd,
+               int64_t N, int64_t D, float eps, cudaStream_t st) {
+    int tpr = 32;
+    while (tpr * EL < D) tpr *= 2;
+    const int threads = VEC == 1 ? (tpr > 256 ? tpr : 256) : (tpr > 128 ? tpr : 128);
+    const int64_t groups = threads / tpr, need = (N + groups - 1) / groups;
+    auto k = tpr == 32 ? fwd_kernel<TX, TY, VEC, EL, true> : fwd_kernel<TX, TY, VEC, EL, false>;
+    const size_t smem = VEC == 8 ? (size_t)Ring<TX, fwd_stages<TX, EL>(), EL>::BYTES * threads : 0;
+    if (int rc = allow_smem(k, smem, "concord_layer_norm_fwd")) return rc;
+    // one wave of resident blocks (asked for once per form; the answer is the architecture's)
+    static std::atomic<int> resident[8];
+    std::atomic<int>& known = resident[__builtin_ctz(tpr) - 5];
+    int per_sm = known.load();
+    if (per_sm == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, threads, smem) != cudaSuccess || per_sm < 1)
+            per_sm = 1;
+        known.store(per_sm);
+    }
+    const int64_t wave = (int64_t)sm_count() * per_sm;
+    k<<<(int)(need < wave ? need : wave), threads, smem, st>>>(static_cast<const TX*>(x), ldx, w, b,
+                                                               static_cast<TY*>(y), mean, rstd, N, (int)D, eps, tpr);
+    return check_launch("concord_layer_norm_fwd");
+}
+
 template <typename TX, typename TY>
 int forward(const void* x, int64_t ldx, const float* w, const float* b, void* y, float* mean, float* rstd, int64_t N,
             int64_t D, float eps, bool vec, cudaStream_t st) {
-    const int tpr = threads_per_row(D), threads = tpr > 256 ? tpr : 256;
-    const int64_t groups = threads / tpr, need = (N + groups - 1) / groups;
-    const int64_t wave = (int64_t)sm_count() * (1024 / threads);
-    const int grid = (int)(need < wave ? need : wave);
-    auto k = vec ? fwd_kernel<TX, TY, 8> : fwd_kernel<TX, TY, 1>;
-    k<<<grid, threads, 0, st>>>(static_cast<const TX*>(x), ldx, w, b, static_cast<TY*>(y), mean, rstd, N, (int)D, eps,
-                                tpr);
-    return check_launch("concord_layer_norm_fwd");
+    if (!vec) return launch_fwd<TX, TY, 1, 16>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
+    if (D <= 512) return launch_fwd<TX, TY, 8, 16>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
+    if (D <= 1024) return launch_fwd<TX, TY, 8, 32>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
+    return launch_fwd<TX, TY, 8, 64>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
 }
 
 template <typename TX, typename TY>
@@ -272,14 +502,13 @@ int backward(const void* x, int64_t ldx, const void* dy, int64_t lddy, const flo
     int threads = 0;
     const int grid = bwd_blocks(N, D, &threads), tpr = threads_per_row(D);
     const bool wide = tpr == 1024;
-    const size_t smem = wide ? 2 * PER * 1024 * sizeof(float) : (size_t)(threads / tpr) * 2 * D * sizeof(float);
+    const size_t sums = (size_t)(threads / tpr) * 2 * D * sizeof(float);
+    constexpr int ST = ring_stages<TX, TY>();
+    const size_t rings = vec ? (size_t)(Ring<TX, ST>::BYTES + Ring<TY, ST>::BYTES) * threads : 0;
+    const size_t smem = wide ? 2 * PER * 1024 * sizeof(float) : sums > rings ? sums : rings;
     auto k = wide ? (vec ? bwd_kernel<TX, TY, 8, true> : bwd_kernel<TX, TY, 1, true>)
                   : (vec ? bwd_kernel<TX, TY, 8, false> : bwd_kernel<TX, TY, 1, false>);
-    if (smem > 48 * 1024) {
-        // 128 KB at most; set on every call that needs it (the attribute is per device and idempotent)
-        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return fail(CONCORD_ELAUNCH, std::string("concord_layer_norm_bwd: ") + cudaGetErrorString(e));
-    }
+    if (int rc = allow_smem(k, smem, "concord_layer_norm_bwd")) return rc;
     if (!dw && !db) part = nullptr;
     k<<<grid, threads, smem, st>>>(static_cast<const TX*>(x), ldx, static_cast<const TY*>(dy), lddy, w, mean, rstd,
                                    static_cast<TX*>(dx), part, N, (int)D, tpr);
@@ -325,7 +554,8 @@ extern "C" int concord_layer_norm_fwd(const void* x, int32_t x_type, int64_t ldx
     if (int rc = norm::check_shape("concord_layer_norm_fwd", x_type, y_type, N, D, ldx)) return rc;
     if (N == 0) return CONCORD_OK;
     if (!x || !y || !mean != !rstd) return fail(CONCORD_EINVAL, "concord_layer_norm_fwd: null pointer");
-    const bool vec = D % 8 == 0 && ldx * norm::esize(x_type) % 16 == 0 && aligned(x, 16) && aligned(y, 16);
+    const bool vec = D % 8 == 0 && ldx * norm::esize(x_type) % 16 == 0 && aligned(x, 16) && aligned(y, 16) &&
+                     aligned(w, 16) && aligned(b, 16);
     NORM_TYPES(x_type, y_type, norm::forward, x, ldx, w, b, y, mean, rstd, N, D, eps, vec, as_stream(stream))
 }
 
@@ -350,7 +580,7 @@ extern "C" int concord_layer_norm_bwd(const void* x, int32_t x_type, int64_t ldx
     if ((dw || db) && (!workspace || workspace_bytes < concord_layer_norm_bwd_workspace_bytes(N, D)))
         return fail(CONCORD_EWORKSPACE, "concord_layer_norm_bwd: workspace too small");
     const bool vec = D % 8 == 0 && ldx * norm::esize(x_type) % 16 == 0 && lddy * norm::esize(dy_type) % 16 == 0 &&
-                     aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) && (!w || aligned(w, 16));
+                     aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) && aligned(w, 16);
     NORM_TYPES(x_type, dy_type, norm::backward, x, ldx, dy, lddy, w, mean, rstd, dx, dw, db, N, D, vec,
                static_cast<float*>(workspace), st)
 }

@@ -78,6 +78,23 @@ template <int VEC, typename T> __device__ __forceinline__ void store_vec(T* p, c
     }
 }
 
+// asynchronous copies of 16 bytes into shared memory, in groups of this thread
+__device__ __forceinline__ void copy16(uint32_t smem, const void* g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(g) : "memory");
+}
+__device__ __forceinline__ uint4 read16(uint32_t smem) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(smem)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 // 2^x, subnormal results flushed to 0 (without .ftz each call costs three more instructions)
 __device__ __forceinline__ float ex2f(float x) {
     float r;
