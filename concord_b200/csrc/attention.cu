@@ -604,36 +604,47 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool live = row < w.lq;
         const int64_t trow = (int64_t)w.q0 + row;
         // delta = do . o, o with its rest: o rounded to 16 bits alone makes the
-        // error of dq and dk a tenth larger.  The halves take alternate 16
-        // bytes, then add in order.
-        float d = 0.f;
-        if (live) {
-            const T* a = static_cast<const T*>(P.dout) + trow * P.do_ts + head * P.do_hs;
-            const T* b = static_cast<const T*>(P.o) + (trow * P.H + head) * P.D;
-            const T* b2 = static_cast<const T*>(P.rest) + (trow * P.H + head) * P.D;
-            for (int c = half * 8; c < P.D; c += 16) {
-                float x[8], y[8], z[8];
-                load_vec<8>(a + c, x);
-                load_vec<8>(b + c, y);
-                load_vec<8>(b2 + c, z);
+        // error of dq and dk a tenth larger.  A row's 16-byte pieces go to
+        // neighbouring lanes (a lane a row would touch 32 lines a load), each
+        // warp takes 16 rows.
+        {
+            constexpr int CH = DP / 8, AT = 32 / CH;           // lanes of a row, rows a load
+            const int sub = lane / CH, c = lane % CH * 8;
+#pragma unroll 4
+            for (int k = 0; k < 16; k += AT) {
+                const int x = (warp - 4) * 16 + k + sub;
+                float d = 0.f;
+                if (r0 + x < w.lq && c < P.D) {
+                    const int64_t tok = (int64_t)w.q0 + r0 + x, at = (tok * P.H + head) * P.D + c;
+                    float g[8], o[8], e[8];
+                    load_vec<8>(static_cast<const T*>(P.dout) + tok * P.do_ts + head * P.do_hs + c, g);
+                    load_vec<8>(static_cast<const T*>(P.o) + at, o);
+                    load_vec<8>(static_cast<const T*>(P.rest) + at, e);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e] + z[e], d);
+                    for (int i = 0; i < 8; ++i) d = fmaf(g[i], o[i] + e[i], d);
+                }
+#pragma unroll
+                for (int i = CH / 2; i > 0; i >>= 1) d += __shfl_xor_sync(0xffffffffu, d, i);
+                if (lane % CH == 0) {
+                    red[x] = d;
+                    if (r0 + x < w.lq) P.delta[(int64_t)head * P.Tq + w.q0 + r0 + x] = d;
+                }
             }
         }
-        red[half * 128 + r] = d;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        d = red[r] + red[128 + r];
+        const float d = red[r];
         float lse = live ? P.lse[(int64_t)head * P.Tq + trow] : 0.f;
         if (lse == -INFINITY) lse = 0.f;           // no key: everything is masked below
-        if (live && half == 0) P.delta[(int64_t)head * P.Tq + trow] = d;
         const float l2 = -lse * LOG2E;
         const uint64_t c2 = f2(P.scale2, P.scale2), l22 = f2(l2, l2), nd2 = f2(-d, -d);
         const int mine = (P.causal ? min(w.lk, row + off + 1) : w.lk) - half * 64;
         const int every = P.causal ? min(w.lk, r0 + off + 1) : w.lk;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         for (int j = 0; j < n; ++j) {
-            float p[64];
-            uint32_t u[64];
+            // S and dP are read whole, which frees their places for the next
+            // block's products, and then meet element by element: exponentials
+            // and the arithmetic of ds overlap
+            uint32_t u[64], v[64];
             if (!mbar_wait(s_full, j & 1, P.err, 32)) goto done;
             fence_after();
             ld32(tmem + lanes + half * 64, u);
@@ -641,31 +652,28 @@ __global__ void __launch_bounds__(THREADS, 1)
             wait_ld();
             fence_before();
             mbar_arrive(s_free);
-#pragma unroll
-            for (int k = 0; k < 64; k += 2) {
-                float a, b;
-                unf2(fma2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, l22), a, b);
-                p[k] = ex2f(a);
-                p[k + 1] = ex2f(b);
-            }
             if (!mbar_wait(dp_full, j & 1, P.err, 33)) goto done;
             fence_after();
-            ld32(tmem + lanes + 128 + half * 64, u);
-            ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
+            ld32(tmem + lanes + 128 + half * 64, v);
+            ld32(tmem + lanes + 128 + half * 64 + 32, v + 32);
             wait_ld();
             fence_before();
             mbar_arrive(dp_free);
+            const bool masked = (j + 1) * 128 > every;
+            auto weigh = [&](bool mask) {
 #pragma unroll
-            for (int k = 0; k < 64; k += 2)
-                unf2(mul2(f2(p[k], p[k + 1]), add2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), nd2)), p[k],
-                     p[k + 1]);
-            if ((j + 1) * 128 > every) {
-#pragma unroll
-                for (int k = 0; k < 64; ++k)
-                    if (j * 128 + k >= mine) p[k] = 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < 32; ++k) u[k] = pack2(p[2 * k], p[2 * k + 1], T());
+                for (int k = 0; k < 64; k += 2) {
+                    float a, b;
+                    unf2(fma2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, l22), a, b);
+                    a = ex2f(a);
+                    b = ex2f(b);
+                    unf2(mul2(f2(a, b), add2(f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), nd2)), a, b);
+                    if (mask && j * 128 + k >= mine) a = 0.f;
+                    if (mask && j * 128 + k + 1 >= mine) b = 0.f;
+                    u[k >> 1] = pack2(a, b, T());
+                }
+            };
+            if (masked) weigh(true); else weigh(false);
             if (j > 0 && !mbar_wait(ds_free, (j - 1) & 1, P.err, 34)) goto done;
             st32(tmem + lanes + 384 + half * 32, u);
             wait_st();

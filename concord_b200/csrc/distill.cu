@@ -53,7 +53,6 @@ struct Args {
     float* row_loss;        // [N]
     float* row_counts;      // [N]: 1 where the row counts
     void* dz;
-    int squarings;          // log2(T) where T = 2, 4, 8
     int tpr;
 };
 
@@ -102,183 +101,230 @@ __device__ __forceinline__ int total_count(const Args& A) {
     return __reduce_add_sync(0xffffffffu, n);
 }
 
+// KIND of a kernel: 0: one temperature serves both terms (or there is one term
+// only); 1: two exponentials; 1 + n: T = 2^n, the second is the first squared n times
 // running maximum with the sums of exp((z - m) / T) and exp(z - m)
 struct Run {
     float m, s, s1;
 };
 
-template <bool TWO>
+template <int KIND>
 __device__ __forceinline__ void merge(Run& a, float m, float s, float s1, float c, float c1) {
     const float top = fmaxf(a.m, m), ref = top == -INFINITY ? 0.f : top;
     a.s = a.s * ex2f((a.m - ref) * c) + s * ex2f((m - ref) * c);
-    if (TWO) a.s1 = a.s1 * ex2f((a.m - ref) * c1) + s1 * ex2f((m - ref) * c1);
+    if (KIND) a.s1 = a.s1 * ex2f((a.m - ref) * c1) + s1 * ex2f((m - ref) * c1);
     a.m = top;
 }
 
-template <bool TWO> struct Exps {
+template <int KIND> struct Exps {
     float c, c1;
-    int squarings;
-    // exp((z - m) / T) and exp(z - m); the difference first, so that rows of the
-    // type's lowest value, or of 1e4 and more, lose nothing in a product
-    __device__ __forceinline__ void at(float z, float m, float& e, float& e1) const {
-        const float d = z - m;
-        e = ex2f(d * c);
-        if (TWO) {
-            if (squarings) {
-                e1 = e * e;
-                if (squarings > 1) e1 *= e1;
-                if (squarings > 2) e1 *= e1;
-            } else e1 = ex2f(d * c1);
+    // exp((z - m) / T) and exp(z - m) of two logits; the difference first, so
+    // that rows of the type's lowest value, or of 1e4 and more, lose nothing in
+    // a product.  `neg`: -m twice.
+    __device__ __forceinline__ void at(uint64_t z, uint64_t neg, uint64_t& e, uint64_t& e1) const {
+        const uint64_t d = add2(z, neg);
+        float a, b;
+        unf2(mul2(d, f2(c, c)), a, b);
+        e = f2(ex2f(a), ex2f(b));
+        e1 = e;
+        if (KIND == 1) {
+            unf2(mul2(d, f2(c1, c1)), a, b);
+            e1 = f2(ex2f(a), ex2f(b));
         }
+#pragma unroll
+        for (int i = 1; i < KIND; ++i) e1 = mul2(e1, e1);
     }
 };
 
-template <bool TWO, int NE>
-__device__ __forceinline__ void take(Run& r, const float* v, const Exps<TWO>& X) {
-    float top = v[0];
+// NE logits (even) into a thread's running maximum and sums
+template <int KIND, int NE>
+__device__ __forceinline__ void take(Run& r, const float* v, const Exps<KIND>& X) {
+    float top = fmaxf(v[0], v[1]);
 #pragma unroll
-    for (int i = 1; i < NE; ++i) top = fmaxf(top, v[i]);
+    for (int i = 2; i < NE; i += 2) top = max3(top, v[i], v[i + 1]);
     if (top > r.m) {
         const float old = r.m;          // -inf at first: exp gives 0
         r.s *= ex2f((old - top) * X.c);
-        if (TWO) r.s1 *= ex2f((old - top) * X.c1);
+        if (KIND) r.s1 *= ex2f((old - top) * X.c1);
         r.m = top;
     }
     const float ref = r.m == -INFINITY ? 0.f : r.m;
+    const uint64_t neg = f2(-ref, -ref);
+    uint64_t s[2] = {0, 0}, s1 = 0;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        float e, e1;
-        X.at(v[i], ref, e, e1);
-        r.s += e;
-        if (TWO) r.s1 += e1;
+    for (int i = 0; i < NE; i += 2) {
+        uint64_t e, e1;
+        X.at(f2(v[i], v[i + 1]), neg, e, e1);
+        s[(i >> 1) & 1] = add2(s[(i >> 1) & 1], e);
+        if (KIND) s1 = add2(s1, e1);
+    }
+    float a, b;
+    unf2(add2(s[0], s[1]), a, b);
+    r.s += a + b;
+    if (KIND) {
+        unf2(s1, a, b);
+        r.s1 += a + b;
     }
 }
 
-// T: logits' type; TWO: both temperatures are needed; MODE 1: statistics and
+// 16 bytes of -inf: what stands for the pieces beyond a row's end
+template <typename T> __device__ __forceinline__ uint4 nothing() {
+    const uint32_t u = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(u, u, u, u);
+}
+
+constexpr int DEEP = 4;              // 16-byte loads of a thread on their way at a time
+
+// T: logits' type; MODE 1: statistics and
 // loss, 2: gradient from given statistics, 3: both
-template <typename T, bool TWO, int MODE>
+template <typename T, int KIND, int MODE>
 __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
     constexpr int W = Pack16<T>::N;
-    extern __shared__ float dyn[];       // groups x (K probabilities, K ids)
+    extern __shared__ float dyn[];       // groups x (K probabilities, K ids, K logits at them)
     __shared__ float red[32][3];
-    __shared__ float shared_row[32][4];
+    __shared__ float teacher[32];        // whether the group's teacher has an entry
     const int tpr = A.tpr, t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tpr >> 5;
-    float* prob = dyn + (size_t)group * 2 * A.K;
-    int* pid = reinterpret_cast<int*>(prob + A.K);
-    Exps<TWO> X;
+    const int V = (int)A.V, K = A.K;
+    float* prob = dyn + (size_t)group * 3 * K;
+    int* pid = reinterpret_cast<int*>(prob + K);
+    float* at_id = prob + 2 * K;
+    Exps<KIND> X;
     X.c = LOG2E / A.temp;
     X.c1 = LOG2E;
-    X.squarings = A.squarings;
     float number = 1.f;
     if (MODE == 3 && A.mean) number = (float)max(1, total_count(A));
     if (MODE == 2 && A.mean) number = *A.number;
 
+    // (a block of more than a warp per row holds one row: its branches are uniform)
     auto sync = [&]() { if (tpr == 32) __syncwarp(); else __syncthreads(); };
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < A.N; r0 += (int64_t)gridDim.x * groups) {
-        const int64_t row = r0 + group;
+    const int64_t row0 = (int64_t)blockIdx.x * groups + group;
+    int64_t next_y = row0 < A.N && A.labels ? entry(A.labels, A.labels64, row0) : -1;      // a row ahead
+    for (int64_t row = row0; row - group < A.N; row += (int64_t)gridDim.x * groups) {
         const bool live = row < A.N;
-        const int64_t V = A.V;
         const T* z = static_cast<const T*>(A.z) + (live ? row * A.ldz : 0);
-        const int64_t y = live && A.labels ? entry(A.labels, A.labels64, row) : -1;
-        // aligned body [head, head + body): 16-byte loads; the rest by element
-        const int64_t head = min(V, (int64_t)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
-        const int64_t nvec = (V - head) / W, tail = head + nvec * W;
+        const int64_t y = next_y;
+        const int64_t ahead = row + (int64_t)gridDim.x * groups;
+        next_y = ahead < A.N && A.labels ? entry(A.labels, A.labels64, ahead) : -1;
+        // aligned body [head, tail): 16-byte loads; the rest by element
+        const int head = min(V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
+        const int nvec = (V - head) / W, tail = head + nvec * W;
         bool counts = live && (!A.labels || label_counts(A, y));
+        float t0 = 0.f;
+        int64_t id0 = -1;
+        if (t < 32 && lane < K && live) {
+            t0 = A.t[row * K + lane];
+            id0 = entry(A.ids, A.ids64, row * K + lane);
+        }
 
-        // ---- the teacher's distribution, by the row's first warp ----
-        float has = 0.f, plogp = 0.f;
-        if (t < 32) {
-            float top = -INFINITY;
-            bool any = false;
-            for (int k = lane; counts && k < A.K; k += 32) {
-                const float tk = A.t[row * A.K + k];
-                const bool ok = entry_counts(A, entry(A.ids, A.ids64, row * A.K + k), tk);
-                any |= ok;
-                if (ok) top = fmaxf(top, tk);
+        // ---- maximum and sums (before the teacher's entries are known: a row
+        // that turns out to have none is read for nothing) ----
+        Run R = {-INFINITY, 0.f, 0.f};
+        if ((MODE & 1) && counts) {
+            for (int i = t; i < head + (V - tail); i += tpr) {
+                const float v[2] = {to_f32(z[i < head ? i : tail + (i - head)]), -INFINITY};
+                take<KIND, 2>(R, v, X);
             }
+            const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+            uint4 u[DEEP];
+            auto take_all = [&]() {
+#pragma unroll
+                for (int k = 0; k < DEEP; k += 2) {
+                    float v[2 * W];
+                    Pack16<T>::unpack(u[k], v);
+                    Pack16<T>::unpack(u[k + 1], v + W);
+                    take<KIND, 2 * W>(R, v, X);
+                }
+            };
+            int i = t;
+            for (; i + (DEEP - 1) * tpr < nvec; i += DEEP * tpr) {
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k) u[k] = zv[i + k * tpr];
+                take_all();
+            }
+            if (i < nvec) {
+#pragma unroll
+                for (int k = 0; k < DEEP; ++k) u[k] = i + k * tpr < nvec ? zv[i + k * tpr] : nothing<T>();
+                take_all();
+            }
+        }
+
+        // ---- the teacher's distribution, and the logits at its places, by the
+        // row's first warp (its first 32 entries are on their way since before
+        // the row was read) ----
+        float plogp = 0.f, zy = 0.f;
+        if (t < 32) {
+            if ((MODE & 1) && A.labels && counts) zy = to_f32(z[y]);
+            float top = -INFINITY;
+            for (int k = lane; k < K; k += 32) {
+                float tk = t0;
+                int64_t id = id0;
+                if (k >= 32 && counts) { tk = A.t[row * K + k]; id = entry(A.ids, A.ids64, row * K + k); }
+                const bool ok = counts && entry_counts(A, id, tk);
+                pid[k] = ok ? (int)id : -1;
+                prob[k] = tk;
+                if (ok) {
+                    top = fmaxf(top, tk);
+                    at_id[k] = to_f32(z[id]);
+                }
+            }
+            bool any = false;
+            for (int k = lane; k < K; k += 32) any |= pid[k] >= 0;
             any = __any_sync(0xffffffffu, any);
             top = warp_maxf(top);
             float sum = 0.f;
-            for (int k = lane; k < A.K; k += 32) {
-                float e = 0.f;
-                int id = -1;
-                if (counts) {
-                    const float tk = A.t[row * A.K + k];
-                    const int64_t i64 = entry(A.ids, A.ids64, row * A.K + k);
-                    if (entry_counts(A, i64, tk)) {
-                        id = (int)i64;
-                        e = expf((tk - top) / A.temp);
-                    }
-                }
+            for (int k = lane; k < K; k += 32) {
+                const float d = (prob[k] - top) / A.temp, e = pid[k] >= 0 ? expf(d) : 0.f;
+                if ((MODE & 1) && pid[k] >= 0 && !(e == 0.f)) plogp += e * d;
                 prob[k] = e;
-                pid[k] = id;
                 sum += e;
             }
             sum = warp_sum(sum);
-            for (int k = lane; k < A.K; k += 32) {
-                const float p = any ? prob[k] / sum : 0.f;
-                if ((MODE & 1) && pid[k] >= 0 && !(p == 0.f))
-                    plogp += p * ((A.t[row * A.K + k] - top) / A.temp - logf(sum));
-                prob[k] = p;
+            if (any) {
+                for (int k = lane; k < K; k += 32) prob[k] /= sum;
+                // sum_k p_k log p_k
+                if (MODE & 1) plogp = warp_sum(plogp) / sum - logf(sum);
             }
-            if (MODE & 1) plogp = warp_sum(plogp);
-            has = any ? 1.f : 0.f;
-            if (lane == 0) shared_row[group][0] = has;
+            if (lane == 0) teacher[group] = any ? 1.f : 0.f;
         }
-        sync();
-        has = shared_row[group][0];
-        if (!A.labels) counts = counts && has != 0.f;
 
-        // ---- maximum and sums ----
-        Run R = {-INFINITY, 0.f, 0.f};
+        // ---- the row's statistics, the same bits in every thread ----
         if (MODE & 1) {
-            if (counts) {
-                for (int64_t i = t; i < head + (V - tail); i += tpr) {
-                    const float v = to_f32(z[i < head ? i : tail + (i - head)]);
-                    take<TWO, 1>(R, &v, X);
-                }
-                const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-                for (int64_t i = t; i < nvec; i += tpr) {
-                    float v[W];
-                    Pack16<T>::unpack(zv[i], v);
-                    take<TWO, W>(R, v, X);
-                }
-            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 const float m = __shfl_xor_sync(0xffffffffu, R.m, o), s = __shfl_xor_sync(0xffffffffu, R.s, o);
-                const float s1 = TWO ? __shfl_xor_sync(0xffffffffu, R.s1, o) : 0.f;
-                // the lower lane's values first on both sides: the same bits in every lane
-                Run L = {R.m, R.s, R.s1};
-                if (lane & o) { L = {m, s, s1}; merge<TWO>(L, R.m, R.s, R.s1, X.c, X.c1); }
-                else merge<TWO>(L, m, s, s1, X.c, X.c1);
+                const float s1 = KIND ? __shfl_xor_sync(0xffffffffu, R.s1, o) : 0.f;
+                Run L = {R.m, R.s, R.s1};                     // the lower lane's first on both sides
+                if (lane & o) { L = {m, s, s1}; merge<KIND>(L, R.m, R.s, R.s1, X.c, X.c1); }
+                else merge<KIND>(L, m, s, s1, X.c, X.c1);
                 R = L;
             }
-            if (tpr > 32) {
-                if (lane == 0) { red[warp][0] = R.m; red[warp][1] = R.s; red[warp][2] = R.s1; }
-                __syncthreads();
-                const int w0 = warp & ~(nw - 1);
-                R = {red[w0][0], red[w0][1], red[w0][2]};
-                for (int i = 1; i < nw; ++i) merge<TWO>(R, red[w0 + i][0], red[w0 + i][1], red[w0 + i][2], X.c, X.c1);
-            }
-            if (!TWO) R.s1 = R.s;
-        } else if (counts) {
-            R = {A.stats[row * 3], A.stats[row * 3 + 1], A.stats[row * 3 + 2]};
+            if (lane == 0 && tpr > 32) { red[warp][0] = R.m; red[warp][1] = R.s; red[warp][2] = R.s1; }
         }
+        sync();
+        if (MODE & 1) {
+            if (tpr > 32) {
+                R = {red[0][0], red[0][1], red[0][2]};
+                for (int i = 1; i < nw; ++i) merge<KIND>(R, red[i][0], red[i][1], red[i][2], X.c, X.c1);
+            }
+            if (!KIND) R.s1 = R.s;
+        }
+        const float has = teacher[group];
+        if (!A.labels) counts = counts && has != 0.f;
+        if (MODE == 2 && counts) R = {A.stats[row * 3], A.stats[row * 3 + 1], A.stats[row * 3 + 2]};
 
         // ---- loss of the row, by its first warp ----
         if ((MODE & 1) && t < 32) {
             const float lse = R.m / A.temp + logf(R.s);
             float cross = 0.f;           // sum_k p_k (lse(z / T) - z_k / T)
-            for (int k = lane; counts && k < A.K; k += 32)
-                if (pid[k] >= 0 && !(prob[k] == 0.f)) cross += prob[k] * (lse - to_f32(z[pid[k]]) / A.temp);
+            for (int k = lane; counts && k < K; k += 32)
+                if (pid[k] >= 0 && !(prob[k] == 0.f)) cross += prob[k] * (lse - at_id[k] / A.temp);
             cross = warp_sum(cross);
             if (live && lane == 0) {
                 float loss = 0.f;
                 if (counts) {
                     if (has != 0.f) loss = A.alpha * A.temp * A.temp * (plogp + cross);
-                    if (A.labels) loss += (1.f - A.alpha) * (R.m + logf(R.s1) - to_f32(z[y]));
+                    if (A.labels) loss += (1.f - A.alpha) * (R.m + logf(R.s1) - zy);
                 }
                 A.row_loss[row] = loss;
                 if (A.row_counts) A.row_counts[row] = counts ? 1.f : 0.f;
@@ -288,52 +334,65 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
 
         // ---- gradient ----
         if (MODE & 2) {
-            T* dz = static_cast<T*>(A.dz) + (live ? row * V : 0);
+            T* dz = static_cast<T*>(A.dz) + (live ? row * A.V : 0);
             const bool same = (reinterpret_cast<uintptr_t>(dz) & 15) == (reinterpret_cast<uintptr_t>(z) & 15);
-            const int64_t h = same ? head : V, n = same ? nvec : 0, tl = same ? tail : V;
+            const int h = same ? head : V, n = same ? nvec : 0, tl = same ? tail : V;
+            uint4* dv = reinterpret_cast<uint4*>(dz + h);
             if (live && !counts) {
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                for (int64_t i = t; i < h + (V - tl); i += tpr) dz[i < h ? i : tl + (i - h)] = from_f32<T>(0.f);
-                for (int64_t i = t; i < n; i += tpr) reinterpret_cast<uint4*>(dz + h)[i] = zero;
+                for (int i = t; i < h + (V - tl); i += tpr) dz[i < h ? i : tl + (i - h)] = from_f32<T>(0.f);
+                for (int i = t; i < n; i += tpr) dv[i] = make_uint4(0, 0, 0, 0);
             } else if (live) {
                 float g = A.gscale / number;
                 if (A.gout) g *= A.gout[A.gout_stride * row];
                 const float ga = g * A.alpha * A.temp * has, gb = A.labels ? g * (1.f - A.alpha) : 0.f;
-                const float a = ga / R.s, b = TWO ? gb / R.s1 : 0.f;
                 const float ref = R.m == -INFINITY ? 0.f : R.m;
                 // one temperature: both terms share the exponential
-                const float ab = TWO ? a : a + gb / R.s;
-                auto dense = [&](float v) {
-                    float e, e1 = 0.f;
-                    X.at(v, ref, e, e1);
-                    return TWO ? fmaf(b, e1, ab * e) : ab * e;
+                const float a = KIND ? ga / R.s : ga / R.s + gb / R.s, b = gb / R.s1;
+                const uint64_t neg = f2(-ref, -ref), a2 = f2(a, a), b2 = f2(b, b);
+                auto dense = [&](uint64_t v) -> uint64_t {
+                    uint64_t e, e1;
+                    X.at(v, neg, e, e1);
+                    return KIND ? fma2(b2, e1, mul2(a2, e)) : mul2(a2, e);
                 };
-                for (int64_t i = t; i < h + (V - tl); i += tpr) {
-                    const int64_t c = i < h ? i : tl + (i - h);
-                    dz[c] = from_f32<T>(dense(to_f32(z[c])));
+                auto dense1 = [&](float v) {
+                    float p, q;
+                    unf2(dense(f2(v, v)), p, q);
+                    return p;
+                };
+                for (int i = t; i < h + (V - tl); i += tpr) {
+                    const int c = i < h ? i : tl + (i - h);
+                    dz[c] = from_f32<T>(dense1(to_f32(z[c])));
                 }
                 const uint4* zv = reinterpret_cast<const uint4*>(z + h);
-                uint4* dv = reinterpret_cast<uint4*>(dz + h);
-                for (int64_t i = t; i < n; i += tpr) {
+                uint4 u[DEEP];
+                auto put = [&](int at, const uint4& x) {
                     float v[W];
-                    Pack16<T>::unpack(zv[i], v);
+                    Pack16<T>::unpack(x, v);
 #pragma unroll
-                    for (int j = 0; j < W; ++j) v[j] = dense(v[j]);
-                    dv[i] = Pack16<T>::pack(v);
+                    for (int j = 0; j < W; j += 2) unf2(dense(f2(v[j], v[j + 1])), v[j], v[j + 1]);
+                    __stcs(dv + at, Pack16<T>::pack(v));     // not read again here: the L2 is z's
+                };
+                int i = t;
+                for (; i + (DEEP - 1) * tpr < n; i += DEEP * tpr) {
+#pragma unroll
+                    for (int k = 0; k < DEEP; ++k) u[k] = zv[i + k * tpr];
+#pragma unroll
+                    for (int k = 0; k < DEEP; ++k) put(i + k * tpr, u[k]);
                 }
+                for (; i < n; i += tpr) put(i, zv[i]);
                 sync();
-                for (int k = t; k <= A.K; k += tpr) {
-                    const int id = k < A.K ? pid[k] : (A.labels ? (int)y : -1);
+                for (int k = t; k <= K; k += tpr) {
+                    const int id = k < K ? pid[k] : (A.labels ? (int)y : -1);
                     if (id < 0) continue;
                     float p = 0.f;
-                    for (int j = 0; j < A.K; ++j) p += pid[j] == id ? prob[j] : 0.f;
-                    float v = dense(to_f32(z[id])) - ga * p;
+                    for (int j = 0; j < K; ++j) p += pid[j] == id ? prob[j] : 0.f;
+                    float v = dense1(k < K ? at_id[k] : to_f32(z[id])) - ga * p;
                     if (A.labels && id == (int)y) v -= gb;
                     dz[id] = from_f32<T>(v);
                 }
             }
         }
-        sync();          // prob / pid / red are written again by the next row
+        sync();          // prob, pid and red are written again by the next row
     }
 }
 
@@ -368,25 +427,31 @@ int sm_count() {
     return n;
 }
 
-template <typename T, bool TWO, int MODE>
+template <typename T, int KIND, int MODE>
 void launch(Args& A, cudaStream_t st) {
     // threads of a row: a warp for short rows, a block otherwise
     A.tpr = A.V <= 1024 ? 32 : A.V <= 4096 ? 128 : A.V <= 65536 ? 256 : 1024;
     if (A.N < sm_count() && A.V > 4096) A.tpr = 1024;
-    const int threads = A.tpr == 32 ? 256 : A.tpr, groups = threads / A.tpr;
+    const int threads = A.tpr > 32 ? A.tpr : A.K > 256 ? 128 : 256, groups = threads / A.tpr;
     const int64_t need = (A.N + groups - 1) / groups, wave = (int64_t)sm_count() * (2048 / threads);
-    const size_t smem = (size_t)groups * 2 * A.K * sizeof(float);
-    row_kernel<T, TWO, MODE><<<(int)(need < wave ? need : wave), threads, smem, st>>>(A);
+    const size_t smem = (size_t)groups * 3 * A.K * sizeof(float);       // 24 KB at most
+    row_kernel<T, KIND, MODE><<<(int)(need < wave ? need : wave), threads, smem, st>>>(A);
+}
+
+template <typename T, int MODE>
+void launch_kind(Args& A, cudaStream_t st) {
+    if (!A.labels || A.temp == 1.0f) launch<T, 0, MODE>(A, st);
+    else if (A.temp == 2.0f) launch<T, 2, MODE>(A, st);
+    else if (A.temp == 4.0f) launch<T, 3, MODE>(A, st);
+    else if (A.temp == 8.0f) launch<T, 4, MODE>(A, st);
+    else launch<T, 1, MODE>(A, st);
 }
 
 template <int MODE>
 int run(Args& A, int32_t type, cudaStream_t st, const char* name) {
-    const bool two = A.labels && A.temp != 1.0f;
-    A.squarings = A.temp == 2.0f ? 1 : A.temp == 4.0f ? 2 : A.temp == 8.0f ? 3 : 0;
-    if (type == 0) { if (two) launch<float, true, MODE>(A, st); else launch<float, false, MODE>(A, st); }
-    else if (type == 1) {
-        if (two) launch<__nv_bfloat16, true, MODE>(A, st); else launch<__nv_bfloat16, false, MODE>(A, st);
-    } else { if (two) launch<__half, true, MODE>(A, st); else launch<__half, false, MODE>(A, st); }
+    if (type == 0) launch_kind<float, MODE>(A, st);
+    else if (type == 1) launch_kind<__nv_bfloat16, MODE>(A, st);
+    else launch_kind<__half, MODE>(A, st);
     return check_launch(name);
 }
 

@@ -93,7 +93,7 @@ def check(z, ids, t, y, temp=1.0, alpha=1.0):
 
 
 @pytest.mark.parametrize("N,V,K", [(1, 1, 1), (3, 2, 2), (5, 65, 16), (700, 65, 3), (33, 1024, 64), (7, 1025, 8),
-                                   (4, 4097, 5), (300, 5000, 32), (3, 32000, 100), (2, 70001, 512), (160, 8191, 1)])
+                                   (4, 4097, 5), (300, 5000, 32), (3, 32000, 100), (2, 70001, 512), (160, 8191, 1), (11, 900, 512), (9, 700, 257)])
 def test_shapes(N, V, K):
     check(*inputs(N, V, K, torch.bfloat16, seed=N + V), temp=1.5, alpha=0.6)
 
