@@ -293,54 +293,55 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        // ---- products ----
+        // ---- products (the whole warp, one value of everything) ----
         constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_O = instr_desc(BF, DP, 1);
+        const uint32_t one = elect_one(), tm = uniform(tmem), sm = uniform(base);
+        const int nu[2] = {uniform(n[0]), uniform(n[1])}, nm = max(nu[0], nu[1]), lk = uniform(w.lk);
+        const uint64_t dq = desc_k(sm), dk = desc_k(sm + C::RING), dv = desc_mn(sm + C::RING);
         auto mma_s = [&](int i, int s) {
-            if (lane == 0) {
+            const uint64_t a = dq + i * (TILE >> 4), b = dk + s * (TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_ss(tmem + i * 128, desc_k(base + i * TILE, kk), desc_k(ring + s * TILE, kk), ID_S, kk != 0);
-                mma_commit(s_full(i));
-            }
+            for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm + i * 128, a + step_k(kk), b + step_k(kk), ID_S, kk != 0, one);
+            mma_commit(s_full(i), one);
         };
-        if (nmax > 0) {
-            if (!mbar_wait(full(0), 0, P.err, 3)) goto done;
+        if (nm > 0) {
+            if (!warp_wait(full(0), 0, P.err, 3)) goto done;
+#pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (n[i] == 0) continue;
-                if (!mbar_wait(q_full(i), 0, P.err, 4)) goto done;
+                if (nu[i] == 0) continue;
+                if (!warp_wait(q_full(i), 0, P.err, 4)) goto done;
                 fence_after();
                 mma_s(i, 0);
             }
-            if (lane == 0) mma_commit(empty(0));
+            mma_commit(empty(0), one);
         }
-        for (int j = 0; j < nmax; ++j) {
-            const int xv = 2 * j + 1, xk = 2 * j + 2, sv = xv % ST, sk = xk % ST;
-            const bool more = j + 1 < nmax;
-            if (!mbar_wait(full(sv), (xv / ST) & 1, P.err, 5)) goto done;
-            if (w.lk - j * 128 < 128) zero_rows<DP>(smem + C::RING + sv * TILE, w.lk - j * 128);
-            if (more && !mbar_wait(full(sk), (xk / ST) & 1, P.err, 6)) goto done;
+        int sv = 1, sk = 2;
+        uint32_t pv = 0, pk = 0;                  // phases of their barriers
+        for (int j = 0; j < nm; ++j) {
+            const bool more = j + 1 < nm;
+            if (!warp_wait(full(sv), pv, P.err, 5)) goto done;
+            if (lk - j * 128 < 128) zero_rows<DP>(smem + C::RING + sv * TILE, lk - j * 128);
+            if (more && !warp_wait(full(sk), pk, P.err, 6)) goto done;
+            const uint64_t b = dv + sv * (TILE >> 4);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (j >= n[i]) continue;
-                if (!mbar_wait(p_full(i), j & 1, P.err, 7)) goto done;
+                if (j >= nu[i]) continue;
+                if (!warp_wait(p_full(i), j & 1, P.err, 7)) goto done;
                 fence_after();
-                if (lane == 0) {
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        mma_ts(tmem + 256 + i * DP, tmem + i * 128 + kk * 8, desc_mn(ring + sv * TILE, kk), ID_O,
-                               (j | kk) != 0);
-                    mma_commit(pv_done(i));
-                }
-                if (j + 1 < n[i]) {     // S_i takes P_i's place: only after the product that reads P_i
-                    if (!mbar_wait(pv_done(i), j & 1, P.err, 8)) goto done;
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ts(tm + 256 + i * DP, tm + i * 128 + kk * 8, b + step_mn(kk), ID_O, (j | kk) != 0, one);
+                mma_commit(pv_done(i), one);
+                if (j + 1 < nu[i]) {    // S_i takes P_i's place: only after the product that reads P_i
+                    if (!warp_wait(pv_done(i), j & 1, P.err, 8)) goto done;
                     fence_after();
                     mma_s(i, sk);
                 }
             }
-            if (lane == 0) {
-                mma_commit(empty(sv));
-                if (more) mma_commit(empty(sk));
-            }
+            mma_commit(empty(sv), one);
+            if (more) mma_commit(empty(sk), one);
+            sv += 2; if (sv >= ST) { sv -= ST; pv ^= 1; }
+            sk += 2; if (sk >= ST) { sk -= ST; pk ^= 1; }
         }
     } else if (warp >= 4) {
         // ---- softmax: one row a thread ----
@@ -553,50 +554,57 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else if (warp == 1) {
         constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_Q = instr_desc(BF, DP, 1);
-        auto dq_product = [&](int j) {        // dQ += dS_j K_j
-            if (lane == 0) {
-                const uint32_t kt = base + C::K_OFF + (j % KS) * TILE;
+        const uint32_t el = elect_one(), tm = uniform(tmem), sm = uniform(base);
+        const int nu = uniform(n), lk = uniform(w.lk);
+        const uint64_t dq = desc_k(sm), ddo = desc_k(sm + TILE), dk = desc_k(sm + C::K_OFF), dv = desc_k(sm + C::V_OFF),
+                       dkt = desc_mn(sm + C::K_OFF);
+        auto dq_product = [&](int j, int s) {        // dQ += dS_j K_j
+            const uint64_t b = dkt + s * (TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    mma_ts(tmem + 256, tmem + 384 + kk * 8, desc_mn(kt, kk), ID_Q, (j | kk) != 0);
-                mma_commit(k_empty(j % KS));
-                mma_commit(ds_free);
-            }
+            for (int kk = 0; kk < 8; ++kk)
+                mma_ts(tm + 256, tm + 384 + kk * 8, b + step_mn(kk), ID_Q, (j | kk) != 0, el);
+            mma_commit(k_empty(s), el);
+            mma_commit(ds_free, el);
         };
-        if (n > 0 && !mbar_wait(q_full, 0, P.err, 25)) goto done;
-        for (int j = 0; j < n; ++j) {
-            const int sk = j % KS, sv = j % VS;
-            if (!mbar_wait(k_full(sk), (j / KS) & 1, P.err, 26)) goto done;
+        if (nu > 0 && !warp_wait(q_full, 0, P.err, 25)) goto done;
+        int sk = 0, sv = 0, before = 0;              // slots; that of the block before
+        uint32_t pk = 0, pv = 0;
+        for (int j = 0; j < nu; ++j) {
+            if (!warp_wait(k_full(sk), pk, P.err, 26)) goto done;
             // rows of another sequence: dS is 0 there, and 0 * NaN must not reach dQ
-            if (w.lk - j * 128 < 128) zero_rows<DP>(smem + C::K_OFF + sk * TILE, w.lk - j * 128);
-            if (j > 0 && !mbar_wait(s_free, (j - 1) & 1, P.err, 27)) goto done;
+            if (lk - j * 128 < 128) zero_rows<DP>(smem + C::K_OFF + sk * TILE, lk - j * 128);
+            if (j > 0 && !warp_wait(s_free, (j - 1) & 1, P.err, 27)) goto done;
             fence_after();
-            if (lane == 0) {
+            {
+                const uint64_t b = dk + sk * (TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_ss(tmem, desc_k(base, kk), desc_k(base + C::K_OFF + sk * TILE, kk), ID_S, kk != 0);
-                mma_commit(s_full);
+                for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm, dq + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+                mma_commit(s_full, el);
             }
-            if (!mbar_wait(v_full(sv), (j / VS) & 1, P.err, 28)) goto done;
-            if (j > 0 && !mbar_wait(dp_free, (j - 1) & 1, P.err, 29)) goto done;
+            if (!warp_wait(v_full(sv), pv, P.err, 28)) goto done;
+            if (j > 0 && !warp_wait(dp_free, (j - 1) & 1, P.err, 29)) goto done;
             fence_after();
-            if (lane == 0) {
+            {
+                const uint64_t b = dv + sv * (TILE >> 4);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_ss(tmem + 128, desc_k(base + TILE, kk), desc_k(base + C::V_OFF + sv * TILE, kk), ID_S, kk != 0);
-                mma_commit(dp_full);
-                mma_commit(v_empty(sv));
+                    mma_ss(tm + 128, ddo + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+                mma_commit(dp_full, el);
+                mma_commit(v_empty(sv), el);
             }
             if (j > 0) {
-                if (!mbar_wait(ds_full, (j - 1) & 1, P.err, 30)) goto done;
+                if (!warp_wait(ds_full, (j - 1) & 1, P.err, 30)) goto done;
                 fence_after();
-                dq_product(j - 1);
+                dq_product(j - 1, before);
             }
+            before = sk;
+            if (++sk == KS) { sk = 0; pk ^= 1; }
+            if (++sv == VS) { sv = 0; pv ^= 1; }
         }
-        if (n > 0) {
-            if (!mbar_wait(ds_full, (n - 1) & 1, P.err, 31)) goto done;
+        if (nu > 0) {
+            if (!warp_wait(ds_full, (nu - 1) & 1, P.err, 31)) goto done;
             fence_after();
-            dq_product(n - 1);
+            dq_product(nu - 1, before);
         }
     } else if (warp >= 4) {
         const int half = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
@@ -608,31 +616,38 @@ __global__ void __launch_bounds__(THREADS, 1)
         // neighbouring lanes (a lane a row would touch 32 lines a load), each
         // warp takes 16 rows.
         {
-            constexpr int CH = DP / 8, AT = 32 / CH;           // lanes of a row, rows a load
+            constexpr int CH = DP / 8, AT = 32 / CH, NL = 16 / AT;      // lanes of a row, rows a load, loads
             const int sub = lane / CH, c = lane % CH * 8;
-#pragma unroll 4
-            for (int k = 0; k < 16; k += AT) {
-                const int x = (warp - 4) * 16 + k + sub;
-                float d = 0.f;
-                if (r0 + x < w.lq && c < P.D) {
-                    const int64_t tok = (int64_t)w.q0 + r0 + x, at = (tok * P.H + head) * P.D + c;
-                    float g[8], o[8], e[8];
-                    load_vec<8>(static_cast<const T*>(P.dout) + tok * P.do_ts + head * P.do_hs + c, g);
-                    load_vec<8>(static_cast<const T*>(P.o) + at, o);
-                    load_vec<8>(static_cast<const T*>(P.rest) + at, e);
+            uint4 g[NL], o[NL], e[NL];                                  // all on their way at once
+            const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) d = fmaf(g[i], o[i] + e[i], d);
+            for (int k = 0; k < NL; ++k) {
+                const int x = r0 + (warp - 4) * 16 + k * AT + sub;
+                g[k] = o[k] = e[k] = none;
+                if (x < w.lq && c < P.D) {
+                    const int64_t tok = (int64_t)w.q0 + x, at = (tok * P.H + head) * P.D + c;
+                    g[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(P.dout) + tok * P.do_ts +
+                                                                head * P.do_hs + c));
+                    o[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(P.o) + at));
+                    e[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(P.rest) + at));
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < NL; ++k) {
+                float gv[8], ov[8], ev[8], d = 0.f;
+                Pack16<T>::unpack(g[k], gv);
+                Pack16<T>::unpack(o[k], ov);
+                Pack16<T>::unpack(e[k], ev);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d = fmaf(gv[i], ov[i] + ev[i], d);
 #pragma unroll
                 for (int i = CH / 2; i > 0; i >>= 1) d += __shfl_xor_sync(0xffffffffu, d, i);
-                if (lane % CH == 0) {
-                    red[x] = d;
-                    if (r0 + x < w.lq) P.delta[(int64_t)head * P.Tq + w.q0 + r0 + x] = d;
-                }
+                if (lane % CH == 0) red[(warp - 4) * 16 + k * AT + sub] = d;
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const float d = red[r];
+        if (live && half == 0) P.delta[(int64_t)head * P.Tq + trow] = d;
         float lse = live ? P.lse[(int64_t)head * P.Tq + trow] : 0.f;
         if (lse == -INFINITY) lse = 0.f;           // no key: everything is masked below
         const float l2 = -lse * LOG2E;
@@ -800,65 +815,71 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else if (warp == 1) {
         constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_D = instr_desc(BF, DP, 1);
-        const uint32_t qt = base + C::Q_OFF, ot = base + C::O_OFF;
+        const uint32_t el = elect_one(), tm = uniform(tmem), sm = uniform(base);
+        const int nu = uniform(n), per = uniform(nq), left = uniform(w.lq - jq * 128);
+        const uint64_t dk = desc_k(sm), dv = desc_k(sm + TILE), dq = desc_k(sm + C::Q_OFF), ddo = desc_k(sm + C::O_OFF),
+                       dqt = desc_mn(sm + C::Q_OFF), dot = desc_mn(sm + C::O_OFF);
         // rows of another sequence hold anything: p and ds are 0 there, and 0 * NaN must not reach dk and dv
-        auto short_by = [&](int x) { return w.lq - (jq + x % nq) * 128; };
-        auto s_product = [&](int x) -> bool {
-            const int s = x % QS;
-            if (!mbar_wait(q_full(s), (x / QS) & 1, P.err, 45)) return false;
-            if (short_by(x) < 128) zero_rows<DP>(smem + C::Q_OFF + s * TILE, short_by(x));
+        int sq = 0, so = 0, bq = 0, bo = 0;          // slots and query blocks (of their head) of the next S and dP
+        uint32_t pq = 0, po = 0;
+        auto s_product = [&]() -> bool {
+            if (!warp_wait(q_full(sq), pq, P.err, 45)) return false;
+            if (left - bq * 128 < 128) zero_rows<DP>(smem + C::Q_OFF + sq * TILE, left - bq * 128);
             fence_after();
-            if (lane == 0) {
+            const uint64_t b = dq + sq * (TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_ss(tmem, desc_k(base, kk), desc_k(qt + s * TILE, kk), ID_S, kk != 0);
-                mma_commit(s_full);
-            }
+            for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm, dk + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+            mma_commit(s_full, el);
+            if (++bq == per) bq = 0;
+            if (++sq == QS) { sq = 0; pq ^= 1; }
             return true;
         };
-        auto dp_product = [&](int x) -> bool {
-            const int s = x % OS;
-            if (!mbar_wait(o_full(s), (x / OS) & 1, P.err, 46)) return false;
-            if (short_by(x) < 128) zero_rows<DP>(smem + C::O_OFF + s * TILE, short_by(x));
+        auto dp_product = [&]() -> bool {
+            if (!warp_wait(o_full(so), po, P.err, 46)) return false;
+            if (left - bo * 128 < 128) zero_rows<DP>(smem + C::O_OFF + so * TILE, left - bo * 128);
             fence_after();
-            if (lane == 0) {
+            const uint64_t b = ddo + so * (TILE >> 4);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_ss(tmem + 128, desc_k(base + TILE, kk), desc_k(ot + s * TILE, kk), ID_S, kk != 0);
-                mma_commit(dp_full);
-            }
+            for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm + 128, dv + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+            mma_commit(dp_full, el);
+            if (++bo == per) bo = 0;
+            if (++so == OS) { so = 0; po ^= 1; }
             return true;
         };
-        if (n > 0) {
-            if (!mbar_wait(kv_full, 0, P.err, 47)) goto done;
-            if (!s_product(0) || !dp_product(0)) goto done;
+        if (nu > 0) {
+            if (!warp_wait(kv_full, 0, P.err, 47)) goto done;
+            if (!s_product() || !dp_product()) goto done;
         }
-        for (int x = 0; x < n; ++x) {
-            if (!mbar_wait(p_full, x & 1, P.err, 48)) goto done;
+        int cq = 0, co = 0;                          // slots of the present dK and dV
+        for (int x = 0; x < nu; ++x) {
+            if (!warp_wait(p_full, x & 1, P.err, 48)) goto done;
             fence_after();
-            if (lane == 0) {
+            {
+                const uint64_t b = dot + co * (TILE >> 4);
 #pragma unroll
                 for (int kk = 0; kk < 8; ++kk)
-                    mma_ts(tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8, desc_mn(ot + (x % OS) * TILE, kk), ID_D,
-                           (x | kk) != 0);
-                mma_commit(dv_done);
-                mma_commit(o_empty(x % OS));
+                    mma_ts(tm + 256, tm + (kk >> 2) * 64 + (kk & 3) * 8, b + step_mn(kk), ID_D, (x | kk) != 0, el);
+                mma_commit(dv_done, el);
+                mma_commit(o_empty(co), el);
+                if (++co == OS) co = 0;
             }
-            if (!mbar_wait(dv_done, x & 1, P.err, 49)) goto done;      // S takes P's place
-            if (x + 1 < n && !s_product(x + 1)) goto done;
-            if (!mbar_wait(ds_full, x & 1, P.err, 50)) goto done;
+            if (!warp_wait(dv_done, x & 1, P.err, 49)) goto done;      // S takes P's place
+            if (x + 1 < nu && !s_product()) goto done;
+            if (!warp_wait(ds_full, x & 1, P.err, 50)) goto done;
             fence_after();
-            if (lane == 0) {
+            {
+                const uint64_t b = dqt + cq * (TILE >> 4);
 #pragma unroll
                 for (int kk = 0; kk < 8; ++kk)
-                    mma_ts(tmem + 256 + DP, tmem + 128 + (kk >> 2) * 64 + (kk & 3) * 8, desc_mn(qt + (x % QS) * TILE, kk),
-                           ID_D, (x | kk) != 0);
-                mma_commit(dk_done);
-                mma_commit(q_empty(x % QS));
+                    mma_ts(tm + 256 + DP, tm + 128 + (kk >> 2) * 64 + (kk & 3) * 8, b + step_mn(kk), ID_D, (x | kk) != 0,
+                           el);
+                mma_commit(dk_done, el);
+                mma_commit(q_empty(cq), el);
+                if (++cq == QS) cq = 0;
             }
-            if (x + 1 < n) {
-                if (!mbar_wait(dk_done, x & 1, P.err, 51)) goto done;  // dP takes dS's place
-                if (!dp_product(x + 1)) goto done;
+            if (x + 1 < nu) {
+                if (!warp_wait(dk_done, x & 1, P.err, 51)) goto done;  // dP takes dS's place
+                if (!dp_product()) goto done;
             }
         }
     } else if (warp < 4) {

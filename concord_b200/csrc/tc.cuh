@@ -66,6 +66,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
     return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, err, code);
 }
 
+// the same by a whole warp, with one answer for all lanes
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
 // one box {64 columns, 1 head, 128 rows} into 128 rows of 128 swizzled bytes
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int head,
                                          int row) {
@@ -82,27 +87,47 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// The products are issued by a whole warp, converged, the instruction itself
+// predicated on one elected lane: the operands then stay in uniform registers.
+// Issued from inside a branch on the lane, each needs its descriptors moved
+// there first: eight take 750 cycles in place of 60 to 125 (and 512 to run).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p;
+}
+// a value that all lanes hold, known to be the same
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // D (tensor memory) = A (shared memory) B (shared memory) [+ D]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
         : "memory");
 }
 // D (tensor memory) = A (tensor memory) B (shared memory) [+ D]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
         : "memory");
 }
-// one arrival on `bar` once every MMA that this thread has issued is complete
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// one arrival on `bar` once every MMA that the elected lane has issued is complete
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(one)
+        : "memory");
 }
 
 template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t slot) {
@@ -154,12 +179,12 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
 // A tile of 128 rows x 64 or 128 columns is one or two boxes of 128 rows x 64
 // columns (16 KB each, 8-row groups of swizzled 128-byte rows 1024 B apart).
 constexpr uint32_t BOX = 16384;
-// columns are the reduction (K-major): the kk-th 16 columns
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int kk) {
-    return smem_desc(tile + (kk >> 2) * BOX + (kk & 3) * 32, 16, 1024);
-}
-// rows are the reduction (MN-major): the kk-th 16 rows; the second 64 columns one box on
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int kk) { return smem_desc(tile + kk * 2048, BOX, 1024); }
+// columns are the reduction (K-major); the kk-th 16 columns are at + step_k(kk)
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile) { return smem_desc(tile, 16, 1024); }
+__host__ __device__ constexpr uint64_t step_k(int kk) { return ((kk >> 2) * BOX + (kk & 3) * 32) >> 4; }
+// rows are the reduction (MN-major), the second 64 columns one box on; the kk-th 16 rows are at + step_mn(kk)
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile) { return smem_desc(tile, BOX, 1024); }
+__host__ __device__ constexpr uint64_t step_mn(int kk) { return (kk * 2048) >> 4; }
 
 // instruction descriptor: fp32 accumulator, A and B of one 16-bit type, M = 128
 __host__ __device__ constexpr uint32_t instr_desc(int bf16, int n, int b_mn) {
