@@ -721,15 +721,43 @@ done:
 // ds are the A operands of their products as they come from the softmax.
 // Tensor memory: S 0, dP 128, dV 256, dK 256 + DP.  P takes half of each half
 // of S (columns 0-31 and 64-95), dS the same of dP: each softmax warp writes
-// only where it has read itself.  The order of the products, dV, next S, dK,
+// only where it has read itself.  lse and delta belong to columns here: read
+// per column from shared memory they met the products there (2730 cycles of
+// softmax a block in place of the 1100 of its exponentials), so the products
+// subtract them themselves: one more step of 16, a row of ones against the
+// value in three 16-bit parts (24 bits of it).  The order of the products, dV, next S, dK,
 // next dP, lets the exponentials run beside dK and dP, and ds beside dV and S.
 template <int DP> struct BwdK {
     static constexpr int TILE = 256 * DP;
     static constexpr int QS = DP == 128 ? 2 : 3, OS = DP == 128 ? 2 : 3;
     static constexpr int Q_OFF = 2 * TILE, O_OFF = Q_OFF + QS * TILE;
     static constexpr int BARS = O_OFF + OS * TILE;
-    static constexpr int STAT = BARS + 512;                    // 2 stages of (-lse log2(e), -delta)[128]
-    static constexpr size_t SMEM = STAT + 2 * 1024 + 1024;
+    static constexpr int ONES = BARS + 512;                    // the row of ones, for every key
+    static constexpr int STAT = ONES + THIN;                   // 2 stages of (-lse / scale, -delta), a query a row
+    static constexpr size_t SMEM = STAT + 4 * THIN + 1024;
+};
+
+// What the ones are, and a value's parts against them.  fp16 cannot hold what
+// lse / scale may be (scores before scaling), so its ones are 2^15, 2^4 and
+// 2^-7: values up to 2^31, each part 11 bits of what the one before left.
+template <typename T> struct Parts;
+template <> struct Parts<__nv_bfloat16> {
+    static __device__ __forceinline__ uint4 ones() { return make_uint4(0x3f803f80u, 0x3f80u, 0, 0); }
+    static __device__ __forceinline__ uint4 of(float v) {
+        const float a = __bfloat162float(__float2bfloat16_rn(v)), b = __bfloat162float(__float2bfloat16_rn(v - a));
+        return make_uint4(pack2(a, b, __nv_bfloat16()), pack2(v - a - b, 0.f, __nv_bfloat16()), 0, 0);
+    }
+};
+template <> struct Parts<__half> {
+    static __device__ __forceinline__ uint4 ones() {
+        return make_uint4(pack2(32768.f, 16.f, __half()), pack2(1.f / 128.f, 0.f, __half()), 0, 0);
+    }
+    static __device__ __forceinline__ uint4 of(float v) {
+        v = fminf(fmaxf(v, -2.1e9f), 2.1e9f);
+        const float a = __half2float(__float2half_rn(v * (1.f / 32768.f))), r = v - a * 32768.f;
+        const float b = __half2float(__float2half_rn(r * (1.f / 16.f)));
+        return make_uint4(pack2(a, b, __half()), pack2((r - b * 16.f) * 128.f, 0.f, __half()), 0, 0);
+    }
 };
 
 template <typename T, int DP>
@@ -745,7 +773,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
     uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * QS + 2 * OS + 12);
     Work* work = reinterpret_cast<Work*>(slot + 4);
-    float* stat = reinterpret_cast<float*>(smem + C::STAT);
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto q_full = [&](int s) { return bar0 + 8u * s; };
     auto q_empty = [&](int s) { return bar0 + 8u * (QS + s); };
@@ -767,12 +794,20 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(kv_full, 1);
             mbar_init(s_full, 1); mbar_init(p_full, 256); mbar_init(dv_done, 1);
             mbar_init(dp_full, 1); mbar_init(ds_full, 256); mbar_init(dk_done, 1);
-            for (int s = 0; s < 2; ++s) { mbar_init(st_full(s), 64); mbar_init(st_empty(s), 256); }
+            for (int s = 0; s < 2; ++s) { mbar_init(st_full(s), 64); mbar_init(st_empty(s), 1); }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         find_tile(P, true, t, gridDim.x / HK, 128, false, work);
     }
     if (warp == 1) tmem_alloc<512>(smem_u32(slot));
+    if (warp >= 4) {          // the ones, and zeros beside them and beside the values
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x - 128; i < 5 * 256; i += 256) {
+            const uint32_t at = base + C::ONES + (i >> 8) * THIN + (i & 255) * 16;
+            sts16(at, (i < 256 && !(i & 8)) ? Parts<T>::ones() : z);
+        }
+        fence_async();
+    }
     fence_before();
     __syncthreads();
     fence_after();
@@ -819,17 +854,22 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int nu = uniform(n), per = uniform(nq), left = uniform(w.lq - jq * 128);
         const uint64_t dk = desc_k(sm), dv = desc_k(sm + TILE), dq = desc_k(sm + C::Q_OFF), ddo = desc_k(sm + C::O_OFF),
                        dqt = desc_mn(sm + C::Q_OFF), dot = desc_mn(sm + C::O_OFF);
+        const uint64_t ones = desc_thin(sm + C::ONES), stat = desc_thin(sm + C::STAT);
         // rows of another sequence hold anything: p and ds are 0 there, and 0 * NaN must not reach dk and dv
         int sq = 0, so = 0, bq = 0, bo = 0;          // slots and query blocks (of their head) of the next S and dP
-        uint32_t pq = 0, po = 0;
+        uint32_t pq = 0, po = 0, ss = 0, sp = 0, ps = 0;      // ss, sp: slots of lse and delta; ps: their phase
         auto s_product = [&]() -> bool {
             if (!warp_wait(q_full(sq), pq, P.err, 45)) return false;
             if (left - bq * 128 < 128) zero_rows<DP>(smem + C::Q_OFF + sq * TILE, left - bq * 128);
+            if (!warp_wait(st_full(ss), ps, P.err, 53)) return false;
             fence_after();
             const uint64_t b = dq + sq * (TILE >> 4);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm, dk + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+            mma_ss(tm, ones, stat + ss * (2 * THIN >> 4), ID_S, 1, el);
             mma_commit(s_full, el);
+            ss ^= 1;
+            if (ss == 0) ps ^= 1;
             if (++bq == per) bq = 0;
             if (++sq == QS) { sq = 0; pq ^= 1; }
             return true;
@@ -841,7 +881,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t b = ddo + so * (TILE >> 4);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm + 128, dv + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
+            mma_ss(tm + 128, ones, stat + (2 * sp + 1) * (THIN >> 4), ID_S, 1, el);
             mma_commit(dp_full, el);
+            mma_commit(st_empty(sp), el);
+            sp ^= 1;
             if (++bo == per) bo = 0;
             if (++so == OS) { so = 0; po ^= 1; }
             return true;
@@ -883,24 +926,36 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
     } else if (warp < 4) {
-        // ---- lse and delta of the query rows, for the softmax warps ----
+        // ---- lse and delta of the query rows, for the products ----
         const int i = threadIdx.x - 64;
+        const float unscale = -1.0f / P.scale;
         for (int x = 0; x < n; ++x) {
             const int s = x & 1, head = kvh * P.G + x / nq, row0 = (jq + x % nq) * 128;
-            if (!mbar_wait(st_empty(s), ((x >> 1) & 1) ^ 1, P.err, 52)) goto done;
-            for (int k = i; k < 128; k += 64) {
-                float l = INFINITY, d = 0.f;       // no such row, or one without keys: p = 0
-                if (row0 + k < w.lq) {
-                    const int64_t at = (int64_t)head * P.Tq + w.q0 + row0 + k;
-                    l = P.lse[at];
-                    l = l == -INFINITY ? INFINITY : l * LOG2E;
-                    d = P.delta[at];
+            float l[2], d[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = row0 + i + k * 64;
+                l[k] = -INFINITY;
+                d[k] = 0.f;
+                if (r < w.lq) {
+                    const int64_t at = (int64_t)head * P.Tq + w.q0 + r;
+                    l[k] = P.lse[at];
+                    d[k] = P.delta[at];
                 }
-                stat[s * 256 + k] = -l;
-                stat[s * 256 + 128 + k] = -d;
             }
+            if (!mbar_wait(st_empty(s), ((x >> 1) & 1) ^ 1, P.err, 52)) goto done;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t at = base + C::STAT + 2 * s * THIN + thin_row(i + k * 64);
+                // no such row, or one without keys: far below every score, so p = 0
+                sts16(at, Parts<T>::of(l[k] == -INFINITY ? -1e30f : l[k] * unscale));
+                sts16(at + THIN, Parts<T>::of(-d[k]));
+            }
+            fence_async();
             mbar_arrive(st_full(s));
         }
+        for (int x = 0; x < 2 && x < n; ++x)       // the last use of each stage
+            if (!mbar_wait(st_empty((n - 1 - x) & 1), ((n - 1 - x) >> 1) & 1, P.err, 57)) goto done;
     } else {
         const int half = (warp - 4) >> 2, q = warp & 3;
         const int key = k0 + q * 32 + lane;
@@ -908,31 +963,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const uint64_t c2 = f2(P.scale2, P.scale2);
         for (int x = 0; x < n; ++x) {
-            const int s = x & 1, row0 = (jq + x % nq) * 128 + half * 64;
-            const float4* l4 = reinterpret_cast<const float4*>(stat + s * 256 + half * 64);
-            const float4* d4 = reinterpret_cast<const float4*>(stat + s * 256 + 128 + half * 64);
+            const int row0 = (jq + x % nq) * 128 + half * 64;
             // the first query of this half that sees the key, as a column
             const int from = P.causal ? key - off - row0 : 0;
             const bool masked = P.causal && row0 + off < k0 + 127;
             float p[64];
             uint32_t u[64], v[32];
-            if (!mbar_wait(st_full(s), (x >> 1) & 1, P.err, 53)) goto done;
             if (!mbar_wait(s_full, x & 1, P.err, 54)) goto done;
             fence_after();
             ld32(tmem + lanes + half * 64, u);
             ld32(tmem + lanes + half * 64 + 32, u + 32);
             wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float4 l = l4[k];
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    float a, b;
-                    unf2(fma2(f2(__uint_as_float(u[4 * k + e]), __uint_as_float(u[4 * k + e + 1])), c2,
-                              e ? f2(l.z, l.w) : f2(l.x, l.y)), a, b);
-                    p[4 * k + e] = ex2f(a);
-                    p[4 * k + e + 1] = ex2f(b);
-                }
+            for (int k = 0; k < 64; k += 2) {
+                float a, b;
+                unf2(mul2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2), a, b);
+                p[k] = ex2f(a);
+                p[k + 1] = ex2f(b);
             }
             if (masked) {
 #pragma unroll
@@ -951,15 +998,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
             wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float4 d = d4[k];
-#pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    unf2(mul2(f2(p[4 * k + e], p[4 * k + e + 1]),
-                              add2(f2(__uint_as_float(u[4 * k + e]), __uint_as_float(u[4 * k + e + 1])),
-                                   e ? f2(d.z, d.w) : f2(d.x, d.y))), p[4 * k + e], p[4 * k + e + 1]);
-            }
-            mbar_arrive(st_empty(s));
+            for (int k = 0; k < 64; k += 2)
+                unf2(mul2(f2(p[k], p[k + 1]), f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1]))), p[k], p[k + 1]);
             if (masked) {
 #pragma unroll
                 for (int k = 0; k < 64; ++k)

@@ -186,6 +186,14 @@ __host__ __device__ constexpr uint64_t step_k(int kk) { return ((kk >> 2) * BOX 
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile) { return smem_desc(tile, BOX, 1024); }
 __host__ __device__ constexpr uint64_t step_mn(int kk) { return (kk * 2048) >> 4; }
 
+// 128 rows of 16 columns (K-major, one step), no swizzle: 8 rows of 8 columns
+// are 128 consecutive bytes, the second 8 columns 128 B on, the next rows 256 B
+constexpr uint32_t THIN = 4096;
+__device__ __forceinline__ uint64_t desc_thin(uint32_t tile) {
+    return (uint64_t)((tile >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ uint32_t thin_row(int r) { return (r >> 3) * 256 + (r & 7) * 16; }    // its first 8 columns
+
 // instruction descriptor: fp32 accumulator, A and B of one 16-bit type, M = 128
 __host__ __device__ constexpr uint32_t instr_desc(int bf16, int n, int b_mn) {
     return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)b_mn << 16) |
