@@ -66,9 +66,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
     return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, err, code);
 }
 
-// the same by a whole warp, with one answer for all lanes
+// The same by a whole warp, which stays converged: every branch goes by a vote.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+    const uint64_t t0 = now_ns();
+#pragma unroll 1
+    while (!__all_sync(0xffffffffu, mbar_try(bar, parity))) {
+        if (__any_sync(0xffffffffu, now_ns() - t0 > WAIT_NS)) {
+            atomicCAS(err, 0, code);
+            return false;
+        }
+    }
+    return true;
 }
 
 // one box {64 columns, 1 head, 128 rows} into 128 rows of 128 swizzled bytes
