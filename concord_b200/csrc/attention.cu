@@ -858,10 +858,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         // rows of another sequence hold anything: p and ds are 0 there, and 0 * NaN must not reach dk and dv
         int sq = 0, so = 0, bq = 0, bo = 0;          // slots and query blocks (of their head) of the next S and dP
         uint32_t pq = 0, po = 0, ss = 0, sp = 0, ps = 0;      // ss, sp: slots of lse and delta; ps: their phase
-        auto s_product = [&]() -> bool {
+        // the operands of the next S: waited for before its place is free
+        auto s_ready = [&]() -> bool {
             if (!warp_wait(q_full(sq), pq, P.err, 45)) return false;
             if (left - bq * 128 < 128) zero_rows<DP>(smem + C::Q_OFF + sq * TILE, left - bq * 128);
-            if (!warp_wait(st_full(ss), ps, P.err, 53)) return false;
+            return warp_wait(st_full(ss), ps, P.err, 53);
+        };
+        auto s_product = [&]() {
             fence_after();
             const uint64_t b = dq + sq * (TILE >> 4);
 #pragma unroll
@@ -872,11 +875,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (ss == 0) ps ^= 1;
             if (++bq == per) bq = 0;
             if (++sq == QS) { sq = 0; pq ^= 1; }
-            return true;
         };
-        auto dp_product = [&]() -> bool {
+        auto dp_ready = [&]() -> bool {
             if (!warp_wait(o_full(so), po, P.err, 46)) return false;
             if (left - bo * 128 < 128) zero_rows<DP>(smem + C::O_OFF + so * TILE, left - bo * 128);
+            return true;
+        };
+        auto dp_product = [&]() {
             fence_after();
             const uint64_t b = ddo + so * (TILE >> 4);
 #pragma unroll
@@ -887,11 +892,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             sp ^= 1;
             if (++bo == per) bo = 0;
             if (++so == OS) { so = 0; po ^= 1; }
-            return true;
         };
         if (nu > 0) {
             if (!warp_wait(kv_full, 0, P.err, 47)) goto done;
-            if (!s_product() || !dp_product()) goto done;
+            if (!s_ready()) goto done;
+            s_product();
+            if (!dp_ready()) goto done;
+            dp_product();
         }
         int cq = 0, co = 0;                          // slots of the present dK and dV
         for (int x = 0; x < nu; ++x) {
@@ -906,8 +913,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mma_commit(o_empty(co), el);
                 if (++co == OS) co = 0;
             }
+            if (x + 1 < nu && !s_ready()) goto done;
             if (!warp_wait(dv_done, x & 1, P.err, 49)) goto done;      // S takes P's place
-            if (x + 1 < nu && !s_product()) goto done;
+            if (x + 1 < nu) s_product();
             if (!warp_wait(ds_full, x & 1, P.err, 50)) goto done;
             fence_after();
             {
@@ -921,8 +929,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (++cq == QS) cq = 0;
             }
             if (x + 1 < nu) {
+                if (!dp_ready()) goto done;
                 if (!warp_wait(dk_done, x & 1, P.err, 51)) goto done;  // dP takes dS's place
-                if (!dp_product()) goto done;
+                dp_product();
             }
         }
     } else if (warp < 4) {
