@@ -1,16 +1,31 @@
 """What the training operators (layer norm, packed attention, distillation
-loss) share: type codes of the C ABI, checks of arguments, the call itself."""
-import ctypes
+loss) share: checks of arguments, and the extension that runs them."""
+import importlib.machinery
+import importlib.util
+import os
 
 import torch
 
 from . import _abi
 
 TYPES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
+NATIVE_PATH = os.path.join(os.path.dirname(_abi.LIB_PATH), "_native.so")
+_NATIVE = None
 
 
-def ptr(t):
-    return None if t is None else t.data_ptr()
+def native():
+    """The extension of csrc/torch_ops.cpp (raises if it was not built)."""
+    global _NATIVE
+    if _NATIVE is None:
+        _abi.load()
+        if not os.path.exists(NATIVE_PATH):
+            raise RuntimeError(f"concord_b200 extension not built: {NATIVE_PATH} is missing "
+                               "(run `python -m concord_b200.build`); there is no CPU fallback")
+        loader = importlib.machinery.ExtensionFileLoader("_native", NATIVE_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_native", loader))
+        loader.exec_module(module)
+        _NATIVE = module
+    return _NATIVE
 
 
 def need_cuda(*named):
@@ -27,31 +42,8 @@ def need_cuda(*named):
             dev = t.device
         elif t.device != dev:
             raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {dev}")
-    return dev
 
 
 def need_type(name, t, types):
     if t.dtype not in types:
         raise TypeError(f"{name} must be one of {[str(x) for x in types]}, got {t.dtype}")
-
-
-_FN = {}
-_raw_stream = torch._C._cuda_getCurrentRawStream     # current_stream(...).cuda_stream without the Stream object
-
-
-def call(name, index, *args):
-    """Call `name` of the C ABI on CUDA device `index` and its current stream
-    (appended as the last argument)."""
-    fn = _FN.get(name)
-    if fn is None:
-        fn = _FN[name] = getattr(_abi.load(), name)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
-    else:
-        status = fn(*args, _raw_stream(index))
-    if status != 0:
-        _abi.check(status, name)
-
-
-byref = ctypes.byref

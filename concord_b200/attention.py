@@ -6,65 +6,10 @@ here a batch is its documents one after the other, with no padding between
 them, read in place from the projection's output.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _abi, _ops
+from . import _ops
 
 _HALVES = (torch.bfloat16, torch.float16)
-
-
-def _operand(t):
-    """t [T, H, D] as the kernels read it (a copy only where its strides or its
-    address do not fit 16-byte rows)."""
-    if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(0) <= 0 or t.stride(1) <= 0
-            or t.data_ptr() % 16):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
-
-
-def _params(q, k, cu_q, cu_k, causal, scale):
-    return _abi.AttentionParams(cu_q=cu_q.data_ptr(), cu_k=cu_k.data_ptr(), seqs=cu_q.numel() - 1,
-                                tokens_q=q.shape[0], tokens_k=k.shape[0], heads=q.shape[1], kv_heads=k.shape[1],
-                                head_dim=q.shape[2], type=_ops.TYPES[q.dtype], causal=int(causal), scale=scale)
-
-
-def _arg(t):
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
-        q, k, v = _operand(q), _operand(k), _operand(v)
-        o = q.new_empty(q.shape)
-        rest = torch.empty_like(o) if any(ctx.needs_input_grad[:3]) else None
-        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
-        if k.shape[0] == 0:
-            o.zero_()
-            lse.fill_(float("-inf"))
-        elif q.shape[0]:
-            _ops.call("concord_attention_fwd", q.get_device(), _ops.byref(_params(q, k, cu_q, cu_k, causal, scale)),
-                      *_arg(q), *_arg(k), *_arg(v), o.data_ptr(), _ops.ptr(rest), lse.data_ptr())
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, rest, lse)
-        ctx.causal, ctx.scale = causal, scale
-        ctx.mark_non_differentiable(lse)
-        return o, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do, _):
-        q, k, v, cu_q, cu_k, o, rest, lse = ctx.saved_tensors
-        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
-        if q.shape[0] == 0 or k.shape[0] == 0:
-            return dq.zero_(), dk.zero_(), dv.zero_(), None, None, None, None
-        do = _operand(do)
-        delta = torch.empty_like(lse)
-        _ops.call("concord_attention_bwd", q.get_device(), _ops.byref(_params(q, k, cu_q, cu_k, ctx.causal, ctx.scale)),
-                  *_arg(q), *_arg(k), *_arg(v), o.data_ptr(), rest.data_ptr(), lse.data_ptr(), *_arg(do),
-                  delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
-        return dq, dk, dv, None, None, None, None
 
 
 def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=None, return_lse=False):
@@ -119,5 +64,5 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale must be positive, got {scale}")
-    o, lse = _Attention.apply(q, k, v, cus[0], cus[1], bool(causal), scale)
+    o, lse = _ops.native().attention(q, k, v, cus[0], cus[1], causal, scale)
     return (o, lse) if return_lse else o

@@ -7,7 +7,9 @@ links one shared library with a plain C ABI (include/concord_b200.h).  The
 step kernels are built with -fmad=false: the reference's arithmetic rounds
 every fp32 multiply and add separately, and bit-exact words depend on the
 compiler not fusing them.  Also builds the host copy of the correctly
-rounded log2/exp2 (libcrmath_check.so) that the CPU tests check.
+rounded log2/exp2 (libcrmath_check.so) that the CPU tests check, and
+`_lib/_native.so`, the Python extension with the training operators' autograd
+nodes (csrc/torch_ops.cpp, compiled by g++ against the installed torch).
 """
 import glob
 import os
@@ -18,6 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(LIBDIR, "libconcord_b200.so")
+NATIVE = os.path.join(LIBDIR, "_native.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC",
@@ -57,6 +60,21 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _native_command(src):
+    """g++ command of the Python extension: torch's headers and libraries, and
+    libconcord_b200 beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += ["-I" + p for p in include_paths("cuda") + [sysconfig.get_paths()["include"]]]
+    cmd += ["-I" + os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), src, "-o", NATIVE]
+    cmd += ["-L" + LIBDIR, "-lconcord_b200", "-Wl,-rpath,$ORIGIN"] + ["-L" + p for p in library_paths("cuda")]
+    return cmd + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+
+
 def build(verbose=False, force=False):
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(LIBDIR, "obj")
@@ -78,6 +96,12 @@ def build(verbose=False, force=False):
     src = os.path.join(CSRC, "crmath_check.cpp")
     if force or _newer(chk, [src, os.path.join(CSRC, "crmath.h")]):
         subprocess.check_call(["g++", "-O2", "-fPIC", "-ffp-contract=off", "-shared", "-o", chk, src])
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    if force or _newer(NATIVE, [src, os.path.join(HERE, "..", "include", "concord_b200.h")]):
+        cmd = _native_command(src)
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
     return OUT
 
 

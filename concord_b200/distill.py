@@ -13,11 +13,11 @@ probabilities: one pass reads the logits and, in `distill_loss_and_grad`,
 writes their gradient.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _abi, _ops
+from . import _ops
 
 _INTS = (torch.int64, torch.int32)
+_REDUCTIONS = ("mean", "sum", "none")
 
 
 def _check(logits, top_ids, top_logits, labels, temperature, alpha):
@@ -45,60 +45,6 @@ def _check(logits, top_ids, top_logits, labels, temperature, alpha):
         raise ValueError("alpha < 1 weighs hard labels: pass labels")
 
 
-def _flat(logits, top_ids, top_logits, labels):
-    V, K = logits.shape[-1], top_ids.shape[-1]
-    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if not z.is_contiguous() and (z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < V)):
-        z = z.contiguous()
-    ids = top_ids if top_ids.dim() == 2 else top_ids.reshape(-1, K)
-    t = top_logits if top_logits.dim() == 2 else top_logits.reshape(-1, K)
-    if labels is not None:
-        labels = (labels if labels.dim() == 1 else labels.reshape(-1)).contiguous()
-    return z, ids.contiguous(), t.float().contiguous(), labels
-
-
-def _params(ids, labels, temperature, alpha, ignore_index, mean, scale=1.0):
-    return _abi.DistillParams(temperature, alpha, scale, mean, ids.dtype == torch.int64,
-                              labels is not None and labels.dtype == torch.int64, ignore_index)
-
-
-def _loss(z, ids, t, labels, params, loss, row_loss, stats, dz):
-    N, V = z.shape
-    nbytes = 512 + 8 * N          # concord_distill_workspace_bytes(N)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
-    _ops.call("concord_distill_loss", z.get_device(), _ops.byref(params), z.data_ptr(), _ops.TYPES[z.dtype],
-              z.stride(0) if N > 1 else V, ids.data_ptr(), t.data_ptr(), _ops.ptr(labels), _ops.ptr(loss),
-              _ops.ptr(row_loss), _ops.ptr(stats), _ops.ptr(dz), N, V, ids.shape[1], ws.data_ptr(), nbytes)
-
-
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_ids, top_logits, labels, temperature, alpha, ignore_index, reduction):
-        z, ids, t, lab = _flat(logits, top_ids, top_logits, labels)
-        params = _params(ids, lab, temperature, alpha, ignore_index, reduction == "mean")
-        f32 = dict(dtype=torch.float32, device=z.device)
-        per_row = reduction == "none"
-        out = torch.empty(logits.shape[:-1] if per_row else (), **f32)
-        stats = torch.empty(3 * z.shape[0] + 1, **f32) if ctx.needs_input_grad[0] else None
-        _loss(z, ids, t, lab, params, None if per_row else out, out if per_row else None, stats, None)
-        if stats is not None:
-            ctx.save_for_backward(z, ids, t, lab, stats)
-            ctx.params, ctx.shape, ctx.per_row = params, logits.shape, per_row
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        z, ids, t, lab, stats = ctx.saved_tensors
-        N, V = z.shape
-        grad = grad.contiguous()
-        dz = torch.empty(ctx.shape, dtype=z.dtype, device=z.device)
-        _ops.call("concord_distill_grad", z.get_device(), _ops.byref(ctx.params), z.data_ptr(), _ops.TYPES[z.dtype],
-                  z.stride(0) if N > 1 else V, ids.data_ptr(), t.data_ptr(), _ops.ptr(lab), stats.data_ptr(),
-                  grad.data_ptr(), ctx.per_row, dz.data_ptr(), N, V, ids.shape[1])
-        return dz, None, None, None, None, None, None, None
-
-
 def distill_loss(logits, top_ids, top_logits, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100,
                  reduction="mean"):
     """Distillation loss of `logits` [..., V] against a teacher's top logits.
@@ -117,12 +63,12 @@ def distill_loss(logits, top_ids, top_logits, labels=None, temperature=1.0, alph
     """
     temperature, alpha = float(temperature), float(alpha)
     _check(logits, top_ids, top_logits, labels, temperature, alpha)
-    if reduction not in ("mean", "sum", "none"):
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
-    return _Distill.apply(logits, top_ids, top_logits, labels, temperature, alpha, ignore_index, reduction)
+    return _ops.native().distill_loss(logits, top_ids, top_logits, labels, temperature, alpha, ignore_index,
+                                      _REDUCTIONS.index(reduction))
 
 
-@torch.no_grad()
 def distill_loss_and_grad(logits, top_ids, top_logits, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100,
                           reduction="mean", grad_scale=1.0):
     """(loss, d loss / d logits * grad_scale) in one pass over the logits, for
@@ -134,9 +80,5 @@ def distill_loss_and_grad(logits, top_ids, top_logits, labels=None, temperature=
     _check(logits, top_ids, top_logits, labels, temperature, alpha)
     if reduction not in ("mean", "sum"):
         raise ValueError(f"reduction must be 'mean' or 'sum', not {reduction!r}")
-    z, ids, t, lab = _flat(logits, top_ids, top_logits, labels)
-    params = _params(ids, lab, temperature, alpha, ignore_index, reduction == "mean", float(grad_scale))
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
-    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    _loss(z, ids, t, lab, params, loss, None, None, dz)
-    return loss, dz.view(logits.shape)
+    return _ops.native().distill_loss_and_grad(logits, top_ids, top_logits, labels, temperature, alpha, ignore_index,
+                                               reduction == "mean", grad_scale)
