@@ -34,6 +34,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -197,8 +198,11 @@ __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f,
 // ---------------------------------------------------------------- forward
 // A block owns 256 query rows (two tiles, one softmax warpgroup each) of one
 // head; K and V tiles go through one ring and serve both.  Tensor memory: S_0,
-// S_1 (128 columns each; P_i, as 16-bit pairs, takes the first 64 of S_i once
-// it has been read), O_0, O_1.
+// S_1 (128 columns each), O_0, O_1 and, with heads up to 64, P_0, P_1 (16-bit
+// pairs): the next S is then computed as soon as the present one is read.  With
+// 128 there is no room, P_i takes the first 64 columns of S_i once they have
+// been read, and the next S waits for P V.  The product P V begins with the
+// first 64 keys while the exponentials of the others still run.
 template <int DP> struct Fwd {
     static constexpr int TILE = 256 * DP;               // bytes of 128 rows
     static constexpr int ST = DP == 128 ? 5 : 8;        // ring of K and V tiles
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = align1024(raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 10);
+    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 14);
     Work* work = reinterpret_cast<Work*>(slot + 4);
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
@@ -226,6 +230,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto s_full = [&](int i) { return bar0 + 8u * (2 * ST + 2 + i); };
     auto p_full = [&](int i) { return bar0 + 8u * (2 * ST + 4 + i); };
     auto pv_done = [&](int i) { return bar0 + 8u * (2 * ST + 6 + i); };
+    auto p_half = [&](int i) { return bar0 + 8u * (2 * ST + 8 + i); };
+    auto s_free = [&](int i) { return bar0 + 8u * (2 * ST + 10 + i); };
+    constexpr bool APART = DP == 64;             // P has columns of its own
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.x % P.H, t = blockIdx.x / P.H, kvh = head / P.G;
 
@@ -234,6 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(q_full(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 128); mbar_init(pv_done(i), 1);
+                mbar_init(p_half(i), 128); mbar_init(s_free(i), 128);
             }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -326,13 +334,22 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (j >= nu[i]) continue;
-                if (!warp_wait(p_full(i), j & 1, P.err, 7)) goto done;
-                fence_after();
+                if (APART && j + 1 < nu[i]) {
+                    if (!warp_wait(s_free(i), j & 1, P.err, 11)) goto done;
+                    fence_after();
+                    mma_s(i, sk);
+                }
+                const uint32_t p = APART ? tm + 384 + i * 64 : tm + i * 128;
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    mma_ts(tm + 256 + i * DP, tm + i * 128 + kk * 8, b + step_mn(kk), ID_O, (j | kk) != 0, one);
+                for (int h = 0; h < 2; ++h) {
+                    if (!warp_wait(h ? p_full(i) : p_half(i), j & 1, P.err, 7)) goto done;
+                    fence_after();
+#pragma unroll
+                    for (int kk = h * 4; kk < h * 4 + 4; ++kk)
+                        mma_ts(tm + 256 + i * DP, p + kk * 8, b + step_mn(kk), ID_O, (j | kk) != 0, one);
+                }
                 mma_commit(pv_done(i), one);
-                if (j + 1 < nu[i]) {    // S_i takes P_i's place: only after the product that reads P_i
+                if (!APART && j + 1 < nu[i]) {    // S_i takes P_i's place: only after the product that reads P_i
                     if (!warp_wait(pv_done(i), j & 1, P.err, 8)) goto done;
                     fence_after();
                     mma_s(i, sk);
@@ -351,6 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool live = row < w.lq;
         const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + i * 128;
         const uint32_t to = tmem + ((uint32_t)(q * 32) << 16) + 256 + i * DP;
+        const uint32_t tp = APART ? tmem + ((uint32_t)(q * 32) << 16) + 384 + i * 64 : ts;
         const float c = P.scale2, slack = 8.0f / c;
         // keys this row sees; and those every row of the tile sees
         const int mine = P.causal ? min(w.lk, row + off + 1) : w.lk;
@@ -379,26 +397,30 @@ __global__ void __launch_bounds__(THREADS, 1)
             auto largest = [&]() {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4) {
-                    tops[0] = max3(tops[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                    tops[1] = max3(tops[1], __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
-                    tops[2] = max3(tops[2], __uint_as_float(y[k]), __uint_as_float(y[k + 1]));
-                    tops[3] = max3(tops[3], __uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
+                    tops[0] = max3_nan(tops[0], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                    tops[1] = max3_nan(tops[1], __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                    tops[2] = max3_nan(tops[2], __uint_as_float(y[k]), __uint_as_float(y[k + 1]));
+                    tops[3] = max3_nan(tops[3], __uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
                 }
             };
             load(64);
             largest();
             load(0);
             largest();
-            const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+            const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
             // the reference maximum follows only where it has fallen 2^8 behind:
             // p up to 256 is as exact, and O is rescaled a few times in all
-            const bool up = top > m + slack || (m == -INFINITY && top > m);
+            // (a NaN score, or one of +inf, makes the row NaN here: the exponentials
+            // on the fma pipe would hide it)
+            if (APART && j > 0 && !mbar_wait(pv_done(i), (j - 1) & 1, P.err, 12)) goto done;     // O and P are free
+            const bool up = !(top <= m + slack);
             if (__any_sync(0xffffffffu, up)) {
-                const float to_m = fmaxf(m, top);
+                float to_m = up ? max3_nan(m, top, top) : m;     // a row moves by its own scores alone
+                if (to_m == INFINITY) to_m = NAN;
                 const float f = m == to_m ? 1.0f : ex2f((m - to_m) * c);
                 m = to_m;
                 l *= f;
-                if (j > 0) {            // P_i V of block j - 1 is complete: S_i was issued after it
+                if (j > 0) {            // P_i V of block j - 1 is complete
 #pragma unroll
                     for (int k = 0; k < DP; k += 32) {
                         uint32_t o[32];
@@ -413,24 +435,40 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float mc = m == -INFINITY ? 0.f : -m * c;
             const uint64_t c2 = f2(c, c), mc2 = f2(mc, mc);
             uint64_t sum[2] = {0, 0};
-            auto weigh = [&](const uint32_t* v, int at) {       // P of 32 columns, into columns of S that are done with
+            auto weigh = [&](const uint32_t* v, int at, auto fma_pipe) {       // P of 32 columns
                 uint32_t w16[16];
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
                     float a, b;
-                    unf2(fma2(f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, mc2), a, b);
-                    a = ex2f(a);
-                    b = ex2f(b);
+                    const uint64_t x2 = fma2(f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, mc2);
+                    // every fourth pair on the fma pipe (where nothing is masked: it has no exact 0)
+                    if (decltype(fma_pipe)::value && k % 8 == 6) ex2_fma2(x2, a, b);
+                    else {
+                        unf2(x2, a, b);
+                        a = ex2f(a);
+                        b = ex2f(b);
+                    }
                     sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], f2(a, b));
                     w16[k >> 1] = pack2(a, b, T());
                 }
-                st16(ts + at, w16);
+                st16(tp + at, w16);
             };
-            weigh(x, 0);
-            weigh(y, 16);
-            load(64);
-            weigh(x, 32);
-            weigh(y, 48);
+            auto block = [&](auto fma_pipe) {
+                weigh(x, 0, fma_pipe);
+                weigh(y, 16, fma_pipe);
+                wait_st();
+                fence_before();
+                mbar_arrive(p_half(i));
+                load(64);
+                if (APART) {
+                    fence_before();
+                    mbar_arrive(s_free(i));
+                }
+                weigh(x, 32, fma_pipe);
+                weigh(y, 48, fma_pipe);
+            };
+            if (masked) block(std::false_type());
+            else block(std::true_type());
             float sa, sb;
             unf2(add2(sum[0], sum[1]), sa, sb);
             l += sa + sb;
@@ -445,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!mbar_wait(pv_done(i), (ni - 1) & 1, P.err, 10)) goto done;
             fence_after();
             const int64_t stride = (int64_t)P.H * P.D, at0 = at - lane * stride;
-            store_rows<T, DP, true>(to, base + i * TILE + q * (TILE / 4), l == 0.f ? 0.f : 1.0f / l, out + at0, stride,
+            store_rows<T, DP, true>(to, base + i * TILE + q * (TILE / 4), m == -INFINITY ? 0.f : 1.0f / l, out + at0, stride,
                                     0, P.D, w.lq - (row - lane), rest ? rest + at0 : nullptr);
         } else if (live) {
             for (int d = 0; d < P.D; d += 8) {
@@ -453,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (rest) *reinterpret_cast<uint4*>(rest + at + d) = make_uint4(0, 0, 0, 0);
             }
         }
-        if (live) P.lse[(int64_t)head * P.Tq + trow] = l == 0.f ? -INFINITY : fmaf(m, P.scale, logf(l));
+        if (live) P.lse[(int64_t)head * P.Tq + trow] = m == -INFINITY ? -INFINITY : fmaf(m, P.scale, logf(l));
     }
 done:
     fence_before();

@@ -132,6 +132,35 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// the same, a NaN among them wins
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two values on the fma pipe, beside the special-function unit (which
+// gives 4 a cycle and scheduler): x = n + f with n the nearest whole number, a
+// polynomial in f whose relative error is least on [-1/2, 1/2] (2.6e-6; fitted
+// by least squares reweighted by the error, Lawson's method), n added to the
+// exponent.  x below -126 counts as -126; x is not NaN and below 128.
+__device__ __forceinline__ void ex2_fma2(uint64_t x, float& a, float& b) {
+    unf2(x, a, b);
+    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t shift = f2(12582912.f, 12582912.f), back = f2(-12582912.f, -12582912.f);     // 1.5 * 2^23
+    const uint64_t r = add2(x, shift), n = add2(r, back);
+    const uint64_t f = fma2(n, f2(-1.f, -1.f), x);
+    uint64_t p = fma2(f, f2(0.009570101434f, 0.009570101434f), f2(0.05591786028f, 0.05591786028f));
+    p = fma2(p, f, f2(0.2402474484f, 0.2402474484f));
+    p = fma2(p, f, f2(0.6931218147f, 0.6931218147f));
+    p = fma2(p, f, f2(0.9999992614f, 0.9999992614f));
+    float ra, rb;
+    unf2(r, ra, rb);
+    unf2(p, a, b);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ra) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(rb) << 23));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
