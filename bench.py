@@ -488,6 +488,22 @@ def bench_chargpt(args, cores):
     emit(d)
 
 
+def bench_chardistill(args):
+    """The char GPT distilled on packed documents, on one GPU: tokens/s."""
+    import workloads
+    r = workloads.train_chardistill(steps=args.steps, graph=args.graph)
+    ms = sum(r["ms"]) / len(r["ms"])
+    emit({"metric": "char-GPT distillation on packed documents, train tokens/s", "unit": "tokens/s", "n_gpus": 1,
+          "steps": args.steps, "warmup": 10, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+          "dtype": "bf16 autocast; packed int32 words",
+          "data": "synthetic: order-2 Markov chain, 65 symbols, its rows' top 16 as the teacher",
+          "config": {"workload": "6L/6H/384d char-GPT student, 64 documents of 1-256 tokens packed, T 2, alpha 0.5",
+                     "seq_len": 256, "global_batch": 64},
+          "value": 1e3 * r["tokens_per_step"] / ms, "ms_per_step": ms, "losses": [r["losses"][0], r["losses"][-1]],
+          "concord_params": r["concord_params"], "cuda_graph": args.graph,
+          "timing": "CUDA events around each training step, mean; rows of no document count as tokens"})
+
+
 def bench_llama(args, rank, world, steps=None, warmup=None, ret=False):
     """Config 5: weak-scaling data-parallel training step (whole job tokens/s).
     With `ret` the line is returned (rank 0; None elsewhere) instead of printed."""
@@ -767,9 +783,10 @@ def main():
     ap.add_argument("--layers", type=int, default=24, help="llama: decoder layers")
     ap.add_argument("--nogate", action="store_true", help="sdxl: disable_cohpre on every layer")
     ap.add_argument("--ckpt", action="store_true", help="sdxl: activation checkpointing per block")
-    ap.add_argument("--workload", default="c2", choices=["c2", "chargpt", "llama", "sdxl", "conv", "gemm"],
+    ap.add_argument("--workload", default="c2", choices=["c2", "chargpt", "chardistill", "llama", "sdxl", "conv", "gemm"],
                     help="c2: the packed-step path on config 2's largest layer (default); "
                          "chargpt: config 3's char-level GPT trained end to end; "
+                         "chardistill: the same architecture distilled on packed documents; "
                          "llama: config 5's data-parallel decoder (weak scaling); "
                          "sdxl: config 4's UNet fine-tune (weak scaling); "
                          "conv: the conv layer's convolutions per backend; "
@@ -822,6 +839,10 @@ def main():
     if args.workload == "chargpt":
         if rank == 0:
             bench_chargpt(args, cores)
+        return
+    if args.workload == "chardistill":
+        if rank == 0:
+            bench_chardistill(args)
         return
     if args.workload == "conv":
         if rank == 0:

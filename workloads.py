@@ -8,6 +8,9 @@ checkpoint is read.
   MLP, learned positions, causal SDPA), 6 layers, 6 heads, d=384, context
   256, vocab 65, batch 64, on tokens from a seeded order-2 Markov chain over
   65 symbols whose transition rows are Dirichlet(0.3).
+* The char-level GPT as a student, distilled on packed documents of different
+  lengths from its teacher's top logits (the chain's own transition rows),
+  on this package's layer norm, packed attention and distillation loss.
 * Config 5, Llama-style decoder (24 layers, d=2048, 16 heads, SwiGLU 5504,
   vocab 32000, seq 2048) on uniform random token ids.
 """
@@ -194,6 +197,120 @@ def _chargpt_loop(steps, lr, warmup, layers, data, batch, block, x, y, graph, st
         if g is None:
             del loss
     return log, t_dev, g
+
+
+# ---------------------------------------------------------------- the char GPT distilled on packed documents
+class PackedGPTBlock(nn.Module):
+    """GPTBlock over documents packed one after the other: x [tokens, d]."""
+
+    def __init__(self, d, h):
+        super().__init__()
+        from concord_b200 import LayerNorm
+        self.ln_1, self.ln_2 = (LayerNorm(d, out_dtype=torch.bfloat16) for _ in range(2))
+        self.c_attn, self.c_proj = nn.Linear(d, 3 * d, bias=False), nn.Linear(d, d, bias=False)
+        self.c_fc, self.mlp_proj = nn.Linear(d, 4 * d, bias=False), nn.Linear(4 * d, d, bias=False)
+        self.h = h
+
+    def forward(self, x, cu_seqlens):
+        from concord_b200 import packed_attention
+        T, d = x.shape
+        q, k, v = self.c_attn(self.ln_1(x)).view(T, 3, self.h, d // self.h).unbind(1)
+        x = x + self.c_proj(packed_attention(q, k, v, cu_seqlens).view(T, d))
+        return x + self.mlp_proj(F.gelu(self.c_fc(self.ln_2(x))))
+
+
+class PackedCharGPT(nn.Module):
+    """CharGPT's architecture for packed documents: logits [tokens, vocab]."""
+
+    def __init__(self, vocab=65, block=256, n_layer=6, n_head=6, d=384):
+        super().__init__()
+        from concord_b200 import LayerNorm
+        self.wte, self.wpe = nn.Embedding(vocab, d), nn.Embedding(block, d)
+        self.blocks = nn.ModuleList([PackedGPTBlock(d, n_head) for _ in range(n_layer)])
+        self.ln_f = LayerNorm(d, out_dtype=torch.bfloat16)
+        self.lm_head = nn.Linear(d, vocab, bias=False)
+        for m in self.modules():
+            if isinstance(m, (nn.Linear, nn.Embedding)):
+                nn.init.normal_(m.weight, 0.0, 0.02)
+        for b in self.blocks:
+            for lin in (b.c_proj, b.mlp_proj):
+                nn.init.normal_(lin.weight, 0.0, 0.02 / math.sqrt(2 * n_layer))
+
+    def forward(self, idx, pos, cu_seqlens):
+        x = self.wte(idx) + self.wpe(pos)
+        for b in self.blocks:
+            x = b(x, cu_seqlens)
+        return self.lm_head(self.ln_f(x))
+
+
+class PackedDocuments:
+    """Batches of `docs` documents of 1 to `block` tokens from a MarkovChars,
+    packed into `tokens` rows (the rest belongs to no document), with the
+    teacher's `top` logits per token: the chain's own transition row, known
+    from a document's second token on."""
+
+    def __init__(self, data, docs, block, top):
+        self.data, self.docs, self.block, self.top = data, docs, block, top
+        self.tokens = docs * block
+        self.logits = data.P.clamp_min(1e-30).log()
+
+    def batch(self):
+        d, dev = self.data, self.data.toks.device
+        n, L = d.toks.shape
+        rand = lambda hi: torch.randint(0, hi, (self.docs,), generator=d.gen, device=dev)  # noqa: E731
+        lens, chain, start = rand(self.block) + 1, rand(n), rand(L - self.block - 1)
+        cu = torch.zeros(self.docs + 1, dtype=torch.int32, device=dev)
+        cu[1:] = lens.cumsum(0)
+        row = torch.arange(self.tokens, device=dev)
+        doc = torch.searchsorted(cu[1:].long(), row, right=True).clamp_max(self.docs - 1)
+        inside = row < cu[-1]
+        pos = torch.where(inside, row - cu[doc], 0)
+        at = start[doc] + pos
+        x, y = d.toks[chain[doc], at], d.toks[chain[doc], at + 1]
+        before = d.toks[chain[doc], (at - 1).clamp_min(0)]
+        t, ids = self.logits[before * d.vocab + x].topk(self.top, dim=1)
+        ids = torch.where((inside & (pos > 0))[:, None], ids, -1)
+        return x, pos, torch.where(inside, y, -100), ids, t, cu
+
+
+def train_chardistill(steps=200, docs=64, block=256, top=16, temperature=2.0, alpha=0.5, lr=5e-4, aux_lr=0.05, seed=0,
+                      device="cuda", n_layer=6, warmup=100, graph=True):
+    """The char GPT distilled on packed documents, one GPU: Concord on every
+    Linear, this package's layer norms and attention around them, and the
+    loss and its gradient in one call (`distill_loss_and_grad`), which starts
+    the backward that steps the packed layers.  Lengths change from batch to
+    batch under one CUDA graph: they are read on the device.  Returns per-step
+    device times and losses."""
+    from concord_b200 import distill_loss_and_grad
+    from concord_b200.convert import aux_parameters, concordify
+    torch.manual_seed(seed)
+    batches = PackedDocuments(MarkovChars(seed=seed, device=device), docs, block, top)
+    model = PackedCharGPT(block=block, n_layer=n_layer).to(device)
+    layers = concordify(model, lr=lr)
+    aux = aux_parameters(model)
+    opt = torch.optim.SGD(aux, lr=aux_lr, momentum=0.9)
+    static = [t.clone() for t in batches.batch()]
+    for p in aux:
+        p.grad = torch.zeros_like(p)
+
+    def refill(it):
+        for dst, src in zip(static, batches.batch()):
+            dst.copy_(src)
+
+    def step():
+        x, pos, y, ids, t, cu = static
+        opt.zero_grad(set_to_none=False)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            logits = model(x, pos, cu)
+        loss, dlogits = distill_loss_and_grad(logits, ids, t, labels=y, temperature=temperature, alpha=alpha)
+        logits.backward(dlogits)              # Concord layers step inside the backward
+        opt.step()
+        for l in layers:
+            l.rebalance()
+        return loss
+
+    times, losses = run_steps(step, refill, steps, 10, layers, lr, graph)
+    return dict(ms=times, losses=losses, tokens_per_step=batches.tokens, concord_params=sum(l.packed_w.numel() for l in layers))
 
 
 def run_steps(step_fn, refill, steps, warmup, layers, lr, graph, world=1, group=None):
