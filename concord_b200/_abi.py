@@ -265,7 +265,9 @@ _SIGS = [
     ("concord_attention_fwd", ctypes.c_int,
      [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P] * 4),
     ("concord_attention_bwd", ctypes.c_int,
-     [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P, _P, _P, _P, _I64, _I64] + [_P] * 5),
+     [ctypes.POINTER(AttentionParams)] + [_P, _I64, _I64] * 3 + [_P, _P, _P, _P, _I64, _I64] + [_P] * 5 +
+     [ctypes.c_size_t, _P]),
+    ("concord_attention_bwd_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(AttentionParams)]),
     ("concord_attention_error", ctypes.c_int, [_I32]),
 ]
 

@@ -66,6 +66,8 @@ struct Params {
     int64_t do_ts, do_hs;
     float* delta;         // [H, Tq]
     void *dq, *dk, *dv;
+    float* part;          // splits > 1: [splits][dk, dv][Tk, key heads, D] in fp32
+    int splits, per;      // parts of a key head's query heads, and heads of a part
     int* err;
 };
 
@@ -148,7 +150,7 @@ __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
 template <typename T, int COLS, bool REST = false>
 __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f, T* out, int64_t stride, int col0,
                                            int D, int rows, T* rest = nullptr) {
-    constexpr int CH = COLS / 8;                 // 16-byte pieces of a row
+    constexpr int E = Pack16<T>::N, CH = COLS / E;             // elements of 16 bytes, such pieces of a row
     const int lane = threadIdx.x & 31;
     auto place = [](int row, int c) -> uint32_t { return (row * CH + (c ^ (CH >= 8 ? row & 7 : (row >> 1) & 3))) * 16; };
 #pragma unroll
@@ -160,19 +162,19 @@ __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f,
             ld32(tm + c, r);
             wait_ld();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float v[8];
+            for (int k = 0; k < 32 / E; ++k) {
+                float v[E];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[k * 8 + e]) * f;
+                for (int e = 0; e < E; ++e) v[e] = __uint_as_float(r[k * E + e]) * f;
                 uint4 o = Pack16<T>::pack(v);
                 if (pass) {
-                    float h[8];
+                    float h[E];
                     Pack16<T>::unpack(o, h);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] -= h[e];
+                    for (int e = 0; e < E; ++e) v[e] -= h[e];
                     o = Pack16<T>::pack(v);
                 }
-                sts16(stage + place(lane, c / 8 + k), o);
+                sts16(stage + place(lane, c / E + k), o);
             }
         }
         __syncwarp();
@@ -187,7 +189,7 @@ __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f,
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int at = (i + k) * 32 + lane, row = at / CH, col = col0 + at % CH * 8;
+                const int at = (i + k) * 32 + lane, row = at / CH, col = col0 + at % CH * E;
                 if (row < rows && col < D) *reinterpret_cast<uint4*>(dst + row * stride + col) = o[k];
             }
         }
@@ -269,10 +271,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t ring = base + C::RING;
 
     if (w.tile < 0) {
-        if (w.first + (P.Tq - w.last) > 0) {
+        const int rows = w.first + (P.Tq - w.last);
+        if (rows > 0) {
             zero_uncovered(out, w, P.Tq, P.H, head, P.D);
-            for (int64_t r = (int64_t)w.spare * blockDim.x + threadIdx.x; r < w.first + (P.Tq - w.last);
-                 r += (int64_t)w.spares * blockDim.x)
+            for (int64_t r = (int64_t)w.spare * blockDim.x + threadIdx.x; r < rows; r += (int64_t)w.spares * blockDim.x)
                 P.lse[(int64_t)head * P.Tq + (r < w.first ? r : w.last + (r - w.first))] = 0.f;
         }
     } else if (warp == 0) {
@@ -713,7 +715,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             fence_before();
             mbar_arrive(dp_free);
             const bool masked = (j + 1) * 128 > every;
-            auto weigh = [&](bool mask) {
+            auto weigh = [&](auto with_mask) {
+                constexpr bool mask = decltype(with_mask)::value;
 #pragma unroll
                 for (int k = 0; k < 64; k += 2) {
                     float a, b;
@@ -726,7 +729,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     u[k >> 1] = pack2(a, b, T());
                 }
             };
-            if (masked) weigh(true); else weigh(false);
+            if (masked) weigh(std::true_type());
+            else weigh(std::false_type());
             if (j > 0 && !mbar_wait(ds_free, (j - 1) & 1, P.err, 34)) goto done;
             st32(tmem + lanes + 384 + half * 32, u);
             wait_st();
@@ -755,7 +759,8 @@ done:
 
 // ---------------------------------------------------------------- backward: dk and dv
 // A block owns 128 keys of one key head and walks the query blocks of every
-// head that shares it.  The scores are transposed (a key is a row), so p and
+// head that shares it, or, where there are few key blocks, of some of these
+// heads: the parts' sums then meet in fp32 and are added in part order.  The scores are transposed (a key is a row), so p and
 // ds are the A operands of their products as they come from the softmax.
 // Tensor memory: S 0, dP 128, dV 256, dK 256 + DP.  P takes half of each half
 // of S (columns 0-31 and 64-95), dS the same of dP: each softmax warp writes
@@ -823,7 +828,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto st_empty = [&](int s) { return one + 72u + 8u * s; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int HK = P.H / P.G;
-    const int kvh = blockIdx.x % HK, t = blockIdx.x / HK;
+    const int kvh = blockIdx.x % HK, part = blockIdx.x / HK % P.splits, t = blockIdx.x / HK / P.splits;
+    const int head0 = kvh * P.G + part * P.per;                      // its first query head
 
     if (warp == 0) {
         if (lane == 0) {
@@ -835,7 +841,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int s = 0; s < 2; ++s) { mbar_init(st_full(s), 64); mbar_init(st_empty(s), 1); }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        find_tile(P, true, t, gridDim.x / HK, 128, false, work);
+        find_tile(P, true, t, gridDim.x / HK / P.splits, 128, false, work);
     }
     if (warp == 1) tmem_alloc<512>(smem_u32(slot));
     if (warp >= 4) {          // the ones, and zeros beside them and beside the values
@@ -858,11 +864,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int first = P.causal ? max(0, k0 - off) : 0;
         if (first < w.lq) { jq = first / 128; nq = (w.lq + 127) / 128 - jq; }
     }
-    const int n = nq * P.G;
+    const int n = nq * min(P.per, P.G - part * P.per);
+    const int64_t all = (int64_t)P.Tk * HK * P.D;
+    float* dkp = P.part + 2 * all * part;                            // splits > 1
 
     if (w.tile < 0) {
-        zero_uncovered(P.dk, w, P.Tk, HK, kvh, P.D);
-        zero_uncovered(P.dv, w, P.Tk, HK, kvh, P.D);
+        // (an fp32 row is two 16-bit ones)
+        const int width = P.splits > 1 ? 2 * P.D : P.D;
+        zero_uncovered(P.splits > 1 ? dkp : P.dk, w, P.Tk, HK, kvh, width);
+        zero_uncovered(P.splits > 1 ? dkp + all : P.dv, w, P.Tk, HK, kvh, width);
     } else if (warp == 0) {
         if (lane == 0 && n > 0) {
             auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int h, int row) {
@@ -873,7 +883,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             load(base + TILE, &mv, kv_full, kvh, w.k0 + k0);
             for (int x = 0; x < n; ++x) {
                 const int sq = x % QS, so = x % OS;
-                const int head = kvh * P.G + x / nq, row = w.q0 + (jq + x % nq) * 128;
+                const int head = head0 + x / nq, row = w.q0 + (jq + x % nq) * 128;
                 if (!mbar_wait(q_empty(sq), ((x / QS) & 1) ^ 1, P.err, 41)) goto done;
                 mbar_expect(q_full(sq), TILE);
                 load(base + C::Q_OFF + sq * TILE, &mq, q_full(sq), head, row);
@@ -977,7 +987,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int i = threadIdx.x - 64;
         const float unscale = -1.0f / P.scale;
         for (int x = 0; x < n; ++x) {
-            const int s = x & 1, head = kvh * P.G + x / nq, row0 = (jq + x % nq) * 128;
+            const int s = x & 1, head = head0 + x / nq, row0 = (jq + x % nq) * 128;
             float l[2], d[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -1059,23 +1069,29 @@ __global__ void __launch_bounds__(THREADS, 1)
             fence_before();
             mbar_arrive(ds_full);
         }
-        const int64_t trow = (int64_t)w.k0 + key;
-        T* dk = static_cast<T*>(P.dk) + (trow * HK + kvh) * P.D;
-        T* dv = static_cast<T*>(P.dv) + (trow * HK + kvh) * P.D;
+        const int64_t at = (((int64_t)w.k0 + key - lane) * HK + kvh) * P.D, stride = (int64_t)HK * P.D;   // lane 0's row
+        const int col = half * (DP / 2), rows = w.lk - (key - lane);
+        auto store = [&](auto* dk, auto* dv) {
+            using O = std::remove_pointer_t<decltype(dk)>;
+            const uint32_t stage = base + half * TILE + q * (TILE / 16 * sizeof(O));
+            store_rows<O, DP / 2>(tmem + lanes + 256 + col, stage, 1.0f, dv + at, stride, col, P.D, rows);
+            store_rows<O, DP / 2>(tmem + lanes + 256 + DP + col, stage, P.scale, dk + at, stride, col, P.D, rows);
+        };
+        auto clear = [&](auto* dk, auto* dv) {
+            constexpr int E = 16 / sizeof(*dk);
+            for (int d = half * E; d < P.D; d += 2 * E) {
+                *reinterpret_cast<uint4*>(dk + at + lane * stride + d) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(dv + at + lane * stride + d) = make_uint4(0, 0, 0, 0);
+            }
+        };
         if (n > 0) {
             if (!mbar_wait(dk_done, (n - 1) & 1, P.err, 56)) goto done;      // and dV before it
             fence_after();
-            const int64_t stride = (int64_t)HK * P.D;
-            const int col = half * (DP / 2), rows = w.lk - (key - lane);
-            const uint32_t stage = base + half * TILE + q * (TILE / 8);
-            store_rows<T, DP / 2>(tmem + lanes + 256 + col, stage, 1.0f, dv - lane * stride, stride, col, P.D, rows);
-            store_rows<T, DP / 2>(tmem + lanes + 256 + DP + col, stage, P.scale, dk - lane * stride, stride, col, P.D,
-                                  rows);
+            if (P.splits > 1) store(dkp, dkp + all);
+            else store(static_cast<T*>(P.dk), static_cast<T*>(P.dv));
         } else if (live) {
-            for (int d = half * 8; d < P.D; d += 16) {
-                *reinterpret_cast<uint4*>(dk + d) = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(dv + d) = make_uint4(0, 0, 0, 0);
-            }
+            if (P.splits > 1) clear(dkp, dkp + all);
+            else clear(static_cast<T*>(P.dk), static_cast<T*>(P.dv));
         }
     }
 done:
@@ -1085,6 +1101,22 @@ done:
         fence_after();
         tmem_free<512>(tmem);
     }
+}
+
+// dk, dv from the parts' sums, in part order (8 elements a thread)
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, int64_t all,
+                                                   T* __restrict__ dk, T* __restrict__ dv) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= 2 * all) return;
+    float s[8], v[8];
+    load_vec<8>(part + i, s);
+    for (int k = 1; k < splits; ++k) {
+        load_vec<8>(part + 2 * all * k + i, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += v[e];
+    }
+    store_vec<8>(i < all ? dk + i : dv + (i - all), s);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1167,7 +1199,8 @@ int check(const char* name, const concord_attention_params* p) {
         return fail(CONCORD_ESHAPE, n + ": head_dim must be a multiple of 8 up to 128");
     if (!(p->scale > 0.f) || !(p->scale < INFINITY)) return fail(CONCORD_EINVAL, n + ": scale must be positive");
     if (!p->cu_q || !p->cu_k) return fail(CONCORD_EINVAL, n + ": null pointer");
-    if (tiles_bound(std::max(p->tokens_q, p->tokens_k), p->seqs, 128) * p->heads > INT32_MAX)
+    if (tiles_bound(std::max(p->tokens_q, p->tokens_k), p->seqs, 128) * p->heads > INT32_MAX ||
+        p->tokens_k * p->kv_heads * p->head_dim / 4 / 256 >= INT32_MAX)
         return fail(CONCORD_ETOOBIG, n + ": too many tiles");
     return CONCORD_OK;
 }
@@ -1196,13 +1229,38 @@ void launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v
     fwd_kernel<T, DP><<<grid, THREADS, Fwd<DP>::SMEM, st>>>(q, k, v, P);
 }
 
+// multiprocessors (asked for once: the sizes of workspaces go by it, so it is one number for the process)
+int sm_count() {
+    static const int n = [] {
+        int d = 0, c = 148;
+        if (cudaGetDevice(&d) == cudaSuccess) cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, d);
+        return c;
+    }();
+    return n;
+}
+
+// Parts of a key head's query heads: with fewer key blocks than two for each
+// SM, as many parts as make up two.  One key head of 16 query heads, 2048
+// tokens, heads of 128: 420 us with one part, 45 us with 16 and 33 MB to join.
+int splits_of(int64_t tokens_k, int64_t heads, int64_t kv_heads, int* per) {
+    const int64_t G = heads / kv_heads, blocks = (tokens_k + 127) / 128 * kv_heads;
+    const int64_t want = std::min<int64_t>(G, (2 * sm_count() + blocks - 1) / blocks);
+    *per = (int)((G + want - 1) / want);
+    return (int)((G + *per - 1) / *per);
+}
+
 template <typename T, int DP>
 void launch_bwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& d,
                 const Params& P, cudaStream_t st) {
     if (P.Tq > 0)
         bwd_q_kernel<T, DP><<<(int)(tiles_bound(P.Tq, P.B, 128) * P.H), THREADS, BwdQ<DP>::SMEM, st>>>(q, k, v, d, P);
-    bwd_k_kernel<T, DP><<<(int)(tiles_bound(P.Tk, P.B, 128) * (P.H / P.G)), THREADS, BwdK<DP>::SMEM, st>>>(q, k, v, d,
-                                                                                                         P);
+    bwd_k_kernel<T, DP><<<(int)(tiles_bound(P.Tk, P.B, 128) * (P.H / P.G) * P.splits), THREADS, BwdK<DP>::SMEM, st>>>(
+        q, k, v, d, P);
+    if (P.splits > 1) {
+        const int64_t all = (int64_t)P.Tk * (P.H / P.G) * P.D;
+        join_kernel<T><<<(int)((2 * all / 8 + 255) / 256), 256, 0, st>>>(P.part, P.splits, all, static_cast<T*>(P.dk),
+                                                                        static_cast<T*>(P.dv));
+    }
 }
 
 }  // namespace attn
@@ -1246,10 +1304,19 @@ extern "C" int concord_attention_fwd(const concord_attention_params* p, const vo
     return check_launch(name);
 }
 
+// workspace: the parts' sums, where the query heads of a key head are split
+extern "C" size_t concord_attention_bwd_workspace_bytes(const concord_attention_params* p) {
+    if (attn::check("concord_attention_bwd_workspace_bytes", p) != CONCORD_OK || p->tokens_k == 0) return 0;
+    int per = 1;
+    const int splits = attn::splits_of(p->tokens_k, p->heads, p->kv_heads, &per);
+    return splits > 1 ? (size_t)splits * 2 * p->tokens_k * p->kv_heads * p->head_dim * sizeof(float) : 0;
+}
+
 extern "C" int concord_attention_bwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs,
                                      const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
                                      int64_t v_hs, const void* o, const void* o_rest, const float* lse,
-                                     const void* dout, int64_t do_ts, int64_t do_hs, float* delta, void* dq, void* dk, void* dv, void* stream) {
+                                     const void* dout, int64_t do_ts, int64_t do_hs, float* delta, void* dq, void* dk, void* dv,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
     const char* name = "concord_attention_bwd";
     if (int rc = attn::check(name, p)) return rc;
     if (p->tokens_q == 0 || p->tokens_k == 0) return fail(CONCORD_ESHAPE, "concord_attention_bwd: no rows");
@@ -1260,6 +1327,9 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
     if (!o || !o_rest || !lse || !delta || !dq || !dk || !dv) return fail(CONCORD_EINVAL, "concord_attention_bwd: null pointer");
     if (!aligned(o, 16) || !aligned(o_rest, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16))
         return fail(CONCORD_EALIGN, "concord_attention_bwd: tensors must be 16-byte aligned");
+    if (workspace_bytes < concord_attention_bwd_workspace_bytes(p) || (!workspace && workspace_bytes) ||
+        !aligned(workspace, 16))
+        return fail(CONCORD_EWORKSPACE, "concord_attention_bwd: workspace too small or not 16-byte aligned");
     if (int rc = bind_current_context(name)) return rc;
     CUtensorMap mq, mk, mv, md;
     const int bf = p->type == CONCORD_BF16;
@@ -1281,6 +1351,8 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
     P.dq = dq;
     P.dk = dk;
     P.dv = dv;
+    P.splits = attn::splits_of(p->tokens_k, p->heads, p->kv_heads, &P.per);
+    P.part = static_cast<float*>(workspace);
     cudaStream_t st = as_stream(stream);
     if (bf) {
         if (p->head_dim <= 64) attn::launch_bwd<__nv_bfloat16, 64>(mq, mk, mv, md, P, st);

@@ -296,10 +296,13 @@ struct AttentionBackward : public torch::autograd::Node {
                 out = {at::empty(q.sizes(), plain), at::empty(k.sizes(), plain), at::empty(v.sizes(), plain)};
                 const Tensor up = operand(g[0]), delta = at::empty(lse.sizes(), lse.options());
                 const auto p = attention_params(q, k, cu_q, cu_k, causal, scale);
+                const size_t bytes = concord_attention_bwd_workspace_bytes(&p);
+                Tensor ws;
+                if (bytes > 0) ws = at::empty({(int64_t)bytes}, plain.dtype(at::kByte));
                 check(concord_attention_bwd(&p, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1),
                                             ptr(v), v.stride(0), v.stride(1), ptr(o), ptr(rest), ptr<float>(lse),
                                             ptr(up), up.stride(0), up.stride(1), ptr<float>(delta), ptr(out[0]),
-                                            ptr(out[1]), ptr(out[2]), current_stream()),
+                                            ptr(out[1]), ptr(out[2]), ptr(ws), bytes, current_stream()),
                       "concord_attention_bwd");
             }
         }

@@ -629,7 +629,8 @@ int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t
  * gradients are contiguous; o_rest (o's layout; NULL in the forward where no
  * backward follows) is what o's rounding left over, from which the backward
  * has delta = dout . o to fp32; lse and delta are fp32 [heads, tokens_q], delta
- * being scratch that the backward fills.  concord_attention_error: non-zero
+ * being scratch that the backward fills, as is its workspace (16-byte aligned;
+ * often of 0 bytes).  concord_attention_error: non-zero
  * once a barrier wait inside a kernel has run out (2 s of GPU time per wait).
  */
 typedef struct concord_attention_params {
@@ -646,7 +647,8 @@ int concord_attention_fwd(const concord_attention_params* p, const void* q, int6
 int concord_attention_bwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
                           int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, const void* o,
                           const void* o_rest, const float* lse, const void* dout, int64_t do_ts, int64_t do_hs, float* delta, void* dq,
-                          void* dk, void* dv, void* stream);
+                          void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+size_t concord_attention_bwd_workspace_bytes(const concord_attention_params* p);
 int concord_attention_error(int32_t reset);
 
 #ifdef __cplusplus

@@ -119,6 +119,17 @@ def test_shared_heads(H, Hk, D):
     check(*inputs(333, H, Hk, D, seed=H * Hk), cum([200, 133]))
 
 
+def test_shared_heads_in_uneven_parts():
+    """Five query heads of one key head, at 110 key blocks: parts of two, two and one."""
+    from concord_b200 import _abi
+    lens = [128] * 100 + [1, 0, 127, 300, 90, 130, 128, 60]
+    q, k, v, do = inputs(sum(lens), 5, 1, 64, seed=11)
+    p = _abi.AttentionParams(cu_q=1, cu_k=1, seqs=1, tokens_q=len(q), tokens_k=len(k), heads=5, kv_heads=1, head_dim=64,
+                             type=_abi.BF16, causal=1, scale=1.0)
+    assert _abi.load().concord_attention_bwd_workspace_bytes(p) == 3 * 2 * len(k) * 64 * 4
+    check(q, k, v, do, cum(lens))
+
+
 @pytest.mark.parametrize("lq,lk", [([5], [400]), ([400], [5]), ([130, 1, 300], [77, 500, 140]), ([0, 7], [9, 0]),
                                    ([1, 1, 1], [1000, 129, 0]), ([300, 20], [300, 700])])
 @pytest.mark.parametrize("causal", [True, False])
