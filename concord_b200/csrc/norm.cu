@@ -157,19 +157,20 @@ template <typename T, int STAGES, int EL = PER> struct Ring {
     }
 };
 
-template <typename TX, int EL> constexpr int fwd_stages() { return EL == 64 || sizeof(TX) == 4 ? 3 : 4; }
+template <typename TX> constexpr int fwd_stages() { return sizeof(TX) == 4 ? 3 : 4; }
 
-// EL elements a thread.  With 64 of them a row of 2048 belongs to one warp: no
-// barrier, and the two sums cost a third of an instruction an element; with 16
-// (four warps a row) the kernel issued 25 an element and took 135 us for 65533
-// x 2048 bf16, above the 82 us of its bytes.
-// ONE: a row is one warp's (the columns' distances are then constants).
+// EL elements a thread, whose weight and bias stay in its registers (VEC 8).
+// Measured for 65533 x 2048 bf16 (82 us of bytes): 16 elements, four warps a
+// row, 135 us (25 instructions an element, half of them the two sums); 64, one
+// warp a row, weight and bias from the L1, 125 us (90 without them: the L1
+// gives 128 bytes a cycle, they are 8 an element); 32 in registers, two warps a
+// row, 105 us.  ONE: a row is one warp's (the columns' distances are constants).
 template <typename TX, typename TY, int VEC, int EL, bool ONE>
-__global__ void __launch_bounds__(VEC == 1 ? 1024 : 256)
+__global__ void __launch_bounds__(VEC == 1 ? 1024 : 512)
     fwd_kernel(const TX* __restrict__ x, int64_t ldx, const float* __restrict__ w, const float* __restrict__ b,
                TY* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int64_t N, int D, float eps,
                int threads_per_row) {
-    constexpr int NV = EL / VEC, STAGES = fwd_stages<TX, EL>();
+    constexpr int NV = EL / VEC, STAGES = fwd_stages<TX>();
     extern __shared__ __align__(16) uint8_t dyn_f[];
     __shared__ float2 red[64];
     int turn = 0;
@@ -183,7 +184,17 @@ __global__ void __launch_bounds__(VEC == 1 ? 1024 : 256)
     Ring<TX, STAGES, EL> ring(static_cast<uint32_t>(__cvta_generic_to_shared(dyn_f)), x + row * ldx + here,
                               step * ldx);
     TY* dst = y + row * D + here;
+    PairsOf<EL> wv, bv;
     if constexpr (VEC == 8) {
+        wv.fill(1.0f);
+        bv.fill(0.0f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (here + i * cols < D) {
+                if (w) wv.template load<VEC>(i, w + here + i * cols);
+                if (b) bv.template load<VEC>(i, b + here + i * cols);
+            }
+        }
 #pragma unroll
         for (int k = 0; k < STAGES - 1; ++k)
             ring.fetch(row + k * step < N, cols * (int)sizeof(TX), here, D, cols);
@@ -225,7 +236,10 @@ __global__ void __launch_bounds__(VEC == 1 ? 1024 : 256)
         const float rs = rsqrtf(sq * inv + eps);
         const uint64_t rs2 = f2(rs, rs);
 #pragma unroll
-        for (int e = 0; e < EL / 2; ++e) v.v[e] = mul2(v.v[e], rs2);
+        for (int e = 0; e < EL / 2; ++e) {
+            v.v[e] = mul2(v.v[e], rs2);
+            if constexpr (VEC == 8) v.v[e] = fma2(v.v[e], wv.v[e], bv.v[e]);
+        }
         if (live) {
             if (mean && t == 0) {
                 mean[row] = mu;
@@ -234,18 +248,8 @@ __global__ void __launch_bounds__(VEC == 1 ? 1024 : 256)
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = here + i * cols;
-                if (c < D) {                          // weight and bias stay in the L1
-                    if constexpr (VEC == 1) {
-                        v.set(i, fmaf(v.get(i), w ? w[c] : 1.0f, b ? b[c] : 0.0f));
-                    } else {
-                        PairsOf<8> wv, bv;
-                        wv.fill(1.0f);
-                        bv.fill(0.0f);
-                        if (w) wv.template load<8>(0, w + here + i * cols);
-                        if (b) bv.template load<8>(0, b + here + i * cols);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v.v[i * 4 + j] = fma2(v.v[i * 4 + j], wv.v[j], bv.v[j]);
-                    }
+                if (c < D) {
+                    if constexpr (VEC == 1) v.set(i, fmaf(v.get(i), w ? w[c] : 1.0f, b ? b[c] : 0.0f));
                     v.template store<VEC>(i, dst + i * cols);
                 }
             }
@@ -469,7 +473,7 @@ int launch_fwd(const void* x, int64_t ldx, const float* w, const float* b, void*
     const int threads = VEC == 1 ? (tpr > 256 ? tpr : 256) : (tpr > 128 ? tpr : 128);
     const int64_t groups = threads / tpr, need = (N + groups - 1) / groups;
     auto k = tpr == 32 ? fwd_kernel<TX, TY, VEC, EL, true> : fwd_kernel<TX, TY, VEC, EL, false>;
-    const size_t smem = VEC == 8 ? (size_t)Ring<TX, fwd_stages<TX, EL>(), EL>::BYTES * threads : 0;
+    const size_t smem = VEC == 8 ? (size_t)Ring<TX, fwd_stages<TX>(), EL>::BYTES * threads : 0;
     if (int rc = allow_smem(k, smem, "concord_layer_norm_fwd")) return rc;
     // one wave of resident blocks (asked for once per form; the answer is the architecture's)
     static std::atomic<int> resident[8];
@@ -491,8 +495,7 @@ int forward(const void* x, int64_t ldx, const float* w, const float* b, void* y,
             int64_t D, float eps, bool vec, cudaStream_t st) {
     if (!vec) return launch_fwd<TX, TY, 1, 16>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
     if (D <= 512) return launch_fwd<TX, TY, 8, 16>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
-    if (D <= 1024) return launch_fwd<TX, TY, 8, 32>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
-    return launch_fwd<TX, TY, 8, 64>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
+    return launch_fwd<TX, TY, 8, 32>(x, ldx, w, b, y, mean, rstd, N, D, eps, st);
 }
 
 template <typename TX, typename TY>
