@@ -29,6 +29,7 @@
 // alternative adds dq atomically into an fp32 buffer, which is another order of
 // the sums on every run, and a pass to clear and one to round it.
 #include <cuda.h>
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -80,38 +81,49 @@ struct Work {
 };
 
 // The t-th tile of `rows` rows, sequences in order, a sequence's last tile
-// first where `back` (causal queries: the longest first).  Whole warp.
+// first where `back` (causal queries: the longest first).  Whole warp, four
+// sequences a lane.
 __device__ __forceinline__ void find_tile(const Params& P, bool keys, int t, int tiles_bound, int rows, bool back,
                                           Work* w) {
+    constexpr int EACH = 4;
     const int lane = threadIdx.x & 31;
     const int* cu = keys ? P.cuk : P.cuq;
     const int T = keys ? P.Tk : P.Tq;
     int before = 0;
-    for (int b0 = 0; b0 < P.B; b0 += 32) {
-        const int b = b0 + lane;
-        int n = 0, s = 0, len = 0;
-        if (b < P.B) {
-            s = min(max(cu[b], 0), T);
-            len = min(max(cu[b + 1], s), T) - s;
-            n = (len + rows - 1) / rows;
+    for (int b0 = 0; b0 < P.B; b0 += 32 * EACH) {
+        const int b = b0 + lane * EACH;
+        int at[EACH + 1], n[EACH], sum = 0;
+#pragma unroll
+        for (int k = 0; k <= EACH; ++k) at[k] = min(max(b + k <= P.B ? cu[b + k] : INT_MAX, 0), T);
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            n[k] = b + k < P.B ? (max(at[k + 1] - at[k], 0) + rows - 1) / rows : 0;
+            sum += n[k];
         }
-        int incl = n;
+        int incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        const int lo = before + incl - n;
-        const bool mine = t >= lo && t < lo + n;
+        int lo = before + incl - sum;
+        const bool mine = t >= lo && t < lo + sum;
         if (mine) {
             const int* other = keys ? P.cuq : P.cuk;
             const int To = keys ? P.Tq : P.Tk;
-            const int so = min(max(other[b], 0), To), lo2 = min(max(other[b + 1], so), To) - so;
-            w->q0 = keys ? so : s;
-            w->lq = keys ? lo2 : len;
-            w->k0 = keys ? s : so;
-            w->lk = keys ? len : lo2;
-            w->tile = back ? n - 1 - (t - lo) : t - lo;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                if (t >= lo && t < lo + n[k]) {
+                    const int s = at[k], len = max(at[k + 1] - s, 0);
+                    const int so = min(max(other[b + k], 0), To), lo2 = max(min(max(other[b + k + 1], 0), To) - so, 0);
+                    w->q0 = keys ? so : s;
+                    w->lq = keys ? lo2 : len;
+                    w->k0 = keys ? s : so;
+                    w->lk = keys ? len : lo2;
+                    w->tile = back ? n[k] - 1 - (t - lo) : t - lo;
+                }
+                lo += n[k];
+            }
         }
         if (__any_sync(0xffffffffu, mine)) return;
         before += __shfl_sync(0xffffffffu, incl, 31);

@@ -50,15 +50,19 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-// a backward that may run once: its results refuse to be differentiated
+// A gradient that has no gradient itself: where the upstream one would pass on
+// a second derivative, the results get a node that says so when it is reached
+// (which DelayedError attaches to inputs that require a gradient only).
 variable_list once(variable_list grads, const variable_list& upstream) {
     if (!at::GradMode::is_enabled()) return grads;
-    for (const Tensor& g : upstream)
-        if (wants_grad(g))
-            return torch::autograd::DelayedError(
-                "trying to differentiate twice a function that was marked with @once_differentiable",
-                (int64_t)grads.size())(variable_list(grads));
-    return grads;
+    bool second = false;
+    for (const Tensor& g : upstream) second |= wants_grad(g);
+    if (!second) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g.set_requires_grad(true);
+    return torch::autograd::DelayedError(
+        "trying to differentiate twice a function that was marked with @once_differentiable",
+        (int64_t)grads.size())(std::move(grads));
 }
 
 template <typename Node, typename... In> std::shared_ptr<Node> link(const In&... in) {

@@ -101,7 +101,8 @@ def check(q, k, v, do, cu, cuk=None, causal=True, scale=None):
 
 # lengths of one and none, around the tiles of 128 and 256 rows, and several of them
 @pytest.mark.parametrize("lens", [[1], [2, 1, 1], [127], [128], [129], [255, 1], [256, 257], [0, 5, 0, 0, 300, 0],
-                                  [640], [64] * 37, [1] * 70, [1000, 3, 513]])
+                                  [640], [64] * 37, [1] * 70, [1000, 3, 513], [1, 0, 2, 5] * 90,
+                                  [0] * 300 + [140, 3]])
 @pytest.mark.parametrize("causal", [True, False])
 def test_lengths(lens, causal):
     check(*inputs(sum(lens), 2, 2, 64, seed=len(lens)), cum(lens), causal=causal)
