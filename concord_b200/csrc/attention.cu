@@ -217,6 +217,10 @@ __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f,
 // 128 there is no room, P_i takes the first 64 columns of S_i once they have
 // been read, and the next S waits for P V.  The product P V begins with the
 // first 64 keys while the exponentials of the others still run.
+// Bound by the chain of a tile, S -> softmax -> P V -> next S, of which two run
+// against each other (2900 cycles a pair of 128 x 128 blocks, 2048 of products);
+// short sequences by a block's start and end.  8 x 2048 tokens, 16 heads of 128,
+// causal: 192 us, 716 TFLOP/s; one sequence of 8191: 253 us, 1087 TFLOP/s.
 template <int DP> struct Fwd {
     static constexpr int TILE = 256 * DP;               // bytes of 128 rows
     static constexpr int ST = DP == 128 ? 5 : 8;        // ring of K and V tiles
@@ -520,6 +524,9 @@ done:
 // A block owns 128 query rows of one head.  Tensor memory: S 0, dP 128, dQ
 // 256, dS (16-bit pairs) 384.  S and dP of the next key block are computed as
 // soon as the softmax warps have read the present ones.
+// Bound by the softmax warps (1970 cycles a block, 1024 of exponentials) beside
+// 1536 cycles of products.  8 x 2048, 16 heads of 128, causal: 240 us, 860
+// TFLOP/s of its three products.
 template <int DP> struct BwdQ {
     static constexpr int TILE = 256 * DP;
     static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 128 ? 2 : 4;
@@ -782,6 +789,10 @@ done:
 // subtract them themselves: one more step of 16, a row of ones against the
 // value in three 16-bit parts (24 bits of it).  The order of the products, dV, next S, dK,
 // next dP, lets the exponentials run beside dK and dP, and ds beside dV and S.
+// Bound by the chain P -> dV -> next S -> exponentials (about 2900 cycles a
+// block) and by shared memory, which S and dP read at its full rate: 2048 cycles
+// of products.  8 x 2048, 16 heads of 128, causal: 303 us, 907 TFLOP/s of its
+// four products.
 template <int DP> struct BwdK {
     static constexpr int TILE = 256 * DP;
     static constexpr int QS = DP == 128 ? 2 : 3, OS = DP == 128 ? 2 : 3;

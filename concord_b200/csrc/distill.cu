@@ -13,7 +13,10 @@
 // Bound by memory, near the rate of the exponentials: a row is read once for
 // its maximum and sums (one running maximum, one or two sums), and once more
 // while it is still in the L2 to write dz, so the HBM sees z once and dz once.
-// Where T is a power of two, exp(z) is exp(z / T) squared log2(T) times
+// 16384 x 32000 bf16, T = 2, value and gradient: 500 us, 4.2 TB/s, the
+// special-function unit 64 % busy (256 threads a row, four 16-byte loads each on
+// their way; 512 threads 729 us, 128 518, two loads 539).
+// Where T is 2, 4 or 8, exp(z) is exp(z / T) squared log2(T) times
 // (relative error T times that of one exponential), which halves the
 // exponentials.  A row belongs to 32 to 1024 threads of a block, by its
 // length.  The K teacher entries and the label touch few places of dz: their

@@ -6,10 +6,10 @@
 //
 // Bound by memory: the forward reads x and writes y once, the backward reads
 // x and dy and writes dx once.  A row stays in the registers of the threads
-// that own it (16 elements each: 32 threads up to 512 columns, 1024 at the
-// largest width), so the variance is the mean of squared deviations from the
-// finished mean and nothing is read twice.  The grid is one wave of resident
-// blocks that walk the rows; each thread keeps its columns' weight, and in the
+// that own it (16 elements each, 32 in the forward above 512 columns), so the
+// variance is the mean of squared deviations from the finished mean and nothing
+// is read twice.  The grid is one wave of resident blocks that walk the rows;
+// each thread keeps its columns' weight and bias, and in the
 // backward its columns' sums of dy xh and dy, from row to row.  Rows whose
 // pieces are 16 bytes come through a ring in shared memory, three rows ahead
 // of their use: a thread copies only what it reads itself, so the ring needs no
@@ -164,7 +164,7 @@ template <typename TX> constexpr int fwd_stages() { return sizeof(TX) == 4 ? 3 :
 // row, 135 us (25 instructions an element, half of them the two sums); 64, one
 // warp a row, weight and bias from the L1, 125 us (90 without them: the L1
 // gives 128 bytes a cycle, they are 8 an element); 32 in registers, two warps a
-// row, 105 us.  ONE: a row is one warp's (the columns' distances are constants).
+// row, 105 us (5.1 TB/s).  ONE: a row is one warp's (the columns' distances are constants).
 template <typename TX, typename TY, int VEC, int EL, bool ONE>
 __global__ void __launch_bounds__(VEC == 1 ? 1024 : 512)
     fwd_kernel(const TX* __restrict__ x, int64_t ldx, const float* __restrict__ w, const float* __restrict__ b,
@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(VEC == 1 ? 1024 : 512)
     }
 }
 
+// 65533 x 2048 bf16: 152 us, 5.3 TB/s of x, dy and dx (82 % of a plain copy's
+// rate); issue slots 59 %.
 // dx, and this block's column sums to part[block][0: dy xh, 1: dy][D].  WIDE
 // (above 8192 columns, 1024 threads of at most 64 registers): the column sums
 // live in the thread's own shared-memory slots instead of its registers.
