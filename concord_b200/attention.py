@@ -32,7 +32,9 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     log-sum-exp [H, T] (not differentiable).  Scores, sums and lse are fp32;
     the probabilities and their gradients are rounded to the inputs' type for
     their products with v, k and q.  Differentiable once, without atomics: the
-    same bits on every run.
+    same bits on every run.  A call that is differentiated keeps q, k, v, o, lse
+    and what o's rounding left over (as large as o); few keys with shared heads
+    take an fp32 workspace in the backward.
     """
     _ops.need_cuda(("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k))
     _ops.need_type("q", q, _HALVES)
