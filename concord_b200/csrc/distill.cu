@@ -318,16 +318,18 @@ __global__ void __launch_bounds__(1024) row_kernel(const Args A) {
 
         // ---- loss of the row, by its first warp ----
         if ((MODE & 1) && t < 32) {
-            const float lse = R.m / A.temp + logf(R.s);
+            // differences from the maximum first here too: added to log(sum), a
+            // maximum of 1e4 would leave 1e-3 of a loss that may be no larger
+            const float logs = logf(R.s);
             float cross = 0.f;           // sum_k p_k (lse(z / T) - z_k / T)
             for (int k = lane; counts && k < K; k += 32)
-                if (pid[k] >= 0 && !(prob[k] == 0.f)) cross += prob[k] * (lse - at_id[k] / A.temp);
+                if (pid[k] >= 0 && !(prob[k] == 0.f)) cross += prob[k] * (logs + (R.m - at_id[k]) / A.temp);
             cross = warp_sum(cross);
             if (live && lane == 0) {
                 float loss = 0.f;
                 if (counts) {
                     if (has != 0.f) loss = A.alpha * A.temp * A.temp * (plogp + cross);
-                    if (A.labels) loss += (1.f - A.alpha) * (R.m + logf(R.s1) - zy);
+                    if (A.labels) loss += (1.f - A.alpha) * (logf(R.s1) + (R.m - zy));
                 }
                 A.row_loss[row] = loss;
                 if (A.row_counts) A.row_counts[row] = counts ? 1.f : 0.f;
