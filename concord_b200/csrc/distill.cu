@@ -495,14 +495,16 @@ extern "C" int concord_distill_loss(const concord_distill_params* p, const void*
                                     float* row_loss, float* stats, void* dz, int64_t N, int64_t V, int64_t K,
                                     void* workspace, size_t workspace_bytes, void* stream) {
     const char* name = "concord_distill_loss";
-    if (!p || (!loss && !row_loss)) return fail(CONCORD_EINVAL, "concord_distill_loss: null pointer");
+    // (a tensor of no rows has no address)
+    if (!p || (!loss && !row_loss && N != 0)) return fail(CONCORD_EINVAL, "concord_distill_loss: null pointer");
     distill::Args A = distill::make_args(p, z, ldz, ids, t, labels, N, V, K);
     if (int rc = distill::check(name, A, z_type)) return rc;
     if (!workspace || workspace_bytes < concord_distill_workspace_bytes(N))
         return fail(CONCORD_EWORKSPACE, "concord_distill_loss: workspace too small");
     cudaStream_t st = as_stream(stream);
     if (N == 0) {
-        if (loss) cudaMemsetAsync(loss, 0, sizeof(float), st);
+        if (!loss) return CONCORD_OK;
+        cudaMemsetAsync(loss, 0, sizeof(float), st);
         return check_launch(name);
     }
     int* counts = static_cast<int*>(workspace);

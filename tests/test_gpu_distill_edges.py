@@ -46,3 +46,13 @@ def test_cross_entropy_of_confident_rows(offset):
     ref = -torch.log_softmax(z.double(), 1).gather(1, y[:, None])[:, 0]
     assert 1e-4 < float(ref.min()) and float(ref.max()) < 1e-2
     assert float((rows.double() - ref).abs().max()) <= 32 * 2.0 ** -24
+
+
+def test_no_rows():
+    from concord_b200 import distill_loss
+    z, ids, t, y = (x[:0] for x in _grid(2, 70, 0))
+    z.requires_grad_()
+    rows = distill_loss(z, ids, t, y, 2.0, 0.5, reduction="none")
+    assert rows.shape == (0,)
+    (dz,) = torch.autograd.grad(rows, z, torch.zeros(0, device=DEV))
+    assert dz.shape == (0, 70)

@@ -1,0 +1,27 @@
+"""CPU-only checks of the training operators' C entries at the ends of their ranges: what they answer before anything
+reaches a device."""
+import ctypes
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from concord_b200 import _abi, build
+    build.build()
+    return _abi.load()
+
+
+ONE = ctypes.c_void_p(16)
+
+
+def _loss(lib, N=4, V=8, K=2, ldz=None, loss=ONE, row_loss=None):
+    from concord_b200 import _abi
+    p = _abi.DistillParams(temperature=1.0, alpha=1.0, grad_scale=1.0)
+    return lib.concord_distill_loss(p, ONE, 0, ldz or V, ONE, ONE, None, loss, row_loss, None, None, N, V, K, ONE, 10 ** 6,
+                                    None)
+
+
+def test_a_loss_per_row_of_no_rows_has_no_address(lib):
+    assert _loss(lib, N=0, loss=None) == 0
+    assert _loss(lib, N=1, loss=None) == -1
