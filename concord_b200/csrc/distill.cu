@@ -33,6 +33,7 @@ namespace distill {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_K = 512;
+constexpr int MAX_V = INT32_MAX - 1024;      // a thread's column and the next one of its 1024 neighbours' fit 32 bits
 constexpr int COUNT_BLOCKS = 128;
 
 struct Args {
@@ -462,8 +463,9 @@ int run(Args& A, int32_t type, cudaStream_t st, const char* name) {
 
 int check(const char* name, const Args& A, int32_t type) {
     if (type < 0 || type > 2) return fail(CONCORD_EINVAL, std::string(name) + ": unknown element type");
-    if (A.N < 0 || A.V <= 0 || A.K <= 0 || A.ldz < A.V || A.V > INT32_MAX)
+    if (A.N < 0 || A.V <= 0 || A.K <= 0 || A.ldz < A.V)
         return fail(CONCORD_ESHAPE, std::string(name) + ": bad extents or row stride");
+    if (A.V > MAX_V) return fail(CONCORD_ETOOBIG, std::string(name) + ": more than 2^31 - 1025 columns");
     if (A.K > MAX_K) return fail(CONCORD_ETOOBIG, std::string(name) + ": more than 512 teacher entries");
     if (!(A.temp > 0.f) || !(A.temp <= FLT_MAX)) return fail(CONCORD_EINVAL, std::string(name) + ": temperature must be positive");
     if (A.N > 0 && (!A.z || !A.ids || !A.t)) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");

@@ -25,3 +25,13 @@ def _loss(lib, N=4, V=8, K=2, ldz=None, loss=ONE, row_loss=None):
 def test_a_loss_per_row_of_no_rows_has_no_address(lib):
     assert _loss(lib, N=0, loss=None) == 0
     assert _loss(lib, N=1, loss=None) == -1
+
+
+@pytest.mark.parametrize("V", [2 ** 31 - 1024, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
+def test_rows_beyond_32_bits_of_columns_are_refused(lib, V):
+    """A thread steps from column to column by up to 1024: beyond these widths the step would pass 32 bits and the
+    gradient be written in front of its tensor."""
+    assert _loss(lib, V=V) == -7
+    from concord_b200 import _abi
+    p = _abi.DistillParams(temperature=1.0, alpha=1.0, grad_scale=1.0)
+    assert lib.concord_distill_grad(p, ONE, 0, V, ONE, ONE, None, ONE, None, 0, ONE, 4, V, 2, None) == -7
