@@ -341,10 +341,12 @@ __global__ void __launch_bounds__(WIDE ? 1024 : 512)
         }
         xr.next();
         yr.next();
-        const uint64_t rs2 = f2(rs, rs), mr2 = f2(-mu * rs, -mu * rs);
+        // (x - mean first, as in the forward: the rounding of mean * rstd would
+        // give rows far off centre a deviation that they do not have)
+        const uint64_t rs2 = f2(rs, rs), mu2 = f2(-mu, -mu);
 #pragma unroll
         for (int e = 0; e < PER / 2; ++e) {
-            xh.v[e] = fma2(xh.v[e], rs2, mr2);
+            xh.v[e] = mul2(add2(xh.v[e], mu2), rs2);
             if constexpr (WIDE) {
                 float ga, gb, xa, xb;
                 unf2(g.v[e], ga, gb);
