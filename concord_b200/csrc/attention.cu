@@ -803,28 +803,15 @@ template <int DP> struct BwdK {
     static constexpr size_t SMEM = STAT + 4 * THIN + 1024;
 };
 
-// What the ones are, and a value's parts against them.  fp16 cannot hold what
-// lse / scale may be (scores before scaling), so its ones are 2^15, 2^4 and
-// 2^-7: values up to 2^31, each part 11 bits of what the one before left.
-template <typename T> struct Parts;
-template <> struct Parts<__nv_bfloat16> {
-    static __device__ __forceinline__ uint4 ones() { return make_uint4(0x3f803f80u, 0x3f80u, 0, 0); }
-    static __device__ __forceinline__ uint4 of(float v) {
-        const float a = __bfloat162float(__float2bfloat16_rn(v)), b = __bfloat162float(__float2bfloat16_rn(v - a));
-        return make_uint4(pack2(a, b, __nv_bfloat16()), pack2(v - a - b, 0.f, __nv_bfloat16()), 0, 0);
-    }
-};
-template <> struct Parts<__half> {
-    static __device__ __forceinline__ uint4 ones() {
-        return make_uint4(pack2(32768.f, 16.f, __half()), pack2(1.f / 128.f, 0.f, __half()), 0, 0);
-    }
-    static __device__ __forceinline__ uint4 of(float v) {
-        v = fminf(fmaxf(v, -2.1e9f), 2.1e9f);
-        const float a = __half2float(__float2half_rn(v * (1.f / 32768.f))), r = v - a * 32768.f;
-        const float b = __half2float(__float2half_rn(r * (1.f / 16.f)));
-        return make_uint4(pack2(a, b, __half()), pack2((r - b * 16.f) * 128.f, 0.f, __half()), 0, 0);
-    }
-};
+// A value's parts against the ones: three of 8 bits each, in bf16 for fp16
+// operands too (an instruction's operands have one type, but the step of 16 that
+// holds these is an instruction of its own): lse / scale is a score before
+// scaling, which fp16 does not hold.  NaN comes through, an infinity as NaN.
+__device__ __forceinline__ uint4 parts_ones() { return make_uint4(0x3f803f80u, 0x3f80u, 0, 0); }
+__device__ __forceinline__ uint4 parts_of(float v) {
+    const float a = __bfloat162float(__float2bfloat16_rn(v)), b = __bfloat162float(__float2bfloat16_rn(v - a));
+    return make_uint4(pack2(a, b, __nv_bfloat16()), pack2(v - a - b, 0.f, __nv_bfloat16()), 0, 0);
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -871,7 +858,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint4 z = make_uint4(0, 0, 0, 0);
         for (int i = threadIdx.x - 128; i < 5 * 256; i += 256) {
             const uint32_t at = base + C::ONES + (i >> 8) * THIN + (i & 255) * 16;
-            sts16(at, (i < 256 && !(i & 8)) ? Parts<T>::ones() : z);
+            sts16(at, (i < 256 && !(i & 8)) ? parts_ones() : z);
         }
         fence_async();
     }
@@ -920,7 +907,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!mbar_wait(o_empty((n - 1 - x) % OS), ((n - 1 - x) / OS) & 1, P.err, 44)) goto done;
         }
     } else if (warp == 1) {
-        constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_D = instr_desc(BF, DP, 1);
+        constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_D = instr_desc(BF, DP, 1), ID_STAT = instr_desc(1, 128, 0);
         const uint32_t el = elect_one(), tm = uniform(tmem), sm = uniform(base);
         const int nu = uniform(n), per = uniform(nq), left = uniform(w.lq - jq * 128);
         const uint64_t dk = desc_k(sm), dv = desc_k(sm + TILE), dq = desc_k(sm + C::Q_OFF), ddo = desc_k(sm + C::O_OFF),
@@ -940,7 +927,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t b = dq + sq * (TILE >> 4);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm, dk + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
-            mma_ss(tm, ones, stat + ss * (2 * THIN >> 4), ID_S, 1, el);
+            mma_ss(tm, ones, stat + ss * (2 * THIN >> 4), ID_STAT, 1, el);
             mma_commit(s_full, el);
             ss ^= 1;
             if (ss == 0) ps ^= 1;
@@ -957,7 +944,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t b = ddo + so * (TILE >> 4);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) mma_ss(tm + 128, dv + step_k(kk), b + step_k(kk), ID_S, kk != 0, el);
-            mma_ss(tm + 128, ones, stat + (2 * sp + 1) * (THIN >> 4), ID_S, 1, el);
+            mma_ss(tm + 128, ones, stat + (2 * sp + 1) * (THIN >> 4), ID_STAT, 1, el);
             mma_commit(dp_full, el);
             mma_commit(st_empty(sp), el);
             sp ^= 1;
@@ -1028,8 +1015,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int k = 0; k < 2; ++k) {
                 const uint32_t at = base + C::STAT + 2 * s * THIN + thin_row(i + k * 64);
                 // no such row, or one without keys: far below every score, so p = 0
-                sts16(at, Parts<T>::of(l[k] == -INFINITY ? -1e30f : l[k] * unscale));
-                sts16(at + THIN, Parts<T>::of(-d[k]));
+                sts16(at, parts_of(l[k] == -INFINITY ? -1e30f : l[k] * unscale));
+                sts16(at + THIN, parts_of(-d[k]));
             }
             fence_async();
             mbar_arrive(st_full(s));
