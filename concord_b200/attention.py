@@ -31,10 +31,12 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     Returns o [T, H, D], contiguous, and with return_lse also the fp32
     log-sum-exp [H, T] (not differentiable).  Scores, sums and lse are fp32;
     the probabilities and their gradients are rounded to the inputs' type for
-    their products with v, k and q.  Differentiable once, without atomics: the
+    their products with v, k and q (in fp16's backward after scaling by powers
+    of two, so that neither many keys nor small upstream gradients take them
+    below fp16's range).  Differentiable once, without atomics: the
     same bits on every run.  A call that is differentiated keeps q, k, v, o, lse
-    and what o's rounding left over (as large as o); few keys with shared heads
-    take an fp32 workspace in the backward.
+    and what o's rounding left over (as large as o); the backward takes an fp32
+    workspace for few keys with shared heads, and a small one in fp16.
     """
     _ops.need_cuda(("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k))
     _ops.need_type("q", q, _HALVES)

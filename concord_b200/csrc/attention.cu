@@ -69,6 +69,13 @@ struct Params {
     void *dq, *dk, *dv;
     float* part;          // splits > 1: [splits][dk, dv][Tk, key heads, D] in fp32
     int splits, per;      // parts of a key head's query heads, and heads of a part
+    // fp16 backward (see lift): v, the largest |v| of each part of a sequence's keys
+    // [B][key heads][chunks], and the largest sum of |dout| of a row [B][H]
+    const void* v;
+    int64_t v_ts, v_hs;
+    float* vmax;
+    int chunks;
+    int* dmax;            // (fp32 of no sign, ordered as whole numbers)
     int* err;
 };
 
@@ -78,6 +85,7 @@ struct Work {
     int tile;             // -1: none left; then `spare` of `spares` blocks zero the rows of no sequence
     int spare, spares;
     int first, last;      // rows [0, first) and [last, T) belong to no sequence
+    int seq;              // its number
 };
 
 // The t-th tile of `rows` rows, sequences in order, a sequence's last tile
@@ -120,6 +128,7 @@ __device__ __forceinline__ void find_tile(const Params& P, bool keys, int t, int
                     w->lq = keys ? lo2 : len;
                     w->k0 = keys ? s : so;
                     w->lk = keys ? len : lo2;
+                    w->seq = b + k;
                     w->tile = back ? n[k] - 1 - (t - lo) : t - lo;
                 }
                 lo += n[k];
@@ -520,6 +529,66 @@ done:
     }
 }
 
+// ---------------------------------------------------------------- the range of fp16
+// ds = p (dp - delta) is far smaller than its sums where keys are many or
+// gradients small: 4096 keys and upstream gradients of 1e-5 give 2e-9, and fp16
+// ends at 6e-8.  So in fp16 p is held times 2^12 in dk / dv (exponents + 12),
+// and ds times a power of two that cannot take it past 2^12 (16 times below the
+// largest number): |dp| and |delta| are at most max|v| times the row's sum of
+// |do|.  The factor goes by the row in dq, by the sequence and the key head's
+// query heads in dk, so no other sequence has a part in it; it is never below 1,
+// and the results are divided by it in fp32.  bf16 has fp32's range.
+constexpr float P_LIFT = 4096.f, P_LIFT_LOG2 = 12.f;
+__device__ __forceinline__ float lift(float l1, float vmax) {
+    const float bound = 2.f * l1 * vmax;
+    if (!(bound > 0.f && bound < 2048.f)) return 1.f;        // (NaN, infinities and zeros too)
+    return __uint_as_float((uint32_t)(127 + 11 + 127) * (1u << 23) - (__float_as_uint(bound) & 0x7f800000u));
+}
+__device__ __forceinline__ float largest_v(const Params& P, int seq, int kvh) {       // (whole warp)
+    const float* at = P.vmax + ((int64_t)seq * (P.H / P.G) + kvh) * P.chunks;
+    const int lane = threadIdx.x & 31;
+    return warp_maxf(lane < P.chunks ? at[lane] : 0.f);
+}
+
+// vmax, and zeros to dmax: a block takes a chunk of a sequence's keys of one
+// head, 16 or 32 rows a step, eight 16-byte loads of a thread on their way.
+// Reads v once more: 15 us beside 520 (8 x 2048 tokens, 16 heads of 128), 7
+// beside 780 (8191 tokens, 4 key heads).
+__global__ void __launch_bounds__(256) range_kernel(const __grid_constant__ Params P) {
+    __shared__ float red[8];
+    const int HK = P.H / P.G, c = blockIdx.x % P.chunks, kvh = blockIdx.x / P.chunks % HK, b = blockIdx.x / P.chunks / HK;
+    if (c == 0)
+        for (int i = threadIdx.x; i < P.G; i += 256) P.dmax[b * P.H + kvh * P.G + i] = 0;
+    const int k0 = min(max(P.cuk[b], 0), P.Tk), lk = max(min(max(P.cuk[b + 1], 0), P.Tk) - k0, 0);
+    const int rows = (lk + P.chunks - 1) / P.chunks, first = min((int64_t)c * rows, (int64_t)lk), left = min(rows, lk - first);
+    const int wide = P.D > 64, step = wide ? 16 : 32, row = threadIdx.x >> (wide ? 4 : 3),
+              col = (threadIdx.x & (wide ? 15 : 7)) * 8;
+    const __half* v = static_cast<const __half*>(P.v) + ((int64_t)k0 + first + row) * P.v_ts + kvh * P.v_hs + col;
+    float m = 0.f;
+    if (col < P.D) {
+        for (int r = row; r < left; r += 8 * step, v += 8 * step * P.v_ts) {
+            uint4 u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                u[k] = r + k * step < left ? *reinterpret_cast<const uint4*>(v + k * step * P.v_ts) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float x[8];
+                Pack16<__half>::unpack(u[k], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+            }
+        }
+    }
+    m = warp_maxf(m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+        P.vmax[blockIdx.x] = m;
+    }
+}
+
 // ---------------------------------------------------------------- backward: dq and delta
 // A block owns 128 query rows of one head.  Tensor memory: S 0, dP 128, dQ
 // 256, dS (16-bit pairs) 384.  S and dP of the next key block are computed as
@@ -532,7 +601,7 @@ template <int DP> struct BwdQ {
     static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 128 ? 2 : 4;
     static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + KS * TILE;
     static constexpr int BARS = V_OFF + VS * TILE;
-    static constexpr int RED = BARS + 512;                     // 256 halves of delta
+    static constexpr int RED = BARS + 512;                     // delta, and (fp16) the sum of |do|, of 128 rows
     static constexpr size_t SMEM = RED + 1024 + 1024;
 };
 
@@ -693,15 +762,24 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
 #pragma unroll
             for (int k = 0; k < NL; ++k) {
-                float gv[8], ov[8], ev[8], d = 0.f;
+                float gv[8], ov[8], ev[8], d = 0.f, a = 0.f;
                 Pack16<T>::unpack(g[k], gv);
                 Pack16<T>::unpack(o[k], ov);
                 Pack16<T>::unpack(e[k], ev);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d = fmaf(gv[i], ov[i] + ev[i], d);
+                for (int i = 0; i < 8; ++i) {
+                    d = fmaf(gv[i], ov[i] + ev[i], d);
+                    if (!BF) a += fabsf(gv[i]);
+                }
 #pragma unroll
-                for (int i = CH / 2; i > 0; i >>= 1) d += __shfl_xor_sync(0xffffffffu, d, i);
-                if (lane % CH == 0) red[(warp - 4) * 16 + k * AT + sub] = d;
+                for (int i = CH / 2; i > 0; i >>= 1) {
+                    d += __shfl_xor_sync(0xffffffffu, d, i);
+                    if (!BF) a += __shfl_xor_sync(0xffffffffu, a, i);
+                }
+                if (lane % CH == 0) {
+                    red[(warp - 4) * 16 + k * AT + sub] = d;
+                    if (!BF) red[128 + (warp - 4) * 16 + k * AT + sub] = a;
+                }
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -709,8 +787,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (live && half == 0) P.delta[(int64_t)head * P.Tq + trow] = d;
         float lse = live ? P.lse[(int64_t)head * P.Tq + trow] : 0.f;
         if (lse == -INFINITY) lse = 0.f;           // no key: everything is masked below
+        float up = 1.f;                            // fp16: ds is held times this
+        if (!BF) {
+            const float a = red[128 + r];
+            up = lift(a, largest_v(P, w.seq, kvh));
+            const float most = warp_maxf(live ? a : 0.f);
+            if (half == 0 && lane == 0) atomicMax(P.dmax + w.seq * P.H + head, __float_as_int(most));
+        }
         const float l2 = -lse * LOG2E;
-        const uint64_t c2 = f2(P.scale2, P.scale2), l22 = f2(l2, l2), nd2 = f2(-d, -d);
+        const uint64_t c2 = f2(P.scale2, P.scale2), l22 = f2(l2, l2), nd2 = f2(-d * up, -d * up), up2 = f2(up, up);
         const int mine = (P.causal ? min(w.lk, row + off + 1) : w.lk) - half * 64;
         const int every = P.causal ? min(w.lk, r0 + off + 1) : w.lk;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -742,7 +827,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     unf2(fma2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2, l22), a, b);
                     a = ex2f(a);
                     b = ex2f(b);
-                    unf2(mul2(f2(a, b), add2(f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), nd2)), a, b);
+                    const uint64_t dp = f2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                    unf2(mul2(f2(a, b), BF ? add2(dp, nd2) : fma2(dp, up2, nd2)), a, b);
                     if (mask && j * 128 + k >= mine) a = 0.f;
                     if (mask && j * 128 + k + 1 >= mine) b = 0.f;
                     u[k >> 1] = pack2(a, b, T());
@@ -761,7 +847,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!mbar_wait(ds_free, (n - 1) & 1, P.err, 35)) goto done;
             fence_after();
             const int64_t stride = (int64_t)P.H * P.D;
-            store_rows<T, DP / 2>(tmem + lanes + 256 + half * (DP / 2), base + half * TILE + q * (TILE / 8), P.scale,
+            store_rows<T, DP / 2>(tmem + lanes + 256 + half * (DP / 2), base + half * TILE + q * (TILE / 8), P.scale / up,
                                   dst - lane * stride, stride, half * (DP / 2), P.D, w.lq - (row - lane));
         } else if (live) {
             for (int x = half * 8; x < P.D; x += 16) *reinterpret_cast<uint4*>(dst + x) = make_uint4(0, 0, 0, 0);
@@ -874,7 +960,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int first = P.causal ? max(0, k0 - off) : 0;
         if (first < w.lq) { jq = first / 128; nq = (w.lq + 127) / 128 - jq; }
     }
-    const int n = nq * min(P.per, P.G - part * P.per);
+    const int heads = min(P.per, P.G - part * P.per), n = nq * heads;
     const int64_t all = (int64_t)P.Tk * HK * P.D;
     float* dkp = P.part + 2 * all * part;                            // splits > 1
 
@@ -1028,7 +1114,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int key = k0 + q * 32 + lane;
         const bool live = key < w.lk;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const uint64_t c2 = f2(P.scale2, P.scale2);
+        const uint64_t c2 = f2(P.scale2, P.scale2), lift2 = f2(P_LIFT_LOG2, P_LIFT_LOG2);
+        float up = 1.f;                            // fp16: ds is held times this, p times P_LIFT
+        if (!BF && n > 0) {
+            int most = 0;
+            for (int h = 0; h < heads; ++h) most = max(most, P.dmax[w.seq * P.H + head0 + h]);
+            up = lift(__int_as_float(most), largest_v(P, w.seq, kvh));
+        }
+        const uint64_t up2 = f2(up / P_LIFT, up / P_LIFT);
         for (int x = 0; x < n; ++x) {
             const int row0 = (jq + x % nq) * 128 + half * 64;
             // the first query of this half that sees the key, as a column
@@ -1044,7 +1137,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 64; k += 2) {
                 float a, b;
-                unf2(mul2(f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), c2), a, b);
+                const uint64_t s = f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1]));
+                unf2(BF ? mul2(s, c2) : fma2(s, c2, lift2), a, b);
                 p[k] = ex2f(a);
                 p[k + 1] = ex2f(b);
             }
@@ -1065,8 +1159,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
             wait_ld();
 #pragma unroll
-            for (int k = 0; k < 64; k += 2)
-                unf2(mul2(f2(p[k], p[k + 1]), f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1]))), p[k], p[k + 1]);
+            for (int k = 0; k < 64; k += 2) {
+                const uint64_t ds = mul2(f2(p[k], p[k + 1]), f2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])));
+                unf2(BF ? ds : mul2(ds, up2), p[k], p[k + 1]);
+            }
             if (masked) {
 #pragma unroll
                 for (int k = 0; k < 64; ++k)
@@ -1084,8 +1180,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto store = [&](auto* dk, auto* dv) {
             using O = std::remove_pointer_t<decltype(dk)>;
             const uint32_t stage = base + half * TILE + q * (TILE / 16 * sizeof(O));
-            store_rows<O, DP / 2>(tmem + lanes + 256 + col, stage, 1.0f, dv + at, stride, col, P.D, rows);
-            store_rows<O, DP / 2>(tmem + lanes + 256 + DP + col, stage, P.scale, dk + at, stride, col, P.D, rows);
+            store_rows<O, DP / 2>(tmem + lanes + 256 + col, stage, BF ? 1.0f : 1.0f / P_LIFT, dv + at, stride, col, P.D, rows);
+            store_rows<O, DP / 2>(tmem + lanes + 256 + DP + col, stage, P.scale / up, dk + at, stride, col, P.D, rows);
         };
         auto clear = [&](auto* dk, auto* dv) {
             constexpr int E = 16 / sizeof(*dk);
@@ -1259,9 +1355,29 @@ int splits_of(int64_t tokens_k, int64_t heads, int64_t kv_heads, int* per) {
     return (int)((G + *per - 1) / *per);
 }
 
+// chunks of a sequence's keys in range_kernel: of about 256 keys, 32 at most (a lane each)
+int chunks_of(int64_t tokens_k, int64_t seqs) {
+    return (int)std::min<int64_t>(32, std::max<int64_t>(1, (tokens_k + 256 * seqs - 1) / (256 * seqs)));
+}
+
+// workspace of the backward: the parts' sums, where the query heads of a key
+// head are split; in fp16 the largest |v| and rows of dout behind them
+struct Space {
+    size_t vmax, dmax, bytes;
+    int splits, per, chunks;
+    explicit Space(const concord_attention_params* p) {
+        splits = splits_of(p->tokens_k, p->heads, p->kv_heads, &per);
+        vmax = splits > 1 ? (size_t)splits * 2 * p->tokens_k * p->kv_heads * p->head_dim * sizeof(float) : 0;
+        chunks = chunks_of(p->tokens_k, p->seqs);
+        dmax = vmax + (size_t)p->seqs * p->kv_heads * chunks * sizeof(float);
+        bytes = p->type == CONCORD_F16 ? dmax + (size_t)p->seqs * p->heads * sizeof(int) : vmax;
+    }
+};
+
 template <typename T, int DP>
 void launch_bwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& d,
                 const Params& P, cudaStream_t st) {
+    if constexpr (__is_same(T, __half)) range_kernel<<<P.B * (P.H / P.G) * P.chunks, 256, 0, st>>>(P);
     if (P.Tq > 0)
         bwd_q_kernel<T, DP><<<(int)(tiles_bound(P.Tq, P.B, 128) * P.H), THREADS, BwdQ<DP>::SMEM, st>>>(q, k, v, d, P);
     bwd_k_kernel<T, DP><<<(int)(tiles_bound(P.Tk, P.B, 128) * (P.H / P.G) * P.splits), THREADS, BwdK<DP>::SMEM, st>>>(
@@ -1314,12 +1430,9 @@ extern "C" int concord_attention_fwd(const concord_attention_params* p, const vo
     return check_launch(name);
 }
 
-// workspace: the parts' sums, where the query heads of a key head are split
 extern "C" size_t concord_attention_bwd_workspace_bytes(const concord_attention_params* p) {
     if (attn::check("concord_attention_bwd_workspace_bytes", p) != CONCORD_OK || p->tokens_k == 0) return 0;
-    int per = 1;
-    const int splits = attn::splits_of(p->tokens_k, p->heads, p->kv_heads, &per);
-    return splits > 1 ? (size_t)splits * 2 * p->tokens_k * p->kv_heads * p->head_dim * sizeof(float) : 0;
+    return attn::Space(p).bytes;
 }
 
 extern "C" int concord_attention_bwd(const concord_attention_params* p, const void* q, int64_t q_ts, int64_t q_hs,
@@ -1361,8 +1474,16 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
     P.dq = dq;
     P.dk = dk;
     P.dv = dv;
-    P.splits = attn::splits_of(p->tokens_k, p->heads, p->kv_heads, &P.per);
+    const attn::Space space(p);
+    P.splits = space.splits;
+    P.per = space.per;
+    P.chunks = space.chunks;
     P.part = static_cast<float*>(workspace);
+    P.vmax = reinterpret_cast<float*>(static_cast<char*>(workspace) + space.vmax);
+    P.dmax = reinterpret_cast<int*>(static_cast<char*>(workspace) + space.dmax);
+    P.v = v;
+    P.v_ts = v_ts;
+    P.v_hs = v_hs;
     cudaStream_t st = as_stream(stream);
     if (bf) {
         if (p->head_dim <= 64) attn::launch_bwd<__nv_bfloat16, 64>(mq, mk, mv, md, P, st);

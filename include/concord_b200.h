@@ -630,7 +630,7 @@ int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t
  * backward follows) is what o's rounding left over, from which the backward
  * has delta = dout . o to fp32; lse and delta are fp32 [heads, tokens_q], delta
  * being scratch that the backward fills, as is its workspace (16-byte aligned;
- * often of 0 bytes).  concord_attention_error: non-zero
+ * of 0 bytes for bf16 unless query heads are split).  concord_attention_error: non-zero
  * once a barrier wait inside a kernel has run out (2 s of GPU time per wait).
  */
 typedef struct concord_attention_params {

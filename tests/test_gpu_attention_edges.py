@@ -6,9 +6,14 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import DEV, U, check, cum, inputs, run
+from test_gpu_attention import DEV, U, check, cum, inputs, reference, run
 
 pytestmark = pytest.mark.gpu
+
+
+def close(name, got, ref, mag, u, least):
+    err, lim = (got.double() - ref).abs(), u * (ref.abs() + mag) + least
+    assert bool((err <= lim).all()), (name, float((err / lim).max()))
 
 
 @pytest.mark.parametrize("dtype", list(U))
@@ -41,3 +46,62 @@ def test_scores_beyond_two_to_the_31(dtype):
     own.fill_diagonal_(-math.inf)
     assert float(own.max()) < 2.0 ** 32 - 2.0 ** 29
     check(q, q.clone(), v, do, cum([150]), causal=False)
+
+
+def test_fp16_gradients_of_small_upstream_gradients():
+    """4096 keys, upstream gradients of 1e-5: a gradient of one score is of the size 2e-9, below what fp16 holds, and
+    the sums of 4096 of them are not."""
+    g = torch.Generator(device=DEV).manual_seed(24)
+    n = 4096
+    q, v = torch.randn(n, 1, 64, generator=g, device=DEV), torch.randn(n, 1, 64, generator=g, device=DEV)
+    do = q * 1e-5
+    q, v, do = q.half(), v.half(), do.half()
+    k = v.clone()                            # sums that add up: dq follows do, dk follows v
+    got = run(q, k, v, do, cum([n]), causal=False, scale=0.05)
+    ref, mag = reference(q, k, v, do, cum([n]), cum([n]), False, 0.05)
+    assert float(ref["dq"].abs().mean()) > 2.0 ** -22 and float(ref["dk"].abs().mean()) > 2.0 ** -22
+    for name in ("o", "dq", "dk", "dv"):
+        close(name, got[name], ref[name], mag[name], U[torch.float16], 2.0 ** -25)
+
+
+@pytest.mark.parametrize("size", [1e-6, 1.0, 300.0])
+@pytest.mark.parametrize("heads", [(2, 1), (1, 1)])
+def test_fp16_gradients_of_any_size(size, heads):
+    """Sequences whose upstream gradients and values differ by powers of ten, side by side."""
+    lens = [300, 1, 0, 140, 500]
+    q, k, v, do = inputs(sum(lens), *heads, 64, torch.float16, seed=25)
+    do[:300] *= size
+    v[301:441] *= 1e-3
+    cu = cum(lens)
+    for causal in (True, False):
+        got = run(q, k, v, do, cu, causal=causal)
+        ref, mag = reference(q, k, v, do, cu, cu, causal, 0.125)
+        for name in ("o", "dq", "dk", "dv"):
+            close(name, got[name], ref[name], mag[name], U[torch.float16], 2.0 ** -25)
+
+
+def test_fp16_probabilities_of_a_million_keys():
+    q, k, v, do = inputs(8, 1, 1, 64, torch.float16, Tk=1 << 20, seed=26)
+    do = do * 64
+    cu, cuk = cum([8]), cum([1 << 20])
+    got = run(q, k, v, do, cu, cuk, causal=False)
+    ref, mag = reference(q, k, v, do, cu, cuk, False, 0.125)
+    for name in ("o", "dq", "dk", "dv"):
+        close(name, got[name], ref[name], mag[name], U[torch.float16], 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", list(U))
+def test_extreme_neighbours_change_no_bit(dtype):
+    """The range of one sequence is no other's: the same bits beside a sequence, or rows of none, of the largest
+    numbers and of NaN."""
+    q, k, v, do = inputs(300, 2, 1, 64, dtype, seed=27)
+    do = do * 1e-4
+    want = run(q[100:200], k[100:200], v[100:200], do[100:200], cum([100]))
+    for value in (60000.0, math.nan):
+        wild = [t.clone() for t in (q, k, v, do)]
+        for t in wild:
+            t[:100] = value
+            t[200:] = -value
+        for cu in (cum([100, 100, 100]), cum([100]) + 100):
+            got = run(*wild, cu)
+            assert all(torch.equal(got[n][100:200], want[n]) for n in ("o", "dq", "dk", "dv"))
