@@ -251,13 +251,16 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
 }
 
 // ---------------------------------------------------------------- attention
-// t [T, H, D] as the kernels read it (a copy only where its strides or its address do not fit 16-byte rows)
+// t [T, H, D] as the kernels read it (a copy only where its strides or its
+// address do not fit 16-byte rows).  The stride of a dimension of size one says
+// nothing: the dense one is taken for it.
 Tensor operand(const Tensor& t) {
-    if (t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) > 0 && t.stride(1) > 0 &&
+    const int64_t H = t.size(1), D = t.size(2);
+    const int64_t ts = t.size(0) > 1 ? t.stride(0) : H * D, hs = H > 1 ? t.stride(1) : D;
+    if (t.stride(2) == 1 && ts % 8 == 0 && hs % 8 == 0 && ts > 0 && hs > 0 &&
         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
-        return t;
-    Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+        return ts == t.stride(0) && hs == t.stride(1) ? t : t.as_strided(t.sizes(), {ts, hs, 1});
+    return at::empty(t.sizes(), t.options()).copy_(t);
 }
 
 concord_attention_params attention_params(const Tensor& q, const Tensor& k, const Tensor& cu_q, const Tensor& cu_k,

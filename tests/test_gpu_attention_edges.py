@@ -105,3 +105,22 @@ def test_extreme_neighbours_change_no_bit(dtype):
         for cu in (cum([100, 100, 100]), cum([100]) + 100):
             got = run(*wild, cu)
             assert all(torch.equal(got[n][100:200], want[n]) for n in ("o", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_row_or_one_head_of_any_stride(D):
+    """The stride of a dimension of size one says nothing."""
+    g = torch.Generator(device=DEV).manual_seed(28)
+    buf = torch.randn(4, 3000, generator=g, device=DEV).bfloat16()
+    row = lambda i: buf.as_strided((1, 6, D), (1003, D, 1), 3000 * i)  # noqa: E731
+    want = run(*(row(i).clone() for i in range(4)), cum([1]))
+    got = run(*(row(i) for i in range(4)), cum([1]))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    head = lambda i: buf.as_strided((20, 1, D), (136, 3, 1), 3000 * i)  # noqa: E731
+    want = run(*(head(i).clone(memory_format=torch.contiguous_format).view(20, 1, D) for i in range(4)), cum([15, 5]))
+    got = run(*(head(i) for i in range(4)), cum([15, 5]))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    both = lambda i: buf.as_strided((1, 1, D), (5, 7, 1), 3000 * i)  # noqa: E731
+    want = run(*(both(i).clone().view(-1).view(1, 1, D) for i in range(4)), cum([1]))
+    got = run(*(both(i) for i in range(4)), cum([1]))
+    assert all(torch.equal(got[n], want[n]) for n in want)
