@@ -38,7 +38,7 @@ from .packed_b import (  # noqa: F401
     V_SLOW_FACTOR,
     MANTISSA_BIAS,
 )
-from .attention import packed_attention  # noqa: F401
+from .attention import attention_error, packed_attention  # noqa: F401
 from .distill import distill_loss, distill_loss_and_grad  # noqa: F401
 from .norm import LayerNorm, layer_norm  # noqa: F401
 
@@ -60,6 +60,7 @@ __all__ = [
     "V_SLOW_FACTOR",
     "MANTISSA_BIAS",
     "packed_attention",
+    "attention_error",
     "LayerNorm",
     "layer_norm",
     "distill_loss",

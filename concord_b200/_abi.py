@@ -48,7 +48,7 @@ ERRORS = {
     -5: "CUDA launch/runtime error",
     -6: "no usable CUDA device",
     -7: "size above the fixed maximum",
-    -8: "a cross-GPU wait ran out",
+    -8: "a wait ran out",
 }
 
 
@@ -269,6 +269,8 @@ _SIGS = [
      [ctypes.c_size_t, _P]),
     ("concord_attention_bwd_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(AttentionParams)]),
     ("concord_attention_error", ctypes.c_int, [_I32]),
+    ("concord_attention_error_word", ctypes.POINTER(_I32), []),
+    ("concord_attention_wait_check", ctypes.c_int, [_P]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

@@ -7,7 +7,7 @@ them, read in place from the projection's output.
 """
 import torch
 
-from . import _ops
+from . import _abi, _ops
 
 _HALVES = (torch.bfloat16, torch.float16)
 
@@ -37,6 +37,10 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     same bits on every run.  A call that is differentiated keeps q, k, v, o, lse
     and what o's rounding left over (as large as o); the backward takes an fp32
     workspace for few keys with shared heads, and a small one in fp16.
+
+    Waits inside the kernels are bounded (2 s).  If one runs out, the results
+    hold NaN and every later call on the device raises until
+    `attention_error(reset=True)`.
     """
     _ops.need_cuda(("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("cu_seqlens_k", cu_seqlens_k))
     _ops.need_type("q", q, _HALVES)
@@ -70,3 +74,10 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
         raise ValueError(f"scale must be positive, got {scale}")
     o, lse = _ops.native().attention(q, k, v, cus[0], cus[1], causal, scale)
     return (o, lse) if return_lse else o
+
+
+def attention_error(reset=False):
+    """Code of the first wait inside an attention kernel of the current device
+    that ran out, 0 if none did.  Synchronises; `reset` clears it, after which
+    calls are taken again."""
+    return _abi.load().concord_attention_error(int(reset))

@@ -18,9 +18,12 @@
 // a tile that lie beyond its sequence: they belong to another sequence, or to
 // nobody, and 0 * NaN is NaN), warps 4-11 do the softmax arithmetic, one row
 // of 128 a thread in the forward, half a row in the backward.  Every wait on a
-// barrier is bounded (2 s of GPU time): the role then records an error word
-// and stops, the others run out too, and the block frees its tensor memory and
-// returns.
+// barrier is bounded (2 s, see tc.cuh).  Where one runs out the loads and the
+// products stop; the softmax warps go on through their loop on whatever is there
+// (they never branch on a wait: their tcgen05 instructions want whole warps),
+// and the block waits (bounded again) for its loads and products in flight,
+// fills its results with NaN, frees its tensor memory and returns.  The next
+// call finds the host's error word and fails.
 //
 // The backward is two kernels without atomics, so gradients are the same bits
 // on every run: one owns 128 rows of q and walks the keys (dq, and delta), the
@@ -31,6 +34,7 @@
 #include <cuda.h>
 #include <limits.h>
 #include <math.h>
+#include <string.h>
 
 #include <algorithm>
 #include <atomic>
@@ -76,7 +80,8 @@ struct Params {
     float* vmax;
     int chunks;
     int* dmax;            // (fp32 of no sign, ordered as whole numbers)
-    int* err;
+    int* err;             // error word of the device, and the host's
+    int* err_host;
 };
 
 // a block's work: sequence bounds (clamped to the tensors) and tile
@@ -161,6 +166,54 @@ __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
 
+// Behind the barriers: the tensor memory's address, and 12 bytes on the block's
+// work, which is then read word by word: read in vectors its fields take
+// neighbouring registers (8 x 2048: forward 174 -> 191 us, dq 229 -> 240).
+__device__ __forceinline__ uint32_t* slot_of(uint64_t* bars, int n) { return reinterpret_cast<uint32_t*>(bars + n); }
+__device__ __forceinline__ Work* work_of(uint64_t* bars, int n) { return reinterpret_cast<Work*>(slot_of(bars, n) + 3); }
+
+// `rows` rows of `bytes`, the first of them the `row`-th such, `step` of them apart
+__device__ __forceinline__ void spoil(void* out, int64_t row, int rows, int64_t step, int bytes) {
+    const int words = bytes / 4;
+    uint32_t* at = static_cast<uint32_t*>(out) + row * words;
+#pragma unroll 1
+    for (int64_t i = threadIdx.x & 31; i < (int64_t)rows * words; i += 32) at[i / words * step * words + i % words] = 0x7fff7fffu;
+}
+// What the product warp does at the end of a block whose waits ran out (looked
+// for by all warps it cost the forward of 64 x 256 tokens 2 us of 32): the host
+// is told, the products in flight end (bounded), and NaN (of any type) takes the results'
+// place.  KIND 0: forward, 1: dq, 2: dk and dv; BARS: where its NBARS barriers
+// stand, the last one for this (nothing of the kernel's is kept in registers for it).
+template <int KIND, int BARS, int NBARS> __device__ __noinline__ void spoil_block(const Params& P) {
+    extern __shared__ uint8_t raw[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(align1024(raw) + BARS);
+    const Work* work = work_of(bars, NBARS);
+    const uint32_t drained = smem_u32(bars + NBARS - 1);
+    if ((threadIdx.x & 31) == 0) {
+        *reinterpret_cast<volatile int*>(P.err_host) = *reinterpret_cast<volatile int*>(P.err);
+        __threadfence_system();
+    }
+    __syncwarp();
+    mma_commit(drained, elect_one());
+    Patience patience;
+    while (!__all_sync(0xffffffffu, mbar_try(drained, 0)) && !__any_sync(0xffffffffu, patience.over(P.err))) {}
+    const Work w = *work;
+    if (KIND < 2) {
+        const int r0 = w.tile * (KIND ? 128 : 256), rows = min(KIND ? 128 : 256, w.lq - r0), head = blockIdx.x % P.H;
+        const int64_t first = (int64_t)w.q0 + r0, row = first * P.H + head;
+        spoil(KIND ? P.dq : P.o, row, rows, P.H, P.D * 2);
+        if (!KIND && P.rest) spoil(P.rest, row, rows, P.H, P.D * 2);
+        spoil(KIND ? P.delta : P.lse, (int64_t)head * P.Tq + first, rows, 1, 4);
+    } else {
+        const int HK = P.H / P.G, k0 = w.tile * 128, rows = min(128, w.lk - k0);
+        const int64_t row = ((int64_t)w.k0 + k0) * HK + blockIdx.x % HK, all = (int64_t)P.Tk * HK * P.D;
+        float* part = P.part + 2 * all * (blockIdx.x / HK % P.splits);
+        const bool parts = P.splits > 1;
+        spoil(parts ? part : P.dk, row, rows, HK, P.D * (parts ? 4 : 2));
+        spoil(parts ? part + all : P.dv, row, rows, HK, P.D * (parts ? 4 : 2));
+    }
+}
+
 // COLS columns of the warp's 32 rows in tensor memory, times f (one factor a
 // row), to `rows` rows of `out` (row stride in elements), as columns col0 .. of
 // D.  A lane holds a row, so stores straight from the registers touch 32 rows
@@ -235,7 +288,7 @@ template <int DP> struct Fwd {
     static constexpr int ST = DP == 128 ? 5 : 8;        // ring of K and V tiles
     static constexpr int RING = 2 * TILE;
     static constexpr int BARS = RING + ST * TILE;
-    static constexpr size_t SMEM = BARS + 512 + 1024;
+    static constexpr size_t SMEM = BARS + BARRIERS + 1024;
 };
 
 template <typename T, int DP>
@@ -248,8 +301,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = align1024(raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * ST + 14);
-    Work* work = reinterpret_cast<Work*>(slot + 4);
+    constexpr int NBARS = 2 * ST + 13;
+    uint32_t* slot = slot_of(bars, NBARS);
+    Work* work = work_of(bars, NBARS);
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
@@ -259,6 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto pv_done = [&](int i) { return bar0 + 8u * (2 * ST + 6 + i); };
     auto p_half = [&](int i) { return bar0 + 8u * (2 * ST + 8 + i); };
     auto s_free = [&](int i) { return bar0 + 8u * (2 * ST + 10 + i); };
+    const uint32_t drained = bar0 + 8u * (2 * ST + 12);
     constexpr bool APART = DP == 64;             // P has columns of its own
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.x % P.H, t = blockIdx.x / P.H, kvh = head / P.G;
@@ -270,6 +325,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mbar_init(q_full(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 128); mbar_init(pv_done(i), 1);
                 mbar_init(p_half(i), 128); mbar_init(s_free(i), 128);
             }
+            mbar_init(drained, 1);
+            set_gave_up(bar0, 0);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         find_tile(P, false, t, gridDim.x / P.H, 256, P.causal, work);
@@ -313,18 +370,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (n[i] > 0) load(base + i * TILE, &mq, q_full(i), head, w.q0 + w.tile * 256 + i * 128);
             };
             load_q(0);
-            int s = 0;
+            int s = 0, sent = 0;
             uint32_t ph = 0;
-            for (int x = 0; x < 2 * nmax; ++x) {      // K_0, V_0, K_1, V_1, ...
-                if (!mbar_wait(empty(s), ph ^ 1, P.err, 1)) goto done;
-                load(ring + s * TILE, x & 1 ? &mv : &mk, full(s), kvh, w.k0 + (x >> 1) * 128);
-                if (x == 0) load_q(1);
+            bool ok = true;
+            for (; sent < 2 * nmax; ++sent) {         // K_0, V_0, K_1, V_1, ...
+                if (!(ok = mbar_wait(empty(s), ph ^ 1, P.err, 1))) break;
+                load(ring + s * TILE, sent & 1 ? &mv : &mk, full(s), kvh, w.k0 + (sent >> 1) * 128);
+                if (sent == 0) load_q(1);
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
             // the last use of every slot: nothing arrives on these barriers after the block has left
-            for (int x = 0; x < ST && x < 2 * nmax; ++x) {
+            for (int x = 0; ok && x < ST && x < 2 * nmax; ++x) {
                 const int y = 2 * nmax - 1 - x;
-                if (!mbar_wait(empty(y % ST), (y / ST) & 1, P.err, 2)) goto done;
+                ok = mbar_wait(empty(y % ST), (y / ST) & 1, P.err, 2);
+            }
+            if (!ok) {
+                if ((n[0] == 0 || ring_landed(q_full(0), 1, 1, P.err)) &&
+                    (n[1] == 0 || sent == 0 || ring_landed(q_full(1), 1, 1, P.err)))
+                    ring_landed(full(0), ST, sent, P.err);
+                goto done;
             }
         }
     } else if (warp == 1) {
@@ -402,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int every = P.causal ? min(w.lk, w.tile * 256 + i * 128 + off + 1) : w.lk;
         float m = -INFINITY, l = 0.f;
         for (int j = 0; j < ni; ++j) {
-            if (!mbar_wait(s_full(i), j & 1, P.err, 9)) goto done;
+            mbar_wait(s_full(i), j & 1, P.err, 9);
             fence_after();
             // 32 scores at a time: the second half first, for the maximum alone;
             // the first half stays in registers for the exponentials
@@ -439,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // p up to 256 is as exact, and O is rescaled a few times in all
             // (a NaN score, or one of +inf, makes the row NaN here: the exponentials
             // on the fma pipe would hide it)
-            if (APART && j > 0 && !mbar_wait(pv_done(i), (j - 1) & 1, P.err, 12)) goto done;     // O and P are free
+            if (APART && j > 0) mbar_wait(pv_done(i), (j - 1) & 1, P.err, 12);     // O and P are free
             const bool up = !(top <= m + slack);
             if (__any_sync(0xffffffffu, up)) {
                 float to_m = up ? max3_nan(m, top, top) : m;     // a row moves by its own scores alone
@@ -507,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int64_t at = (trow * P.H + head) * P.D;
         T* rest = static_cast<T*>(P.rest);
         if (ni > 0) {
-            if (!mbar_wait(pv_done(i), (ni - 1) & 1, P.err, 10)) goto done;
+            mbar_wait(pv_done(i), (ni - 1) & 1, P.err, 10);
             fence_after();
             const int64_t stride = (int64_t)P.H * P.D, at0 = at - lane * stride;
             store_rows<T, DP, true>(to, base + i * TILE + q * (TILE / 4), m == -INFINITY ? 0.f : 1.0f / l, out + at0, stride,
@@ -525,6 +589,7 @@ done:
     __syncthreads();
     if (warp == 1) {
         fence_after();
+        if (gave_up(bar0)) spoil_block<0, C::BARS, NBARS>(P);
         tmem_free<512>(tmem);
     }
 }
@@ -601,7 +666,7 @@ template <int DP> struct BwdQ {
     static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 128 ? 2 : 4;
     static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + KS * TILE;
     static constexpr int BARS = V_OFF + VS * TILE;
-    static constexpr int RED = BARS + 512;                     // delta, and (fp16) the sum of |do|, of 128 rows
+    static constexpr int RED = BARS + BARRIERS;                     // delta, and (fp16) the sum of |do|, of 128 rows
     static constexpr size_t SMEM = RED + 1024 + 1024;
 };
 
@@ -616,8 +681,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = align1024(raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * KS + 2 * VS + 9);
-    Work* work = reinterpret_cast<Work*>(slot + 4);
+    constexpr int NBARS = 2 * KS + 2 * VS + 8;
+    uint32_t* slot = slot_of(bars, NBARS);
+    Work* work = work_of(bars, NBARS);
     float* red = reinterpret_cast<float*>(smem + C::RED);
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto k_full = [&](int s) { return bar0 + 8u * s; };
@@ -626,7 +692,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto v_empty = [&](int s) { return bar0 + 8u * (2 * KS + VS + s); };
     const uint32_t one = bar0 + 8u * (2 * KS + 2 * VS);
     const uint32_t q_full = one, s_full = one + 8, s_free = one + 16, dp_full = one + 24, dp_free = one + 32,
-                   ds_full = one + 40, ds_free = one + 48;
+                   ds_full = one + 40, ds_free = one + 48, drained = one + 56;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.x % P.H, t = blockIdx.x / P.H, kvh = head / P.G;
 
@@ -638,6 +704,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(s_full, 1); mbar_init(s_free, 256);
             mbar_init(dp_full, 1); mbar_init(dp_free, 256);
             mbar_init(ds_full, 256); mbar_init(ds_free, 1);
+            mbar_init(drained, 1);
+            set_gave_up(bar0, 0);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         find_tile(P, false, t, gridDim.x / P.H, 128, P.causal, work);
@@ -666,19 +734,28 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_expect(q_full, 2 * TILE);
             load(base, &mq, q_full, head, w.q0 + r0);
             load(base + TILE, &mdo, q_full, head, w.q0 + r0);
+            int nk = 0, nv = 0;                          // tiles sent
+            bool ok = true;
             for (int j = 0; j < n; ++j) {
                 const int sk = j % KS, sv = j % VS;
-                if (!mbar_wait(k_empty(sk), ((j / KS) & 1) ^ 1, P.err, 21)) goto done;
+                if (!(ok = mbar_wait(k_empty(sk), ((j / KS) & 1) ^ 1, P.err, 21))) break;
                 mbar_expect(k_full(sk), TILE);
                 load(base + C::K_OFF + sk * TILE, &mk, k_full(sk), kvh, w.k0 + j * 128);
-                if (!mbar_wait(v_empty(sv), ((j / VS) & 1) ^ 1, P.err, 22)) goto done;
+                ++nk;
+                if (!(ok = mbar_wait(v_empty(sv), ((j / VS) & 1) ^ 1, P.err, 22))) break;
                 mbar_expect(v_full(sv), TILE);
                 load(base + C::V_OFF + sv * TILE, &mv, v_full(sv), kvh, w.k0 + j * 128);
+                ++nv;
             }
-            for (int x = 0; x < KS && x < n; ++x)
-                if (!mbar_wait(k_empty((n - 1 - x) % KS), ((n - 1 - x) / KS) & 1, P.err, 23)) goto done;
-            for (int x = 0; x < VS && x < n; ++x)
-                if (!mbar_wait(v_empty((n - 1 - x) % VS), ((n - 1 - x) / VS) & 1, P.err, 24)) goto done;
+            for (int x = 0; ok && x < KS && x < n; ++x)
+                ok = mbar_wait(k_empty((n - 1 - x) % KS), ((n - 1 - x) / KS) & 1, P.err, 23);
+            for (int x = 0; ok && x < VS && x < n; ++x)
+                ok = mbar_wait(v_empty((n - 1 - x) % VS), ((n - 1 - x) / VS) & 1, P.err, 24);
+            if (!ok) {
+                if (ring_landed(q_full, 1, 1, P.err) && ring_landed(k_full(0), KS, nk, P.err))
+                    ring_landed(v_full(0), VS, nv, P.err);
+                goto done;
+            }
         }
     } else if (warp == 1) {
         constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_Q = instr_desc(BF, DP, 1);
@@ -804,14 +881,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             // block's products, and then meet element by element: exponentials
             // and the arithmetic of ds overlap
             uint32_t u[64], v[64];
-            if (!mbar_wait(s_full, j & 1, P.err, 32)) goto done;
+            mbar_wait(s_full, j & 1, P.err, 32);
             fence_after();
             ld32(tmem + lanes + half * 64, u);
             ld32(tmem + lanes + half * 64 + 32, u + 32);
             wait_ld();
             fence_before();
             mbar_arrive(s_free);
-            if (!mbar_wait(dp_full, j & 1, P.err, 33)) goto done;
+            mbar_wait(dp_full, j & 1, P.err, 33);
             fence_after();
             ld32(tmem + lanes + 128 + half * 64, v);
             ld32(tmem + lanes + 128 + half * 64 + 32, v + 32);
@@ -836,7 +913,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             };
             if (masked) weigh(std::true_type());
             else weigh(std::false_type());
-            if (j > 0 && !mbar_wait(ds_free, (j - 1) & 1, P.err, 34)) goto done;
+            if (j > 0) mbar_wait(ds_free, (j - 1) & 1, P.err, 34);
             st32(tmem + lanes + 384 + half * 32, u);
             wait_st();
             fence_before();
@@ -844,7 +921,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         T* dst = static_cast<T*>(P.dq) + (trow * P.H + head) * P.D;
         if (n > 0) {
-            if (!mbar_wait(ds_free, (n - 1) & 1, P.err, 35)) goto done;
+            mbar_wait(ds_free, (n - 1) & 1, P.err, 35);
             fence_after();
             const int64_t stride = (int64_t)P.H * P.D;
             store_rows<T, DP / 2>(tmem + lanes + 256 + half * (DP / 2), base + half * TILE + q * (TILE / 8), P.scale / up,
@@ -858,6 +935,7 @@ done:
     __syncthreads();
     if (warp == 1) {
         fence_after();
+        if (gave_up(bar0)) spoil_block<1, C::BARS, NBARS>(P);
         tmem_free<512>(tmem);
     }
 }
@@ -884,7 +962,7 @@ template <int DP> struct BwdK {
     static constexpr int QS = DP == 128 ? 2 : 3, OS = DP == 128 ? 2 : 3;
     static constexpr int Q_OFF = 2 * TILE, O_OFF = Q_OFF + QS * TILE;
     static constexpr int BARS = O_OFF + OS * TILE;
-    static constexpr int ONES = BARS + 512;                    // the row of ones, for every key
+    static constexpr int ONES = BARS + BARRIERS;                    // the row of ones, for every key
     static constexpr int STAT = ONES + THIN;                   // 2 stages of (-lse / scale, -delta), a query a row
     static constexpr size_t SMEM = STAT + 4 * THIN + 1024;
 };
@@ -910,8 +988,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = align1024(raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BARS);
-    uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * QS + 2 * OS + 12);
-    Work* work = reinterpret_cast<Work*>(slot + 4);
+    constexpr int NBARS = 2 * QS + 2 * OS + 12;
+    uint32_t* slot = slot_of(bars, NBARS);
+    Work* work = work_of(bars, NBARS);
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto q_full = [&](int s) { return bar0 + 8u * s; };
     auto q_empty = [&](int s) { return bar0 + 8u * (QS + s); };
@@ -922,6 +1001,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                    ds_full = one + 40, dk_done = one + 48;
     auto st_full = [&](int s) { return one + 56u + 8u * s; };
     auto st_empty = [&](int s) { return one + 72u + 8u * s; };
+    const uint32_t drained = one + 88;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int HK = P.H / P.G;
     const int kvh = blockIdx.x % HK, part = blockIdx.x / HK % P.splits, t = blockIdx.x / HK / P.splits;
@@ -935,6 +1015,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(s_full, 1); mbar_init(p_full, 256); mbar_init(dv_done, 1);
             mbar_init(dp_full, 1); mbar_init(ds_full, 256); mbar_init(dk_done, 1);
             for (int s = 0; s < 2; ++s) { mbar_init(st_full(s), 64); mbar_init(st_empty(s), 1); }
+            mbar_init(drained, 1);
+            set_gave_up(bar0, 0);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         find_tile(P, true, t, gridDim.x / HK / P.splits, 128, false, work);
@@ -977,20 +1059,29 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_expect(kv_full, 2 * TILE);
             load(base, &mk, kv_full, kvh, w.k0 + k0);
             load(base + TILE, &mv, kv_full, kvh, w.k0 + k0);
+            int sent_q = 0, sent_o = 0;
+            bool ok = true;
             for (int x = 0; x < n; ++x) {
                 const int sq = x % QS, so = x % OS;
                 const int head = head0 + x / nq, row = w.q0 + (jq + x % nq) * 128;
-                if (!mbar_wait(q_empty(sq), ((x / QS) & 1) ^ 1, P.err, 41)) goto done;
+                if (!(ok = mbar_wait(q_empty(sq), ((x / QS) & 1) ^ 1, P.err, 41))) break;
                 mbar_expect(q_full(sq), TILE);
                 load(base + C::Q_OFF + sq * TILE, &mq, q_full(sq), head, row);
-                if (!mbar_wait(o_empty(so), ((x / OS) & 1) ^ 1, P.err, 42)) goto done;
+                ++sent_q;
+                if (!(ok = mbar_wait(o_empty(so), ((x / OS) & 1) ^ 1, P.err, 42))) break;
                 mbar_expect(o_full(so), TILE);
                 load(base + C::O_OFF + so * TILE, &mdo, o_full(so), head, row);
+                ++sent_o;
             }
-            for (int x = 0; x < QS && x < n; ++x)
-                if (!mbar_wait(q_empty((n - 1 - x) % QS), ((n - 1 - x) / QS) & 1, P.err, 43)) goto done;
-            for (int x = 0; x < OS && x < n; ++x)
-                if (!mbar_wait(o_empty((n - 1 - x) % OS), ((n - 1 - x) / OS) & 1, P.err, 44)) goto done;
+            for (int x = 0; ok && x < QS && x < n; ++x)
+                ok = mbar_wait(q_empty((n - 1 - x) % QS), ((n - 1 - x) / QS) & 1, P.err, 43);
+            for (int x = 0; ok && x < OS && x < n; ++x)
+                ok = mbar_wait(o_empty((n - 1 - x) % OS), ((n - 1 - x) / OS) & 1, P.err, 44);
+            if (!ok) {
+                if (ring_landed(kv_full, 1, 1, P.err) && ring_landed(q_full(0), QS, sent_q, P.err))
+                    ring_landed(o_full(0), OS, sent_o, P.err);
+                goto done;
+            }
         }
     } else if (warp == 1) {
         constexpr uint32_t ID_S = instr_desc(BF, 128, 0), ID_D = instr_desc(BF, DP, 1), ID_STAT = instr_desc(1, 128, 0);
@@ -1096,7 +1187,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     d[k] = P.delta[at];
                 }
             }
-            if (!mbar_wait(st_empty(s), ((x >> 1) & 1) ^ 1, P.err, 52)) goto done;
+            mbar_wait(st_empty(s), ((x >> 1) & 1) ^ 1, P.err, 52);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const uint32_t at = base + C::STAT + 2 * s * THIN + thin_row(i + k * 64);
@@ -1108,7 +1199,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_arrive(st_full(s));
         }
         for (int x = 0; x < 2 && x < n; ++x)       // the last use of each stage
-            if (!mbar_wait(st_empty((n - 1 - x) & 1), ((n - 1 - x) >> 1) & 1, P.err, 57)) goto done;
+            mbar_wait(st_empty((n - 1 - x) & 1), ((n - 1 - x) >> 1) & 1, P.err, 57);
     } else {
         const int half = (warp - 4) >> 2, q = warp & 3;
         const int key = k0 + q * 32 + lane;
@@ -1129,7 +1220,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool masked = P.causal && row0 + off < k0 + 127;
             float p[64];
             uint32_t u[64], v[32];
-            if (!mbar_wait(s_full, x & 1, P.err, 54)) goto done;
+            mbar_wait(s_full, x & 1, P.err, 54);
             fence_after();
             ld32(tmem + lanes + half * 64, u);
             ld32(tmem + lanes + half * 64 + 32, u + 32);
@@ -1153,7 +1244,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             wait_st();
             fence_before();
             mbar_arrive(p_full);
-            if (!mbar_wait(dp_full, x & 1, P.err, 55)) goto done;
+            mbar_wait(dp_full, x & 1, P.err, 55);
             fence_after();
             ld32(tmem + lanes + 128 + half * 64, u);
             ld32(tmem + lanes + 128 + half * 64 + 32, u + 32);
@@ -1191,7 +1282,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         };
         if (n > 0) {
-            if (!mbar_wait(dk_done, (n - 1) & 1, P.err, 56)) goto done;      // and dV before it
+            mbar_wait(dk_done, (n - 1) & 1, P.err, 56);      // and dV before it
             fence_after();
             if (P.splits > 1) store(dkp, dkp + all);
             else store(static_cast<T*>(P.dk), static_cast<T*>(P.dv));
@@ -1205,6 +1296,7 @@ done:
     __syncthreads();
     if (warp == 1) {
         fence_after();
+        if (gave_up(bar0)) spoil_block<2, C::BARS, NBARS>(P);
         tmem_free<512>(tmem);
     }
 }
@@ -1257,11 +1349,65 @@ bool make_map(CUtensorMap* m, const void* base, int bf16, int64_t rows, int64_t 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr int MAX_DEVICES = 64;
 __device__ int g_err;      // first wait that ran out (0: none), per device
 
-int* error_word() {
-    int* p = nullptr;
-    return cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_err) == cudaSuccess ? p : nullptr;
+int device_index() {
+    int d = 0;
+    return cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < MAX_DEVICES ? d : -1;
+}
+
+// the host's error words, one a device, in memory that the kernels write to
+volatile int* host_word() {
+    static int* const words = [] {
+        // (an allocation is no work on a stream: it may come first in a capture)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        if (cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        } else {
+            memset(p, 0, MAX_DEVICES * sizeof(int));
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        return static_cast<int*>(p);
+    }();
+    const int d = device_index();
+    return words && d >= 0 ? words + d : nullptr;
+}
+
+// where this device's kernels tell a wait that ran out; refuses while one is told
+int error_words(int** err, int** err_host, const char* name) {
+    volatile int* host = host_word();
+    void* p = nullptr;
+    if (!host || cudaGetSymbolAddress(&p, g_err) != cudaSuccess) return fail(CONCORD_ELAUNCH, std::string(name) + ": device set-up failed");
+    if (*host)
+        return fail(CONCORD_ETIMEOUT, std::string(name) + ": a wait inside an earlier attention kernel ran out (code " +
+                                          std::to_string(*host) + "), its results hold NaN; concord_attention_error(1) clears this");
+    *err = static_cast<int*>(p);
+    if (cudaHostGetDevicePointer(&p, const_cast<int*>(host), 0) != cudaSuccess)
+        return fail(CONCORD_ELAUNCH, std::string(name) + ": device set-up failed");
+    *err_host = static_cast<int*>(p);
+    return CONCORD_OK;
+}
+
+// a wait on a barrier that nobody arrives on, by a warp and by a thread of another
+__global__ void __launch_bounds__(64) wait_check_kernel(int* err, int* err_host) {
+    __shared__ __align__(BARRIERS) uint8_t bars[BARRIERS];
+    const uint32_t b = smem_u32(bars);
+    if (threadIdx.x == 0) {
+        mbar_init(b, 1);
+        set_gave_up(b, 0);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) warp_wait(b, 0, err, 99);
+    else if (threadIdx.x == 32) mbar_wait(b, 0, err, 99);
+    __syncthreads();
+    if (gave_up(b) && threadIdx.x == 0) {
+        *reinterpret_cast<volatile int*>(err_host) = *reinterpret_cast<volatile int*>(err);
+        __threadfence_system();
+    }
 }
 
 template <typename T, int DP> bool raise_smem() {
@@ -1275,11 +1421,10 @@ template <typename T, int DP> bool raise_smem() {
 
 // the kernels' shared-memory limits, once per device
 bool device_ready() {
-    constexpr int MAX_DEVICES = 64;
     static std::atomic<int> ready[MAX_DEVICES];
     static std::mutex mu;
-    int d = 0;
-    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return false;
+    const int d = device_index();
+    if (d < 0) return false;
     if (ready[d].load()) return true;
     std::lock_guard<std::mutex> g(mu);
     if (!raise_smem<__nv_bfloat16, 64>() || !raise_smem<__nv_bfloat16, 128>() || !raise_smem<__half, 64>() ||
@@ -1319,13 +1464,14 @@ int check_operand(const char* name, const void* x, int64_t ts, int64_t hs) {
     return CONCORD_OK;
 }
 
-Params make_params(const concord_attention_params* p, int* err) {
+Params make_params(const concord_attention_params* p, int* err, int* err_host) {
     Params P{};
     P.cuq = p->cu_q; P.cuk = p->cu_k; P.B = (int)p->seqs;
     P.Tq = (int)p->tokens_q; P.Tk = (int)p->tokens_k;
     P.H = (int)p->heads; P.G = (int)(p->heads / p->kv_heads); P.D = (int)p->head_dim;
     P.causal = p->causal; P.scale = p->scale; P.scale2 = p->scale * LOG2E;
     P.err = err;
+    P.err_host = err_host;
     return P;
 }
 
@@ -1413,9 +1559,10 @@ extern "C" int concord_attention_fwd(const concord_attention_params* p, const vo
         !attn::make_map(&mk, k, bf, p->tokens_k, p->kv_heads, p->head_dim, k_ts, k_hs) ||
         !attn::make_map(&mv, v, bf, p->tokens_k, p->kv_heads, p->head_dim, v_ts, v_hs))
         return fail(CONCORD_ELAUNCH, "concord_attention_fwd: TMA descriptor encoding failed");
-    int* err = attn::error_word();
-    if (!err || !attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_fwd: device set-up failed");
-    attn::Params P = attn::make_params(p, err);
+    int *err, *err_host;
+    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    if (!attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_fwd: device set-up failed");
+    attn::Params P = attn::make_params(p, err, err_host);
     P.o = o;
     P.rest = o_rest;
     P.lse = lse;
@@ -1461,9 +1608,10 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
         !attn::make_map(&mv, v, bf, p->tokens_k, p->kv_heads, p->head_dim, v_ts, v_hs) ||
         !attn::make_map(&md, dout, bf, p->tokens_q, p->heads, p->head_dim, do_ts, do_hs))
         return fail(CONCORD_ELAUNCH, "concord_attention_bwd: TMA descriptor encoding failed");
-    int* err = attn::error_word();
-    if (!err || !attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_bwd: device set-up failed");
-    attn::Params P = attn::make_params(p, err);
+    int *err, *err_host;
+    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    if (!attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_bwd: device set-up failed");
+    attn::Params P = attn::make_params(p, err, err_host);
     P.o = const_cast<void*>(o);
     P.rest = const_cast<void*>(o_rest);
     P.lse = const_cast<float*>(lse);
@@ -1497,10 +1645,26 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
 
 // the attention kernels' error word on the current device (0: no wait ran out)
 extern "C" int concord_attention_error(int32_t reset) {
-    int* err = attn::error_word();
-    if (!err) return -1;
+    volatile int* host = attn::host_word();
+    void* p = nullptr;
     int v = 0;
-    cudaMemcpy(&v, err, sizeof(int), cudaMemcpyDeviceToHost);
-    if (reset) cudaMemset(err, 0, sizeof(int));
+    if (!host || cudaGetSymbolAddress(&p, attn::g_err) != cudaSuccess ||
+        cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
+        return -1;
+    if (!v) v = *host;
+    if (reset) {
+        if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return -1;
+        *host = 0;
+    }
     return v;
+}
+
+extern "C" int32_t* concord_attention_error_word(void) { return const_cast<int32_t*>(attn::host_word()); }
+
+extern "C" int concord_attention_wait_check(void* stream) {
+    const char* name = "concord_attention_wait_check";
+    int *err, *err_host;
+    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    attn::wait_check_kernel<<<1, 64, 0, as_stream(stream)>>>(err, err_host);
+    return check_launch(name);
 }

@@ -9,7 +9,11 @@
 namespace concord {
 namespace tc {
 
-constexpr uint64_t WAIT_NS = 2000000000ull;   // 2 s of GPU time per wait
+// A wait runs out after 2 s in which its warp ran: of the time between two looks
+// at the clock (wall time) at most 100 ms count, so a kernel that was taken off
+// the GPU meanwhile has lost nothing.  Once a wait has run out somewhere on the
+// device the others get 20 ms, so a grid of many blocks still ends soon.
+constexpr uint64_t WAIT_NS = 2000000000ull, LATER_NS = 20000000ull, SLICE_NS = 100000000ull;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -52,30 +56,72 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// false, with the error word set, once WAIT_NS have passed without the phase completing
+struct Patience {
+    uint64_t last = 0, ran = 0;
+    __device__ __forceinline__ bool over(const int* err) {
+        const uint64_t t = now_ns();
+        ran += last ? min(t - last, SLICE_NS) : 0;
+        last = t;
+        return ran > LATER_NS && (ran > WAIT_NS || *reinterpret_cast<const volatile int*>(err) != 0);
+    }
+};
+// The barriers of a block stand in 512 aligned bytes of shared memory, of which
+// the last word says that a wait of the block has run out (the address of any
+// of them leads there, so nothing is kept in registers for it).
+constexpr uint32_t BARRIERS = 512;
+__device__ __forceinline__ uint32_t gave_up_word(uint32_t bar) { return (bar & ~(BARRIERS - 1)) + BARRIERS - 4; }
+__device__ __forceinline__ void set_gave_up(uint32_t bar, uint32_t v) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(gave_up_word(bar)), "r"(v) : "memory");
+}
+__device__ __forceinline__ bool gave_up(uint32_t bar) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(gave_up_word(bar)) : "memory");
+    return v != 0;
+}
+// By one thread: false once the wait has run out, the first such wait's code then
+// in *err, or at once where another of the block has.  (The loops are calls: as
+// code in every place they made the forward of 64 x 256 tokens 4 us slower than
+// its 31.)
 __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
-    const uint64_t t0 = now_ns();
+    Patience patience;
     for (int i = 1;; ++i) {
         if (mbar_try(bar, parity)) return true;
-        if ((i & 63) == 0 && now_ns() - t0 > WAIT_NS) break;
+        if (gave_up(bar)) return false;
+        if ((i & 15) == 0 && patience.over(err)) break;      // (reading the clock is slow)
     }
+    set_gave_up(bar, 1);
     atomicCAS(err, 0, code);
     return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err, int code) {
     return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, err, code);
 }
-
-// The same by a whole warp, which stays converged: every branch goes by a vote.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
-    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-    const uint64_t t0 = now_ns();
+// The same by a whole warp, which stays converged: every branch goes by a vote,
+// so that all lanes go on or none does.
+__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
+    Patience patience;
 #pragma unroll 1
-    while (!__all_sync(0xffffffffu, mbar_try(bar, parity))) {
-        if (__any_sync(0xffffffffu, now_ns() - t0 > WAIT_NS)) {
+    for (int i = 1; !__all_sync(0xffffffffu, mbar_try(bar, parity)); ++i) {
+        if (__any_sync(0xffffffffu, gave_up(bar))) return false;
+        if ((i & 15) == 0 && __any_sync(0xffffffffu, patience.over(err))) {
+            set_gave_up(bar, 1);
             atomicCAS(err, 0, code);
             return false;
         }
+    }
+    return true;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
+    return __all_sync(0xffffffffu, mbar_try(bar, parity)) || warp_wait_slow(bar, parity, err, code);
+}
+// Given up after `sent` tiles into a ring of `stages` (their barriers 8 bytes
+// apart): what is on its way lands first, or that wait too runs out.
+__device__ __noinline__ bool ring_landed(uint32_t full, int stages, int sent, int* err) {
+    for (int x = max(0, sent - stages); x < sent; ++x) {
+        const uint32_t bar = full + 8u * (x % stages), parity = (x / stages) & 1;
+        Patience patience;
+        while (!mbar_try(bar, parity))
+            if (patience.over(err)) return false;
     }
     return true;
 }

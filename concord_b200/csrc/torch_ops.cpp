@@ -35,7 +35,7 @@ void check(int status, const char* name) {
     static const char* const kinds[] = {"invalid argument", "unsupported shape/stride", "unsupported alignment",
                                         "workspace missing or too small", "CUDA launch/runtime error",
                                         "no usable CUDA device", "size above the fixed maximum",
-                                        "a cross-GPU wait ran out"};
+                                        "a wait ran out"};
     const char* kind = status <= -1 && status >= -8 ? kinds[-status - 1] : "error";
     throw std::runtime_error(std::string(name) + " failed: " + kind + ": " + concord_last_error());
 }

@@ -73,7 +73,8 @@ extern "C" {
 #define CONCORD_ELAUNCH      -5  /* CUDA launch / runtime error               */
 #define CONCORD_ENODEVICE    -6  /* no usable CUDA device                      */
 #define CONCORD_ETOOBIG      -7  /* size above a fixed maximum                */
-#define CONCORD_ETIMEOUT     -8  /* a cross-GPU wait ran out (peer transport)  */
+#define CONCORD_ETIMEOUT     -8  /* a wait ran out: between GPUs (peer transport),
+                                    or in an earlier attention kernel          */
 
 /* step-kernel flag bits (the reference's Triton constexprs, packed_b.py:451-458) */
 #define CONCORD_F_MASS_PRESERVE   (1u << 0)
@@ -630,8 +631,16 @@ int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t
  * backward follows) is what o's rounding left over, from which the backward
  * has delta = dout . o to fp32; lse and delta are fp32 [heads, tokens_q], delta
  * being scratch that the backward fills, as is its workspace (16-byte aligned;
- * of 0 bytes for bf16 unless query heads are split).  concord_attention_error: non-zero
- * once a barrier wait inside a kernel has run out (2 s of GPU time per wait).
+ * of 0 bytes for bf16 unless query heads are split). 
+ * Every wait inside these kernels is bounded (2 s of running).  Where one runs
+ * out, the tiles concerned hold NaN and every later attention call on the
+ * device gives CONCORD_ETIMEOUT (the word is in host memory: no call
+ * synchronises to look) until concord_attention_error(1).
+ * concord_attention_error: the code of the first such wait, 0 if there was none
+ * (synchronises; clears it with `reset`).  concord_attention_error_word: the
+ * host's word of the current device, for a program that polls it.
+ * concord_attention_wait_check: launches a wait that nothing ends, for programs
+ * (and tests) that rehearse the failure: 2 s later the error is set.
  */
 typedef struct concord_attention_params {
     const int32_t* cu_q;
@@ -650,6 +659,8 @@ int concord_attention_bwd(const concord_attention_params* p, const void* q, int6
                           void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 size_t concord_attention_bwd_workspace_bytes(const concord_attention_params* p);
 int concord_attention_error(int32_t reset);
+int32_t* concord_attention_error_word(void);
+int concord_attention_wait_check(void* stream);
 
 #ifdef __cplusplus
 }

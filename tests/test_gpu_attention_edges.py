@@ -124,3 +124,39 @@ def test_one_row_or_one_head_of_any_stride(D):
     want = run(*(both(i).clone().view(-1).view(1, 1, D) for i in range(4)), cum([1]))
     got = run(*(both(i) for i in range(4)), cum([1]))
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_a_wait_that_ran_out_is_reported():
+    """A rehearsal: a wait that nothing ends sets the error 2 s later, without a synchronisation of the caller's; then
+    forward and backward refuse, until the error is cleared."""
+    import concord_b200
+    from concord_b200 import _abi, packed_attention
+    lib = _abi.load()
+    q, k, v, do = inputs(300, 2, 2, 64, seed=30)
+    cu = cum([100, 200])
+    want = run(q, k, v, do, cu)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = packed_attention(*leaves, cu)
+    word = lib.concord_attention_error_word()
+    assert word[0] == 0 and concord_b200.attention_error() == 0
+    try:
+        assert lib.concord_attention_wait_check(torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert word[0] == 99 and concord_b200.attention_error() == 99
+        with pytest.raises(RuntimeError, match="a wait inside an earlier attention kernel ran out .code 99."):
+            packed_attention(q, k, v, cu)
+        with pytest.raises(RuntimeError, match="ran out"):
+            torch.autograd.grad(o, leaves, do, retain_graph=True)
+        assert lib.concord_attention_wait_check(None) == -8
+    finally:
+        assert concord_b200.attention_error(reset=True) == 99
+    assert word[0] == 0 and concord_b200.attention_error() == 0
+    again = run(q, k, v, do, cu)
+    assert all(torch.equal(again[n], want[n]) for n in want)
+    word[0] = 5                          # another program's handler, or a kernel, wrote the host's word alone
+    try:
+        with pytest.raises(RuntimeError, match="code 5"):
+            packed_attention(q, k, v, cu)
+    finally:
+        assert concord_b200.attention_error(reset=True) == 5
+    assert torch.equal(packed_attention(q, k, v, cu), want["o"])
