@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <limits>
 #include <optional>
 #include <stdexcept>
@@ -48,6 +49,14 @@ void* current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+// A tangent of forward-mode differentiation is no part of what the kernels read:
+// it would be lost, and the derivative read as zero.
+void refuse_tangents(std::initializer_list<Tensor> inputs, const char* name) {
+    for (const Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name,
+                                    ": forward-mode differentiation is not supported (it has a backward pass only)");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // A gradient that has no gradient itself: where the upstream one would pass on
@@ -117,6 +126,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, int64_t out_code) {
     const Tensor w = get(weight), b = get(bias);
+    refuse_tangents({x, w, b}, "layer_norm");
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b));
     c10::cuda::CUDAGuard guard(x.device());
     Tensor y, x2, stats;
@@ -209,6 +219,7 @@ struct DistillArgs {
 // reduction: 0 mean, 1 sum, 2 none
 Tensor distill_loss(const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits, const MaybeTensor& labels,
                     double temperature, double alpha, int64_t ignore, int64_t reduction) {
+    refuse_tangents({logits, top_logits}, "distill_loss");
     const bool grad = at::GradMode::is_enabled() && wants_grad(logits), per_row = reduction == 2;
     c10::cuda::CUDAGuard guard(logits.device());
     Tensor out, stats;
@@ -240,6 +251,7 @@ Tensor distill_loss(const Tensor& logits, const Tensor& top_ids, const Tensor& t
 std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits,
                                                  const MaybeTensor& labels, double temperature, double alpha,
                                                  int64_t ignore, bool mean, double grad_scale) {
+    refuse_tangents({logits, top_logits}, "distill_loss_and_grad");
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(logits.device());
     const DistillArgs A(logits, top_ids, top_logits, labels);
@@ -319,6 +331,7 @@ struct AttentionBackward : public torch::autograd::Node {
 
 std::tuple<Tensor, Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& cu_q,
                                      const Tensor& cu_k, bool causal, double scale) {
+    refuse_tangents({q0, k0, v0}, "packed_attention");
     const bool grad = at::GradMode::is_enabled() && (wants_grad(q0) || wants_grad(k0) || wants_grad(v0));
     c10::cuda::CUDAGuard guard(q0.device());
     Tensor q, k, v, o, rest, lse;

@@ -59,7 +59,7 @@ def distill_loss(logits, top_ids, top_logits, labels=None, temperature=1.0, alph
 
     reduction: "mean" over the rows that count (0 if none does), "sum", or
     "none" (one loss per row).  The loss is fp32; the gradient, for the logits
-    alone, has their type.  Differentiable once.
+    alone, has their type.  Differentiable once, backward only.
     """
     temperature, alpha = float(temperature), float(alpha)
     _check(logits, top_ids, top_logits, labels, temperature, alpha)

@@ -18,7 +18,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     last dimension that is not contiguous is copied).  weight and bias [D]
     (either may be None); fp32 is read as it is, other types are converted.
     The result has `out_dtype` (default: x's type); statistics, sums and the
-    gradients of weight and bias are fp32.  Differentiable once.
+    gradients of weight and bias are fp32.  Differentiable once, backward only.
     """
     _ops.need_cuda(("x", x), ("weight", weight), ("bias", bias))
     _ops.need_type("x", x, _ops.TYPES)
