@@ -8,12 +8,14 @@
 // functions that call these (norm.py, distill.py, attention.py).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <initializer_list>
@@ -50,9 +52,14 @@ template <typename T> T* ptr(const Tensor& t) { return t.defined() ? static_cast
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 
-// A tangent of forward-mode differentiation is no part of what the kernels read:
-// it would be lost, and the derivative read as zero.
-void refuse_tangents(std::initializer_list<Tensor> inputs, const char* name) {
+// The kernels are no torch operators: a trace would record the allocation of
+// their outputs alone.  And a tangent of forward-mode differentiation is no part
+// of what they read: it would be lost, and the derivative read as zero.
+void refuse_transforms(std::initializer_list<Tensor> inputs, const char* name) {
+    using c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value(),
+                name, " cannot be traced: its kernels are not torch operators");
     for (const Tensor& t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name,
                                     ": forward-mode differentiation is not supported (it has a backward pass only)");
@@ -126,7 +133,7 @@ struct LayerNormBackward : public torch::autograd::Node {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, int64_t out_code) {
     const Tensor w = get(weight), b = get(bias);
-    refuse_tangents({x, w, b}, "layer_norm");
+    refuse_transforms({x, w, b}, "layer_norm");
     const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b));
     c10::cuda::CUDAGuard guard(x.device());
     Tensor y, x2, stats;
@@ -219,7 +226,7 @@ struct DistillArgs {
 // reduction: 0 mean, 1 sum, 2 none
 Tensor distill_loss(const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits, const MaybeTensor& labels,
                     double temperature, double alpha, int64_t ignore, int64_t reduction) {
-    refuse_tangents({logits, top_logits}, "distill_loss");
+    refuse_transforms({logits, top_logits}, "distill_loss");
     const bool grad = at::GradMode::is_enabled() && wants_grad(logits), per_row = reduction == 2;
     c10::cuda::CUDAGuard guard(logits.device());
     Tensor out, stats;
@@ -251,7 +258,7 @@ Tensor distill_loss(const Tensor& logits, const Tensor& top_ids, const Tensor& t
 std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits,
                                                  const MaybeTensor& labels, double temperature, double alpha,
                                                  int64_t ignore, bool mean, double grad_scale) {
-    refuse_tangents({logits, top_logits}, "distill_loss_and_grad");
+    refuse_transforms({logits, top_logits}, "distill_loss_and_grad");
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(logits.device());
     const DistillArgs A(logits, top_ids, top_logits, labels);
@@ -331,7 +338,7 @@ struct AttentionBackward : public torch::autograd::Node {
 
 std::tuple<Tensor, Tensor> attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& cu_q,
                                      const Tensor& cu_k, bool causal, double scale) {
-    refuse_tangents({q0, k0, v0}, "packed_attention");
+    refuse_transforms({q0, k0, v0}, "packed_attention");
     const bool grad = at::GradMode::is_enabled() && (wants_grad(q0) || wants_grad(k0) || wants_grad(v0));
     c10::cuda::CUDAGuard guard(q0.device());
     Tensor q, k, v, o, rest, lse;

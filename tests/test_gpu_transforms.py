@@ -48,3 +48,14 @@ def test_forward_mode_is_refused(make):
                 f(*dual)
     with fwd.dual_level():
         f(*args)                          # nothing to differentiate: as ever
+
+
+@OPERATORS
+def test_tracing_is_refused(make):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, args, _ = make()
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(f, tuple(args), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda *a: f(*a))(*args)
+    f(*args)
