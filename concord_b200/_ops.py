@@ -21,6 +21,10 @@ def native():
         if not os.path.exists(NATIVE_PATH):
             raise RuntimeError(f"concord_b200 extension not built: {NATIVE_PATH} is missing "
                                "(run `python -m concord_b200.build`); there is no CPU fallback")
+        from . import build
+        if build.stamp() not in (None, build.built_for()):
+            raise RuntimeError(f"concord_b200 extension built for {build.stamp()}, this is {build.built_for()}: "
+                               "run `python -m concord_b200.build`")
         loader = importlib.machinery.ExtensionFileLoader("_native", NATIVE_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_native", loader))
         loader.exec_module(module)

@@ -9,7 +9,9 @@ every fp32 multiply and add separately, and bit-exact words depend on the
 compiler not fusing them.  Also builds the host copy of the correctly
 rounded log2/exp2 (libcrmath_check.so) that the CPU tests check, and
 `_lib/_native.so`, the Python extension with the training operators' autograd
-nodes (csrc/torch_ops.cpp, compiled by g++ against the installed torch).
+nodes (csrc/torch_ops.cpp, compiled by g++ against the installed torch and
+again when another torch or Python is installed).  Users of the C ABI need
+neither: `--library` (build(extension=False)) leaves the extension out.
 """
 import glob
 import os
@@ -21,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 OUT = os.path.join(LIBDIR, "libconcord_b200.so")
 NATIVE = os.path.join(LIBDIR, "_native.so")
+STAMP = os.path.join(LIBDIR, "_native.stamp")      # what NATIVE was built for
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC",
@@ -75,7 +78,22 @@ def _native_command(src):
     return cmd + ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
 
 
-def build(verbose=False, force=False):
+def built_for():
+    """The torch and Python that an extension built now works with."""
+    import torch
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def stamp():
+    """What the extension that is there was built for (None: not known)."""
+    try:
+        with open(STAMP) as f:
+            return f.read().strip()
+    except OSError:
+        return None
+
+
+def build(verbose=False, force=False, extension=True):
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(LIBDIR, "obj")
     os.makedirs(objdir, exist_ok=True)
@@ -96,14 +114,18 @@ def build(verbose=False, force=False):
     src = os.path.join(CSRC, "crmath_check.cpp")
     if force or _newer(chk, [src, os.path.join(CSRC, "crmath.h")]):
         subprocess.check_call(["g++", "-O2", "-fPIC", "-ffp-contract=off", "-shared", "-o", chk, src])
+    if not extension:
+        return OUT
     src = os.path.join(CSRC, "torch_ops.cpp")
-    if force or _newer(NATIVE, [src, os.path.join(HERE, "..", "include", "concord_b200.h")]):
+    if force or stamp() != built_for() or _newer(NATIVE, [src, os.path.join(HERE, "..", "include", "concord_b200.h")]):
         cmd = _native_command(src)
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+        with open(STAMP, "w") as f:
+            f.write(built_for() + "\n")
     return OUT
 
 
 if __name__ == "__main__":
-    print(build(verbose=True, force="--force" in sys.argv))
+    print(build(verbose=True, force="--force" in sys.argv, extension="--library" not in sys.argv))
