@@ -160,3 +160,13 @@ def test_a_wait_that_ran_out_is_reported():
     finally:
         assert concord_b200.attention_error(reset=True) == 5
     assert torch.equal(packed_attention(q, k, v, cu), want["o"])
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("lq,lk", [([400], [5]), ([300, 20], [20, 300]), ([260, 1, 700], [3, 0, 200]), ([1], [1000]),
+                                   ([5, 7], [0, 400])])
+def test_wide_heads_with_keys_of_other_lengths(dtype, lq, lk):
+    """Heads of 128: pairs of query tiles of which the first, or both, see no key."""
+    q, k, v, do = inputs(sum(lq), 4, 2, 128, dtype, Tk=sum(lk), seed=29)
+    for causal in (True, False):
+        check(q, k, v, do, cum(lq), cum(lk), causal=causal)
