@@ -282,8 +282,10 @@ def train_chardistill(steps=200, docs=64, block=256, top=16, temperature=2.0, al
     batch under one CUDA graph: they are read on the device.  Returns per-step
     device times and losses."""
     from concord_b200 import distill_loss_and_grad
+    from concord_b200.checkpoint import set_step_salt
     from concord_b200.convert import aux_parameters, concordify
     torch.manual_seed(seed)
+    set_step_salt(torch.device(device), seed)      # the packed steps' rounding too: a seed is a run
     batches = PackedDocuments(MarkovChars(seed=seed, device=device), docs, block, top)
     model = PackedCharGPT(block=block, n_layer=n_layer).to(device)
     layers = concordify(model, lr=lr)
