@@ -274,13 +274,15 @@ class PackedDocuments:
 
 
 def train_chardistill(steps=200, docs=64, block=256, top=16, temperature=2.0, alpha=0.5, lr=5e-4, aux_lr=0.05, seed=0,
-                      device="cuda", n_layer=6, warmup=100, graph=True):
+                      device="cuda", n_layer=6, warmup=10, graph=True):
     """The char GPT distilled on packed documents, one GPU: Concord on every
     Linear, this package's layer norms and attention around them, and the
     loss and its gradient in one call (`distill_loss_and_grad`), which starts
     the backward that steps the packed layers.  Lengths change from batch to
-    batch under one CUDA graph: they are read on the device.  Returns per-step
-    device times and losses."""
+    batch under one CUDA graph: they are read on the device.  `warmup` eager
+    steps, then `steps` timed ones.  Returns per-step device times, losses, the
+    rows of a step (`tokens_per_step`) and the documents' tokens in the timed
+    steps (of the other rows nothing is learned)."""
     from concord_b200 import distill_loss_and_grad
     from concord_b200.checkpoint import set_step_salt
     from concord_b200.convert import aux_parameters, concordify
@@ -295,9 +297,12 @@ def train_chardistill(steps=200, docs=64, block=256, top=16, temperature=2.0, al
     for p in aux:
         p.grad = torch.zeros_like(p)
 
+    tokens = torch.zeros(warmup + steps, dtype=torch.int64, device=device)      # the documents', by step
+
     def refill(it):
         for dst, src in zip(static, batches.batch()):
             dst.copy_(src)
+        tokens[it] = static[5][-1]
 
     def step():
         x, pos, y, ids, t, cu = static
@@ -311,8 +316,9 @@ def train_chardistill(steps=200, docs=64, block=256, top=16, temperature=2.0, al
             l.rebalance()
         return loss
 
-    times, losses = run_steps(step, refill, steps, 10, layers, lr, graph)
-    return dict(ms=times, losses=losses, tokens_per_step=batches.tokens, concord_params=sum(l.packed_w.numel() for l in layers))
+    times, losses = run_steps(step, refill, steps, warmup, layers, lr, graph)
+    return dict(ms=times, losses=losses, tokens_per_step=batches.tokens, document_tokens=int(tokens[warmup:].sum()),
+                concord_params=sum(l.packed_w.numel() for l in layers))
 
 
 def run_steps(step_fn, refill, steps, warmup, layers, lr, graph, world=1, group=None):
