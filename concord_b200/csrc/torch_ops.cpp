@@ -352,8 +352,11 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q0, const Tensor& k0, const T
         if (grad) rest = at::empty(q.sizes(), plain);
         lse = at::empty({q.size(1), q.size(0)}, plain.dtype(at::kFloat));
         if (k.size(0) == 0) {
+            // (a row of no sequence has lse 0, as the kernels give it)
+            const Tensor row = at::arange(q.size(0), cu_q.options());
+            const Tensor none = row.lt(cu_q[0]).logical_or_(row.ge(cu_q[-1]));
             o.zero_();
-            lse.fill_(-std::numeric_limits<float>::infinity());
+            lse.fill_(-std::numeric_limits<float>::infinity()).masked_fill_(none, 0.f);
         } else if (q.size(0) > 0) {
             const auto p = attention_params(q, k, cu_q, cu_k, causal, scale);
             check(concord_attention_fwd(&p, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v),

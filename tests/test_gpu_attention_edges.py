@@ -170,3 +170,15 @@ def test_wide_heads_with_keys_of_other_lengths(dtype, lq, lk):
     q, k, v, do = inputs(sum(lq), 4, 2, 128, dtype, Tk=sum(lk), seed=29)
     for causal in (True, False):
         check(q, k, v, do, cum(lq), cum(lk), causal=causal)
+
+
+@pytest.mark.parametrize("Tk", [0, 30])
+def test_rows_of_no_sequence_without_any_keys(Tk):
+    """Sequences without keys, whether or not k holds rows of none: o 0 and lse -inf, and lse 0 outside of them."""
+    q, k, v, do = inputs(40, 2, 1, 64, Tk=Tk, seed=31)
+    cu = torch.tensor([3, 10, 10, 33], dtype=torch.int32, device=DEV)
+    got = run(q, k, v, do, cu, torch.full((4,), Tk, dtype=torch.int32, device=DEV))
+    assert all(bool((got[n] == 0).all()) for n in ("o", "dq", "dk", "dv"))
+    want = torch.zeros(2, 40, device=DEV)
+    want[:, 3:33] = -math.inf
+    assert torch.equal(got["lse"], want)
