@@ -20,7 +20,8 @@ def packed_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     strides: views of one projection's output are read in place as long as
     rows start on 16 bytes, other layouts are copied.
     cu_seqlens [B + 1] (int32 on the device; int64 is converted): sequence b
-    is rows cu_seqlens[b] .. cu_seqlens[b + 1], of any length, 0 included.
+    is rows cu_seqlens[b] .. cu_seqlens[b + 1], of any length, 0 included (the
+    bounds do not fall; they are clamped to the tensors, not checked).
     cu_seqlens_k: the same for the keys, where they differ (cross attention, a
     prompt's next chunk after cached keys); default: cu_seqlens.
     causal: query i of a sequence with Lq queries and Lk keys sees the keys up

@@ -1359,22 +1359,30 @@ int device_index() {
 
 // the host's error words, one a device, in memory that the kernels write to
 volatile int* host_word() {
-    static int* const words = [] {
-        // (an allocation is no work on a stream: it may come first in a capture)
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        void* p = nullptr;
-        if (cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
-            cudaGetLastError();
-            p = nullptr;
-        } else {
-            memset(p, 0, MAX_DEVICES * sizeof(int));
-        }
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        return static_cast<int*>(p);
-    }();
+    static std::atomic<int*> words;
+    static std::mutex mu;
     const int d = device_index();
-    return words && d >= 0 ? words + d : nullptr;
+    if (d < 0) return nullptr;
+    int* w = words.load();
+    if (!w) {
+        std::lock_guard<std::mutex> g(mu);
+        w = words.load();
+        if (!w) {
+            // (an allocation is no work on a stream: it may come first in a capture)
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            void* p = nullptr;
+            const cudaError_t e = cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) {
+                cudaGetLastError();
+                return nullptr;
+            }
+            memset(p, 0, MAX_DEVICES * sizeof(int));
+            words.store(w = static_cast<int*>(p));
+        }
+    }
+    return w + d;
 }
 
 // where this device's kernels tell a wait that ran out; refuses while one is told
