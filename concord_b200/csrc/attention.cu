@@ -282,7 +282,7 @@ __device__ __forceinline__ void store_rows(uint32_t tm, uint32_t stage, float f,
 // Bound by the chain of a tile, S -> softmax -> P V -> next S, of which two run
 // against each other (2900 cycles a pair of 128 x 128 blocks, 2048 of products);
 // short sequences by a block's start and end.  8 x 2048 tokens, 16 heads of 128,
-// causal: 192 us, 716 TFLOP/s; one sequence of 8191: 253 us, 1087 TFLOP/s.
+// causal: 166 us, 828 TFLOP/s; one sequence of 8191: 241 us, 1140 TFLOP/s.
 template <int DP> struct Fwd {
     static constexpr int TILE = 256 * DP;               // bytes of 128 rows
     static constexpr int ST = DP == 128 ? 5 : 8;        // ring of K and V tiles
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(256) range_kernel(const __grid_constant__ Para
 // 256, dS (16-bit pairs) 384.  S and dP of the next key block are computed as
 // soon as the softmax warps have read the present ones.
 // Bound by the softmax warps (1970 cycles a block, 1024 of exponentials) beside
-// 1536 cycles of products.  8 x 2048, 16 heads of 128, causal: 240 us, 860
+// 1536 cycles of products.  8 x 2048, 16 heads of 128, causal: 225 us, 917
 // TFLOP/s of its three products.
 template <int DP> struct BwdQ {
     static constexpr int TILE = 256 * DP;
@@ -955,7 +955,7 @@ done:
 // next dP, lets the exponentials run beside dK and dP, and ds beside dV and S.
 // Bound by the chain P -> dV -> next S -> exponentials (about 2900 cycles a
 // block) and by shared memory, which S and dP read at its full rate: 2048 cycles
-// of products.  8 x 2048, 16 heads of 128, causal: 303 us, 907 TFLOP/s of its
+// of products.  8 x 2048, 16 heads of 128, causal: 281 us, 979 TFLOP/s of its
 // four products.
 template <int DP> struct BwdK {
     static constexpr int TILE = 256 * DP;
