@@ -631,7 +631,7 @@ int concord_distill_grad(const concord_distill_params* p, const void* z, int32_t
  * backward follows) is what o's rounding left over, from which the backward
  * has delta = dout . o to fp32; lse and delta are fp32 [heads, tokens_q], delta
  * being scratch that the backward fills, as is its workspace (16-byte aligned;
- * of 0 bytes for bf16 unless query heads are split). 
+ * of 0 bytes for bf16 unless query heads are split).
  * Every wait inside these kernels is bounded (2 s of running).  Where one runs
  * out, the tiles concerned hold NaN and every later attention call on the
  * device gives CONCORD_ETIMEOUT (the word is in host memory: no call
