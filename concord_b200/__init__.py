@@ -39,8 +39,11 @@ from .packed_b import (  # noqa: F401
     MANTISSA_BIAS,
 )
 from .attention import attention_error, packed_attention  # noqa: F401
+from .embed import Embedding, embedding  # noqa: F401
 from .distill import distill_loss, distill_loss_and_grad  # noqa: F401
 from .norm import LayerNorm, layer_norm  # noqa: F401
+from .rotary import QKNormRope, qk_norm_rope, rope_tables  # noqa: F401
+from .saved8 import Saved8, gated_unit, gemm_dw8_error, grad_weight8, save8  # noqa: F401
 
 __all__ = [
     "GatedRebalance",
@@ -65,4 +68,14 @@ __all__ = [
     "layer_norm",
     "distill_loss",
     "distill_loss_and_grad",
+    "Embedding",
+    "embedding",
+    "QKNormRope",
+    "qk_norm_rope",
+    "rope_tables",
+    "Saved8",
+    "save8",
+    "grad_weight8",
+    "gated_unit",
+    "gemm_dw8_error",
 ]

@@ -177,6 +177,26 @@ class AttentionParams(ctypes.Structure):
     ]
 
 
+class QKParams(ctypes.Structure):
+    """Mirror of `concord_qk_params` (include/concord_b200.h)."""
+    _fields_ = [
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("rot", ctypes.c_int64),
+        ("positions", ctypes.c_int64),
+        ("pos64", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 _LIB = None
 
 _P = ctypes.c_void_p
@@ -271,6 +291,24 @@ _SIGS = [
     ("concord_attention_error", ctypes.c_int, [_I32]),
     ("concord_attention_error_word", ctypes.POINTER(_I32), []),
     ("concord_attention_wait_check", ctypes.c_int, [_P]),
+    ("concord_embedding_fwd", ctypes.c_int, [_P, _I32, _P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _F, _P]),
+    ("concord_embedding_bwd_workspace_bytes", ctypes.c_size_t, [_I64, _I64, _I64]),
+    ("concord_embedding_bwd", ctypes.c_int,
+     [_P, _I32, _P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _F, _I64, _P, ctypes.c_size_t, _P]),
+    ("concord_qk_norm_rope_fwd", ctypes.c_int, [ctypes.POINTER(QKParams)] + [_P, _I64, _I64] * 2 + [_P] * 5),
+    ("concord_qk_norm_rope_bwd_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(QKParams)]),
+    ("concord_qk_norm_rope_bwd", ctypes.c_int,
+     [ctypes.POINTER(QKParams)] + [_P, _I64, _I64] * 2 + [_P] * 2 + [_P, _I64, _I64] * 2 + [_P] * 5 +
+     [ctypes.c_size_t, _P]),
+    ("concord_saved8_bytes", ctypes.c_size_t, [_I64, _I64]),
+    ("concord_save8", ctypes.c_int, [_P, _I32, _I64, _P, _I64, _I64, _P]),
+    ("concord_dense8", ctypes.c_int, [_P, _P, _I32, _I64, _I64, _I64, _P]),
+    ("concord_gemm_dw8_workspace_bytes", ctypes.c_size_t, [_I64, _I64, _I64]),
+    ("concord_gemm_dw8", ctypes.c_int, [_P, _I64, _P, _P, _I64, _I64, _I64, _P, ctypes.c_size_t, _P]),
+    ("concord_gemm_dw8_error", ctypes.c_int, [_I32]),
+    ("concord_gated_fwd", ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I64, _I64, _P]),
+    ("concord_gated_bwd", ctypes.c_int,
+     [_P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]

@@ -1,0 +1,396 @@
+// eight.cu — activations kept in 8 bits for the backward pass (the format: eight.cuh):
+// saved, read back, and the gated unit whose gradient is computed from them.
+//
+//   h = act(g) u,  act(g) = g sigmoid(g) or g Phi(g)
+//   dg = dh u act'(g),  du = dh act(g),  g and u as kept (8 bits, or the inputs themselves)
+//   silu'(g) = q + g q (1 - q), q = sigmoid(g);  gelu'(g) = Phi(g) + g phi(g)
+//
+// Bound by memory.  A thread owns a block's 32 tokens of a few neighbouring
+// features (8 bytes of each row): the largest magnitude needs no exchange, all its
+// loads are on their way at once, and what it writes are whole pieces of 16 codes.
+#include "common.cuh"
+#include "eight.cuh"
+
+namespace concord {
+namespace eight {
+
+constexpr int THREADS = 128;
+
+
+template <typename T, int EL>
+__global__ void __launch_bounds__(THREADS)
+    save_kernel(const T* x, int64_t ldx, int8_t* codes, uint8_t* scales, int64_t M, int K) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
+    const int64_t tb = blockIdx.x, t0 = tb * BLOCK;
+    if (k >= K) return;
+    Tile<T, EL> A;
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) A.load_row(i, x + (t0 + i) * ldx + k, t0 + i < M);
+    A.save(codes, scales, tb, K, k);
+}
+
+// a thread: 16 tokens of EL features
+template <typename T, int EL>
+__global__ void __launch_bounds__(THREADS)
+    dense_kernel(const int8_t* codes, const uint8_t* scales, T* out, int64_t ldo, int64_t M, int K) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
+    const int64_t tb = blockIdx.x, t0 = tb * 16;
+    if (k >= K || t0 >= M) return;
+    uint4 c[EL];
+    float scale[EL];
+#pragma unroll
+    for (int j = 0; j < EL; ++j) c[j] = reinterpret_cast<const uint4*>(codes)[tb * K + k + j];
+#pragma unroll
+    for (int j = 0; j < EL; ++j) scale[j] = scale_of(scales[(tb >> 1) * scale_row(K) + k + j]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (t0 + i >= M) break;
+        T v[EL];
+#pragma unroll
+        for (int j = 0; j < EL; ++j) {
+            const uint32_t w = (i < 4 ? c[j].x : i < 8 ? c[j].y : i < 12 ? c[j].z : c[j].w) ^ 0x80808080u;
+            v[j] = from_f32<T>(value(w, i & 3, scale[j], value_off(scale[j])));
+        }
+        T* p = out + (t0 + i) * ldo + k;
+        if constexpr (EL * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(v);
+        else if constexpr (EL * sizeof(T) == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+        else p[0] = v[0];
+    }
+}
+
+// ---------------------------------------------------------------- the gated unit
+constexpr int SILU = 0, GELU = 1;
+
+__device__ __forceinline__ float sigmoid(float g) { return __frcp_rn(1.f + ex2f(-1.4426950408889634f * g)); }
+
+template <int ACT> __device__ __forceinline__ float act(float g) {
+    if constexpr (ACT == SILU) return g * sigmoid(g);
+    else return 0.5f * g * (1.f + erff(g * 0.7071067811865476f));
+}
+// act(g) and its derivative
+template <int ACT> __device__ __forceinline__ float2 act2(float g) {
+    if constexpr (ACT == SILU) {
+        const float q = sigmoid(g), a = g * q;
+        return make_float2(a, q + a * (1.f - q));
+    } else {
+        const float p = 0.5f + 0.5f * erff(g * 0.7071067811865476f);
+        return make_float2(g * p, p + g * 0.3989422804014327f * ex2f(-0.7213475204444817f * g * g));
+    }
+}
+
+struct Unit {
+    const void *gate, *up;       // NULL gate in the backward: from the codes
+    int64_t ldg, ldu;
+    int8_t *g8, *u8, *h8;        // NULL: not kept; their bytes stand behind the codes
+    int64_t M;
+    int K;
+};
+__device__ __forceinline__ uint8_t* scales_of(int8_t* codes, int64_t M, int64_t K) {
+    return reinterpret_cast<uint8_t*>(codes) + code_bytes(M, K);
+}
+
+// forward of 32 tokens x EL features a thread, with what is asked for kept in 8 bits
+template <typename T, int EL, int ACT>
+__global__ void __launch_bounds__(THREADS) fwd8_kernel(const __grid_constant__ Unit U, T* h) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
+    const int64_t tb = blockIdx.x, t0 = tb * BLOCK;
+    if (k >= U.K) return;
+    Tile<T, EL> G, P;
+    const T *g = static_cast<const T*>(U.gate) + t0 * U.ldg + k, *u = static_cast<const T*>(U.up) + t0 * U.ldu + k;
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) G.load_row(i, g + i * U.ldg, t0 + i < U.M);
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) P.load_row(i, u + i * U.ldu, t0 + i < U.M);
+    if (U.g8) G.save(U.g8, scales_of(U.g8, U.M, U.K), tb, U.K, k);
+    if (U.u8) P.save(U.u8, scales_of(U.u8, U.M, U.K), tb, U.K, k);
+    T* out = h + t0 * U.K + k;
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) {
+        float v[EL];
+#pragma unroll
+        for (int j = 0; j < EL; ++j) v[j] = act<ACT>(G.get(i, j)) * P.get(i, j);
+        G.set_row(i, v);
+        if (t0 + i < U.M) G.store_row(i, out + (int64_t)i * U.K);
+    }
+    if (U.h8) G.save(U.h8, scales_of(U.h8, U.M, U.K), tb, U.K, k);
+}
+
+// backward from the codes, 16 tokens x EL features a thread
+template <typename T, int EL, int ACT>
+__global__ void __launch_bounds__(THREADS)
+    bwd8_kernel(const __grid_constant__ Unit U, const T* dh, int64_t lddh, T* dg, int64_t lddg, T* du, int64_t lddu) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
+    const int64_t tb = blockIdx.x, t0 = tb * 16;
+    if (k >= U.K || t0 >= U.M) return;
+    Tile<T, EL> D;
+    uint4 cg[EL], cu[EL];
+    float sg[EL], su[EL];
+#pragma unroll
+    for (int j = 0; j < EL; ++j) {
+        cg[j] = reinterpret_cast<const uint4*>(U.g8)[tb * U.K + k + j];
+        cu[j] = reinterpret_cast<const uint4*>(U.u8)[tb * U.K + k + j];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) D.load_row(i, dh + (t0 + i) * lddh + k, t0 + i < U.M);
+#pragma unroll
+    for (int j = 0; j < EL; ++j) {
+        sg[j] = scale_of(scales_of(U.g8, U.M, U.K)[(tb >> 1) * scale_row(U.K) + k + j]);
+        su[j] = scale_of(scales_of(U.u8, U.M, U.K)[(tb >> 1) * scale_row(U.K) + k + j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float a[EL], b[EL];
+#pragma unroll
+        for (int j = 0; j < EL; ++j) {
+            const uint32_t wg = (i < 4 ? cg[j].x : i < 8 ? cg[j].y : i < 12 ? cg[j].z : cg[j].w) ^ 0x80808080u;
+            const uint32_t wu = (i < 4 ? cu[j].x : i < 8 ? cu[j].y : i < 12 ? cu[j].z : cu[j].w) ^ 0x80808080u;
+            const float g = value(wg, i & 3, sg[j], value_off(sg[j])), u = value(wu, i & 3, su[j], value_off(su[j]));
+            const float2 f = act2<ACT>(g);
+            const float d = D.get(i, j);
+            a[j] = d * u * f.y;
+            b[j] = d * f.x;
+        }
+        if (t0 + i < U.M) {
+            Tile<T, EL> O;
+            O.set_row(0, a);
+            O.store_row(0, dg + (t0 + i) * lddg + k);
+            O.set_row(0, b);
+            O.store_row(0, du + (t0 + i) * lddu + k);
+        }
+    }
+}
+
+// forward and backward on the inputs themselves: VEC features of ROWS tokens a thread
+template <typename T, int VEC, int ROWS, int ACT>
+__global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Unit U, T* h) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
+    if (k >= U.K) return;
+    float g[ROWS][VEC], u[ROWS][VEC];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (t0 + r >= U.M) break;
+        load_vec<VEC>(static_cast<const T*>(U.gate) + (t0 + r) * U.ldg + k, g[r]);
+        load_vec<VEC>(static_cast<const T*>(U.up) + (t0 + r) * U.ldu + k, u[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (t0 + r >= U.M) break;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) g[r][j] = act<ACT>(g[r][j]) * u[r][j];
+        store_vec<VEC>(h + (t0 + r) * U.K + k, g[r]);
+    }
+}
+
+template <typename T, int VEC, int ROWS, int ACT>
+__global__ void __launch_bounds__(256)
+    bwd_kernel(const __grid_constant__ Unit U, const T* dh, int64_t lddh, T* dg, int64_t lddg, T* du, int64_t lddu) {
+    const int k = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
+    if (k >= U.K) return;
+    float g[ROWS][VEC], u[ROWS][VEC], d[ROWS][VEC];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (t0 + r >= U.M) break;
+        load_vec<VEC>(static_cast<const T*>(U.gate) + (t0 + r) * U.ldg + k, g[r]);
+        load_vec<VEC>(static_cast<const T*>(U.up) + (t0 + r) * U.ldu + k, u[r]);
+        load_vec<VEC>(dh + (t0 + r) * lddh + k, d[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (t0 + r >= U.M) break;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float2 f = act2<ACT>(g[r][j]);
+            g[r][j] = d[r][j] * u[r][j] * f.y;
+            u[r][j] = d[r][j] * f.x;
+        }
+        store_vec<VEC>(dg + (t0 + r) * lddg + k, g[r]);
+        store_vec<VEC>(du + (t0 + r) * lddu + k, u[r]);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+size_t esize(int32_t t) { return t == CONCORD_F32 ? 4 : 2; }
+
+// blocks of whole warps over pieces of `el` features
+void across(int64_t K, int el, int* threads, int* blocks) {
+    const int64_t pieces = (K + el - 1) / el, n = (pieces + THREADS - 1) / THREADS;
+    *blocks = (int)n;
+    *threads = (int)(((pieces + n - 1) / n + 31) / 32 * 32);
+}
+// the same for the elementwise kernels, several rows a block
+void tall(int64_t K, int vec, dim3* threads, int* blocks) {
+    const int64_t pieces = (K + vec - 1) / vec, x = pieces < 256 ? pieces : 256;
+    *threads = dim3((unsigned)x, (unsigned)(256 / x), 1);
+    *blocks = (int)((pieces + x - 1) / x);
+}
+
+int check_shape(const char* name, int32_t type, int64_t M, int64_t K, int64_t ld) {
+    if (type < 0 || type > 2) return fail(CONCORD_EINVAL, std::string(name) + ": unknown element type");
+    if (M < 0 || K <= 0 || ld < K) return fail(CONCORD_ESHAPE, std::string(name) + ": bad extents or row stride");
+    if (K > (1 << 20) || M > ((int64_t)1 << 31))
+        return fail(CONCORD_ETOOBIG, std::string(name) + ": more than 2^20 features or 2^31 tokens");
+    return CONCORD_OK;
+}
+// rows of whole pieces of 8 bytes (`wide`: 16)
+bool rows_fit(const void* p, int64_t ld, int64_t K, int32_t type, int bytes) {
+    const int64_t el = bytes / (int64_t)esize(type);
+    return K % el == 0 && ld % el == 0 && aligned(p, bytes);
+}
+
+template <typename T> int save(const void* x, int64_t ldx, int32_t type, int8_t* codes, int64_t M, int64_t K, cudaStream_t st) {
+    constexpr int EL = 8 / sizeof(T);
+    const bool vec = rows_fit(x, ldx, K, type, 8);
+    int threads, blocks_k;
+    across(K, vec ? EL : 1, &threads, &blocks_k);
+    uint8_t* scales = reinterpret_cast<uint8_t*>(codes) + code_bytes(M, K);
+    auto k = vec ? save_kernel<T, EL> : save_kernel<T, 1>;
+    k<<<dim3((unsigned)blocks(M), blocks_k), threads, 0, st>>>(static_cast<const T*>(x), ldx, codes, scales, M, (int)K);
+    return check_launch("concord_save8");
+}
+
+template <typename T> int dense(const int8_t* codes, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
+    constexpr int EL = 8 / sizeof(T);
+    const bool vec = rows_fit(out, ldo, K, type, 8);
+    int threads, blocks_k;
+    across(K, vec ? EL : 1, &threads, &blocks_k);
+    const uint8_t* scales = reinterpret_cast<const uint8_t*>(codes) + code_bytes(M, K);
+    auto k = vec ? dense_kernel<T, EL> : dense_kernel<T, 1>;
+    k<<<dim3((unsigned)(2 * blocks(M)), blocks_k), threads, 0, st>>>(codes, scales, static_cast<T*>(out), ldo, M, (int)K);
+    return check_launch("concord_dense8");
+}
+
+template <typename T, int ACT> int forward(const Unit& U, void* h, int32_t type, cudaStream_t st) {
+    T* out = static_cast<T*>(h);
+    if (U.g8 || U.u8 || U.h8) {
+        constexpr int EL = 8 / sizeof(T);
+        const bool vec = rows_fit(U.gate, U.ldg, U.K, type, 8) && rows_fit(U.up, U.ldu, U.K, type, 8) && aligned(h, 8);
+        int threads, blocks_k;
+        across(U.K, vec ? EL : 1, &threads, &blocks_k);
+        auto k = vec ? fwd8_kernel<T, EL, ACT> : fwd8_kernel<T, 1, ACT>;
+        k<<<dim3((unsigned)blocks(U.M), blocks_k), threads, 0, st>>>(U, out);
+        return check_launch("concord_gated_fwd");
+    }
+    const bool vec = U.K % 8 == 0 && rows_fit(U.gate, U.ldg, U.K, type, 16) && rows_fit(U.up, U.ldu, U.K, type, 16) && aligned(h, 16);
+    dim3 threads;
+    int blocks_k;
+    tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
+    const int64_t rows = (vec ? 2 : 1) * threads.y;
+    auto k = vec ? fwd_kernel<T, 8, 2, ACT> : fwd_kernel<T, 1, 1, ACT>;
+    k<<<dim3((unsigned)((U.M + rows - 1) / rows), blocks_k), threads, 0, st>>>(U, out);
+    return check_launch("concord_gated_fwd");
+}
+
+template <typename T, int ACT>
+int backward(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg, void* du, int64_t lddu, int32_t type,
+             cudaStream_t st) {
+    const T* up = static_cast<const T*>(dh);
+    T *og = static_cast<T*>(dg), *ou = static_cast<T*>(du);
+    if (U.g8) {
+        constexpr int EL = 8 / sizeof(T);
+        const bool vec = rows_fit(dh, lddh, U.K, type, 8) && rows_fit(dg, lddg, U.K, type, 8) && rows_fit(du, lddu, U.K, type, 8);
+        int threads, blocks_k;
+        across(U.K, vec ? EL : 1, &threads, &blocks_k);
+        auto k = vec ? bwd8_kernel<T, EL, ACT> : bwd8_kernel<T, 1, ACT>;
+        k<<<dim3((unsigned)(2 * blocks(U.M)), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
+        return check_launch("concord_gated_bwd");
+    }
+    const bool vec = U.K % 8 == 0 && rows_fit(U.gate, U.ldg, U.K, type, 16) && rows_fit(U.up, U.ldu, U.K, type, 16) &&
+                     rows_fit(dh, lddh, U.K, type, 16) && rows_fit(dg, lddg, U.K, type, 16) && rows_fit(du, lddu, U.K, type, 16);
+    dim3 threads;
+    int blocks_k;
+    tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
+    const int64_t rows = threads.y;
+    auto k = vec ? bwd_kernel<T, 8, 1, ACT> : bwd_kernel<T, 1, 1, ACT>;
+    k<<<dim3((unsigned)((U.M + rows - 1) / rows), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
+    return check_launch("concord_gated_bwd");
+}
+
+#define EIGHT_TYPES(type, F, ...)                                         \
+    switch (type) {                                                       \
+        case CONCORD_F32: return F<float>(__VA_ARGS__);                   \
+        case CONCORD_BF16: return F<__nv_bfloat16>(__VA_ARGS__);          \
+        default: return F<__half>(__VA_ARGS__);                           \
+    }
+#define GATED_TYPES(type, a, F, ...)                                                                                    \
+    switch ((type) * 2 + (a)) {                                                                                         \
+        case 0: return F<float, SILU>(__VA_ARGS__);                                                                     \
+        case 1: return F<float, GELU>(__VA_ARGS__);                                                                     \
+        case 2: return F<__nv_bfloat16, SILU>(__VA_ARGS__);                                                             \
+        case 3: return F<__nv_bfloat16, GELU>(__VA_ARGS__);                                                             \
+        case 4: return F<__half, SILU>(__VA_ARGS__);                                                                    \
+        default: return F<__half, GELU>(__VA_ARGS__);                                                                   \
+    }
+
+int save_any(const void* x, int64_t ldx, int32_t type, int8_t* codes, int64_t M, int64_t K, cudaStream_t st) {
+    EIGHT_TYPES(type, save, x, ldx, type, codes, M, K, st)
+}
+int dense_any(const int8_t* codes, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
+    EIGHT_TYPES(type, dense, codes, out, ldo, type, M, K, st)
+}
+int forward_any(const Unit& U, void* h, int32_t type, int a, cudaStream_t st) {
+    GATED_TYPES(type, a, forward, U, h, type, st)
+}
+int backward_any(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg, void* du, int64_t lddu,
+                 int32_t type, int a, cudaStream_t st) {
+    GATED_TYPES(type, a, backward, U, dh, lddh, dg, lddg, du, lddu, type, st)
+}
+
+}  // namespace eight
+}  // namespace concord
+
+using namespace concord;
+
+extern "C" size_t concord_saved8_bytes(int64_t M, int64_t K) {
+    if (M <= 0 || K <= 0 || K > (1 << 20) || M > ((int64_t)1 << 31)) return 0;
+    return (size_t)(eight::code_bytes(M, K) + eight::blocks(M) * eight::scale_row(K));
+}
+
+extern "C" int concord_save8(const void* x, int32_t type, int64_t ldx, void* saved, int64_t M, int64_t K, void* stream) {
+    if (int rc = eight::check_shape("concord_save8", type, M, K, ldx)) return rc;
+    if (M == 0) return CONCORD_OK;
+    if (!x || !saved) return fail(CONCORD_EINVAL, "concord_save8: null pointer");
+    if (!aligned(saved, 16)) return fail(CONCORD_EALIGN, "concord_save8: saved must be 16-byte aligned");
+    return eight::save_any(x, ldx, type, static_cast<int8_t*>(saved), M, K, as_stream(stream));
+}
+
+extern "C" int concord_dense8(const void* saved, void* out, int32_t type, int64_t ldo, int64_t M, int64_t K, void* stream) {
+    if (int rc = eight::check_shape("concord_dense8", type, M, K, ldo)) return rc;
+    if (M == 0) return CONCORD_OK;
+    if (!out || !saved) return fail(CONCORD_EINVAL, "concord_dense8: null pointer");
+    if (!aligned(saved, 16)) return fail(CONCORD_EALIGN, "concord_dense8: saved must be 16-byte aligned");
+    return eight::dense_any(static_cast<const int8_t*>(saved), out, ldo, type, M, K, as_stream(stream));
+}
+
+extern "C" int concord_gated_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t type, int32_t act,
+                                 void* h, void* saved_gate, void* saved_up, void* saved_h, int64_t M, int64_t K,
+                                 void* stream) {
+    if (int rc = eight::check_shape("concord_gated_fwd", type, M, K, ldg < ldu ? ldg : ldu)) return rc;
+    if (act < 0 || act > 1) return fail(CONCORD_EINVAL, "concord_gated_fwd: unknown activation");
+    if (M == 0) return CONCORD_OK;
+    if (!gate || !up || !h) return fail(CONCORD_EINVAL, "concord_gated_fwd: null pointer");
+    if (!aligned(saved_gate, 16) || !aligned(saved_up, 16) || !aligned(saved_h, 16))
+        return fail(CONCORD_EALIGN, "concord_gated_fwd: saved tensors must be 16-byte aligned");
+    const eight::Unit U{gate, up, ldg, ldu, static_cast<int8_t*>(saved_gate), static_cast<int8_t*>(saved_up),
+                        static_cast<int8_t*>(saved_h), M, (int)K};
+    return eight::forward_any(U, h, type, act, as_stream(stream));
+}
+
+extern "C" int concord_gated_bwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, const void* saved_gate,
+                                 const void* saved_up, int32_t type, int32_t act, const void* dh, int64_t lddh,
+                                 void* dgate, int64_t lddg, void* dup, int64_t lddu, int64_t M, int64_t K, void* stream) {
+    const char* name = "concord_gated_bwd";
+    const int64_t lo = lddh < lddg ? lddh : lddg;
+    if (int rc = eight::check_shape(name, type, M, K, lo < lddu ? lo : lddu)) return rc;
+    if (act < 0 || act > 1) return fail(CONCORD_EINVAL, std::string(name) + ": unknown activation");
+    if (M == 0) return CONCORD_OK;
+    if (!dh || !dgate || !dup || !saved_gate != !saved_up || (!saved_gate && (!gate || !up)))
+        return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
+    if (!saved_gate && (ldg < K || ldu < K)) return fail(CONCORD_ESHAPE, std::string(name) + ": bad row stride");
+    if (!aligned(saved_gate, 16) || !aligned(saved_up, 16))
+        return fail(CONCORD_EALIGN, std::string(name) + ": saved tensors must be 16-byte aligned");
+    const eight::Unit U{gate, up, ldg, ldu, static_cast<int8_t*>(const_cast<void*>(saved_gate)),
+                        static_cast<int8_t*>(const_cast<void*>(saved_up)), nullptr, M, (int)K};
+    return eight::backward_any(U, dh, lddh, dgate, lddg, dup, lddu, type, act, as_stream(stream));
+}

@@ -82,7 +82,7 @@ __device__ __forceinline__ bool gave_up(uint32_t bar) {
 // in *err, or at once where another of the block has.  (The loops are calls: as
 // code in every place they made the forward of 64 x 256 tokens 4 us slower than
 // its 31.)
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
     Patience patience;
     for (int i = 1;; ++i) {
         if (mbar_try(bar, parity)) return true;
@@ -98,7 +98,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
 }
 // The same by a whole warp, which stays converged: every branch goes by a vote,
 // so that all lanes go on or none does.
-__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
+static __device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, int code) {
     Patience patience;
 #pragma unroll 1
     for (int i = 1; !__all_sync(0xffffffffu, mbar_try(bar, parity)); ++i) {
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* er
 }
 // Given up after `sent` tiles into a ring of `stages` (their barriers 8 bytes
 // apart): what is on its way lands first, or that wait too runs out.
-__device__ __noinline__ bool ring_landed(uint32_t full, int stages, int sent, int* err) {
+static __device__ __noinline__ bool ring_landed(uint32_t full, int stages, int sent, int* err) {
     for (int x = max(0, sent - stages); x < sent; ++x) {
         const uint32_t bar = full + 8u * (x % stages), parity = (x / stages) & 1;
         Patience patience;

@@ -5,7 +5,7 @@
 // engine's thread, a dozen converted arguments a call), of which the kernels
 // need a third.  Here a call allocates its outputs, hands over plain pointers
 // and links one node into the graph.  Arguments are checked by the Python
-// functions that call these (norm.py, distill.py, attention.py).
+// functions that call these (norm.py, distill.py, attention.py, embed.py, rotary.py, saved8.py).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -381,6 +381,304 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q0, const Tensor& k0, const T
     return {o, lse};
 }
 
+// ---------------------------------------------------------------- embedding
+at::ScalarType type_of(int64_t code) {
+    return code == CONCORD_F32 ? at::kFloat : code == CONCORD_BF16 ? at::kBFloat16 : at::kHalf;
+}
+Tensor bytes_like(const Tensor& t, size_t bytes) {
+    return at::empty({(int64_t)bytes}, t.options().requires_grad(false).dtype(at::kByte));
+}
+
+struct EmbeddingBackward : public torch::autograd::Node {
+    SavedVariable ids_;
+    at::TensorOptions options;
+    int64_t V = 0, D = 0, padding = -1;
+    double scale = 1;
+    std::string name() const override { return "ConcordEmbeddingBackward"; }
+    void release_variables() override { ids_.reset_data(); }
+    variable_list apply(variable_list&& g) override {
+        const Tensor ids = ids_.unpack();
+        variable_list out(1);
+        if (!g[0].defined()) return out;
+        {
+            at::NoGradGuard no_grad;
+            c10::cuda::CUDAGuard guard(ids.device());
+            const Tensor dy = rows(g[0], D);
+            const int64_t T = ids.numel();
+            out[0] = at::empty({V, D}, options);
+            const size_t bytes = concord_embedding_bwd_workspace_bytes(T, V, D);
+            const Tensor ws = bytes_like(ids, bytes);
+            check(concord_embedding_bwd(ptr(ids), ids.scalar_type() == at::kLong, ptr(dy), type_code(dy), ld(dy, D),
+                                        ptr(out[0]), type_code(out[0]), T, V, D, (float)scale, padding, ptr(ws), bytes,
+                                        current_stream()),
+                  "concord_embedding_bwd");
+        }
+        return once(std::move(out), g);
+    }
+};
+
+Tensor embedding(const Tensor& ids0, const Tensor& weight, double scale, int64_t padding, int64_t out_code) {
+    refuse_transforms({weight}, "embedding");
+    const bool grad = at::GradMode::is_enabled() && wants_grad(weight);
+    c10::cuda::CUDAGuard guard(weight.device());
+    const int64_t V = weight.size(0), D = weight.size(1);
+    Tensor y, ids;
+    {
+        at::NoGradGuard no_grad;
+        ids = ids0.reshape({-1}).contiguous();
+        const Tensor w = rows(weight, D);
+        auto shape = ids0.sizes().vec();
+        shape.push_back(D);
+        y = at::empty(shape, weight.options().requires_grad(false).dtype(type_of(out_code)));
+        check(concord_embedding_fwd(ptr(ids), ids.scalar_type() == at::kLong, ptr(w), type_code(w), ld(w, D), ptr(y),
+                                    (int32_t)out_code, ids.numel(), V, D, (float)scale, current_stream()),
+              "concord_embedding_fwd");
+    }
+    if (grad) {
+        auto node = link<EmbeddingBackward>(weight);
+        node->ids_ = SavedVariable(ids, false);
+        node->options = weight.options().requires_grad(false);
+        node->V = V;
+        node->D = D;
+        node->padding = padding;
+        node->scale = scale;
+        torch::autograd::set_history(y, node);
+    }
+    return y;
+}
+
+// ---------------------------------------------------------------- norm and rotation of queries and keys
+// t [T, H, D] with contiguous columns, and its strides (of a dimension of size one: the dense one)
+struct Heads {
+    Tensor t;
+    int64_t ts = 0, hs = 0;
+    explicit Heads(const Tensor& x) {
+        if (!x.defined()) return;
+        t = x.size(2) > 1 && x.stride(2) != 1 ? x.contiguous() : x;
+        hs = t.size(1) > 1 ? t.stride(1) : t.size(2);
+        ts = t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+    }
+};
+
+struct QKArgs {
+    Tensor cos, sin, pos;
+    bool norm = true, interleaved = false;
+    double eps = 0;
+    concord_qk_params params(const Tensor& like, int64_t heads, int64_t kv_heads) const {
+        concord_qk_params p{};
+        p.cos = ptr<const float>(cos);
+        p.sin = ptr<const float>(sin);
+        p.pos = ptr(pos);
+        p.pos64 = pos.defined() && pos.scalar_type() == at::kLong;
+        p.tokens = like.size(0);
+        p.heads = heads;
+        p.kv_heads = kv_heads;
+        p.head_dim = like.size(2);
+        p.rot = cos.defined() ? 2 * cos.size(1) : 0;
+        p.positions = cos.defined() ? cos.size(0) : 0;
+        p.type = type_code(like);
+        p.norm = norm;
+        p.interleaved = interleaved;
+        p.eps = (float)eps;
+        return p;
+    }
+};
+
+struct QKNormRopeBackward : public torch::autograd::Node {
+    SavedVariable q_, k_, qw_, kw_, cos_, sin_, pos_;
+    bool norm = true, interleaved = false, has_k = false;
+    double eps = 0;
+    std::string name() const override { return "ConcordQKNormRopeBackward"; }
+    void release_variables() override {
+        for (SavedVariable* v : {&q_, &k_, &qw_, &kw_, &cos_, &sin_, &pos_}) v->reset_data();
+    }
+    variable_list apply(variable_list&& g) override {
+        const Tensor q = q_.unpack(), k = k_.unpack(), qw = qw_.unpack(), kw = kw_.unpack();
+        QKArgs A;
+        A.cos = cos_.unpack();
+        A.sin = sin_.unpack();
+        A.pos = pos_.unpack();
+        A.norm = norm;
+        A.interleaved = interleaved;
+        A.eps = eps;
+        variable_list out(4);
+        const bool has_q = g[0].defined(), with_k = has_k && g.size() > 1 && g[1].defined();
+        if (!has_q && !with_k) return out;
+        {
+            at::NoGradGuard no_grad;
+            const Tensor& like = has_q ? g[0] : g[1];
+            c10::cuda::CUDAGuard guard(like.device());
+            const Heads dq(has_q ? g[0] : Tensor()), dk(with_k ? g[1] : Tensor());
+            const Heads xq(has_q ? q : Tensor()), xk(with_k ? k : Tensor());
+            const auto plain = like.options().requires_grad(false);
+            if (has_q) out[0] = at::empty(g[0].sizes(), plain);
+            if (with_k) out[1] = at::empty(g[1].sizes(), plain);
+            if (has_q && qw.defined() && task_should_compute_output(2)) out[2] = at::empty(qw.sizes(), qw.options().requires_grad(false));
+            if (with_k && kw.defined() && task_should_compute_output(3)) out[3] = at::empty(kw.sizes(), kw.options().requires_grad(false));
+            const auto p = A.params(like, has_q ? g[0].size(1) : 0, with_k ? g[1].size(1) : 0);
+            Tensor ws;
+            size_t bytes = 0;
+            if (out[2].defined() || out[3].defined()) {
+                bytes = concord_qk_norm_rope_bwd_workspace_bytes(&p);
+                ws = bytes_like(like, bytes);
+            }
+            check(concord_qk_norm_rope_bwd(&p, ptr(xq.t), xq.ts, xq.hs, ptr(xk.t), xk.ts, xk.hs, ptr<const float>(qw),
+                                           ptr<const float>(kw), ptr(dq.t), dq.ts, dq.hs, ptr(dk.t), dk.ts, dk.hs, ptr(out[0]),
+                                           ptr(out[1]), ptr<float>(out[2]), ptr<float>(out[3]), ptr(ws), bytes,
+                                           current_stream()),
+                  "concord_qk_norm_rope_bwd");
+        }
+        return once(std::move(out), g);
+    }
+};
+
+std::tuple<Tensor, MaybeTensor> qk_norm_rope(const Tensor& q, const MaybeTensor& k_in, const MaybeTensor& cos,
+                                             const MaybeTensor& sin, const MaybeTensor& pos, const MaybeTensor& q_weight,
+                                             const MaybeTensor& k_weight, bool norm, double eps, bool interleaved) {
+    const Tensor k = get(k_in), qw = get(q_weight), kw = get(k_weight);
+    QKArgs A;
+    A.cos = get(cos);
+    A.sin = get(sin);
+    A.pos = get(pos);
+    A.norm = norm;
+    A.interleaved = interleaved;
+    A.eps = eps;
+    refuse_transforms({q, k, qw, kw, A.cos, A.sin}, "qk_norm_rope");
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw));
+    c10::cuda::CUDAGuard guard(q.device());
+    Tensor q_out, k_out;
+    const Heads hq(q.detach()), hk(k.defined() ? k.detach() : k);
+    {
+        at::NoGradGuard no_grad;
+        const auto plain = q.options().requires_grad(false);
+        q_out = at::empty(q.sizes(), plain);
+        if (k.defined()) k_out = at::empty(k.sizes(), plain);
+        const auto p = A.params(q, q.size(1), k.defined() ? k.size(1) : 0);
+        check(concord_qk_norm_rope_fwd(&p, ptr(hq.t), hq.ts, hq.hs, ptr(hk.t), hk.ts, hk.hs, ptr<const float>(qw),
+                                       ptr<const float>(kw), ptr(q_out), ptr(k_out), current_stream()),
+              "concord_qk_norm_rope_fwd");
+    }
+    if (grad) {
+        auto node = link<QKNormRopeBackward>(q, k, qw, kw);
+        if (norm) {                      // (the rotation's gradient does not read them)
+            node->q_ = SavedVariable(hq.t, false);
+            node->k_ = SavedVariable(hk.t, false);
+            node->qw_ = SavedVariable(qw, false);
+            node->kw_ = SavedVariable(kw, false);
+        }
+        node->cos_ = SavedVariable(A.cos, false);
+        node->sin_ = SavedVariable(A.sin, false);
+        node->pos_ = SavedVariable(A.pos, false);
+        node->norm = norm;
+        node->interleaved = interleaved;
+        node->eps = eps;
+        node->has_k = k.defined();
+        torch::autograd::set_history(q_out, node);
+        if (k.defined()) torch::autograd::set_history(k_out, node);
+    }
+    return {q_out, k_out.defined() ? MaybeTensor(k_out) : MaybeTensor()};
+}
+
+// ---------------------------------------------------------------- activations in 8 bits
+Tensor save8(const Tensor& x) {
+    refuse_transforms({x}, "save8");
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t K = x.size(-1);
+    const Tensor x2 = rows(x, K);
+    const Tensor out = bytes_like(x, concord_saved8_bytes(x2.size(0), K));
+    check(concord_save8(ptr(x2), type_code(x2), ld(x2, K), ptr(out), x2.size(0), K, current_stream()), "concord_save8");
+    return out;
+}
+
+Tensor dense8(const Tensor& saved, int64_t M, int64_t K, int64_t code) {
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(saved.device());
+    const Tensor out = at::empty({M, K}, saved.options().dtype(type_of(code)));
+    check(concord_dense8(ptr(saved), ptr(out), (int32_t)code, K, M, K, current_stream()), "concord_dense8");
+    return out;
+}
+
+Tensor grad_weight8(const Tensor& dy0, const Tensor& saved, int64_t M, int64_t K) {
+    refuse_transforms({dy0}, "grad_weight8");
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(saved.device());
+    const int64_t N = dy0.size(-1);
+    Tensor dy = rows(dy0, N);
+    if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 || ld(dy, N) % 8) dy = at::empty(dy.sizes(), dy.options()).copy_(dy);
+    const Tensor dw = at::empty({N, K}, dy.options().requires_grad(false));
+    const size_t bytes = concord_gemm_dw8_workspace_bytes(M, N, K);
+    const Tensor ws = bytes_like(dy, bytes);
+    check(concord_gemm_dw8(ptr<const uint16_t>(dy), ld(dy, N), ptr(saved), ptr<uint16_t>(dw), M, N, K, ptr(ws), bytes,
+                           current_stream()),
+          "concord_gemm_dw8");
+    return dw;
+}
+
+struct GatedBackward : public torch::autograd::Node {
+    SavedVariable gate_, up_;            // [M, K], or their 8-bit form
+    bool eight = false;
+    int64_t act = 0, M = 0, K = 0;
+    std::vector<int64_t> shape;
+    std::string name() const override { return "ConcordGatedBackward"; }
+    void release_variables() override { gate_.reset_data(); up_.reset_data(); }
+    variable_list apply(variable_list&& g) override {
+        const Tensor gate = gate_.unpack(), up = up_.unpack();
+        variable_list out(2);
+        if (!g[0].defined()) return out;
+        {
+            at::NoGradGuard no_grad;
+            c10::cuda::CUDAGuard guard(gate.device());
+            const Tensor dh = rows(g[0], K);
+            out[0] = at::empty(shape, dh.options().requires_grad(false));
+            out[1] = at::empty(shape, dh.options().requires_grad(false));
+            check(concord_gated_bwd(eight ? nullptr : ptr(gate), eight ? 0 : ld(gate, K), eight ? nullptr : ptr(up),
+                                    eight ? 0 : ld(up, K), eight ? ptr(gate) : nullptr, eight ? ptr(up) : nullptr,
+                                    type_code(dh), (int32_t)act, ptr(dh), ld(dh, K), ptr(out[0]), K, ptr(out[1]), K, M, K,
+                                    current_stream()),
+                  "concord_gated_bwd");
+        }
+        return once(std::move(out), g);
+    }
+};
+
+std::tuple<Tensor, MaybeTensor> gated_unit(const Tensor& gate0, const Tensor& up0, int64_t act, bool keep8, bool out8) {
+    refuse_transforms({gate0, up0}, "gated_unit");
+    const bool grad = at::GradMode::is_enabled() && (wants_grad(gate0) || wants_grad(up0));
+    c10::cuda::CUDAGuard guard(gate0.device());
+    const int64_t K = gate0.size(-1);
+    Tensor gate, up, h, g8, u8, h8;
+    int64_t M;
+    {
+        at::NoGradGuard no_grad;
+        gate = rows(gate0, K);
+        up = rows(up0, K);
+        M = gate.size(0);
+        h = at::empty(gate0.sizes(), gate0.options().requires_grad(false));
+        const size_t bytes = concord_saved8_bytes(M, K);
+        if (grad && keep8) {
+            g8 = bytes_like(gate, bytes);
+            u8 = bytes_like(gate, bytes);
+        }
+        if (out8) h8 = bytes_like(gate, bytes);
+        check(concord_gated_fwd(ptr(gate), ld(gate, K), ptr(up), ld(up, K), type_code(gate), (int32_t)act, ptr(h), ptr(g8),
+                                ptr(u8), ptr(h8), M, K, current_stream()),
+              "concord_gated_fwd");
+    }
+    if (grad) {
+        auto node = link<GatedBackward>(gate0, up0);
+        node->gate_ = SavedVariable(keep8 ? g8 : gate, false);
+        node->up_ = SavedVariable(keep8 ? u8 : up, false);
+        node->eight = keep8;
+        node->act = act;
+        node->M = M;
+        node->K = K;
+        node->shape = gate0.sizes().vec();
+        torch::autograd::set_history(h, node);
+    }
+    return {h, h8.defined() ? MaybeTensor(h8) : MaybeTensor()};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -390,4 +688,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("distill_loss", &distill_loss, release());
     m.def("distill_loss_and_grad", &distill_loss_and_grad, release());
     m.def("attention", &attention, release());
+    m.def("embedding", &embedding, release());
+    m.def("qk_norm_rope", &qk_norm_rope, release());
+    m.def("save8", &save8, release());
+    m.def("dense8", &dense8, release());
+    m.def("grad_weight8", &grad_weight8, release());
+    m.def("gated_unit", &gated_unit, release());
 }

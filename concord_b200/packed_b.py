@@ -19,6 +19,7 @@ import torch.nn as nn
 
 from . import _abi
 from . import gemm as _gemm
+from . import saved8 as _saved8
 
 MANTISSA_BIAS = 15
 INT8_MIN, INT8_MAX = -128, 127
@@ -671,11 +672,13 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
                 optimizer_kind, weight_decay, eps, step_cap, v_scale, precond_p, gf_consol,
                 drift_cancel_C, alpha_v_fast, wd_sv, wd_sf, mass_preserve, apply_chase,
                 track_rebalance, weight_buf, row_max_buf, col_max_buf, v_row, v_col, sum_v_inv,
-                adafactor_beta2, track_adafactor_v, gf_trust_delta_sq, coh_pre, coh_stats=None):
+                adafactor_beta2, track_adafactor_v, gf_trust_delta_sq, coh_pre, coh_stats=None,
+                saved=None):
         bias_bf16 = (bias.to(torch.bfloat16)
                      if bias is not None and bias.dtype != torch.bfloat16 else bias)
         y = _gemm.forward(x, weight_buf, bias_bf16)
-        ctx.save_for_backward(x, weight_buf)
+        ctx.saved8 = None if saved is None else (saved.shape, saved.dtype)
+        ctx.save_for_backward(x if saved is None else saved.data, weight_buf)
         vals = (packed_w, row_exp, col_exp, lr, alpha, beta1, mantissa_bias, optimizer_kind,
                 weight_decay, eps, step_cap, v_scale, precond_p, gf_consol, drift_cancel_C,
                 alpha_v_fast, wd_sv, wd_sf, mass_preserve, apply_chase, track_rebalance,
@@ -696,9 +699,15 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
             grad_y = grad_y.contiguous()
         grad_x = _gemm.grad_input(grad_y, weight)
         out_features, in_features = weight.shape
-        x_flat = x.reshape(-1, in_features)
         grad_y_flat = grad_y.reshape(-1, out_features)
-        if _fused_dw_vhat_ok(ctx, grad_y_flat, x_flat):
+        x_flat = x.reshape(-1, in_features) if ctx.saved8 is None else None
+        if ctx.saved8 is not None:          # the input in 8 bits: dW from these, v-hat by its own launch
+            saved = _saved8.Saved8(x, *ctx.saved8)
+            grad_W = _saved8.grad_weight8(grad_y, saved)
+            if _SIGMAG_NOISE:
+                grad_W = sigmag_noise(grad_W, grad_y_flat, saved.dense(torch.bfloat16).view(-1, in_features))
+            _optimizer_half(ctx, grad_W)
+        elif _fused_dw_vhat_ok(ctx, grad_y_flat, x_flat):
             track = bool(ctx.track_rebalance)
             grad_W = dw_vhat_update(grad_y_flat, x_flat, ctx.v_row, ctx.v_col, ctx.sum_v_inv,
                                     ctx.adafactor_beta2, ctx.row_max_buf if track else None,
@@ -710,7 +719,7 @@ class FusedConcordLinearPackedB(torch.autograd.Function):
                 grad_W = sigmag_noise(grad_W, grad_y_flat, x_flat)
             _optimizer_half(ctx, grad_W)
         grad_bias = grad_y_flat.sum(0) if ctx.has_bias else None
-        return (grad_x, None, None, None, grad_bias) + (None,) * 29
+        return (grad_x, None, None, None, grad_bias) + (None,) * 30
 
 
 class ConcordLinearPackedB(nn.Module):
@@ -758,6 +767,8 @@ class ConcordLinearPackedB(nn.Module):
         self.track_rebalance = True
         # fused coherence meter: (sum of coh, count) accumulated by the step kernel
         self.coh_stats = None
+        # keep the input in 8 bits for the backward (dW is computed from these); see save8
+        self.save8 = False
         self.register_buffer('_reb_seed', torch.zeros(1, dtype=torch.int32, device=device))
         self.register_buffer('packed_w', torch.zeros(out_features, in_features,
                                                      dtype=torch.int32, device=device))
@@ -959,16 +970,25 @@ class ConcordLinearPackedB(nn.Module):
         m_gated = (ss * 128.0 + self.fast_gain * sf + vs * 128.0) * torch.exp2(exp)
         wbuf.copy_(m_gated.to(wbuf.dtype))
 
-    def forward(self, x):
+    def forward(self, x, saved=None):
+        """x W^T + bias.  saved: x in 8 bits (save8(x), where several layers read one x, or
+        what gated_unit returns beside its output), which the backward computes dW
+        from in place of x; with the attribute `save8` set the layer makes it itself."""
+        if saved is not None:
+            _saved8._check_saved(saved)
+            if saved.shape != x.shape:
+                raise ValueError(f"saved is of shape {tuple(saved.shape)}, x of {tuple(x.shape)}")
         in_dtype = x.dtype
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
+        if saved is None and self.save8 and torch.is_grad_enabled():
+            saved = _saved8.save8(x.detach())
         wbuf, rmbuf, cmbuf = self._ensure_buffers()
         if self.fast_gain < 1.0:
             with torch.no_grad():
                 self._gated_forward_weight(wbuf)
         y = FusedConcordLinearPackedB.apply(x, self.packed_w, self.row_exp, self.col_exp,
-                                            self.bias, *self._apply_args(wbuf, rmbuf, cmbuf))
+                                            self.bias, *self._apply_args(wbuf, rmbuf, cmbuf), saved)
         return y.to(in_dtype)
 
     @torch.no_grad()

@@ -662,6 +662,93 @@ int concord_attention_error(int32_t reset);
 int32_t* concord_attention_error_word(void);
 int concord_attention_wait_check(void* stream);
 
+/*
+ * Embedding lookup: y[t] = scale * W[ids[t]] for the table w [V, D] (row stride
+ * ldw, columns contiguous); a row whose id is outside [0, V) is 0.  ids [T]
+ * int32 or int64, y [T, D] contiguous in its own type.  The backward writes the
+ * whole gradient dw [V, D] (contiguous, of dw_type): the sums of scale * dy over a
+ * row's tokens, fp32 in a fixed order, rounded once; ids outside [0, V) and
+ * `padding` (negative: none) get nothing.  At most 2^30 tokens and rows.
+ */
+int concord_embedding_fwd(const void* ids, int32_t ids64, const void* w, int32_t w_type, int64_t ldw, void* y,
+                          int32_t y_type, int64_t T, int64_t V, int64_t D, float scale, void* stream);
+size_t concord_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D);
+int concord_embedding_bwd(const void* ids, int32_t ids64, const void* dy, int32_t dy_type, int64_t lddy, void* dw,
+                          int32_t dw_type, int64_t T, int64_t V, int64_t D, float scale, int64_t padding,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Root-mean-square norm of every head of q [tokens, heads, D] and k [tokens,
+ * kv_heads, D] (norm != 0: x / sqrt(mean(x^2) + eps) * weight, fp32 weights [D] or
+ * NULL), then the rotation of their first `rot` columns: pair i is (2i, 2i + 1)
+ * where interleaved, else (i, i + rot / 2); its angle's cosine and sine stand
+ * in cos / sin [positions, rot / 2] at the token's position, pos [tokens] (int32
+ * or int64) or NULL: the token's number.  A position that the tables do not have gives
+ * NaN.  Inputs take a token and a head stride (elements, columns contiguous);
+ * outputs and gradients are contiguous.  heads or kv_heads may be 0.  D <= 256.
+ * The backward writes dq, dk and, unless NULL, the weights' gradients (fp32 [D],
+ * sums in a fixed order); without the norm it does not read q and k.
+ */
+typedef struct concord_qk_params {
+    const float* cos;
+    const float* sin;
+    const void* pos;
+    int64_t tokens, heads, kv_heads, head_dim, rot, positions;
+    int32_t pos64;
+    int32_t type;
+    int32_t norm;
+    int32_t interleaved;
+    float eps;
+} concord_qk_params;
+int concord_qk_norm_rope_fwd(const concord_qk_params* p, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                             int64_t k_ts, int64_t k_hs, const float* q_weight, const float* k_weight, void* q_out,
+                             void* k_out, void* stream);
+size_t concord_qk_norm_rope_bwd_workspace_bytes(const concord_qk_params* p);
+int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                             int64_t k_ts, int64_t k_hs, const float* q_weight, const float* k_weight,
+                             const void* dq_out, int64_t dq_ts, int64_t dq_hs, const void* dk_out, int64_t dk_ts,
+                             int64_t dk_hs, void* dq, void* dk, float* dq_weight, float* dk_weight, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Activations x [M, K] kept in 8 bits for the backward pass: 32 tokens of one
+ * feature share a power of two 2^e, the least with |x| <= 127 2^e, and a value is
+ * the whole number nearest to x / 2^e (ties to even; in the block of a type's largest
+ * values at most 63, which it can still hold).  A block with a NaN or an infinity
+ * reads back as NaN.  `saved`: concord_saved8_bytes(M, K) bytes, 16-byte aligned:
+ *   int8 codes [ceil(M / 32) * 2][K][16]: token 16 i + j of feature k at [i][k][j],
+ *        zeros beyond M;
+ *   uint8 e + 127 (255: NaN) [ceil(M / 32)][K rounded up to 16].
+ * concord_dense8 reads them back, rounded to the type of out [M, K].
+ * concord_gemm_dw8: dw [N, K] (bf16, contiguous) = dy^T x for dy [M, N] (bf16, row
+ * stride lddy) and x in 8 bits: the values it keeps are exact in bf16, sums are fp32,
+ * rounded once.  N and lddy multiples of 8, dy 16-byte aligned; any M and K.
+ * Workspace: 16-byte aligned (sums of parts where outputs are few).  Its waits are bounded as
+ * concord_gemm2sm's are: concord_gemm_dw8_error reads and clears its error word.
+ */
+size_t concord_saved8_bytes(int64_t M, int64_t K);
+int concord_save8(const void* x, int32_t type, int64_t ldx, void* saved, int64_t M, int64_t K, void* stream);
+int concord_dense8(const void* saved, void* out, int32_t type, int64_t ldo, int64_t M, int64_t K, void* stream);
+size_t concord_gemm_dw8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* saved, uint16_t* dw, int64_t M, int64_t N, int64_t K,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int concord_gemm_dw8_error(int32_t reset);
+
+/*
+ * Gated unit: h [M, K] = act(gate) * up, act CONCORD_SILU or CONCORD_GELU (of the error
+ * function); gate and up of one type with row strides of their own, h contiguous.
+ * saved_gate, saved_up, saved_h: NULL, or where their 8-bit form goes
+ * (concord_saved8_bytes each).  The backward takes gate and up themselves, or (not
+ * NULL) their 8-bit form, and writes dgate and dup (row strides of their own).
+ */
+#define CONCORD_SILU 0
+#define CONCORD_GELU 1
+int concord_gated_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t type, int32_t act, void* h,
+                      void* saved_gate, void* saved_up, void* saved_h, int64_t M, int64_t K, void* stream);
+int concord_gated_bwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, const void* saved_gate,
+                      const void* saved_up, int32_t type, int32_t act, const void* dh, int64_t lddh, void* dgate,
+                      int64_t lddg, void* dup, int64_t lddu, int64_t M, int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
