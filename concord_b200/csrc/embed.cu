@@ -8,17 +8,21 @@
 //
 // The gradient goes by sorted tokens: a stable radix sort of (id, token) gives
 // every row of the table its tokens in order, so that sums are fp32 in token
-// order, without atomics on them: the same bits on every run.  A row of up to
-// SEG tokens is summed by the threads that own it.  A longer one (every symbol
-// of a small vocabulary) is cut where the sorted tokens pass a multiple of SEG;
-// the pieces are summed side by side and joined in order by a second kernel.
+// order, without atomics on them: the same bits on every run.  Up to 65,536 tokens
+// are sorted by one cluster of 8 blocks in its shared memory, in one launch;
+// more go through memory, two launches a digit.  The sorted tokens are cut into
+// chunks of 32, summed side by side, each chunk's rows in order; a row that begins and
+// ends in one is finished there, the pieces of the others are joined in order
+// by a second kernel.  Rows of no token are cleared by other blocks meanwhile.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "vec.cuh"
 
 namespace concord {
 namespace embed {
 
-constexpr int SEG = 64;                    // tokens that one owner sums
+constexpr int SEG = 32;                    // sorted tokens of a chunk
 constexpr int DIGIT = 9, BINS = 1 << DIGIT;
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32;
 constexpr int64_t SORT_CHUNK = 4096;       // tokens of a sorting block, and more where blocks would pass
@@ -144,111 +148,293 @@ __global__ void __launch_bounds__(SORT_THREADS) place_kernel(const __grid_consta
     }
 }
 
-// first[v]: the first sorted place of a key of v or more, v = 0 .. V
-__global__ void __launch_bounds__(256) first_kernel(const uint2* sorted, uint32_t* first, int64_t T, int64_t V) {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v > V) return;
-    uint32_t lo = 0, hi = (uint32_t)T;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (sorted[mid].x < v) lo = mid + 1;
-        else hi = mid;
+// The first of `n` sorted places whose key is v or more, by a whole warp: 32 places looked at at once.
+__device__ __forceinline__ uint32_t lower_bound(const uint2* sorted, uint32_t n, int64_t v) {
+    uint32_t lo = 0, len = n;                     // it is in [lo, lo + len]
+    uint32_t lane;                                // (blocks have two dimensions)
+    asm("mov.u32 %0, %%laneid;" : "=r"(lane));
+    while (len > 0) {
+        const uint32_t step = (len + 31) / 32, at = lane * step;
+        const bool below = at < len && (int64_t)sorted[lo + at].x < v;
+        const uint32_t k = __popc(__ballot_sync(0xffffffffu, below));      // lanes 0 .. k - 1
+        if (k == 0) return lo;
+        const uint32_t from = (k - 1) * step + 1;
+        len = min(step - 1, len - from);
+        lo += from;
     }
-    first[v] = lo;
+    return lo;
+}
+__global__ void __launch_bounds__(32) end_kernel(const uint2* sorted, uint32_t* end, int64_t T, int64_t V) {
+    const uint32_t e = lower_bound(sorted, (uint32_t)T, V);
+    if (threadIdx.x == 0) *end = e;
+}
+
+// The whole sort by one cluster: block r holds places [r n, (r + 1) n)
+// of the list, n a power of two.  A digit takes two exchanges: the blocks' counts,
+// and the items, stored straight into the shared memory of the block that owns their place.
+constexpr int CLUSTER = 8, CT = 1024, CW = CT / 32;
+constexpr int64_t CLUSTER_MOST = 8192;                       // items of a block
+struct ClusterSort {
+    const void* ids;
+    int ids64;
+    int64_t V, padding;
+    int T, n, log_n, passes, digit;       // digit: bits of a pass, up to 9
+    uint2* sorted;
+    uint32_t* end;                                // places of rows; behind them what counts for none
+};
+size_t cluster_smem(int n) { return (size_t)2 * n * sizeof(uint2) + CW * BINS * sizeof(uint16_t) + 2 * BINS * sizeof(uint32_t); }
+
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CT) cluster_sort_kernel(const __grid_constant__ ClusterSort P) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) uint8_t raw[];
+    __shared__ uint32_t sums[CW];
+    uint2* list[2] = {reinterpret_cast<uint2*>(raw), reinterpret_cast<uint2*>(raw) + P.n};
+    uint16_t* run_at = reinterpret_cast<uint16_t*>(list[1] + P.n);         // [warp][digit]
+    uint32_t* mine = reinterpret_cast<uint32_t*>(run_at + CW * BINS);      // this block's counts
+    uint32_t* base = mine + BINS;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int begin = rank * P.n, have = max(0, min(P.n, P.T - begin));    // places of this block, and items in them
+    const int run = max(32, P.n / CW), r0 = min(warp * run, have), r1 = min(r0 + run, have);
+    for (int i = threadIdx.x; i < have; i += CT)
+        list[0][i] = make_uint2(key_of(P.ids, P.ids64, begin + i, P.V, P.padding), (uint32_t)(begin + i));
+    const int bins = 1 << P.digit;
+    for (int pass = 0; pass < P.passes; ++pass) {
+        const uint2* from = list[pass & 1];
+        const int shift = pass * P.digit;
+        for (int i = threadIdx.x; i < CW * bins / 8; i += CT) reinterpret_cast<uint4*>(run_at)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        uint16_t* at = run_at + warp * bins;
+        for (int t = r0; t < r1; t += 32) {
+            const bool is = t + lane < r1;
+            const uint32_t d = is ? (from[t + lane].x >> shift) & (bins - 1) : BINS;
+            const uint32_t same = __match_any_sync(0xffffffffu, d);
+            if (is && lane == __ffs(same) - 1) at[d] += (uint16_t)__popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        if (threadIdx.x < bins) {                 // each run's first place among the block's of this digit
+            uint32_t c[CW], n = 0;
+#pragma unroll
+            for (int w = 0; w < CW; ++w) c[w] = run_at[w * bins + threadIdx.x];
+#pragma unroll
+            for (int w = 0; w < CW; ++w) {
+                run_at[w * bins + threadIdx.x] = (uint16_t)n;
+                n += c[w];
+            }
+            mine[threadIdx.x] = n;
+        }
+        cluster.sync();
+        uint32_t all = 0, before = 0;
+        if (threadIdx.x < bins) {
+#pragma unroll
+            for (int r = 0; r < CLUSTER; ++r) {
+                const uint32_t c = cluster.map_shared_rank(mine, r)[threadIdx.x];
+                all += c;
+                before += r < rank ? c : 0;
+            }
+        }
+        uint32_t incl = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        if (threadIdx.x < bins) {
+            uint32_t b = incl - all + before;
+#pragma unroll
+            for (int w = 0; w < BINS / 32; ++w) b += w < warp ? sums[w] : 0;
+            base[threadIdx.x] = b;
+        }
+        __syncthreads();
+        uint2* to = list[(pass + 1) & 1];
+        for (int t = r0; t < r1; t += 32) {
+            const bool is = t + lane < r1;
+            const uint2 it = is ? from[t + lane] : make_uint2(0, 0);
+            const uint32_t d = is ? (it.x >> shift) & (bins - 1) : BINS;
+            const uint32_t same = __match_any_sync(0xffffffffu, d);
+            if (is) {
+                const uint32_t p = base[d] + at[d] + __popc(same & ((1u << lane) - 1));
+                cluster.map_shared_rank(to, p >> P.log_n)[p & (P.n - 1)] = it;
+            }
+            __syncwarp();
+            if (is && lane == __ffs(same) - 1) at[d] += (uint16_t)__popc(same);
+            __syncwarp();
+        }
+        cluster.sync();
+    }
+    const uint2* done = list[P.passes & 1];
+    for (int i = threadIdx.x; i < have; i += CT) {
+        const uint2 it = done[i];
+        P.sorted[begin + i] = it;
+        const bool none = it.x >= P.V;
+        if (none && begin + i == 0) *P.end = 0;
+        if (!none && begin + i + 1 == P.T) *P.end = (uint32_t)P.T;
+        if (!none && begin + i + 1 < P.T) {
+            const uint32_t next = i + 1 < have ? done[i + 1].x : cluster.map_shared_rank(const_cast<uint2*>(done), rank + 1)[0].x;
+            if (next >= P.V) *P.end = (uint32_t)(begin + i + 1);
+        }
+    }
+    cluster.sync();                               // nobody leaves while its list is read
 }
 
 // ---------------------------------------------------------------- sums
 struct Sums {
     const uint2* sorted;
-    const uint32_t* first;
-    float* part;              // [chunks][2][D]: pieces of the long rows
+    const uint32_t* end;
+    float* part;              // [chunks][2][D]: a row's piece that goes on from the chunk before, one that begins here and goes on
     int64_t T, V, lddy;
     int64_t chunks;
     int D;
     float scale;
 };
 
-// acc += the rows of tokens [a, b) of the sorted ones, in order, four loads on their way
-template <typename TY, int VEC>
-__device__ __forceinline__ void add_rows(const Sums& P, const TY* dy, uint32_t a, uint32_t b, int col, float* acc) {
-    constexpr int AHEAD = 4;
-    uint32_t p = a;
-    for (; p + AHEAD <= b; p += AHEAD) {
-        float v[AHEAD][VEC];
+// VEC columns of a row as they come from memory
+template <typename T, int VEC> struct RawVec {
+    static constexpr int W = VEC * (int)sizeof(T) / 4 > 0 ? VEC * (int)sizeof(T) / 4 : 1;
+    uint32_t v[W];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC == 1) v[0] = __float_as_uint(to_f32(*p));
+        else {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) load_vec<VEC>(dy + P.sorted[p + i].y * P.lddy + col, v[i]);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] += v[i][j];
+            for (int i = 0; i < W / 4; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+            }
+        }
     }
-    for (; p < b; ++p) {
-        float v[VEC];
-        load_vec<VEC>(dy + P.sorted[p].y * P.lddy + col, v);
+    __device__ __forceinline__ void add_to(float* acc) const {
+        if constexpr (VEC == 1) acc[0] += __uint_as_float(v[0]);
+        else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += v[j];
+            for (int i = 0; i < VEC; ++i) {
+                if constexpr (sizeof(T) == 4) acc[i] += __uint_as_float(v[i]);
+                else {
+                    const float2 f = unpack2(v[i / 2], T());
+                    acc[i] += i & 1 ? f.y : f.x;
+                }
+            }
+        }
     }
-}
+};
 
-// The first `chunks` rows of threads take the pieces of long rows, the others a
-// row of the table each.
+// Blocks of two kinds, spread evenly: chunks, one a row of threads (their
+// loads run AHEAD tokens before their sums), and rows of no token to clear.
+constexpr int CLEAR = 64;             // rows of the table that a clearing block looks at
 template <typename TY, typename TW, int VEC>
-__global__ void __launch_bounds__(256) sum_kernel(const TY* dy, TW* dw, const __grid_constant__ Sums P) {
+__global__ void __launch_bounds__(256, 3)
+    sum_kernel(const TY* dy, TW* dw, const __grid_constant__ Sums P, int chunk_blocks, int clear_blocks) {
     const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (col >= P.D || i >= P.chunks + P.V) return;
     float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    if (i >= P.chunks) {
-        const int64_t v = i - P.chunks;
-        const uint32_t a = P.first[v], b = P.first[v + 1];
-        if (b - a > SEG) return;
-        add_rows<TY, VEC>(P, dy, a, b, col, acc);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] *= P.scale;
-        store_vec<VEC>(dw + v * P.D + col, acc);
+    const int64_t both = chunk_blocks + clear_blocks;
+    const int64_t nth = blockIdx.x * (int64_t)chunk_blocks / both;
+    if (nth == (blockIdx.x + 1) * (int64_t)chunk_blocks / both) {          // the (blockIdx.x - nth)-th to clear
+        __shared__ uint32_t some[CLEAR / 32];
+        const int64_t v0 = (blockIdx.x - nth) * CLEAR;
+        const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+        if (thread < CLEAR / 32) some[thread] = 0;
+        __syncthreads();
+        if (thread < (threads & ~31)) {           // (whole warps)
+            const uint32_t a = lower_bound(P.sorted, *P.end, v0), b = lower_bound(P.sorted, *P.end, v0 + CLEAR);
+            for (uint32_t p = a + thread; p < b; p += threads & ~31) {
+                const uint32_t r = P.sorted[p].x - (uint32_t)v0;
+                atomicOr(&some[r / 32], 1u << (r % 32));
+            }
+        }
+        __syncthreads();
+        if (col >= P.D) return;
+        for (int r = threadIdx.y; r < CLEAR && v0 + r < P.V; r += blockDim.y)
+            if (!(some[r / 32] >> (r % 32) & 1)) store_vec<VEC>(dw + (v0 + r) * P.D + col, acc);
         return;
     }
-    const uint32_t p0 = (uint32_t)i * SEG, p1 = min(p0 + SEG, P.first[P.V]);
-    if (p0 >= p1) return;
-    const uint32_t v0 = P.sorted[p0].x, v1 = P.sorted[p1 - 1].x;
-    const uint32_t e0 = P.first[v0 + 1], a1 = P.first[v1];
-    if (e0 - P.first[v0] > SEG) {
-        add_rows<TY, VEC>(P, dy, p0, min(e0, p1), col, acc);
-        store_vec<VEC>(P.part + (2 * i) * P.D + col, acc);
-    }
-    if (v1 != v0 && P.first[v1 + 1] - a1 > SEG) {
+    if (col >= P.D) return;
+    constexpr int AHEAD = VEC == 1 || sizeof(TY) == 2 ? 8 : 4;
+    const int64_t i = nth * blockDim.y + threadIdx.y;
+    const uint32_t end = *P.end;
+    if (i >= P.chunks || (uint32_t)i * SEG >= end) return;
+    const uint32_t p0 = (uint32_t)i * SEG, p1 = min(p0 + SEG, end);
+    const uint2* at = P.sorted;
+    const TY* src = dy + col;
+    RawVec<TY, VEC> ring[AHEAD];
+    uint32_t key[AHEAD];                                  // their rows
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-        add_rows<TY, VEC>(P, dy, a1, p1, col, acc);
-        store_vec<VEC>(P.part + (2 * i + 1) * P.D + col, acc);
+    for (int k = 0; k < AHEAD; ++k) {
+        const uint2 it = at[min(p0 + k, p1 - 1)];
+        key[k] = it.x;
+        ring[k].load(src + it.y * P.lddy);
+    }
+    bool before = p0 > 0 && at[p0 - 1].x == key[0];       // the row goes on from the chunk before
+    const uint32_t after = p1 < end ? at[p1].x : (uint32_t)P.V;
+    for (uint32_t p = p0; p < p1; p += AHEAD) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (p + k >= p1) break;
+            ring[k].add_to(acc);
+            const uint32_t v = key[k];
+            const uint2 it = at[min(p + k + AHEAD, p1 - 1)];      // (the last one again where there are no more)
+            key[k] = it.x;
+            ring[k].load(src + it.y * P.lddy);
+            const bool last = p + k + 1 == p1;
+            const uint32_t next = last ? after : key[(k + 1) % AHEAD];
+            if (next == v && !last) continue;
+            if (!before && next != v) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] *= P.scale;
+                store_vec<VEC>(dw + (int64_t)v * P.D + col, acc);
+            } else {
+                store_vec<VEC>(P.part + (2 * i + !before) * P.D + col, acc);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+            before = false;
+        }
     }
 }
 
-// One long row at most begins in each chunk: its pieces, in order.
+// One row at most begins in a chunk and goes on: its pieces in order, eight runs of
+// them side by side, the runs' sums in order again.
+constexpr int JOIN = 8;
 template <typename TW, int VEC>
 __global__ void __launch_bounds__(256) join_kernel(TW* dw, const __grid_constant__ Sums P) {
-    const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (col >= P.D || i >= P.chunks) return;
-    const uint32_t p0 = (uint32_t)i * SEG, p1 = min(p0 + SEG, P.first[P.V]);
-    if (p0 >= p1) return;
-    const uint32_t v = P.sorted[p1 - 1].x, a = P.first[v], b = P.first[v + 1];
-    if (b - a <= SEG || a < p0) return;
-    const int64_t last = (b - 1) / SEG;
+    __shared__ float runs[JOIN][32][VEC];
+    const int64_t i = blockIdx.x;
+    const uint32_t end = *P.end, p0 = (uint32_t)i * SEG, p1 = p0 + SEG;
+    if (p1 >= end) return;                                // (the last chunk: nothing goes on)
+    const uint32_t v = P.sorted[p1 - 1].x;
+    if (P.sorted[p1].x != v) return;
+    if (p0 > 0 && P.sorted[p0 - 1].x == v) return;        // it began before
+    const uint32_t b = p1 + lower_bound(P.sorted + p1, end - p1, (int64_t)v + 1);
+    const int64_t pieces = (b - 1) / SEG - i;             // besides the first
+    const int col = (blockIdx.y * 32 + threadIdx.x) * VEC;
     float acc[VEC];
-    load_vec<VEC>(P.part + (2 * i + (a != p0)) * P.D + col, acc);
-#pragma unroll 8
-    for (int64_t c = i + 1; c <= last; ++c) {
-        float x[VEC];
-        load_vec<VEC>(P.part + 2 * c * P.D + col, x);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    if (col < P.D) {
+        const int64_t c0 = i + 1 + pieces * threadIdx.y / JOIN, c1 = i + 1 + pieces * (threadIdx.y + 1) / JOIN;
+        if (threadIdx.y == 0) load_vec<VEC>(P.part + (2 * i + 1) * P.D + col, acc);
+#pragma unroll 4
+        for (int64_t c = c0; c < c1; ++c) {
+            float x[VEC];
+            load_vec<VEC>(P.part + 2 * c * P.D + col, x);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+        }
     }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] *= P.scale;
-    store_vec<VEC>(dw + (int64_t)v * P.D + col, acc);
+    for (int j = 0; j < VEC; ++j) runs[threadIdx.y][threadIdx.x][j] = acc[j];
+    __syncthreads();
+    if (threadIdx.y == 0 && col < P.D) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            for (int k = 1; k < JOIN; ++k) acc[j] += runs[k][threadIdx.x][j];
+            acc[j] *= P.scale;
+        }
+        store_vec<VEC>(dw + (int64_t)v * P.D + col, acc);
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -276,9 +462,9 @@ int forward(const void* ids, int ids64, const void* w, int64_t ldw, void* y, int
 
 struct Layout {
     int64_t chunk, blocks, chunks;
-    size_t second, counts, first, part, total;        // offsets (the first list stands at 0)
+    size_t second, counts, end, part, total;        // offsets (the first list stands at 0)
 };
-Layout layout(int64_t T, int64_t V, int64_t D) {
+Layout layout(int64_t T, int64_t D) {
     Layout L;
     L.chunk = SORT_CHUNK;
     while ((T + L.chunk - 1) / L.chunk > SORT_BLOCKS) L.chunk *= 2;
@@ -287,8 +473,8 @@ Layout layout(int64_t T, int64_t V, int64_t D) {
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     L.second = up(T * sizeof(uint2));
     L.counts = L.second + up(T * sizeof(uint2));
-    L.first = L.counts + up(L.blocks * BINS * sizeof(uint32_t));
-    L.part = L.first + up((V + 1) * sizeof(uint32_t));
+    L.end = L.counts + up(L.blocks * BINS * sizeof(uint32_t));
+    L.part = L.end + up(sizeof(uint32_t));
     L.total = L.part + up((size_t)L.chunks * 2 * D * sizeof(float));
     return L;
 }
@@ -296,29 +482,53 @@ Layout layout(int64_t T, int64_t V, int64_t D) {
 template <typename TY, typename TW>
 int backward(const void* ids, int ids64, const void* dy, int64_t lddy, void* dw, int64_t T, int64_t V, int64_t D,
              float scale, int64_t padding, char* ws, bool vec, cudaStream_t st) {
-    const Layout L = layout(T, V, D);
+    const Layout L = layout(T, D);
     uint2 *list[2] = {reinterpret_cast<uint2*>(ws), reinterpret_cast<uint2*>(ws + L.second)};
-    uint32_t* first = reinterpret_cast<uint32_t*>(ws + L.first);
-    Pass P{ids, ids64, nullptr, list[0], reinterpret_cast<uint32_t*>(ws + L.counts), T, V, padding, L.chunk, 0};
-    int turn = 0;
-    for (int shift = 0; shift == 0 || V >> shift; shift += DIGIT) {
-        P.shift = shift;
-        P.to = list[turn];
-        count_kernel<<<(int)L.blocks, SORT_THREADS, 0, st>>>(P);
-        place_kernel<<<(int)L.blocks, SORT_THREADS, 0, st>>>(P);
-        P.from = list[turn];
-        turn ^= 1;
+    uint32_t* end = reinterpret_cast<uint32_t*>(ws + L.end);
+    const uint2* sorted = list[0];
+    int passes = 1;
+    while (V >> (passes * DIGIT)) ++passes;
+    if (T <= CLUSTER * CLUSTER_MOST) {
+        int bits = 1;
+        while (V >> bits) ++bits;
+        ClusterSort C{ids, ids64, V, padding, (int)T, 32, 5, passes, (bits + passes - 1) / passes, list[0], end};
+        if (C.digit < 3) C.digit = 3;             // (whole 16-byte pieces of counts)
+        while ((int64_t)C.n * CLUSTER < T) {
+            C.n *= 2;
+            ++C.log_n;
+        }
+        const size_t smem = cluster_smem(C.n);
+        cudaError_t e = cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)cluster_smem(CLUSTER_MOST));
+        if (e != cudaSuccess) return fail(CONCORD_ELAUNCH, std::string("concord_embedding_bwd: ") + cudaGetErrorString(e));
+        cluster_sort_kernel<<<CLUSTER, CT, smem, st>>>(C);
+    } else {
+        Pass P{ids, ids64, nullptr, list[0], reinterpret_cast<uint32_t*>(ws + L.counts), T, V, padding, L.chunk, 0};
+        for (int pass = 0; pass < passes; ++pass) {
+            P.shift = pass * DIGIT;
+            P.to = list[pass & 1];
+            count_kernel<<<(int)L.blocks, SORT_THREADS, 0, st>>>(P);
+            place_kernel<<<(int)L.blocks, SORT_THREADS, 0, st>>>(P);
+            P.from = P.to;
+        }
+        sorted = P.from;
+        end_kernel<<<1, 32, 0, st>>>(sorted, end, T, V);
     }
-    first_kernel<<<(int)(V / 256 + 1), 256, 0, st>>>(P.from, first, T, V);
-    const Sums S{P.from, first, reinterpret_cast<float*>(ws + L.part), T, V, lddy, L.chunks, (int)D, scale};
+    const Sums S{sorted, end, reinterpret_cast<float*>(ws + L.part), T, V, lddy, L.chunks, (int)D, scale};
     dim3 threads;
     int across;
     shape(D, vec ? 8 : 1, &threads, &across);
-    const dim3 grid((unsigned)((L.chunks + V + threads.y - 1) / threads.y), across, 1);
+    const int chunk_blocks = (int)((L.chunks + threads.y - 1) / threads.y);
+    const int clear_blocks = (int)((V + CLEAR - 1) / CLEAR);
     auto k = vec ? sum_kernel<TY, TW, 8> : sum_kernel<TY, TW, 1>;
-    k<<<grid, threads, 0, st>>>(static_cast<const TY*>(dy), static_cast<TW*>(dw), S);
-    auto j = vec ? join_kernel<TW, 8> : join_kernel<TW, 1>;
-    j<<<dim3((unsigned)((L.chunks + threads.y - 1) / threads.y), across, 1), threads, 0, st>>>(static_cast<TW*>(dw), S);
+    k<<<dim3((unsigned)(chunk_blocks + clear_blocks), across, 1), threads, 0, st>>>(
+        static_cast<const TY*>(dy), static_cast<TW*>(dw), S, chunk_blocks, clear_blocks);
+    if (L.chunks > 1) {
+        auto j = vec ? join_kernel<TW, 8> : join_kernel<TW, 1>;
+        const int wide = 32 * (vec ? 8 : 1);
+        j<<<dim3((unsigned)(L.chunks - 1), (unsigned)((D + wide - 1) / wide), 1), dim3(32, JOIN, 1), 0, st>>>(
+            static_cast<TW*>(dw), S);
+    }
     return check_launch("concord_embedding_bwd");
 }
 
@@ -363,7 +573,7 @@ extern "C" int concord_embedding_fwd(const void* ids, int32_t ids64, const void*
 
 extern "C" size_t concord_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) {
     if (T <= 0 || V <= 0 || D <= 0 || T > (1 << 30) || V > (1 << 30) || D > (1 << 20)) return 0;
-    return embed::layout(T, V, D).total;
+    return embed::layout(T, D).total;
 }
 
 extern "C" int concord_embedding_bwd(const void* ids, int32_t ids64, const void* dy, int32_t dy_type, int64_t lddy,
