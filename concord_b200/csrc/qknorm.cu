@@ -6,15 +6,19 @@
 //   backward: dn = the rotation undone on dy,  g = dn w,
 //   dx = r g - x r^3 sum(g x) / D,  dw = sum over tokens and heads of dn x r
 //
-// Bound by memory: the forward reads and writes q and k once, the backward
-// reads dy and x and writes dx.  A row (one head of one token) stays in the
-// registers of a group of lanes, 8 pairs each, a pair's two halves in one lane
+// Bound by memory: the forward reads and writes q and k once, the backward reads
+// dy and x and writes dx.  A row (one head of one token) stays in the
+// registers of a group of lanes, 8 or 4 pairs each, a pair's two halves in one lane
 // whichever way pairs are laid out, so that the rotation needs no exchange; the
 // group's lanes share sums by shuffles (both sums of the backward in one go:
-// neither needs r).  A thread keeps its part of cos and sin for all heads of a
-// token, and its columns' weights for all tokens.  The weights' gradients are
-// added per thread, then per block, then over blocks in a fixed order: no
-// atomics, the same bits on every run of one device.
+// neither needs r).  Blocks belong to q or to k; a thread walks its tokens' heads
+// with the rows after the present one on their way, as they come from memory, and keeps its
+// part of cos and sin for a token and its columns' weights for all of
+// them.  The weights' gradients are added per thread, then per block,
+// then over blocks in a fixed order: no atomics, the same bits on every run of
+// one device.
+#include <atomic>
+
 #include "common.cuh"
 #include "vec.cuh"
 
@@ -23,37 +27,42 @@ namespace qkn {
 
 constexpr int MAX_DIM = 256, THREADS = 256;
 
+// q or k
+struct Side {
+    const void *x, *dy;
+    void* out;                    // contiguous [T, heads, D]
+    const float* w;               // NULL: ones
+    int64_t ts, hs, dts, dhs;     // token and head strides of x and dy, elements
+    int heads, share;             // share: row groups of a block beside one another in a token's heads
+};
+
 struct Params {
     const float *cos, *sin;       // [positions, rot / 2]
     const void* pos;              // [T], or NULL: the token's number
     int pos64;
     int64_t T, positions;
-    int heads[2], D, rot;         // heads of q and of k
-    int interleaved;
+    int D, rot, interleaved;
     float eps, inv_d;
-    const float* w[2];            // NULL: ones
-    const void* x[2];
-    int64_t ts[2], hs[2];         // token and head strides, elements
-    const void* dy[2];
-    int64_t dts[2], dhs[2];
-    void* out[2];                 // contiguous [T, heads, D]
-    float* part;                  // backward: [blocks][2][D]
-    int share;                    // row groups of a block that share a token's heads
+    Side side[2];
+    int blocks0;                  // blocks of q; the others are k's
+    float* part;                  // backward: [blocks][D]
 };
 
-// What one lane holds of a row: PAIRS pairs (a, b).  VEC: 8 pairs, rotated ones or 16
-// neighbouring plain columns; else 4 pairs 32 apart, for any size and stride.
-template <bool VEC> struct Lane {
-    static constexpr int PAIRS = VEC ? 8 : 4;
-    int at[VEC ? 2 : 1];          // VEC: the first columns of two runs of 8; else the first pair
+// Where a lane's pairs stand in a row.  VEC: N rotated pairs, or 2 N plain columns,
+// as two runs of N columns (PAIRED: pairs, and plain columns, side by side; else first and second
+// halves of the pairs); else N pairs 32 apart, for any size and stride.
+enum Kind { ANY, HALVES, PAIRED };
+template <int N, Kind KIND> struct Lane {
+    static constexpr bool VEC = KIND != ANY;
+    int at[VEC ? 2 : 1];          // VEC: the runs' first columns; else the first pair
     bool live, turns;             // VEC: any columns, rotated ones
     int D, rot, interleaved;
     __device__ __forceinline__ Lane(const Params& P, int lane) : D(P.D), rot(P.rot), interleaved(P.interleaved) {
         if constexpr (VEC) {
-            live = lane * 16 < D;
-            turns = lane * 16 < rot;
-            at[0] = turns && !interleaved ? lane * 8 : lane * 16;
-            at[1] = turns && !interleaved ? rot / 2 + lane * 8 : lane * 16 + 8;
+            live = lane * 2 * N < D;
+            turns = lane * 2 * N < rot;
+            at[0] = !live ? 0 : turns && KIND == HALVES ? lane * N : lane * 2 * N;
+            at[1] = !live ? N : turns && KIND == HALVES ? rot / 2 + lane * N : lane * 2 * N + N;    // (not live: loads need no condition)
         } else {
             live = turns = true;
             at[0] = lane;
@@ -72,323 +81,500 @@ template <bool VEC> struct Lane {
         if (*a >= D) *a = -1;
         if (*b >= D) *b = -1;
     }
-    template <typename T> __device__ __forceinline__ void load(const T* row, float* a, float* b) const {
-        if constexpr (VEC) {
-            load_vec<8>(row + at[0], a);
-            load_vec<8>(row + at[1], b);
-            if (interleaved && turns) {           // (a0 b0 a1 b1 ..) to (a0 a1 ..), (b0 b1 ..)
-                float t[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { t[j] = a[2 * j + 1]; a[j] = a[2 * j]; }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { a[4 + j] = b[2 * j]; t[4 + j] = b[2 * j + 1]; }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) b[j] = t[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < PAIRS; ++j) {
-                int ca, cb;
-                columns(j, &ca, &cb);
-                a[j] = ca >= 0 ? to_f32(row[ca]) : 0.f;
-                b[j] = cb >= 0 ? to_f32(row[cb]) : 0.f;
-            }
-        }
-    }
-    template <typename T> __device__ __forceinline__ void store(T* row, const float* a, const float* b) const {
-        if constexpr (VEC) {
-            if (interleaved && turns) {
-                float lo[8], hi[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    lo[2 * j] = a[j];
-                    lo[2 * j + 1] = b[j];
-                    hi[2 * j] = a[4 + j];
-                    hi[2 * j + 1] = b[4 + j];
-                }
-                store_vec<8>(row + at[0], lo);
-                store_vec<8>(row + at[1], hi);
-            } else {
-                store_vec<8>(row + at[0], a);
-                store_vec<8>(row + at[1], b);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < PAIRS; ++j) {
-                int ca, cb;
-                columns(j, &ca, &cb);
-                if (ca >= 0) row[ca] = from_f32<T>(a[j]);
-                if (cb >= 0) row[cb] = from_f32<T>(b[j]);
-            }
-        }
-    }
     __device__ __forceinline__ bool rotated(int j) const { return VEC ? turns : at[0] + 32 * j < rot / 2; }
-    // cos and sin of token t's position; NaN where the tables have no such position
-    __device__ __forceinline__ void angles(const Params& P, int64_t t, float* c, float* s) const {
-        int64_t p = t;
-        if (P.pos && rot) p = P.pos64 ? static_cast<const int64_t*>(P.pos)[t] : (int64_t)static_cast<const int32_t*>(P.pos)[t];
-        const bool there = p >= 0 && p < P.positions;
-        const int64_t row = p * (rot / 2);
+};
+
+// a lane's part of a row as it comes from memory
+template <typename T, int N, Kind KIND> struct Raw {
+    static constexpr bool VEC = KIND != ANY;
+    static constexpr int RUN = N * (int)sizeof(T), WORDS = VEC ? 2 * RUN / 4 : 2 * N;
+    uint32_t v[WORDS];
+    __device__ __forceinline__ void fetch(const Lane<N, KIND>& L, const T* row) {
         if constexpr (VEC) {
-            if (live && turns && there) {
-                load_vec<8>(P.cos + row + at[0] / (interleaved ? 2 : 1), c);
-                load_vec<8>(P.sin + row + at[0] / (interleaved ? 2 : 1), s);
-                return;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if constexpr (RUN == 8) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(row + L.at[r]);
+                    v[2 * r] = u.x;
+                    v[2 * r + 1] = u.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < RUN / 16; ++i) {
+                        const uint4 u = reinterpret_cast<const uint4*>(row + L.at[r])[i];
+                        v[r * RUN / 4 + 4 * i] = u.x;
+                        v[r * RUN / 4 + 4 * i + 1] = u.y;
+                        v[r * RUN / 4 + 4 * i + 2] = u.z;
+                        v[r * RUN / 4 + 4 * i + 3] = u.w;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                int ca, cb;
+                L.columns(j, &ca, &cb);
+                v[2 * j] = ca >= 0 ? __float_as_uint(to_f32(row[ca])) : 0u;
+                v[2 * j + 1] = cb >= 0 ? __float_as_uint(to_f32(row[cb])) : 0u;
             }
         }
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int j = 0; j < PAIRS; ++j) {
-            const bool here = !VEC && rotated(j) && there;
-            c[j] = here ? P.cos[row + at[0] + 32 * j] : __int_as_float(0x7fffffff);
-            s[j] = here ? P.sin[row + at[0] + 32 * j] : c[j];
+        for (int i = 0; i < WORDS; ++i) v[i] = 0;
+    }
+    __device__ __forceinline__ float element(int i) const {       // VEC: the i-th of both runs
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+        else {
+            const float2 f = unpack2(v[i / 2], T());
+            return i & 1 ? f.y : f.x;
+        }
+    }
+    // as pairs' first and second elements, two a register pair (packed arithmetic)
+    __device__ __forceinline__ void pairs(uint64_t* a, uint64_t* b) const {
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            if constexpr (!VEC) {
+                a[j] = f2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 2]));
+                b[j] = f2(__uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 3]));
+            } else if constexpr (KIND == PAIRED) {
+                a[j] = f2(element(4 * j), element(4 * j + 2));
+                b[j] = f2(element(4 * j + 1), element(4 * j + 3));
+            } else {
+                a[j] = f2(element(2 * j), element(2 * j + 1));
+                b[j] = f2(element(N + 2 * j), element(N + 2 * j + 1));
+            }
         }
     }
 };
 
-// the sum over a row's lanes (a power of two of them)
-template <bool VEC> __device__ __forceinline__ float lane_sum(float v, int lanes) {
-    for (int o = (VEC ? lanes : 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+template <typename T, int N, Kind KIND>
+__device__ __forceinline__ void store_pairs(const Lane<N, KIND>& L, T* row, const uint64_t* a2, const uint64_t* b2) {
+    float a[N], b[N];
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        unf2(a2[j], a[2 * j], a[2 * j + 1]);
+        unf2(b2[j], b[2 * j], b[2 * j + 1]);
+    }
+    if constexpr (KIND != ANY) {
+        float r[2 * N];
+        if constexpr (KIND == PAIRED) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) { r[2 * j] = a[j]; r[2 * j + 1] = b[j]; }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) { r[j] = a[j]; r[N + j] = b[j]; }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            T* p = row + L.at[k];
+            if constexpr (N * sizeof(T) == 8)
+                *reinterpret_cast<uint2*>(p) = make_uint2(pack2(r[k * N], r[k * N + 1], T()), pack2(r[k * N + 2], r[k * N + 3], T()));
+            else {
+                uint4* q = reinterpret_cast<uint4*>(p);
+#pragma unroll
+                for (int i = 0; i < N * (int)sizeof(T) / 16; ++i) q[i] = Pack16<T>::pack(r + k * N + i * Pack16<T>::N);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            int ca, cb;
+            L.columns(j, &ca, &cb);
+            if (ca >= 0) row[ca] = from_f32<T>(a[j]);
+            if (cb >= 0) row[cb] = from_f32<T>(b[j]);
+        }
+    }
+}
+
+// cos, sin and -sin of position p; NaN where the tables have none
+template <int N, Kind KIND>
+__device__ __forceinline__ void angles(const Params& P, const Lane<N, KIND>& L, int64_t p, uint64_t* c2, uint64_t* s2,
+                                       uint64_t* n2) {
+    const bool there = p >= 0 && p < P.positions;
+    const int64_t row = p * (P.rot / 2);
+    float c[N], s[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) c[j] = s[j] = __int_as_float(0x7fffffff);
+    if constexpr (KIND != ANY) {
+        if (L.live && L.turns && there) {
+            const int64_t at = row + (KIND == PAIRED ? L.at[0] / 2 : L.at[0]);
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const float4 u = *reinterpret_cast<const float4*>(P.cos + at + j), v = *reinterpret_cast<const float4*>(P.sin + at + j);
+                c[j] = u.x; c[j + 1] = u.y; c[j + 2] = u.z; c[j + 3] = u.w;
+                s[j] = v.x; s[j + 1] = v.y; s[j + 2] = v.z; s[j + 3] = v.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!L.rotated(j)) {              // (not used: turn leaves these columns alone)
+                c[j] = 1.f;
+                s[j] = 0.f;
+            } else if (there) {
+                c[j] = P.cos[row + L.at[0] + 32 * j];
+                s[j] = P.sin[row + L.at[0] + 32 * j];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        c2[j] = f2(c[2 * j], c[2 * j + 1]);
+        s2[j] = f2(s[2 * j], s[2 * j + 1]);
+        n2[j] = f2(-s[2 * j], -s[2 * j + 1]);
+    }
+}
+// (a, b) -> (a c + b m, b c + a s): m = -s turns, with s and -s in each other's place it turns back
+template <int N, Kind KIND>
+__device__ __forceinline__ void turn(const Lane<N, KIND>& L, uint64_t* a, uint64_t* b, const uint64_t* c, const uint64_t* s,
+                                     const uint64_t* m) {
+    if (KIND != ANY && !L.turns) return;
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        const uint64_t u = fma2(b[j], m[j], mul2(a[j], c[j])), v = fma2(a[j], s[j], mul2(b[j], c[j]));
+        if constexpr (KIND != ANY) {
+            a[j] = u;
+            b[j] = v;
+        } else {
+            float ua, ub, va, vb, oa, ob, pa, pb;
+            unf2(u, ua, ub);
+            unf2(v, va, vb);
+            unf2(a[j], oa, ob);
+            unf2(b[j], pa, pb);
+            const bool first = L.rotated(2 * j), second = L.rotated(2 * j + 1);
+            a[j] = f2(first ? ua : oa, second ? ub : ob);
+            b[j] = f2(first ? va : pa, second ? vb : pb);
+        }
+    }
+}
+
+__device__ __forceinline__ int64_t position(const Params& P, int64_t t) {
+    if (!P.pos || !P.rot) return t;
+    return P.pos64 ? static_cast<const int64_t*>(P.pos)[t] : (int64_t)static_cast<const int32_t*>(P.pos)[t];
+}
+
+// the sum over a row's lanes (a power of two of them; every lane of the warp calls it)
+template <int LANES> __device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// HEADS rows of a thread at a time, so that their loads are on their way together
-constexpr int AHEAD = 4;
+__device__ __forceinline__ float sum2(uint64_t v) {
+    float a, b;
+    unf2(v, a, b);
+    return a + b;
+}
 
-template <typename T, bool VEC, bool NORM>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Params P, int lanes) {
-    constexpr int N = Lane<VEC>::PAIRS;
-    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = THREADS / lanes;
-    const Lane<VEC> L(P, lane);
-    const int64_t step = (int64_t)gridDim.x * (groups / P.share);
-    // every thread of a warp goes round the same number of times (the sums are whole warps')
-    const int64_t t0 = (int64_t)blockIdx.x * (groups / P.share), mine = group / P.share;
-    for (int64_t base = t0; base < P.T; base += step) {
-        const int64_t t = base + mine;
-        const bool here = t < P.T && L.live;
-        float c[N], s[N];
-        L.angles(P, here ? t : base, c, s);
-#pragma unroll 1
-        for (int which = 0; which < 2; ++which) {
-            const int heads = P.heads[which];
-            const T* x = static_cast<const T*>(P.x[which]) + t * P.ts[which];
-            T* out = static_cast<T*>(P.out[which]) + t * heads * P.D;
-            float wa[N], wb[N];
+// A row group's rows in order: its heads of a token (`share` apart, a divisor of the
+// heads), then those of its next token.  Where it stands is the same in
+// all groups of a block, so that branches are uniform; a group whose token lies
+// beyond the last one reads the last one's (loads need no condition then) and stores nothing.
+struct Rows {
+    int base, mine, i, per, step, T;
+    __device__ __forceinline__ Rows(const Params& P, const Side& S, int block, int blocks, int group, int groups) {
+        const int tokens = groups / S.share;
+        T = (int)P.T;
+        mine = group / S.share;
+        base = block * tokens;
+        step = blocks * tokens;
+        per = S.heads / S.share;
+        i = 0;
+    }
+    __device__ __forceinline__ int token() const { return min(base + mine, T - 1); }
+    __device__ __forceinline__ bool here() const { return base + mine < T; }
+    __device__ __forceinline__ int64_t steps() const { return base < T ? (int64_t)((T - 1 - base) / step + 1) * per : 0; }
+    // to the next row; whether it is another token's
+    __device__ __forceinline__ bool next() {
+        if (++i < per) return false;
+        i = 0;
+        base = min(base + step, T);               // (stays there: no overflow)
+        return true;
+    }
+};
+template <typename T> __device__ __forceinline__ const T* row_at(const void* p, int64_t ts, int64_t hs, int t, int h) {
+    return static_cast<const T*>(p) + t * ts + h * hs;
+}
+
+template <typename T, int N, int LANES, Kind KIND, bool NORM>
+__global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const __grid_constant__ Params P) {
+    constexpr int DEPTH = 3;                      // rows of a thread, the present one included
+    const int which = blockIdx.x >= P.blocks0, block = blockIdx.x - (which ? P.blocks0 : 0);
+    const Side& S = P.side[which];
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, h0 = group % S.share;
+    const Lane<N, KIND> L(P, lane);
+    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, group, THREADS / LANES), far = now;
+    const int64_t steps = now.steps(), ts = S.ts, hs = S.hs, in_step = hs * S.share, ld = (int64_t)S.heads * P.D;
+    const int out_step = S.share * P.D;
+    const T* in = row_at<T>(S.x, ts, hs, far.token(), h0);
+    T* out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
+    Raw<T, N, KIND> raw[DEPTH];
+    auto fetch = [&](int k) {
+        raw[k].fetch(L, in);
+        in += in_step;
+        if (far.next()) in = row_at<T>(S.x, ts, hs, far.token(), h0);
+    };
 #pragma unroll
-            for (int j = 0; j < N; ++j) wa[j] = wb[j] = 1.f;
-            if (NORM && P.w[which] && L.live) L.load(P.w[which], wa, wb);
-#pragma unroll 1
-            for (int h0 = group & (P.share - 1); h0 - (group & (P.share - 1)) < heads; h0 += AHEAD * P.share) {
-                float a[AHEAD][N], b[AHEAD][N];
+    for (int k = 0; k < DEPTH - 1; ++k) fetch(k);
+    uint64_t wa[N / 2], wb[N / 2], c[N / 2], s[N / 2], m[N / 2];
+    if (NORM && S.w) {
+        Raw<float, N, KIND> w;
+        w.fetch(L, S.w);
+        w.pairs(wa, wb);
+    } else {
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int h = h0 + i * P.share;
-                    if (here && h < heads) L.load(x + h * P.hs[which], a[i], b[i]);
+        for (int j = 0; j < N / 2; ++j) wa[j] = wb[j] = f2(1.f, 1.f);
+    }
+    const float inv_d = P.inv_d, eps = P.eps;
+    const bool turns = P.rot > 0;
+    bool fresh = turns, keep = now.here() && L.live;
+    int64_t pos = turns ? position(P, now.token()) : 0;                 // of the next token, once this one's is used
+    for (int64_t n = 0; n < steps; n += DEPTH) {
+#pragma unroll
+        for (int k = 0; k < DEPTH; ++k) {
+            fetch((k + DEPTH - 1) % DEPTH);
+            if (fresh) {
+                angles<N, KIND>(P, L, pos, c, s, m);
+                pos = position(P, min(now.base + now.mine + now.step, now.T - 1));
+            }
+            uint64_t a[N / 2], b[N / 2];
+            raw[k].pairs(a, b);
+            if constexpr (NORM) {
+                uint64_t ss = mul2(a[0], a[0]);
+                ss = fma2(b[0], b[0], ss);
+#pragma unroll
+                for (int j = 1; j < N / 2; ++j) ss = fma2(b[j], b[j], fma2(a[j], a[j], ss));
+                const float r = rsqrtf(lane_sum<LANES>(L.live ? sum2(ss) : 0.f) * inv_d + eps);
+                const uint64_t r2 = f2(r, r);
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    a[j] = mul2(a[j], mul2(wa[j], r2));
+                    b[j] = mul2(b[j], mul2(wb[j], r2));
                 }
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int h = h0 + i * P.share;
-                    const bool row = here && h < heads;
-                    if constexpr (NORM) {
-                        float ss = 0.f;
-                        if (row) {
-#pragma unroll
-                            for (int j = 0; j < N; ++j) ss += a[i][j] * a[i][j] + b[i][j] * b[i][j];
-                        }
-                        ss = lane_sum<VEC>(ss, lanes);
-                        const float r = rsqrtf(ss * P.inv_d + P.eps);
-#pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            a[i][j] *= r * wa[j];
-                            b[i][j] *= r * wb[j];
-                        }
-                    }
-                    if (!row) continue;
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        if (!L.rotated(j)) continue;
-                        const float u = a[i][j], v = b[i][j];
-                        a[i][j] = u * c[j] - v * s[j];
-                        b[i][j] = u * s[j] + v * c[j];
-                    }
-                    L.store(out + h * P.D, a[i], b[i]);
-                }
+            }
+            if (turns) turn<N, KIND>(L, a, b, c, s, m);
+            if (keep) store_pairs<T, N, KIND>(L, out, a, b);
+            out += out_step;
+            fresh = false;
+            if (now.next()) {
+                out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
+                fresh = turns;
+                keep = now.here() && L.live;
             }
         }
     }
 }
 
-template <typename T, bool VEC, bool NORM>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(const __grid_constant__ Params P, int lanes) {
-    constexpr int N = Lane<VEC>::PAIRS, AHEAD = 2;
-    extern __shared__ float sums[];               // [row groups][2][D]
-    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = THREADS / lanes;
-    const Lane<VEC> L(P, lane);
-    const int64_t step = (int64_t)gridDim.x * (groups / P.share);
-    const int64_t t0 = (int64_t)blockIdx.x * (groups / P.share), mine = group / P.share;
-    float ga[2][N], gb[2][N];                     // this thread's part of the weights' gradients
+template <typename T, int N, int LANES, Kind KIND, bool NORM>
+__global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 3) bwd_kernel(const __grid_constant__ Params P) {
+    constexpr int DEPTH = 2;
+    extern __shared__ float sums[];               // [row groups][D]
+    const int which = blockIdx.x >= P.blocks0, block = blockIdx.x - (which ? P.blocks0 : 0);
+    const Side& S = P.side[which];
+    constexpr int groups = THREADS / LANES;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int h0 = group % S.share;
+    const Lane<N, KIND> L(P, lane);
+    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, group, groups), far = now;
+    const int64_t steps = now.steps(), ts = S.ts, hs = S.hs, dts = S.dts, dhs = S.dhs, ld = (int64_t)S.heads * P.D;
+    const int out_step = S.share * P.D, share = S.share;
+    const T *in = row_at<T>(S.dy, dts, dhs, far.token(), h0), *inx = row_at<T>(S.x, ts, hs, far.token(), h0);
+    T* out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
+    Raw<T, N, KIND> raw[DEPTH], rawx[DEPTH];
+    auto fetch = [&](int k) {
+        raw[k].fetch(L, in);
+        in += dhs * share;
+        if (NORM) {
+            rawx[k].fetch(L, inx);
+            inx += hs * share;
+        }
+        if (far.next()) {
+            in = row_at<T>(S.dy, dts, dhs, far.token(), h0);
+            if (NORM) inx = row_at<T>(S.x, ts, hs, far.token(), h0);
+        }
+    };
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < DEPTH - 1; ++k) fetch(k);
+    uint64_t wa[N / 2], wb[N / 2], c[N / 2], s[N / 2], m[N / 2], ga[N / 2], gb[N / 2];   // ga, gb: of the weights' gradient
+    if (NORM && S.w) {
+        Raw<float, N, KIND> w;
+        w.fetch(L, S.w);
+        w.pairs(wa, wb);
+    } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) ga[k][j] = gb[k][j] = 0.f;
-    for (int64_t base = t0; base < P.T; base += step) {
-        const int64_t t = base + mine;
-        const bool here = t < P.T && L.live;
-        float c[N], s[N];
-        L.angles(P, here ? t : base, c, s);
+        for (int j = 0; j < N / 2; ++j) wa[j] = wb[j] = f2(1.f, 1.f);
+    }
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const int heads = P.heads[which];
-            const T* x = static_cast<const T*>(P.x[which]) + t * P.ts[which];
-            const T* dy = static_cast<const T*>(P.dy[which]) + t * P.dts[which];
-            T* out = static_cast<T*>(P.out[which]) + t * heads * P.D;
-            float wa[N], wb[N];
+    for (int j = 0; j < N / 2; ++j) ga[j] = gb[j] = 0;
+    const float inv_d = P.inv_d, eps = P.eps;
+    const bool turns = P.rot > 0;
+    bool fresh = turns, keep = now.here() && L.live;
+    int64_t pos = turns ? position(P, now.token()) : 0;
+    for (int64_t n = 0; n < steps; n += DEPTH) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) wa[j] = wb[j] = 1.f;
-            if (NORM && P.w[which] && L.live) L.load(P.w[which], wa, wb);
-#pragma unroll 1
-            for (int h0 = group & (P.share - 1); h0 - (group & (P.share - 1)) < heads; h0 += AHEAD * P.share) {
-                float a[AHEAD][N], b[AHEAD][N], xa[AHEAD][N], xb[AHEAD][N];
+        for (int k = 0; k < DEPTH; ++k) {
+            fetch((k + DEPTH - 1) % DEPTH);
+            if (fresh) {
+                angles<N, KIND>(P, L, pos, c, s, m);
+                pos = position(P, min(now.base + now.mine + now.step, now.T - 1));
+            }
+            uint64_t a[N / 2], b[N / 2];
+            raw[k].pairs(a, b);
+            if (turns) turn<N, KIND>(L, a, b, c, m, s);
+            if constexpr (NORM) {
+                uint64_t xa[N / 2], xb[N / 2], ss = 0, gx = 0;
+                rawx[k].pairs(xa, xb);
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int h = h0 + i * P.share;
-                    if (here && h < heads) {
-                        L.load(dy + h * P.dhs[which], a[i], b[i]);
-                        if (NORM) L.load(x + h * P.hs[which], xa[i], xb[i]);
-                    }
+                for (int j = 0; j < N / 2; ++j) {
+                    ss = fma2(xb[j], xb[j], fma2(xa[j], xa[j], ss));
+                    gx = fma2(mul2(b[j], wb[j]), xb[j], fma2(mul2(a[j], wa[j]), xa[j], gx));
                 }
+                const float sq = lane_sum<LANES>(L.live ? sum2(ss) : 0.f), gs = lane_sum<LANES>(L.live ? sum2(gx) : 0.f);
+                const float r = rsqrtf(sq * inv_d + eps), q = -r * r * r * gs * inv_d;
+                const float rg = keep ? r : 0.f;           // (a row that is not there is another's copy)
+                const uint64_t r2 = f2(r, r), q2 = f2(q, q), rg2 = f2(rg, rg);
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int h = h0 + i * P.share;
-                    const bool row = here && h < heads;
-                    if (row) {
-#pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            if (!L.rotated(j)) continue;
-                            const float u = a[i][j], v = b[i][j];
-                            a[i][j] = u * c[j] + v * s[j];
-                            b[i][j] = v * c[j] - u * s[j];
-                        }
-                    }
-                    if constexpr (NORM) {
-                        float ss = 0.f, gx = 0.f;
-                        if (row) {
-#pragma unroll
-                            for (int j = 0; j < N; ++j) {
-                                ss += xa[i][j] * xa[i][j] + xb[i][j] * xb[i][j];
-                                gx += a[i][j] * wa[j] * xa[i][j] + b[i][j] * wb[j] * xb[i][j];
-                            }
-                        }
-                        ss = lane_sum<VEC>(ss, lanes);
-                        gx = lane_sum<VEC>(gx, lanes);
-                        const float r = rsqrtf(ss * P.inv_d + P.eps), m = r * r * gx * P.inv_d;
-                        if (row) {
-#pragma unroll
-                            for (int j = 0; j < N; ++j) {
-                                ga[which][j] += a[i][j] * (xa[i][j] * r);
-                                gb[which][j] += b[i][j] * (xb[i][j] * r);
-                                a[i][j] = r * (a[i][j] * wa[j] - xa[i][j] * m);
-                                b[i][j] = r * (b[i][j] * wb[j] - xb[i][j] * m);
-                            }
-                        }
-                    }
-                    if (row) L.store(out + h * P.D, a[i], b[i]);
+                for (int j = 0; j < N / 2; ++j) {
+                    ga[j] = fma2(a[j], mul2(xa[j], rg2), ga[j]);
+                    gb[j] = fma2(b[j], mul2(xb[j], rg2), gb[j]);
+                    a[j] = fma2(xa[j], q2, mul2(mul2(a[j], wa[j]), r2));
+                    b[j] = fma2(xb[j], q2, mul2(mul2(b[j], wb[j]), r2));
                 }
+            }
+            if (keep) store_pairs<T, N, KIND>(L, out, a, b);
+            out += out_step;
+            fresh = false;
+            if (now.next()) {
+                out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
+                fresh = turns;
+                keep = now.here() && L.live;
             }
         }
     }
     if (NORM && P.part) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (L.live) L.store(sums + (group * 2 + k) * P.D, ga[k], gb[k]);
+        if (L.live) store_pairs<float, N, KIND>(L, sums + group * P.D, ga, gb);
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * P.D; i += THREADS) {
+        for (int i = threadIdx.x; i < P.D; i += THREADS) {
             float v = sums[i];
-            for (int g = 1; g < groups; ++g) v += sums[g * 2 * P.D + i];
-            P.part[(int64_t)blockIdx.x * 2 * P.D + i] = v;
+            for (int g = 1; g < groups; ++g) v += sums[g * P.D + i];
+            P.part[(int64_t)blockIdx.x * P.D + i] = v;
         }
     }
 }
 
-// the blocks' sums in a fixed order: 8 columns x 32 strides a block
-__global__ void __launch_bounds__(256) sum_kernel(const float* part, int blocks, int D, float* dqw, float* dkw) {
+// the blocks' sums in a fixed order: 8 columns x 32 strides a block; the first
+// blocks of this grid are q's
+__global__ void __launch_bounds__(256) sum_kernel(const float* part, int blocks0, int blocks, int D, float* dqw, float* dkw) {
     __shared__ float red[32][9];
-    const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3, c = blockIdx.x * 8 + cx;
+    const int per = (D + 7) / 8, side = blockIdx.x >= per;
+    const int cx = threadIdx.x & 7, ry = threadIdx.x >> 3, c = (blockIdx.x - side * per) * 8 + cx;
+    const int first = side ? blocks0 : 0, last = side ? blocks : blocks0;
     float v = 0.f;
-    if (c < 2 * D) {
-#pragma unroll 4
-        for (int k = ry; k < blocks; k += 32) v += part[(int64_t)k * 2 * D + c];
+    if (c < D) {
+#pragma unroll 8
+        for (int k = first + ry; k < last; k += 32) v += part[(int64_t)k * D + c];
     }
     red[ry][cx] = v;
     __syncthreads();
-    if (ry == 0 && c < 2 * D) {
+    if (ry == 0 && c < D) {
         v = 0.f;
 #pragma unroll
         for (int k = 0; k < 32; ++k) v += red[k][cx];
-        float* out = c < D ? dqw : dkw;
-        if (out) out[c < D ? c : c - D] = v;
+        float* out = side ? dkw : dqw;
+        if (out) out[c] = v;
     }
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int MAX_BLOCKS = 148 * 4;       // of the backward, whose blocks each leave a row of sums
+constexpr int MAX_BLOCKS = 148 * 8;       // of the backward, whose blocks each leave a row of sums
 
-int lanes_of(int64_t D, bool vec) {
-    if (!vec) return 32;
-    int n = 1;
-    while (n * 16 < D) n *= 2;
-    return n;
-}
-
-// Groups of a block that share a token: few where tokens are many (cos and sin
-// are then read once for more heads, weights stay), all heads' side by side
-// where they would not fill the GPU.
+// Groups of a block that share a token's heads: one where tokens are many (cos and sin are
+// waited for once for all heads), more where the tokens alone would not fill the GPU twice.
 int share_of(int64_t T, int heads, int groups) {
     int share = 1;
-    while (share < groups && share < heads && (share < 4 || T * share < (int64_t)groups * 148 * 4)) share *= 2;
+    while (share < groups && heads % (2 * share) == 0 && heads > 0 && T * share < (int64_t)groups * 148 * 2) share *= 2;
     return share;
 }
 
-bool vec_of(const Params& P, const concord_qk_params* p, bool bwd) {
-    const int per = p->type == CONCORD_F32 ? 4 : 8;
-    bool ok = P.D % 16 == 0 && P.rot % 16 == 0 && aligned(P.cos, 16) && aligned(P.sin, 16);
-    for (int k = 0; k < 2; ++k) {
-        if (P.heads[k] == 0) continue;
-        ok = ok && aligned(P.x[k], 16) && P.ts[k] % per == 0 && P.hs[k] % per == 0 && aligned(P.out[k], 16) &&
-             aligned(P.w[k], 16);
-        if (bwd) ok = ok && aligned(P.dy[k], 16) && P.dts[k] % per == 0 && P.dhs[k] % per == 0;
+// whether rows are whole runs of 4 columns that loads of 16 bits' worth of them may take (8 pairs a lane
+// instead, for sizes of 16 columns, measured 60 us beside 56 and 124 beside 122, 16384 x 32 heads of 128)
+bool rows_fit(const Params& P, int32_t type, bool bwd) {
+    const int per = type == CONCORD_F32 ? 4 : 8;
+    bool ok = P.D % 8 == 0 && P.rot % 8 == 0 && aligned(P.cos, 16) && aligned(P.sin, 16);
+    for (const Side& S : P.side) {
+        if (S.heads == 0) continue;
+        ok = ok && aligned(S.x, 16) && S.ts % per == 0 && S.hs % per == 0 && aligned(S.out, 16) && aligned(S.w, 16);
+        if (bwd) ok = ok && aligned(S.dy, 16) && S.dts % per == 0 && S.dhs % per == 0;
     }
     return ok;
 }
 
-int64_t blocks_of(const Params& P, int lanes, int share, bool bwd) {
-    const int64_t tokens = THREADS / lanes / share, need = (P.T + tokens - 1) / tokens;
-    const int64_t most = bwd ? MAX_BLOCKS : 148 * 16;
-    return need < most ? need : most;
+template <typename K> int resident_blocks(K k, size_t smem) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, THREADS, smem) != cudaSuccess || per_sm < 1) {
+        cudaGetLastError();
+        per_sm = 1;
+    }
+    int d = 0, sms = 148;
+    if (cudaGetDevice(&d) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d);
+    return sms * per_sm;
 }
 
-template <typename T, bool VEC, bool NORM> int launch(Params P, bool bwd, cudaStream_t st) {
-    const int lanes = lanes_of(P.D, VEC), groups = THREADS / lanes;
-    P.share = share_of(P.T, P.heads[0] > P.heads[1] ? P.heads[0] : P.heads[1], groups);
-    const int blocks = (int)blocks_of(P, lanes, P.share, bwd);
+template <typename T, int N, int LANES, Kind KIND, bool NORM> int launch(Params P, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
+    constexpr int groups = THREADS / LANES;
+    const size_t smem = bwd && NORM && P.part ? (size_t)groups * P.D * sizeof(float) : 0;
+    // one wave of blocks, q's and k's by their heads
+    static std::atomic<int> known[2];
+    int most = known[bwd].load();
+    if (most == 0) {
+        most = bwd ? resident_blocks(bwd_kernel<T, N, LANES, KIND, NORM>, 40 * 1024) : resident_blocks(fwd_kernel<T, N, LANES, KIND, NORM>, 0);
+        if (most > MAX_BLOCKS) most = MAX_BLOCKS;
+        known[bwd].store(most);
+    }
+    int blocks[2];
+    const int heads = P.side[0].heads + P.side[1].heads;
+    for (int k = 0; k < 2; ++k) {
+        Side& S = P.side[k];
+        S.share = share_of(P.T, S.heads, groups);
+        const int64_t tokens = groups / S.share, need = (P.T + tokens - 1) / tokens;
+        int64_t part = k ? most - most * (int64_t)P.side[0].heads / heads : most * (int64_t)P.side[0].heads / heads;
+        if (part < 1) part = 1;
+        blocks[k] = S.heads == 0 ? 0 : (int)(need < part ? need : part);
+    }
+    P.blocks0 = blocks[0];
+    const int all = blocks[0] + blocks[1];
     if (!bwd) {
-        fwd_kernel<T, VEC, NORM><<<blocks, THREADS, 0, st>>>(P, lanes);
+        fwd_kernel<T, N, LANES, KIND, NORM><<<all, THREADS, 0, st>>>(P);
         return check_launch("concord_qk_norm_rope_fwd");
     }
-    const size_t smem = NORM && P.part ? (size_t)groups * 2 * P.D * sizeof(float) : 0;
-    bwd_kernel<T, VEC, NORM><<<blocks, THREADS, smem, st>>>(P, lanes);
-    return check_launch("concord_qk_norm_rope_bwd");
+    bwd_kernel<T, N, LANES, KIND, NORM><<<all, THREADS, smem, st>>>(P);
+    if (int rc = check_launch("concord_qk_norm_rope_bwd")) return rc;
+    if (NORM && P.part) {
+        sum_kernel<<<2 * ((P.D + 7) / 8), 256, 0, st>>>(P.part, blocks[0], all, P.D, dqw, dkw);
+        return check_launch("concord_qk_norm_rope_bwd");
+    }
+    return CONCORD_OK;
 }
 
-template <typename T> int run(const Params& P, bool vec, bool norm, bool bwd, cudaStream_t st) {
-    if (vec) return norm ? launch<T, true, true>(P, bwd, st) : launch<T, true, false>(P, bwd, st);
-    return norm ? launch<T, false, true>(P, bwd, st) : launch<T, false, false>(P, bwd, st);
+template <typename T, bool NORM> int run(const Params& P, bool vec, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
+    // (a lane 8 columns; rows of up to 32 columns leave half of the 8 lanes idle)
+#define QK_LAUNCH(LANES)                                                                                \
+    return P.interleaved ? launch<T, 4, LANES, PAIRED, NORM>(P, bwd, dqw, dkw, st)                     \
+                         : launch<T, 4, LANES, HALVES, NORM>(P, bwd, dqw, dkw, st)
+    if (vec && P.D <= 64) QK_LAUNCH(8);
+    if (vec && P.D <= 128) QK_LAUNCH(16);
+    if (vec) QK_LAUNCH(32);
+    return P.D <= 128 ? launch<T, 2, 32, ANY, NORM>(P, bwd, dqw, dkw, st) : launch<T, 4, 32, ANY, NORM>(P, bwd, dqw, dkw, st);
 }
 
-int dispatch(const Params& P, const concord_qk_params* p, bool bwd, cudaStream_t st) {
-    const bool vec = vec_of(P, p, bwd);
-    if (p->type == CONCORD_F32) return run<float>(P, vec, p->norm != 0, bwd, st);
-    if (p->type == CONCORD_BF16) return run<__nv_bfloat16>(P, vec, p->norm != 0, bwd, st);
-    return run<__half>(P, vec, p->norm != 0, bwd, st);
+int dispatch(const Params& P, const concord_qk_params* p, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
+    const bool vec = rows_fit(P, p->type, bwd);
+    if (p->type == CONCORD_F32)
+        return p->norm ? run<float, true>(P, vec, bwd, dqw, dkw, st) : run<float, false>(P, vec, bwd, dqw, dkw, st);
+    if (p->type == CONCORD_BF16)
+        return p->norm ? run<__nv_bfloat16, true>(P, vec, bwd, dqw, dkw, st)
+                       : run<__nv_bfloat16, false>(P, vec, bwd, dqw, dkw, st);
+    return p->norm ? run<__half, true>(P, vec, bwd, dqw, dkw, st) : run<__half, false>(P, vec, bwd, dqw, dkw, st);
 }
 
 int check_params(const char* name, const concord_qk_params* p) {
@@ -397,8 +583,8 @@ int check_params(const char* name, const concord_qk_params* p) {
     if (p->tokens < 0 || p->heads < 0 || p->kv_heads < 0 || p->heads + p->kv_heads < 1 || p->head_dim < 1 || p->rot < 0 ||
         p->rot % 2 || p->rot > p->head_dim || (p->rot > 0 && p->positions < 1))
         return fail(CONCORD_ESHAPE, std::string(name) + ": bad extents");
-    if (p->head_dim > MAX_DIM || p->heads > 65536 || p->kv_heads > 65536 || p->tokens > (int64_t)1 << 40)
-        return fail(CONCORD_ETOOBIG, std::string(name) + ": heads of more than 256, or more than 65536 heads or 2^40 tokens");
+    if (p->head_dim > MAX_DIM || p->heads > 65536 || p->kv_heads > 65536 || p->tokens > (int64_t)1 << 30)
+        return fail(CONCORD_ETOOBIG, std::string(name) + ": heads of more than 256, or more than 65536 heads or 2^30 tokens");
     if (p->rot > 0 && (!p->cos || !p->sin)) return fail(CONCORD_EINVAL, std::string(name) + ": null table");
     return CONCORD_OK;
 }
@@ -411,8 +597,8 @@ Params params(const concord_qk_params* p) {
     P.pos64 = p->pos64;
     P.T = p->tokens;
     P.positions = p->positions;
-    P.heads[0] = (int)p->heads;
-    P.heads[1] = (int)p->kv_heads;
+    P.side[0].heads = (int)p->heads;
+    P.side[1].heads = (int)p->kv_heads;
     P.D = (int)p->head_dim;
     P.rot = (int)p->rot;
     P.interleaved = p->interleaved;
@@ -421,13 +607,13 @@ Params params(const concord_qk_params* p) {
     return P;
 }
 
-int operand(const char* name, Params& P, int k, const void* x, int64_t ts, int64_t hs, const float* w, void* out) {
-    P.x[k] = x;
-    P.ts[k] = ts;
-    P.hs[k] = hs;
-    P.w[k] = w;
-    P.out[k] = out;
-    if (P.heads[k] > 0 && !out) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
+int operand(const char* name, Side& S, const void* x, int64_t ts, int64_t hs, const float* w, void* out) {
+    S.x = x;
+    S.ts = ts;
+    S.hs = hs;
+    S.w = w;
+    S.out = out;
+    if (S.heads > 0 && !out) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
     if (ts < 0 || hs < 0) return fail(CONCORD_ESHAPE, std::string(name) + ": negative stride");
     return CONCORD_OK;
 }
@@ -444,15 +630,15 @@ extern "C" int concord_qk_norm_rope_fwd(const concord_qk_params* p, const void* 
     if (int rc = qkn::check_params(name, p)) return rc;
     if (p->tokens == 0) return CONCORD_OK;
     qkn::Params P = qkn::params(p);
-    if (int rc = qkn::operand(name, P, 0, q, q_ts, q_hs, q_weight, q_out)) return rc;
-    if (int rc = qkn::operand(name, P, 1, k, k_ts, k_hs, k_weight, k_out)) return rc;
+    if (int rc = qkn::operand(name, P.side[0], q, q_ts, q_hs, q_weight, q_out)) return rc;
+    if (int rc = qkn::operand(name, P.side[1], k, k_ts, k_hs, k_weight, k_out)) return rc;
     if ((p->heads && !q) || (p->kv_heads && !k)) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
-    return qkn::dispatch(P, p, false, as_stream(stream));
+    return qkn::dispatch(P, p, false, nullptr, nullptr, as_stream(stream));
 }
 
 extern "C" size_t concord_qk_norm_rope_bwd_workspace_bytes(const concord_qk_params* p) {
     if (qkn::check_params("concord_qk_norm_rope_bwd_workspace_bytes", p) || !p->norm || p->tokens == 0) return 0;
-    return (size_t)qkn::MAX_BLOCKS * 2 * p->head_dim * sizeof(float);
+    return (size_t)(qkn::MAX_BLOCKS + 2) * p->head_dim * sizeof(float);
 }
 
 extern "C" int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t q_ts, int64_t q_hs,
@@ -471,30 +657,21 @@ extern "C" int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* 
         return check_launch(name);
     }
     qkn::Params P = qkn::params(p);
-    if (int rc = qkn::operand(name, P, 0, q, q_ts, q_hs, q_weight, dq)) return rc;
-    if (int rc = qkn::operand(name, P, 1, k, k_ts, k_hs, k_weight, dk)) return rc;
+    if (int rc = qkn::operand(name, P.side[0], q, q_ts, q_hs, q_weight, dq)) return rc;
+    if (int rc = qkn::operand(name, P.side[1], k, k_ts, k_hs, k_weight, dk)) return rc;
     if ((p->heads && (!dq_out || (p->norm && !q))) || (p->kv_heads && (!dk_out || (p->norm && !k))))
         return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
     if (dq_ts < 0 || dq_hs < 0 || dk_ts < 0 || dk_hs < 0) return fail(CONCORD_ESHAPE, std::string(name) + ": negative stride");
-    P.dy[0] = dq_out;
-    P.dts[0] = dq_ts;
-    P.dhs[0] = dq_hs;
-    P.dy[1] = dk_out;
-    P.dts[1] = dk_ts;
-    P.dhs[1] = dk_hs;
+    P.side[0].dy = dq_out;
+    P.side[0].dts = dq_ts;
+    P.side[0].dhs = dq_hs;
+    P.side[1].dy = dk_out;
+    P.side[1].dts = dk_ts;
+    P.side[1].dhs = dk_hs;
     if (weights) {
         if (!workspace || workspace_bytes < concord_qk_norm_rope_bwd_workspace_bytes(p))
             return fail(CONCORD_EWORKSPACE, std::string(name) + ": workspace too small");
         P.part = static_cast<float*>(workspace);
     }
-    if (int rc = qkn::dispatch(P, p, true, st)) return rc;
-    if (weights) {
-        const bool vec = qkn::vec_of(P, p, true);
-        const int lanes = qkn::lanes_of(P.D, vec), groups = qkn::THREADS / lanes;
-        const int share = qkn::share_of(P.T, P.heads[0] > P.heads[1] ? P.heads[0] : P.heads[1], groups);
-        qkn::sum_kernel<<<(2 * P.D + 7) / 8, 256, 0, st>>>(P.part, (int)qkn::blocks_of(P, lanes, share, true), P.D,
-                                                           dq_weight, dk_weight);
-        return check_launch(name);
-    }
-    return CONCORD_OK;
+    return qkn::dispatch(P, p, true, dq_weight, dk_weight, st);
 }

@@ -685,7 +685,7 @@ int concord_embedding_bwd(const void* ids, int32_t ids64, const void* dy, int32_
  * in cos / sin [positions, rot / 2] at the token's position, pos [tokens] (int32
  * or int64) or NULL: the token's number.  A position that the tables do not have gives
  * NaN.  Inputs take a token and a head stride (elements, columns contiguous);
- * outputs and gradients are contiguous.  heads or kv_heads may be 0.  D <= 256.
+ * outputs and gradients are contiguous.  heads or kv_heads may be 0.  D <= 256, at most 2^30 tokens.
  * The backward writes dq, dk and, unless NULL, the weights' gradients (fp32 [D],
  * sums in a fixed order); without the norm it does not read q and k.
  */
@@ -715,10 +715,11 @@ int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t 
  * feature share a power of two 2^e, the least with |x| <= 127 2^e, and a value is
  * the whole number nearest to x / 2^e (ties to even; in the block of a type's largest
  * values at most 63, which it can still hold).  A block with a NaN or an infinity
- * reads back as NaN.  `saved`: concord_saved8_bytes(M, K) bytes, 16-byte aligned:
- *   int8 codes [ceil(M / 32) * 2][K][16]: token 16 i + j of feature k at [i][k][j],
- *        zeros beyond M;
- *   uint8 e + 127 (255: NaN) [ceil(M / 32)][K rounded up to 16].
+ * reads back as NaN.  `saved`: concord_saved8_bytes(M, K) bytes, 32-byte aligned,
+ * tiles of 64 tokens x 128 features in order of tokens, then features, each
+ *   int8 codes [4][features][16], 16 tokens of a feature side by side, and
+ *   uint8 e + 127 (255: NaN) [2][features],
+ * features filled up to a multiple of 16 (the last tile of 64 tokens is narrower), tokens to one of 64.
  * concord_dense8 reads them back, rounded to the type of out [M, K].
  * concord_gemm_dw8: dw [N, K] (bf16, contiguous) = dy^T x for dy [M, N] (bf16, row
  * stride lddy) and x in 8 bits: the values it keeps are exact in bf16, sums are fp32,
