@@ -15,33 +15,46 @@ namespace concord {
 namespace eight {
 
 constexpr int THREADS = 128;
+#ifndef SAVE_BY
+#define SAVE_BY 8
+#define FWD_BY 4
+#define BWD_BY 8
+#endif
 
+
+template <int EL> __device__ __forceinline__ void load_codes(const uint8_t* p, uint4* c) {
+    if constexpr (EL == 1) c[0] = *reinterpret_cast<const uint4*>(p);
+    else {
+#pragma unroll
+        for (int j = 0; j < EL; j += 2) load32(p + j * 16, c[j], c[j + 1]);
+    }
+}
 
 template <typename T, int EL>
 __global__ void __launch_bounds__(THREADS)
-    save_kernel(const T* x, int64_t ldx, int8_t* codes, uint8_t* scales, int64_t M, int K) {
+    save_kernel(const T* x, int64_t ldx, uint8_t* saved, int64_t M, int K) {
     const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
     const int64_t tb = blockIdx.x, t0 = tb * BLOCK;
     if (k >= K) return;
     Tile<T, EL> A;
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i) A.load_row(i, x + (t0 + i) * ldx + k, t0 + i < M);
-    A.save(codes, scales, tb, K, k);
+    A.save(saved, tb, K, k);
 }
 
 // a thread: 16 tokens of EL features
 template <typename T, int EL>
 __global__ void __launch_bounds__(THREADS)
-    dense_kernel(const int8_t* codes, const uint8_t* scales, T* out, int64_t ldo, int64_t M, int K) {
+    dense_kernel(const uint8_t* saved, T* out, int64_t ldo, int64_t M, int K) {
     const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
     const int64_t tb = blockIdx.x, t0 = tb * 16;
     if (k >= K || t0 >= M) return;
+    const Place at(tb >> 2, k, K);
     uint4 c[EL];
     float scale[EL];
+    load_codes<EL>(saved + at.codes(tb & 3), c);
 #pragma unroll
-    for (int j = 0; j < EL; ++j) c[j] = reinterpret_cast<const uint4*>(codes)[tb * K + k + j];
-#pragma unroll
-    for (int j = 0; j < EL; ++j) scale[j] = scale_of(scales[(tb >> 1) * scale_row(K) + k + j]);
+    for (int j = 0; j < EL; ++j) scale[j] = scale_of(saved[at.scale((tb >> 1) & 1) + j]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         if (t0 + i >= M) break;
@@ -61,7 +74,11 @@ __global__ void __launch_bounds__(THREADS)
 // ---------------------------------------------------------------- the gated unit
 constexpr int SILU = 0, GELU = 1;
 
-__device__ __forceinline__ float sigmoid(float g) { return __frcp_rn(1.f + ex2f(-1.4426950408889634f * g)); }
+__device__ __forceinline__ float sigmoid(float g) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2f(-1.4426950408889634f * g)));
+    return r;
+}
 
 template <int ACT> __device__ __forceinline__ float act(float g) {
     if constexpr (ACT == SILU) return g * sigmoid(g);
@@ -81,13 +98,10 @@ template <int ACT> __device__ __forceinline__ float2 act2(float g) {
 struct Unit {
     const void *gate, *up;       // NULL gate in the backward: from the codes
     int64_t ldg, ldu;
-    int8_t *g8, *u8, *h8;        // NULL: not kept; their bytes stand behind the codes
+    uint8_t *g8, *u8, *h8;       // NULL: not kept
     int64_t M;
     int K;
 };
-__device__ __forceinline__ uint8_t* scales_of(int8_t* codes, int64_t M, int64_t K) {
-    return reinterpret_cast<uint8_t*>(codes) + code_bytes(M, K);
-}
 
 // forward of 32 tokens x EL features a thread, with what is asked for kept in 8 bits
 template <typename T, int EL, int ACT>
@@ -101,8 +115,8 @@ __global__ void __launch_bounds__(THREADS) fwd8_kernel(const __grid_constant__ U
     for (int i = 0; i < BLOCK; ++i) G.load_row(i, g + i * U.ldg, t0 + i < U.M);
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i) P.load_row(i, u + i * U.ldu, t0 + i < U.M);
-    if (U.g8) G.save(U.g8, scales_of(U.g8, U.M, U.K), tb, U.K, k);
-    if (U.u8) P.save(U.u8, scales_of(U.u8, U.M, U.K), tb, U.K, k);
+    if (U.g8) G.save(U.g8, tb, U.K, k);
+    if (U.u8) P.save(U.u8, tb, U.K, k);
     T* out = h + t0 * U.K + k;
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i) {
@@ -112,7 +126,7 @@ __global__ void __launch_bounds__(THREADS) fwd8_kernel(const __grid_constant__ U
         G.set_row(i, v);
         if (t0 + i < U.M) G.store_row(i, out + (int64_t)i * U.K);
     }
-    if (U.h8) G.save(U.h8, scales_of(U.h8, U.M, U.K), tb, U.K, k);
+    if (U.h8) G.save(U.h8, tb, U.K, k);
 }
 
 // backward from the codes, 16 tokens x EL features a thread
@@ -122,20 +136,18 @@ __global__ void __launch_bounds__(THREADS)
     const int k = (blockIdx.y * blockDim.x + threadIdx.x) * EL;
     const int64_t tb = blockIdx.x, t0 = tb * 16;
     if (k >= U.K || t0 >= U.M) return;
+    const Place at(tb >> 2, k, U.K);
     Tile<T, EL> D;
     uint4 cg[EL], cu[EL];
     float sg[EL], su[EL];
-#pragma unroll
-    for (int j = 0; j < EL; ++j) {
-        cg[j] = reinterpret_cast<const uint4*>(U.g8)[tb * U.K + k + j];
-        cu[j] = reinterpret_cast<const uint4*>(U.u8)[tb * U.K + k + j];
-    }
+    load_codes<EL>(U.g8 + at.codes(tb & 3), cg);
+    load_codes<EL>(U.u8 + at.codes(tb & 3), cu);
 #pragma unroll
     for (int i = 0; i < 16; ++i) D.load_row(i, dh + (t0 + i) * lddh + k, t0 + i < U.M);
 #pragma unroll
     for (int j = 0; j < EL; ++j) {
-        sg[j] = scale_of(scales_of(U.g8, U.M, U.K)[(tb >> 1) * scale_row(U.K) + k + j]);
-        su[j] = scale_of(scales_of(U.u8, U.M, U.K)[(tb >> 1) * scale_row(U.K) + k + j]);
+        sg[j] = scale_of(U.g8[at.scale((tb >> 1) & 1) + j]);
+        su[j] = scale_of(U.u8[at.scale((tb >> 1) & 1) + j]);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -239,32 +251,30 @@ bool rows_fit(const void* p, int64_t ld, int64_t K, int32_t type, int bytes) {
     return K % el == 0 && ld % el == 0 && aligned(p, bytes);
 }
 
-template <typename T> int save(const void* x, int64_t ldx, int32_t type, int8_t* codes, int64_t M, int64_t K, cudaStream_t st) {
-    constexpr int EL = 8 / sizeof(T);
+template <typename T> int save(const void* x, int64_t ldx, int32_t type, uint8_t* saved, int64_t M, int64_t K, cudaStream_t st) {
+    constexpr int EL = SAVE_BY / sizeof(T);
     const bool vec = rows_fit(x, ldx, K, type, 8);
     int threads, blocks_k;
     across(K, vec ? EL : 1, &threads, &blocks_k);
-    uint8_t* scales = reinterpret_cast<uint8_t*>(codes) + code_bytes(M, K);
     auto k = vec ? save_kernel<T, EL> : save_kernel<T, 1>;
-    k<<<dim3((unsigned)blocks(M), blocks_k), threads, 0, st>>>(static_cast<const T*>(x), ldx, codes, scales, M, (int)K);
+    k<<<dim3((unsigned)blocks(M), blocks_k), threads, 0, st>>>(static_cast<const T*>(x), ldx, saved, M, (int)K);
     return check_launch("concord_save8");
 }
 
-template <typename T> int dense(const int8_t* codes, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
-    constexpr int EL = 8 / sizeof(T);
+template <typename T> int dense(const uint8_t* saved, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
+    constexpr int EL = SAVE_BY / sizeof(T);
     const bool vec = rows_fit(out, ldo, K, type, 8);
     int threads, blocks_k;
     across(K, vec ? EL : 1, &threads, &blocks_k);
-    const uint8_t* scales = reinterpret_cast<const uint8_t*>(codes) + code_bytes(M, K);
     auto k = vec ? dense_kernel<T, EL> : dense_kernel<T, 1>;
-    k<<<dim3((unsigned)(2 * blocks(M)), blocks_k), threads, 0, st>>>(codes, scales, static_cast<T*>(out), ldo, M, (int)K);
+    k<<<dim3((unsigned)(2 * blocks(M)), blocks_k), threads, 0, st>>>(saved, static_cast<T*>(out), ldo, M, (int)K);
     return check_launch("concord_dense8");
 }
 
 template <typename T, int ACT> int forward(const Unit& U, void* h, int32_t type, cudaStream_t st) {
     T* out = static_cast<T*>(h);
     if (U.g8 || U.u8 || U.h8) {
-        constexpr int EL = 8 / sizeof(T);
+        constexpr int EL = FWD_BY / sizeof(T);
         const bool vec = rows_fit(U.gate, U.ldg, U.K, type, 8) && rows_fit(U.up, U.ldu, U.K, type, 8) && aligned(h, 8);
         int threads, blocks_k;
         across(U.K, vec ? EL : 1, &threads, &blocks_k);
@@ -288,7 +298,7 @@ int backward(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg
     const T* up = static_cast<const T*>(dh);
     T *og = static_cast<T*>(dg), *ou = static_cast<T*>(du);
     if (U.g8) {
-        constexpr int EL = 8 / sizeof(T);
+        constexpr int EL = BWD_BY / sizeof(T);
         const bool vec = rows_fit(dh, lddh, U.K, type, 8) && rows_fit(dg, lddg, U.K, type, 8) && rows_fit(du, lddu, U.K, type, 8);
         int threads, blocks_k;
         across(U.K, vec ? EL : 1, &threads, &blocks_k);
@@ -323,11 +333,11 @@ int backward(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg
         default: return F<__half, GELU>(__VA_ARGS__);                                                                   \
     }
 
-int save_any(const void* x, int64_t ldx, int32_t type, int8_t* codes, int64_t M, int64_t K, cudaStream_t st) {
-    EIGHT_TYPES(type, save, x, ldx, type, codes, M, K, st)
+int save_any(const void* x, int64_t ldx, int32_t type, uint8_t* saved, int64_t M, int64_t K, cudaStream_t st) {
+    EIGHT_TYPES(type, save, x, ldx, type, saved, M, K, st)
 }
-int dense_any(const int8_t* codes, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
-    EIGHT_TYPES(type, dense, codes, out, ldo, type, M, K, st)
+int dense_any(const uint8_t* saved, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
+    EIGHT_TYPES(type, dense, saved, out, ldo, type, M, K, st)
 }
 int forward_any(const Unit& U, void* h, int32_t type, int a, cudaStream_t st) {
     GATED_TYPES(type, a, forward, U, h, type, st)
@@ -344,23 +354,23 @@ using namespace concord;
 
 extern "C" size_t concord_saved8_bytes(int64_t M, int64_t K) {
     if (M <= 0 || K <= 0 || K > (1 << 20) || M > ((int64_t)1 << 31)) return 0;
-    return (size_t)(eight::code_bytes(M, K) + eight::blocks(M) * eight::scale_row(K));
+    return (size_t)eight::all_bytes(M, K);
 }
 
 extern "C" int concord_save8(const void* x, int32_t type, int64_t ldx, void* saved, int64_t M, int64_t K, void* stream) {
     if (int rc = eight::check_shape("concord_save8", type, M, K, ldx)) return rc;
     if (M == 0) return CONCORD_OK;
     if (!x || !saved) return fail(CONCORD_EINVAL, "concord_save8: null pointer");
-    if (!aligned(saved, 16)) return fail(CONCORD_EALIGN, "concord_save8: saved must be 16-byte aligned");
-    return eight::save_any(x, ldx, type, static_cast<int8_t*>(saved), M, K, as_stream(stream));
+    if (!aligned(saved, 32)) return fail(CONCORD_EALIGN, "concord_save8: saved must be 32-byte aligned");
+    return eight::save_any(x, ldx, type, static_cast<uint8_t*>(saved), M, K, as_stream(stream));
 }
 
 extern "C" int concord_dense8(const void* saved, void* out, int32_t type, int64_t ldo, int64_t M, int64_t K, void* stream) {
     if (int rc = eight::check_shape("concord_dense8", type, M, K, ldo)) return rc;
     if (M == 0) return CONCORD_OK;
     if (!out || !saved) return fail(CONCORD_EINVAL, "concord_dense8: null pointer");
-    if (!aligned(saved, 16)) return fail(CONCORD_EALIGN, "concord_dense8: saved must be 16-byte aligned");
-    return eight::dense_any(static_cast<const int8_t*>(saved), out, ldo, type, M, K, as_stream(stream));
+    if (!aligned(saved, 32)) return fail(CONCORD_EALIGN, "concord_dense8: saved must be 32-byte aligned");
+    return eight::dense_any(static_cast<const uint8_t*>(saved), out, ldo, type, M, K, as_stream(stream));
 }
 
 extern "C" int concord_gated_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t type, int32_t act,
@@ -370,10 +380,10 @@ extern "C" int concord_gated_fwd(const void* gate, int64_t ldg, const void* up, 
     if (act < 0 || act > 1) return fail(CONCORD_EINVAL, "concord_gated_fwd: unknown activation");
     if (M == 0) return CONCORD_OK;
     if (!gate || !up || !h) return fail(CONCORD_EINVAL, "concord_gated_fwd: null pointer");
-    if (!aligned(saved_gate, 16) || !aligned(saved_up, 16) || !aligned(saved_h, 16))
-        return fail(CONCORD_EALIGN, "concord_gated_fwd: saved tensors must be 16-byte aligned");
-    const eight::Unit U{gate, up, ldg, ldu, static_cast<int8_t*>(saved_gate), static_cast<int8_t*>(saved_up),
-                        static_cast<int8_t*>(saved_h), M, (int)K};
+    if (!aligned(saved_gate, 32) || !aligned(saved_up, 32) || !aligned(saved_h, 32))
+        return fail(CONCORD_EALIGN, "concord_gated_fwd: saved tensors must be 32-byte aligned");
+    const eight::Unit U{gate, up, ldg, ldu, static_cast<uint8_t*>(saved_gate), static_cast<uint8_t*>(saved_up),
+                        static_cast<uint8_t*>(saved_h), M, (int)K};
     return eight::forward_any(U, h, type, act, as_stream(stream));
 }
 
@@ -388,9 +398,9 @@ extern "C" int concord_gated_bwd(const void* gate, int64_t ldg, const void* up, 
     if (!dh || !dgate || !dup || !saved_gate != !saved_up || (!saved_gate && (!gate || !up)))
         return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
     if (!saved_gate && (ldg < K || ldu < K)) return fail(CONCORD_ESHAPE, std::string(name) + ": bad row stride");
-    if (!aligned(saved_gate, 16) || !aligned(saved_up, 16))
-        return fail(CONCORD_EALIGN, std::string(name) + ": saved tensors must be 16-byte aligned");
-    const eight::Unit U{gate, up, ldg, ldu, static_cast<int8_t*>(const_cast<void*>(saved_gate)),
-                        static_cast<int8_t*>(const_cast<void*>(saved_up)), nullptr, M, (int)K};
+    if (!aligned(saved_gate, 32) || !aligned(saved_up, 32))
+        return fail(CONCORD_EALIGN, std::string(name) + ": saved tensors must be 32-byte aligned");
+    const eight::Unit U{gate, up, ldg, ldu, static_cast<uint8_t*>(const_cast<void*>(saved_gate)),
+                        static_cast<uint8_t*>(const_cast<void*>(saved_up)), nullptr, M, (int)K};
     return eight::backward_any(U, dh, lddh, dgate, lddg, dup, lddu, type, act, as_stream(stream));
 }

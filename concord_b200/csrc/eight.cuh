@@ -7,10 +7,13 @@
 // most 7 significant bits, so it is the same in fp32, bf16 and fp16.  A block
 // is one feature's because features differ in size far more than a feature does from token to token.
 //
-// Stored: codes [ceil(M / 32) * 2][K][16], 16 tokens of a feature side by side
-// (the piece that a lane of the weight gradient's product reads at once), rows
-// beyond M as zeros; then one byte e + 127 a block, [ceil(M / 32)][K rounded up to 16].  A block
-// with a NaN or an infinity has the byte 255 and codes 0: 0 * 2^128 reads as NaN.
+// Stored in tiles of 64 tokens x 128 features, a tile's bytes together (one
+// copy fetches what a step of the weight gradient's product reads): codes
+// [4][features][16], 16 tokens of a feature side by side, then the bytes e +
+// 127, [2][features].  Tiles stand in order of tokens, then features; features
+// are filled up to a multiple of 16 (the last tile of a row of tiles is narrower),
+// tokens to one of 64, with zeros.  A block with a NaN or an infinity has the byte
+// 255 and codes 0: 0 * 2^128 reads as NaN.
 #pragma once
 
 #include "vec.cuh"
@@ -20,9 +23,29 @@ namespace eight {
 
 constexpr int BLOCK = 32;
 
-__host__ __device__ constexpr int64_t blocks(int64_t M) { return (M + BLOCK - 1) / BLOCK; }
-__host__ __device__ constexpr int64_t code_bytes(int64_t M, int64_t K) { return blocks(M) * BLOCK * K; }
-__host__ __device__ constexpr int64_t scale_row(int64_t K) { return (K + 15) / 16 * 16; }
+constexpr int TOKENS = 64, FEATS = 128, TILE_BYTES = TOKENS * FEATS + 2 * FEATS;
+
+__host__ __device__ constexpr int64_t token_tiles(int64_t M) { return (M + TOKENS - 1) / TOKENS; }
+__host__ __device__ constexpr int64_t blocks(int64_t M) { return 2 * token_tiles(M); }     // of 32 tokens
+// features of a row of tiles, its bytes, and those of all rows
+__host__ __device__ constexpr int64_t padded(int64_t K) { return (K + 15) / 16 * 16; }
+__host__ __device__ constexpr int64_t row_bytes(int64_t K) { return padded(K) * (TOKENS + 2); }
+__host__ __device__ constexpr int64_t all_bytes(int64_t M, int64_t K) { return token_tiles(M) * row_bytes(K); }
+
+// where the codes of 16 tokens (t16: the token's number / 16) of feature k stand, and the byte of block tb
+struct Place {
+    int64_t tile;             // offset of the tile
+    int width, k;             // its features, and k's place among them
+    __host__ __device__ __forceinline__ Place(int64_t token_tile, int feature, int64_t K) {
+        const int col = feature / FEATS;
+        tile = token_tile * row_bytes(K) + (int64_t)col * TILE_BYTES;
+        const int64_t left = padded(K) - (int64_t)col * FEATS;
+        width = left < FEATS ? (int)left : FEATS;
+        k = feature % FEATS;
+    }
+    __host__ __device__ __forceinline__ int64_t codes(int t16) const { return tile + ((int64_t)t16 * width + k) * 16; }
+    __host__ __device__ __forceinline__ int64_t scale(int block) const { return tile + TOKENS * width + block * width + k; }
+};
 
 // the byte of a block whose largest magnitude has these bits (a NaN's are the largest)
 __device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
@@ -49,6 +72,18 @@ __device__ __forceinline__ float value(uint32_t flipped, int j, float scale, flo
 }
 __device__ __forceinline__ float value_off(float scale) { return -8388736.f * scale; }
 
+// 32 bytes at once
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+    asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+        : "l"(p));
+}
+
 // EL features of 32 tokens in registers, as loaded
 template <typename T, int EL> struct Tile {
     static constexpr int W = EL * (int)sizeof(T) / 4 > 0 ? EL * (int)sizeof(T) / 4 : 1;
@@ -57,23 +92,21 @@ template <typename T, int EL> struct Tile {
         if (!have) {
 #pragma unroll
             for (int w = 0; w < W; ++w) raw[i][w] = 0;
-        } else if constexpr (EL == 1) {
-            if constexpr (sizeof(T) == 4) raw[i][0] = *reinterpret_cast<const uint32_t*>(p);
-            else raw[i][0] = *reinterpret_cast<const uint16_t*>(p);
+        } else if constexpr (EL * sizeof(T) == 2) {
+            raw[i][0] = *reinterpret_cast<const uint16_t*>(p);
+        } else if constexpr (W == 1) {
+            raw[i][0] = *reinterpret_cast<const uint32_t*>(p);
         } else {
-            static_assert(W == 2, "8 bytes a row");
+            static_assert(W == 2, "up to 8 bytes a row");
             const uint2 v = *reinterpret_cast<const uint2*>(p);
             raw[i][0] = v.x;
             raw[i][1] = v.y;
         }
     }
     __device__ __forceinline__ void store_row(int i, T* p) const {
-        if constexpr (EL == 1) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = raw[i][0];
-            else *reinterpret_cast<uint16_t*>(p) = (uint16_t)raw[i][0];
-        } else {
-            *reinterpret_cast<uint2*>(p) = make_uint2(raw[i][0], raw[i][1]);
-        }
+        if constexpr (EL * sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)raw[i][0];
+        else if constexpr (W == 1) *reinterpret_cast<uint32_t*>(p) = raw[i][0];
+        else *reinterpret_cast<uint2*>(p) = make_uint2(raw[i][0], raw[i][1]);
     }
     __device__ __forceinline__ float get(int i, int j) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i][j]);
@@ -93,44 +126,83 @@ template <typename T, int EL> struct Tile {
             for (int w = 0; w < W; ++w) raw[i][w] = pack2(v[2 * w], v[2 * w + 1], T());
         }
     }
-    // feature j's byte and codes
-    __device__ __forceinline__ uint32_t quantize(int j, uint4* lo, uint4* hi) const {
-        uint32_t most = 0;
+    // the bits of feature j's largest magnitude, as fp32; word w's two features at once where types are 16 bits wide
+    __device__ __forceinline__ void largest(uint32_t* most) const {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < BLOCK; ++i) most = max(most, __float_as_uint(get(i, j)) & 0x7fffffffu);
-        const uint32_t byte = scale_byte(most);
-        const float inv = byte == 255 ? 0.f : __uint_as_float((254 - byte) << 23), magic = 12582912.f;
-        const float cap = byte == TOP<T> ? 63.f : 127.f;
+            for (int j = 0; j < EL; ++j) {
+                most[j] = 0;
+#pragma unroll
+                for (int i = 0; i < BLOCK; ++i) most[j] = max(most[j], raw[i][j] & 0x7fffffffu);
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                uint32_t m = 0;           // magnitudes of 16 bits are ordered as signed whole numbers
+#pragma unroll
+                for (int i = 0; i < BLOCK; i += 2)
+                    m = __vimax3_s16x2(m, raw[i][w] & 0x7fff7fffu, raw[i + 1][w] & 0x7fff7fffu);
+                const float2 f = unpack2(m, T());
+                most[2 * w] = __float_as_uint(f.x);
+                if (EL > 1) most[2 * w + 1] = __float_as_uint(f.y);
+            }
+        }
+    }
+    // feature j's codes
+    template <bool CAPPED> __device__ __forceinline__ void quantize(int j, uint32_t byte, uint4* lo, uint4* hi) const {
+        const float inv = __uint_as_float((254 - byte) << 23), magic = 12582912.f;
         uint32_t word[8];
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
             float f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float x = get(4 * w + i, j);
-                if (byte >= TOP<T>) x = byte == 255 ? 0.f : fminf(fmaxf(x * inv, -cap), cap) * scale_of(byte);
-                f[i] = fmaf(x, inv, magic);
+                const float x = get(4 * w + i, j);
+                f[i] = CAPPED ? fminf(fmaxf(x * inv, -63.f), 63.f) + magic : fmaf(x, inv, magic);
             }
             word[w] = pack_codes(f[0], f[1], f[2], f[3]);
         }
         *lo = make_uint4(word[0], word[1], word[2], word[3]);
         *hi = make_uint4(word[4], word[5], word[6], word[7]);
-        return byte;
     }
     // all features of token block tb, k the first of them
-    __device__ __forceinline__ void save(int8_t* codes, uint8_t* scales, int64_t tb, int64_t K, int k) const {
-        uint4* at = reinterpret_cast<uint4*>(codes) + 2 * tb * K + k;
-        uint32_t bytes = 0;
+    __device__ __forceinline__ void save(uint8_t* saved, int64_t tb, int64_t K, int k) const {
+        const Place at(tb >> 1, k, K);
+        const int block = (int)(tb & 1);
+        uint4* lo = reinterpret_cast<uint4*>(saved + at.codes(2 * block));
+        uint4* hi = reinterpret_cast<uint4*>(saved + at.codes(2 * block + 1));
+        uint32_t bytes = 0, most[EL > 1 ? EL : 2];
+        largest(most);
+        uint4 a[EL], b[EL];
 #pragma unroll
         for (int j = 0; j < EL; ++j) {
-            uint4 lo, hi;
-            const uint32_t b = quantize(j, &lo, &hi);
-            at[j] = lo;
-            at[K + j] = hi;
-            bytes |= b << (8 * j);
+            const uint32_t byte = scale_byte(most[j]);
+            if (byte < TOP<T>) quantize<false>(j, byte, &a[j], &b[j]);
+            else if (byte < 255) quantize<true>(j, byte, &a[j], &b[j]);
+            else a[j] = b[j] = make_uint4(0, 0, 0, 0);
+            bytes |= byte << (8 * j);
+            if constexpr (EL == 1) {
+                lo[0] = a[0];
+                hi[0] = b[0];
+            } else if (j % 2) {
+                store32(lo + j - 1, a[j - 1], a[j]);
+                store32(hi + j - 1, b[j - 1], b[j]);
+            }
         }
+        uint8_t* sc = saved + at.scale(block);
+        if constexpr (EL == 4) *reinterpret_cast<uint32_t*>(sc) = bytes;
+        else if constexpr (EL == 2) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)bytes;
+        else {
 #pragma unroll
-        for (int j = 0; j < EL; ++j) scales[tb * scale_row(K) + k + j] = (uint8_t)(bytes >> (8 * j));
+            for (int j = 0; j < EL; ++j) sc[j] = (uint8_t)(bytes >> (8 * j));
+        }
+        // the features that fill the row of tiles up
+        if (k + EL >= K) {
+            for (int j = 0; k + EL + j < padded(K); ++j) {
+                lo[EL + j] = hi[EL + j] = make_uint4(0, 0, 0, 0);
+                sc[EL + j] = 1;
+            }
+        }
     }
 };
 

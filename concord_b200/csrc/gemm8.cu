@@ -11,15 +11,18 @@
 // which holds a half of dy's tile a CTA as the B operand and is read once a
 // pair for it, is less busy than with two 16-bit operands.
 //
-// Warp roles: warp 0 loads (dy by TMA tiles, codes and scales by bulk copies),
+// Warp roles: warp 0 loads (dy by TMA tiles, a tile of codes and scales by one bulk copy),
 // warp 1 of the leader issues the products, warps 4-11 convert, alternate stages
 // of 64 tokens by the two groups of four, and afterwards store the
 // accumulator (256 columns; the other 256 hold 8 stages of A).
 //
-// Work is the line of all (output tile, stage) in order; pair p takes an equal
-// part of it.  Tiles cut by parts' ends leave fp32 pieces in the workspace, which a
-// second kernel adds in token order: the same bits on every run of one device.
-// Where the tiles themselves share out well, parts end at tiles' ends.
+// Whole tiles go round the pairs, which walk the tokens in step, so that a stage's
+// data come from memory once and are in the L2 for everybody else (parts of equal
+// length but different beginnings read 16384 x 2048 x 2048 from memory eight times:
+// 150 us for the loads alone).  The tiles that are left over when rounds no longer fill
+// are cut: each has a pair for its first tokens, as many as shared out evenly, and
+// the other pairs share the line of their ends.  Cut tiles leave fp32 pieces in
+// the workspace, which a second kernel adds in token order: the same bits on every run of one device.
 //
 // Every wait is bounded (tc.cuh): where one runs out, loads and products stop,
 // what is in flight lands (bounded again), the pair's remaining outputs become NaN and
@@ -45,9 +48,9 @@ constexpr int THREADS = 384;
 constexpr int FEATS = 128, OUTS = 128;            // of one CTA; a pair has twice both
 constexpr int TOKENS = 64;                        // a stage
 constexpr int STAGES = 8;
-constexpr int DY_BYTES = TOKENS * OUTS * 2, CODE_BYTES = TOKENS * FEATS, SCALE_BYTES = 2 * FEATS;
-constexpr int CODES = STAGES * DY_BYTES, SCALES = CODES + STAGES * CODE_BYTES;
-constexpr int BARS = SCALES + STAGES * SCALE_BYTES;
+constexpr int DY_BYTES = TOKENS * OUTS * 2, X_BYTES = eight::TILE_BYTES;
+static_assert(FEATS == eight::FEATS && TOKENS == eight::TOKENS, "a stage reads one tile of codes");
+constexpr int CODES = STAGES * DY_BYTES, BARS = CODES + STAGES * X_BYTES;
 constexpr int NBARS = 4 * STAGES + 3;
 static_assert(BARS % BARRIERS == 0 && NBARS * 8 + 4 <= (int)BARRIERS - 4, "barriers, the tensor memory's address, the word");
 constexpr size_t SMEM = BARS + BARRIERS + 1024;
@@ -57,41 +60,54 @@ constexpr int TILE = 256;
 struct Params {
     int64_t M;
     int N, K, tiles_n, stages;                    // stages of a tile
-    int64_t quanta;                               // the line, in units of `unit` stages
-    int unit;
-    const int8_t* codes;
-    const uint8_t* scales;
+    int full, rest, cut, helpers;                 // tiles of full rounds, the others, their first part's stages, pairs for the ends
+    const uint8_t* saved;
     __nv_bfloat16* dw;
-    float* part;                                  // [pairs][2][256 outputs][256 features]
+    float* part;                                  // pieces of the rest: [2 pairs][256 outputs][256 features]
     int* err;
 };
 
-// the first stage of pair p's part
-__host__ __device__ inline int64_t part_start(const Params& P, int64_t p, int64_t pairs) {
-    return p * P.quanta / pairs * P.unit;
+// The rest's ends, tile after tile, are one line of stages.  Where helper h of them begins:
+__device__ __forceinline__ int64_t end_start(const Params& P, int64_t h) {
+    return h * ((int64_t)P.rest * (P.stages - P.cut)) / P.helpers;
+}
+// and whose part stage t is in
+__device__ __forceinline__ int helper_of(const Params& P, int64_t t) {
+    return (int)(((t + 1) * P.helpers - 1) / ((int64_t)P.rest * (P.stages - P.cut)));
 }
 
-// one piece of a pair's part after another
+// one piece of a pair's work after another
 struct Pieces {
-    int64_t at, end;
-    int first;                                    // 1: the part's first piece
-    int tile, s0, s1;
-    __device__ __forceinline__ Pieces(const Params& P) {
-        const int64_t pairs = gridDim.x >> 1, p = blockIdx.x >> 1;
-        at = part_start(P, p, pairs);
-        end = part_start(P, p + 1, pairs);
-        first = 2;
+    int64_t at, end;                              // a helper's part of the line
+    int next_tile, pairs, pair;
+    int tile, s0, s1, slot;                       // slot: of the workspace; -1: a whole tile
+    __device__ __forceinline__ Pieces(const Params& P) : at(0), end(0) {
+        pairs = (int)(gridDim.x >> 1);
+        next_tile = pair = (int)(blockIdx.x >> 1);
+        const int h = pair - P.rest;
+        if (h >= 0 && h < P.helpers) {
+            at = end_start(P, h);
+            end = end_start(P, h + 1);
+        }
     }
     __device__ __forceinline__ bool next(const Params& P) {
+        if (next_tile < P.full + P.rest) {
+            tile = next_tile;
+            next_tile += pairs;
+            s0 = 0;
+            s1 = tile < P.full ? P.stages : P.cut;
+            slot = s1 == P.stages ? -1 : tile - P.full;
+            return true;
+        }
         if (at >= end) return false;
-        first = first == 2;
-        tile = (int)(at / P.stages);
-        s0 = (int)(at % P.stages);
+        const int len = P.stages - P.cut, j = (int)(at / len);
+        tile = P.full + j;
+        s0 = P.cut + (int)(at % len);
         s1 = (int)min((int64_t)P.stages, s0 + (end - at));
+        slot = P.rest + j + pair - P.rest;        // (j + helper grows from piece to piece along the line)
         at += s1 - s0;
         return true;
     }
-    __device__ __forceinline__ bool whole(const Params& P) const { return s0 == 0 && s1 == P.stages; }
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -108,21 +124,38 @@ __device__ __forceinline__ uint32_t leaders(uint32_t addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
+// What the arrival says is ordered is in tensor memory alone (tcgen05.wait::st or ::ld
+// and the fence before it), so it need not release memory to the cluster: that
+// takes 1400 cycles, which the stages' arrivals would wait for one after another.
 __device__ __forceinline__ void arrive_leader(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leaders(bar)) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leaders(bar)) : "memory");
 }
-// a tile {64 outputs, 64 tokens} of dy into this CTA, counted on the leader's barrier
-__device__ __forceinline__ void load_dy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int n, int t) {
+// By a converged warp, one elected lane: a tile {64 outputs, 64 tokens} of dy
+// into this CTA, counted on the leader's barrier
+__device__ __forceinline__ void load_dy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int n, int t, uint32_t one) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(n), "r"(t)
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(n), "r"(t), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+__device__ __forceinline__ void load_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %4, 0;\n\t"
+        "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(dst),
+        "l"(src), "r"(bytes), "r"(bar), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes), "r"(one)
+        : "memory");
 }
 // accumulator (both CTAs' tensor memory) = A (tensor memory) B (both CTAs' shared memory) [+ itself]
 __device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
@@ -146,6 +179,12 @@ __device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t one) {
 }
 // 256 features (A, tensor memory) x 256 outputs (B, rows are the reduction), bf16, fp32 accumulator
 constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+
+__device__ __forceinline__ uint32_t lds1(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
 
 // Two codes (the low bytes of both halves) as bf16.  128 + their low 7 bits is
 // 0x4300 | bits; what has to come off, 128 or (negative ones) 256, is 0x4300 |
@@ -198,40 +237,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t tm = *slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            Pieces pc(P);
-            int s = 0, sent = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            const int64_t blocks = eight::blocks(P.M);
-            while (ok && pc.next(P)) {
-                const int k0 = pc.tile / P.tiles_n * TILE + (int)rank * FEATS, n0 = pc.tile % P.tiles_n * TILE + (int)rank * OUTS;
-                const int feats = max(0, min(FEATS, P.K - k0)), padded = max(0, min(FEATS, (int)eight::scale_row(P.K) - k0));
-                for (int i = pc.s0; i < pc.s1; ++i) {
-                    if (!(ok = mbar_wait(empty(s), ph ^ 1, P.err, 1))) break;
-                    if (rank == 0) mbar_expect(bfull(s), 2 * DY_BYTES);
-                    const uint32_t lb = leaders(bfull(s)), dy = base + s * DY_BYTES;
-                    load_dy(dy, &map_dy, lb, n0, i * TOKENS);
-                    load_dy(dy + DY_BYTES / 2, &map_dy, lb, n0 + 64, i * TOKENS);
-                    const int64_t b0 = 2 * (int64_t)i;
-                    const int nb = b0 + 1 < blocks ? 2 : 1;          // blocks of 32 tokens that there are
-                    mbar_expect(cfull(s), nb * (2 * feats * 16 + padded));
-                    if (feats > 0) {
-                        const uint32_t c = base + CODES + s * CODE_BYTES, sc = base + SCALES + s * SCALE_BYTES;
-                        for (int j = 0; j < 2 * nb; ++j)
-                            load_bytes(c + j * FEATS * 16, P.codes + ((2 * b0 + j) * P.K + k0) * 16, feats * 16, cfull(s));
-                        for (int j = 0; j < nb; ++j)
-                            load_bytes(sc + j * FEATS, P.scales + (b0 + j) * eight::scale_row(P.K) + k0, padded, cfull(s));
-                    }
-                    ++sent;
-                    if (++s == STAGES) { s = 0; ph ^= 1; }
-                }
-            }
-            if (!ok) {
-                ring_landed(cfull(0), STAGES, sent, P.err);
-                if (rank == 0) ring_landed(bfull(0), STAGES, sent, P.err);
+        const uint32_t one = elect_one();
+        const int64_t row = eight::row_bytes(P.K);
+        Pieces pc(P);
+        int s = 0, sent = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        while (ok && pc.next(P)) {
+            const int k0 = pc.tile / P.tiles_n * TILE + (int)rank * FEATS, n0 = pc.tile % P.tiles_n * TILE + (int)rank * OUTS;
+            const uint32_t bytes = max(0, min(FEATS, (int)eight::padded(P.K) - k0)) * (TOKENS + 2);
+            const uint8_t* x = P.saved + pc.s0 * row + (int64_t)(k0 / FEATS) * X_BYTES;
+            for (int i = pc.s0; i < pc.s1; ++i, x += row) {
+                if (!(ok = warp_wait(empty(s), ph ^ 1, P.err, 1))) break;
+                const uint32_t dy = uniform(base + s * DY_BYTES), lb = uniform(leaders(bfull(s))), cb = uniform(cfull(s));
+                if (rank == 0) expect(uniform(bfull(s)), 2 * DY_BYTES, one);
+                expect(cb, bytes, one);
+                load_dy(dy, &map_dy, lb, n0, i * TOKENS, one);
+                load_dy(dy + DY_BYTES / 2, &map_dy, lb, n0 + 64, i * TOKENS, one);
+                if (bytes) load_bytes(uniform(base + CODES + s * X_BYTES), x, bytes, cb, one);
+                ++sent;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
             }
         }
+        if (!ok && lane == 0) {
+            ring_landed(cfull(0), STAGES, sent, P.err);
+            if (rank == 0) ring_landed(bfull(0), STAGES, sent, P.err);
+        }
+        __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t one = elect_one();
@@ -269,26 +301,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         int s = 0, parity = 0;
         uint32_t ph = 0, turn = 0;
         bool ok = true;
-        const int64_t blocks = eight::blocks(P.M);
         while (pc.next(P)) {
+            // (a lane beyond the tile's features converts what stands there: its row of A is no output)
+            const int width = max(16, min(FEATS, (int)eight::padded(P.K) - (pc.tile / P.tiles_n * TILE + (int)rank * FEATS)));
             for (int i = pc.s0; ok && i < pc.s1; ++i) {
                 if (parity == half) {
                     if (!(ok = warp_wait(cfull(s), ph, P.err, 5))) break;
                     fence_after();
-                    const uint32_t at = base + CODES + s * CODE_BYTES + (q * 32 + lane) * 16;
-                    const uint8_t* sc = smem + SCALES + s * SCALE_BYTES + q * 32 + lane;
-                    const bool both = 2 * (int64_t)i + 1 < blocks;
+                    const uint32_t at = base + CODES + s * X_BYTES + (q * 32 + lane) * 16;
+                    const uint32_t sc = base + CODES + s * X_BYTES + TOKENS * width + q * 32 + lane;
+                    uint4 c[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = lds16(at + j * width * 16);
+                    const uint32_t s0 = lds1(sc) * 0x00800080u, s1 = lds1(sc + width) * 0x00800080u;
                     uint32_t r[32];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 c = lds16(at + j * FEATS * 16);
-                        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-                        const uint32_t scale2 = sc[(j >> 1) * FEATS] * 0x00800080u;
+                        const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t x0 = two(w[k], 0x4140, scale2), x1 = two(w[k], 0x4342, scale2);
-                            r[j * 8 + 2 * k] = j < 2 || both ? x0 : 0u;
-                            r[j * 8 + 2 * k + 1] = j < 2 || both ? x1 : 0u;
+                            r[j * 8 + 2 * k] = two(w[k], 0x4140, j < 2 ? s0 : s1);
+                            r[j * 8 + 2 * k + 1] = two(w[k], 0x4342, j < 2 ? s0 : s1);
                         }
                     }
                     st32(tm + ACC + s * 32 + lanes, r);
@@ -306,8 +339,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             // 32 features x 128 outputs a warp, a feature a lane
             const int f0 = (int)rank * FEATS + q * 32 + lane, k = pc.tile / P.tiles_n * TILE + f0;
             const int n0 = pc.tile % P.tiles_n * TILE + half * 128;
-            float* part = P.part + ((int64_t)(blockIdx.x >> 1) * 2 + !pc.first) * (TILE * TILE) + half * 128 * TILE + f0;
-            const bool whole = pc.whole(P);
+            const bool whole = pc.slot < 0;
+            float* part = P.part + (int64_t)max(pc.slot, 0) * (TILE * TILE) + half * 128 * TILE + f0;
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
                 uint32_t r[32];
@@ -340,28 +373,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
 }
 
-// The pieces of every tile that was cut, in token order: a block a row of 256 features.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params P, int pairs) {
-    const int tile = blockIdx.x, row = blockIdx.y;
-    const int64_t t0 = (int64_t)tile * P.stages, t1 = t0 + P.stages;
-    // the pair whose part holds stage t0
-    int64_t lo = 0, hi = pairs - 1;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) / 2;
-        if (part_start(P, mid, pairs) <= t0) lo = mid;
-        else hi = mid - 1;
+// The pieces of every tile that was cut, in token order: a block four rows of 256
+// features, four features a thread.
+constexpr int JOIN_ROWS = 4;
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params P) {
+    const int j = blockIdx.x, tile = P.full + j, len = P.stages - P.cut;
+    const int first = helper_of(P, (int64_t)j * len), pieces = helper_of(P, (int64_t)(j + 1) * len - 1) - first + 1;
+    const int fk = (threadIdx.x & 63) * 4, k0 = tile / P.tiles_n * TILE + fk;
+    const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 6), n = tile % P.tiles_n * TILE + row;
+    if (n >= P.N || k0 >= P.K) return;
+    const float* at = P.part + (int64_t)row * TILE + fk;
+    float4 sum = *reinterpret_cast<const float4*>(at + (int64_t)j * (TILE * TILE));
+#pragma unroll 4
+    for (int p = 0; p < pieces; ++p) {
+        const float4 v = *reinterpret_cast<const float4*>(at + (int64_t)(P.rest + j + first + p) * (TILE * TILE));
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
     }
-    if (part_start(P, lo + 1, pairs) >= t1) return;              // whole
-    const int n = tile % P.tiles_n * TILE + row, k = tile / P.tiles_n * TILE + threadIdx.x;
-    if (n >= P.N || k >= P.K) return;
-    float sum = 0.f;
-    for (int64_t p = lo; p < pairs; ++p) {
-        const int64_t a = part_start(P, p, pairs), b = part_start(P, p + 1, pairs);
-        if (a >= t1) break;
-        if (a == b) continue;
-        sum += P.part[(p * 2 + (a < t0)) * (TILE * TILE) + row * TILE + threadIdx.x];
+    __nv_bfloat16* out = P.dw + (int64_t)n * P.K + k0;
+    if (P.K % 4 == 0) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack2(sum.x, sum.y, __nv_bfloat16()), pack2(sum.z, sum.w, __nv_bfloat16()));
+    } else {
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        for (int i = 0; i < 4; ++i)
+            if (k0 + i < P.K) out[i] = __float2bfloat16_rn(v[i]);
     }
-    P.dw[(int64_t)n * P.K + k] = __float2bfloat16_rn(sum);
 }
 
 // ---------------------------------------------------------------- host side
@@ -421,13 +459,17 @@ int resident_pairs() {
     return n;
 }
 
-// Tiles go whole to pairs where that costs at most a tenth more stages than equal parts do.
-void share_out(Params& P, int64_t tiles, int pairs, int* used) {
-    const int64_t total = tiles * P.stages, rounds = (tiles + pairs - 1) / pairs;
-    const bool whole = rounds * P.stages * pairs <= total + total / 10 + 8 * pairs;
-    P.unit = whole ? P.stages : 1;
-    P.quanta = whole ? tiles : total;
-    *used = (int)std::min<int64_t>(pairs, whole ? tiles : std::max<int64_t>(tiles, total / 4));
+// The pairs, and which tiles are cut: those beyond full rounds, unless cutting
+// saves no more than 16 stages, about what storing and adding the pieces takes.
+int share_out(Params& P, int64_t tiles, int resident) {
+    const int64_t total = tiles * P.stages;
+    const int pairs = (int)std::min<int64_t>(resident, std::max<int64_t>(tiles, total / 4));
+    P.rest = (int)(tiles % pairs);
+    P.full = (int)(tiles - P.rest);
+    P.cut = (int)(((int64_t)P.stages * P.rest + pairs - 1) / pairs);
+    if (P.stages - P.cut <= 16) P.cut = P.stages;
+    P.helpers = (int)std::min<int64_t>(pairs - P.rest, (int64_t)P.rest * (P.stages - P.cut));
+    return pairs;
 }
 
 }  // namespace g8
@@ -455,7 +497,7 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
         return check_launch(name);
     }
     if (!dy || !saved) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
-    if (!aligned(dy, 16) || !aligned(saved, 16)) return fail(CONCORD_EALIGN, std::string(name) + ": operands must be 16-byte aligned");
+    if (!aligned(dy, 16) || !aligned(saved, 32) || !aligned(dw, 8)) return fail(CONCORD_EALIGN, std::string(name) + ": dy must be 16-byte aligned, saved 32, dw 8");
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < concord_gemm_dw8_workspace_bytes(M, N, K))
         return fail(CONCORD_EWORKSPACE, std::string(name) + ": workspace too small, or not 16-byte aligned");
     if (int rc = bind_current_context(name)) return rc;
@@ -467,20 +509,19 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
     P.K = (int)K;
     P.tiles_n = (int)((N + TILE - 1) / TILE);
     P.stages = (int)((M + TOKENS - 1) / TOKENS);
-    P.codes = static_cast<const int8_t*>(saved);
-    P.scales = static_cast<const uint8_t*>(saved) + eight::code_bytes(M, K);
+    P.saved = static_cast<const uint8_t*>(saved);
     P.dw = reinterpret_cast<__nv_bfloat16*>(dw);
     P.part = static_cast<float*>(workspace);
     P.err = error_word();
     const int resident = resident_pairs();
     if (!P.err || resident <= 0) return fail(CONCORD_ELAUNCH, std::string(name) + ": no error word, or shared memory refused");
     const int64_t tiles = (int64_t)P.tiles_n * ((K + TILE - 1) / TILE);
-    int pairs = 1;
-    share_out(P, tiles, resident, &pairs);
+    if (tiles > INT32_MAX / 2) return fail(CONCORD_ETOOBIG, std::string(name) + ": too many tiles");
+    const int pairs = share_out(P, tiles, resident);
     dw8_kernel<<<2 * pairs, THREADS, SMEM, st>>>(map, P);
     if (int rc = check_launch(name)) return rc;
-    if (P.unit == 1) {
-        join_kernel<<<dim3((unsigned)tiles, TILE), 256, 0, st>>>(P, pairs);
+    if (P.helpers > 0) {
+        join_kernel<<<dim3((unsigned)P.rest, TILE / JOIN_ROWS), 256, 0, st>>>(P);
         return check_launch(name);
     }
     return CONCORD_OK;
