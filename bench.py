@@ -505,6 +505,27 @@ def bench_chardistill(args):
                     f"of {r['tokens_per_step']} rows a step"})
 
 
+def bench_packed_llama(args):
+    """The Llama-style decoder on packed documents, on one GPU: rows/s, activations in 8 bits and as they are."""
+    import workloads
+    res = {}
+    for save8 in (True, False):
+        r = workloads.train_packed_llama(steps=args.steps, warmup=args.warmup, n_layer=args.layers, save8=save8, graph=args.graph)
+        res[save8] = (statistics.mean(r["ms"]), r["peak_gb"], r)
+        torch.cuda.empty_cache()
+    ms, peak, r = res[True]
+    emit({"metric": "Llama-style decoder on packed documents, train tokens/s", "unit": "tokens/s", "n_gpus": 1,
+          "steps": args.steps, "warmup": args.warmup, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+          "dtype": "bf16 autocast; packed int32 words; activations in 8 bits for the backward",
+          "data": "synthetic: uniform random token ids, vocab 32000",
+          "config": {"workload": f"{args.layers}-layer d=2048 16/4-head SwiGLU-5504 decoder, 16384 tokens of documents of "
+                                 "1-2048 tokens", "seq_len": 2048, "global_batch": 16384},
+          "value": r["tokens_per_step"] / (ms * 1e-3), "ms_per_step": ms, "loss_first_last": [r["losses"][0], r["losses"][-1]],
+          "peak_mem_gb": peak, "without_8_bits": {"ms_per_step": res[False][0], "peak_mem_gb": res[False][1]},
+          "concord_params": r["concord_params"], "cuda_graph": args.graph,
+          "timing": "CUDA events around each training step, mean"})
+
+
 def bench_llama(args, rank, world, steps=None, warmup=None, ret=False):
     """Config 5: weak-scaling data-parallel training step (whole job tokens/s).
     With `ret` the line is returned (rank 0; None elsewhere) instead of printed."""
@@ -784,7 +805,7 @@ def main():
     ap.add_argument("--layers", type=int, default=24, help="llama: decoder layers")
     ap.add_argument("--nogate", action="store_true", help="sdxl: disable_cohpre on every layer")
     ap.add_argument("--ckpt", action="store_true", help="sdxl: activation checkpointing per block")
-    ap.add_argument("--workload", default="c2", choices=["c2", "chargpt", "chardistill", "llama", "sdxl", "conv", "gemm"],
+    ap.add_argument("--workload", default="c2", choices=["c2", "chargpt", "chardistill", "llama", "packedllama", "sdxl", "conv", "gemm"],
                     help="c2: the packed-step path on config 2's largest layer (default); "
                          "chargpt: config 3's char-level GPT trained end to end; "
                          "chardistill: the same architecture distilled on packed documents; "
@@ -840,6 +861,10 @@ def main():
     if args.workload == "chargpt":
         if rank == 0:
             bench_chargpt(args, cores)
+        return
+    if args.workload == "packedllama":
+        if rank == 0:
+            bench_packed_llama(args)
         return
     if args.workload == "chardistill":
         if rank == 0:

@@ -66,11 +66,10 @@ __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float 
     return __byte_perm(ab, cd, 0x5410);
 }
 // byte j of four codes with their signs flipped (x ^ 0x80808080), times scale: 2^23 + 128 + code is exact, and
-// so is what the fma leaves
-__device__ __forceinline__ float value(uint32_t flipped, int j, float scale, float off) {
-    return fmaf(__uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7650 + j)), scale, off);
+// both operations after it (one fma instead would take 2^23 times the largest scales, which is infinite)
+__device__ __forceinline__ float value(uint32_t flipped, int j, float scale) {
+    return (__uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7650 + j)) - 8388736.f) * scale;
 }
-__device__ __forceinline__ float value_off(float scale) { return -8388736.f * scale; }
 
 // 32 bytes at once
 __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {

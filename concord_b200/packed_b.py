@@ -1123,6 +1123,8 @@ class ConcordConv2dPackedB(ConcordLinearPackedB):
                          device=device, alpha=alpha, beta1=beta1, lr=lr)
 
     def forward(self, x):
+        if self.save8:
+            raise NotImplementedError("save8 is for linear layers: a convolution keeps its input as it is")
         in_dtype = x.dtype
         wbuf, rmbuf, cmbuf = self._ensure_buffers()
         y = FusedConcordConv2dPackedB.apply(

@@ -13,6 +13,8 @@ checkpoint is read.
   on this package's layer norm, packed attention and distillation loss.
 * Config 5, Llama-style decoder (24 layers, d=2048, 16 heads, SwiGLU 5504,
   vocab 32000, seq 2048) on uniform random token ids.
+* The decoder's shapes on packed documents, on this package's operators alone,
+  activations kept in 8 bits.
 """
 import math
 import os
@@ -525,6 +527,137 @@ def train_llama_dp(steps, warmup, batch_per_gpu=8, seq=2048, lr=5e-4, aux_lr=0.0
         st.close()
     return dict(ms=times, losses=losses, concord_params=params, world=world,
                 tokens_per_step=world * batch_per_gpu * seq)
+
+
+# ---------------------------------------------------------------- the decoder on packed documents
+class PackedLlamaBlock(nn.Module):
+    """LlamaBlock over documents packed one after the other, x [tokens, d], on
+    this package's operators: layer norms, heads normed and turned in one pass,
+    packed attention with `kv_heads` key heads, the gated unit.  With `save8`
+    what the backward needs of the block's activations, beside attention's, is
+    kept in 8 bits: one copy for the layers that read one input, and gate, up and
+    their unit's output as the unit leaves them."""
+
+    def __init__(self, d, h, kv_heads, ffn, positions, save8, device=None):
+        super().__init__()
+        from concord_b200 import LayerNorm, QKNormRope
+        hd = d // h
+        self.attn_norm, self.ffn_norm = (LayerNorm(d, bias=False, out_dtype=torch.bfloat16, device=device) for _ in range(2))
+        self.wq, self.wk, self.wv = (nn.Linear(d, n * hd, bias=False, device=device) for n in (h, kv_heads, kv_heads))
+        self.wo = nn.Linear(d, d, bias=False, device=device)
+        self.qk = QKNormRope(hd, positions, device=device)
+        self.w_gate, self.w_up = (nn.Linear(d, ffn, bias=False, device=device) for _ in range(2))
+        self.w_down = nn.Linear(ffn, d, bias=False, device=device)
+        self.hd, self.save8 = hd, save8
+
+    def read(self, x, *layers, saved=None):
+        """x through each of the layers, packed ones keeping it in 8 bits together."""
+        from concord_b200 import ConcordLinearPackedB, save8
+        packed = [self.save8 and isinstance(lin, ConcordLinearPackedB) for lin in layers]
+        if any(packed) and saved is None and torch.is_grad_enabled():
+            saved = save8(x)
+        return [lin(x, saved=saved) if p and saved is not None else lin(x) for lin, p in zip(layers, packed)]
+
+    def forward(self, x, pos, cu_seqlens):
+        from concord_b200 import gated_unit, packed_attention
+        T = x.shape[0]
+        q, k, v = (t.view(T, -1, self.hd) for t in self.read(self.attn_norm(x), self.wq, self.wk, self.wv))
+        q, k = self.qk(q, k, pos)
+        x = x + self.read(packed_attention(q, k, v, cu_seqlens).view(T, -1), self.wo)[0]
+        gate, up = self.read(self.ffn_norm(x), self.w_gate, self.w_up)
+        if self.save8 and torch.is_grad_enabled():
+            h, h8 = gated_unit(gate, up, save8=True, out8=True)
+            return x + self.read(h, self.w_down, saved=h8)[0]
+        return x + self.w_down(gated_unit(gate, up))
+
+
+class PackedLlama(nn.Module):
+    """The Llama-style decoder's shapes for packed documents: logits [tokens, vocab]."""
+
+    def __init__(self, vocab=32000, d=2048, n_layer=24, n_head=16, kv_heads=4, ffn=5504, positions=2048, save8=True,
+                 device=None):
+        super().__init__()
+        from concord_b200 import Embedding, LayerNorm
+        self.emb = Embedding(vocab, d, scale=math.sqrt(d), out_dtype=torch.float32, device=device)
+        self.blocks = nn.ModuleList([PackedLlamaBlock(d, n_head, kv_heads, ffn, positions, save8, device)
+                                     for _ in range(n_layer)])
+        self.norm = LayerNorm(d, bias=False, out_dtype=torch.bfloat16, device=device)
+        self.lm_head = nn.Linear(d, vocab, bias=False, device=device)
+        for m in self.modules():
+            if isinstance(m, nn.Linear):
+                nn.init.normal_(m.weight, 0.0, 0.02)
+        nn.init.normal_(self.emb.weight, 0.0, 1.0 / math.sqrt(d))
+
+    def forward(self, idx, pos, cu_seqlens):
+        x = self.emb(idx)
+        for b in self.blocks:
+            x = b(x, pos, cu_seqlens)
+        return self.lm_head(self.norm(x))
+
+
+def packed_tokens(tokens, longest, vocab, gen, device):
+    """A batch of `tokens` rows: documents of 1 to `longest` uniform random ids, one
+    after the other (the last is cut), their positions, and the next ids as labels
+    (-100 behind a document's last)."""
+    lens, left = [], tokens
+    while left:
+        n = min(left, int(torch.randint(1, longest + 1, (), generator=gen)))
+        lens.append(n)
+        left -= n
+    most = 2 * tokens // longest + 64                      # as many bounds for every batch: one captured graph serves all
+    cu = torch.tensor([0] + lens)[:most].cumsum(0)
+    cu = torch.cat([cu, cu[-1:].expand(most + 1 - len(cu))]) if len(cu) <= most else cu
+    ids = torch.randint(0, vocab, (tokens,), generator=gen)
+    row = torch.arange(tokens)
+    doc = torch.searchsorted(cu[1:].contiguous(), row, right=True).clamp_max(most - 1)
+    inside = row < cu[-1]
+    pos = torch.where(inside, row - cu[doc], 0)
+    labels = torch.cat([ids[1:], ids[:1]])
+    labels = torch.where(inside & (row + 1 < cu[doc + 1]), labels, -100)
+    return ids.to(device), pos.int().to(device), labels.to(device), cu.int().to(device)
+
+
+def train_packed_llama(steps, warmup, tokens=16384, longest=2048, lr=5e-4, aux_lr=0.01, seed=0, n_layer=24, d=2048,
+                       n_head=16, kv_heads=4, ffn=5504, vocab=32000, save8=True, graph=True):
+    """Training steps of the decoder on packed documents, one GPU: Concord on
+    every Linear of the blocks, this package's operators between them, SGD
+    (momentum 0.9) on embedding, norms and lm_head.  Lengths change from batch to
+    batch under one CUDA graph.  Returns per-step device times, losses, rows a
+    step and the peak of allocated memory."""
+    from concord_b200.checkpoint import set_step_salt
+    from concord_b200.convert import concordify
+    dev = torch.device("cuda", torch.cuda.current_device())
+    torch.manual_seed(seed)
+    set_step_salt(dev, seed)
+    torch.cuda.reset_peak_memory_stats()
+    model = PackedLlama(vocab, d, n_layer, n_head, kv_heads, ffn, longest, save8, device=dev)
+    layers = concordify(model, lr=lr, skip=lambda name, m: name == "lm_head")
+    aux = [p for p in model.parameters() if p.requires_grad]
+    opt = torch.optim.SGD(aux, lr=aux_lr, momentum=0.9)
+    gen = torch.Generator().manual_seed(seed)
+    static = list(packed_tokens(tokens, longest, vocab, gen, dev))
+    for p in aux:
+        p.grad = torch.zeros_like(p)
+
+    def refill(it):
+        for dst, src in zip(static, packed_tokens(tokens, longest, vocab, gen, dev)):
+            dst.copy_(src)
+
+    def step():
+        ids, pos, labels, cu = static
+        opt.zero_grad(set_to_none=False)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            logits = model(ids, pos, cu)
+        loss = F.cross_entropy(logits.float(), labels)
+        loss.backward()                       # Concord layers step inside the backward
+        opt.step()
+        for lay in layers:
+            lay.rebalance()
+        return loss
+
+    times, losses = run_steps(step, refill, steps, warmup, layers, lr, graph)
+    return dict(ms=times, losses=losses, tokens_per_step=tokens, peak_gb=torch.cuda.max_memory_allocated() / 1e9,
+                concord_params=sum(lay.packed_w.numel() for lay in layers))
 
 
 # ---------------------------------------------------------------- config 4: SDXL-architecture UNet
