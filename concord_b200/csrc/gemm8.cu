@@ -461,8 +461,13 @@ int resident_pairs() {
 
 // The pairs, and which tiles are cut: those beyond full rounds, unless cutting
 // saves no more than 16 stages, about what storing and adding the pieces takes.
-int share_out(Params& P, int64_t tiles, int resident) {
-    const int64_t total = tiles * P.stages;
+int share_out(Params& P, int64_t M, int64_t N, int64_t K, int resident) {
+    P.M = M;
+    P.N = (int)N;
+    P.K = (int)K;
+    P.tiles_n = (int)((N + TILE - 1) / TILE);
+    P.stages = (int)((M + TOKENS - 1) / TOKENS);
+    const int64_t tiles = (int64_t)P.tiles_n * ((K + TILE - 1) / TILE), total = tiles * P.stages;
     const int pairs = (int)std::min<int64_t>(resident, std::max<int64_t>(tiles, total / 4));
     P.rest = (int)(tiles % pairs);
     P.full = (int)(tiles - P.rest);
@@ -471,6 +476,10 @@ int share_out(Params& P, int64_t tiles, int resident) {
     P.helpers = (int)std::min<int64_t>(pairs - P.rest, (int64_t)P.rest * (P.stages - P.cut));
     return pairs;
 }
+// slots of the workspace: each cut tile's first piece, and the steps along the line of ends
+int64_t slots(const Params& P) { return P.helpers > 0 ? 2 * P.rest + P.helpers - 1 : 0; }
+
+bool fits(int64_t M, int64_t N, int64_t K) { return K <= (1 << 20) && N <= (1 << 20) && M <= INT32_MAX - TOKENS; }
 
 }  // namespace g8
 }  // namespace concord
@@ -478,8 +487,11 @@ int share_out(Params& P, int64_t tiles, int resident) {
 using namespace concord;
 
 extern "C" size_t concord_gemm_dw8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return (size_t)g8::MAX_PAIRS * 2 * g8::TILE * g8::TILE * sizeof(float);
+    if (M <= 0 || N <= 0 || K <= 0 || !g8::fits(M, N, K)) return 0;
+    const int resident = g8::resident_pairs();
+    g8::Params P{};
+    g8::share_out(P, M, N, K, resident > 0 ? resident : g8::MAX_PAIRS);
+    return (size_t)g8::slots(P) * g8::TILE * g8::TILE * sizeof(float);
 }
 
 extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* saved, uint16_t* dw, int64_t M, int64_t N,
@@ -488,7 +500,7 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
     const char* name = "concord_gemm_dw8";
     if (M < 0 || N <= 0 || K <= 0 || lddy < N || N % 8 || lddy % 8)
         return fail(CONCORD_ESHAPE, std::string(name) + ": N and dy's row stride must be multiples of 8, extents positive");
-    if (K > (1 << 20) || N > (1 << 20) || M > INT32_MAX - TOKENS || lddy > ((int64_t)1 << 38))
+    if (!fits(M, N, K) || lddy > ((int64_t)1 << 38))
         return fail(CONCORD_ETOOBIG, std::string(name) + ": more than 2^20 features or outputs, or 2^31 tokens");
     if (!dw) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
     cudaStream_t st = as_stream(stream);
@@ -498,26 +510,20 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
     }
     if (!dy || !saved) return fail(CONCORD_EINVAL, std::string(name) + ": null pointer");
     if (!aligned(dy, 16) || !aligned(saved, 32) || !aligned(dw, 8)) return fail(CONCORD_EALIGN, std::string(name) + ": dy must be 16-byte aligned, saved 32, dw 8");
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < concord_gemm_dw8_workspace_bytes(M, N, K))
+    const size_t need = concord_gemm_dw8_workspace_bytes(M, N, K);
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return fail(CONCORD_EWORKSPACE, std::string(name) + ": workspace too small, or not 16-byte aligned");
     if (int rc = bind_current_context(name)) return rc;
     CUtensorMap map;
     if (!make_map(&map, dy, M, N, lddy)) return fail(CONCORD_ELAUNCH, std::string(name) + ": TMA descriptor encoding failed");
     Params P{};
-    P.M = M;
-    P.N = (int)N;
-    P.K = (int)K;
-    P.tiles_n = (int)((N + TILE - 1) / TILE);
-    P.stages = (int)((M + TOKENS - 1) / TOKENS);
     P.saved = static_cast<const uint8_t*>(saved);
     P.dw = reinterpret_cast<__nv_bfloat16*>(dw);
     P.part = static_cast<float*>(workspace);
     P.err = error_word();
     const int resident = resident_pairs();
     if (!P.err || resident <= 0) return fail(CONCORD_ELAUNCH, std::string(name) + ": no error word, or shared memory refused");
-    const int64_t tiles = (int64_t)P.tiles_n * ((K + TILE - 1) / TILE);
-    if (tiles > INT32_MAX / 2) return fail(CONCORD_ETOOBIG, std::string(name) + ": too many tiles");
-    const int pairs = share_out(P, tiles, resident);
+    const int pairs = share_out(P, M, N, K, resident);
     dw8_kernel<<<2 * pairs, THREADS, SMEM, st>>>(map, P);
     if (int rc = check_launch(name)) return rc;
     if (P.helpers > 0) {

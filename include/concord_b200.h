@@ -724,7 +724,8 @@ int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t 
  * concord_gemm_dw8: dw [N, K] (bf16, contiguous) = dy^T x for dy [M, N] (bf16, row
  * stride lddy) and x in 8 bits: the values it keeps are exact in bf16, sums are fp32,
  * rounded once.  N and lddy multiples of 8, dy 16-byte aligned; any M and K.
- * Workspace: 16-byte aligned (sums of parts where outputs are few).  Its waits are bounded as
+ * Workspace: 16-byte aligned, sums of tiles that are cut (up to 37 MB; as many bytes
+ * as the current device asks for, 0 where no tile is cut).  Its waits are bounded as
  * concord_gemm2sm's are: concord_gemm_dw8_error reads and clears its error word.
  */
 size_t concord_saved8_bytes(int64_t M, int64_t K);

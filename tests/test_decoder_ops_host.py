@@ -87,9 +87,10 @@ def test_saved_entries_refuse(lib):
     assert save(M=-1) == -2 and save(K=2 ** 21, ld=2 ** 21) == -7 and save(out=ctypes.c_void_p(48)) == -3 and save(M=0) == 0
     assert lib.concord_dense8(None, ONE, 0, 8, 4, 8, None) == -1 and lib.concord_dense8(ONE, ONE, 0, 4, 4, 8, None) == -2
 
-    size = lib.concord_gemm_dw8_workspace_bytes(64, 64, 64)
+    size = lib.concord_gemm_dw8_workspace_bytes(4096, 64, 64)          # one tile, cut
+    assert size > 0 and lib.concord_gemm_dw8_workspace_bytes(64, 64, 64) == 0 and lib.concord_gemm_dw8_workspace_bytes(0, 8, 8) == 0
 
-    def dw(dy=ONE, ld=64, s=ONE, out=ONE, M=64, N=64, K=64, ws=ONE, nbytes=size):
+    def dw(dy=ONE, ld=64, s=ONE, out=ONE, M=4096, N=64, K=64, ws=ONE, nbytes=size):
         return lib.concord_gemm_dw8(dy, ld, s, out, M, N, K, ws, nbytes, None)
     assert dw(dy=None) == -1 and dw(s=None) == -1 and dw(out=None) == -1 and dw(N=60) == -2 and dw(ld=60) == -2 and dw(ld=68) == -2
     assert dw(M=-1) == -2 and dw(K=2 ** 21) == -7 and dw(M=2 ** 31) == -7 and dw(nbytes=size - 1) == -4 and dw(ws=None) == -4

@@ -534,8 +534,8 @@ class PackedLlamaBlock(nn.Module):
     """LlamaBlock over documents packed one after the other, x [tokens, d], on
     this package's operators: layer norms, heads normed and turned in one pass,
     packed attention with `kv_heads` key heads, the gated unit.  With `save8`
-    what the backward needs of the block's activations, beside attention's, is
-    kept in 8 bits: one copy for the layers that read one input, and gate, up and
+    what the backward needs of the block's activations, beside attention's
+    and the norms', is kept in 8 bits: one copy for the layers that read one input, and gate, up and
     their unit's output as the unit leaves them."""
 
     def __init__(self, d, h, kv_heads, ffn, positions, save8, device=None):
@@ -563,7 +563,7 @@ class PackedLlamaBlock(nn.Module):
         T = x.shape[0]
         q, k, v = (t.view(T, -1, self.hd) for t in self.read(self.attn_norm(x), self.wq, self.wk, self.wv))
         q, k = self.qk(q, k, pos)
-        x = x + self.read(packed_attention(q, k, v, cu_seqlens).view(T, -1), self.wo)[0]
+        x = x + self.wo(packed_attention(q, k, v, cu_seqlens).view(T, -1))       # (attention keeps its output anyway)
         gate, up = self.read(self.ffn_norm(x), self.w_gate, self.w_up)
         if self.save8 and torch.is_grad_enabled():
             h, h8 = gated_unit(gate, up, save8=True, out8=True)
@@ -634,13 +634,13 @@ def train_packed_llama(steps, warmup, tokens=16384, longest=2048, lr=5e-4, aux_l
     layers = concordify(model, lr=lr, skip=lambda name, m: name == "lm_head")
     aux = [p for p in model.parameters() if p.requires_grad]
     opt = torch.optim.SGD(aux, lr=aux_lr, momentum=0.9)
-    gen = torch.Generator().manual_seed(seed)
-    static = list(packed_tokens(tokens, longest, vocab, gen, dev))
+    batch = lambda it: packed_tokens(tokens, longest, vocab, torch.Generator().manual_seed(seed * 100003 + it), dev)  # noqa: E731
+    static = list(batch(0))
     for p in aux:
         p.grad = torch.zeros_like(p)
 
     def refill(it):
-        for dst, src in zip(static, packed_tokens(tokens, longest, vocab, gen, dev)):
+        for dst, src in zip(static, batch(it)):
             dst.copy_(src)
 
     def step():
