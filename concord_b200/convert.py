@@ -12,13 +12,15 @@ from .packed_b import ConcordConv2dPackedB, ConcordLinearPackedB
 
 
 @torch.no_grad()
-def concordify(model, lr, convs=False, finetune=False, skip=None, device=None):
+def concordify(model, lr, convs=False, finetune=False, skip=None, device=None, save8=False):
     """Replace every nn.Linear (and nn.Conv2d with groups == 1 when `convs`)
     in `model` by the packed layer, in place; returns the list of new layers.
 
     `finetune` loads with load_weights_finetune (pretrained weights at the
     steady state) instead of load_weights (the whole weight in the fast
-    accumulator, the from-scratch recipe).  `skip(name, module)` may return
+    accumulator, the from-scratch recipe).  `save8` makes the linear layers keep
+    their inputs in 8 bits for the backward (a copy each: where several layers
+    read one input, passing them one `save8(x)` is less).  `skip(name, module)` may return
     True to leave a module alone."""
     made = []
     for parent_name, parent in list(model.named_modules()):
@@ -30,6 +32,7 @@ def concordify(model, lr, convs=False, finetune=False, skip=None, device=None):
             if isinstance(child, nn.Linear):
                 new = ConcordLinearPackedB(child.in_features, child.out_features,
                                            bias=child.bias is not None, device=dev, lr=lr)
+                new.save8 = save8
                 W = child.weight.float()
             elif convs and isinstance(child, nn.Conv2d) and child.groups == 1 and \
                     child.dilation == (1, 1) and child.padding_mode == "zeros" and \

@@ -90,7 +90,10 @@ template <typename T, int N, Kind KIND> struct Raw {
     static constexpr int RUN = N * (int)sizeof(T), WORDS = VEC ? 2 * RUN / 4 : 2 * N;
     uint32_t v[WORDS];
     __device__ __forceinline__ void fetch(const Lane<N, KIND>& L, const T* row) {
-        if constexpr (VEC) {
+        if constexpr (KIND == PAIRED && RUN == 8) {           // both runs side by side
+            const uint4 u = *reinterpret_cast<const uint4*>(row + L.at[0]);
+            v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        } else if constexpr (VEC) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 if constexpr (RUN == 8) {
@@ -163,6 +166,10 @@ __device__ __forceinline__ void store_pairs(const Lane<N, KIND>& L, T* row, cons
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j) { r[j] = a[j]; r[N + j] = b[j]; }
+        }
+        if constexpr (KIND == PAIRED && N * sizeof(T) == 8) {
+            *reinterpret_cast<uint4*>(row + L.at[0]) = Pack16<T>::pack(r);
+            return;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {

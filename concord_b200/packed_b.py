@@ -981,7 +981,8 @@ class ConcordLinearPackedB(nn.Module):
         in_dtype = x.dtype
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
-        if saved is None and self.save8 and torch.is_grad_enabled():
+        if saved is None and self.save8 and torch.is_grad_enabled() and (
+                x.requires_grad or (self.bias is not None and self.bias.requires_grad)):
             saved = _saved8.save8(x.detach())
         wbuf, rmbuf, cmbuf = self._ensure_buffers()
         if self.fast_gain < 1.0:
