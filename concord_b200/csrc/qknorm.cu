@@ -373,8 +373,10 @@ __global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const
 }
 
 template <typename T, int N, int LANES, Kind KIND, bool NORM>
-__global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 3) bwd_kernel(const __grid_constant__ Params P) {
-    constexpr int DEPTH = 2;
+__global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(const __grid_constant__ Params P) {
+    // (16384 tokens, 2 x 16 heads of 128: neighbours' rows, one load each, 76 us with three rows ahead and 84 with
+    // one and more blocks, halves' rows 99 and 85)
+    constexpr int DEPTH = KIND == PAIRED ? 4 : 2;
     extern __shared__ float sums[];               // [row groups][D]
     const int which = blockIdx.x >= P.blocks0, block = blockIdx.x - (which ? P.blocks0 : 0);
     const Side& S = P.side[which];

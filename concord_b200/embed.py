@@ -21,9 +21,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     padding, is 0.  The result has `out_dtype` (default: weight's type).
 
     The gradient, of weight's type, is dense: each row the sum of its tokens'
-    upstream gradients times scale, in fp32, in token order for up to 64 tokens
-    and by pieces of 64 places of the sorted tokens beyond, rounded once: the
-    same bits on every run.  Ids outside the table and `padding_idx` (a row that is
+    upstream gradients times scale, in fp32, by pieces of up to 32 tokens in
+    order, rounded once: the same bits on every run.  Ids outside the table and `padding_idx` (a row that is
     looked up as any other) get none.  Differentiable once, backward only.
     """
     _ops.need_cuda(("ids", ids), ("weight", weight))

@@ -978,6 +978,8 @@ class ConcordLinearPackedB(nn.Module):
             _saved8._check_saved(saved)
             if saved.shape != x.shape:
                 raise ValueError(f"saved is of shape {tuple(saved.shape)}, x of {tuple(x.shape)}")
+            if saved.data.device != x.device:
+                raise RuntimeError(f"saved is on {saved.data.device}, x on {x.device}")
         in_dtype = x.dtype
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)

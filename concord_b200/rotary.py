@@ -45,40 +45,43 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
     gradients of the weights are fp32 sums in a fixed order: the same bits on
     every run.  Differentiable once, backward only, for q, k and the weights.
     """
-    named = (("q", q), ("k", k), ("cos", cos), ("sin", sin), ("positions", positions), ("q_weight", q_weight),
-             ("k_weight", k_weight))
-    _ops.need_cuda(*named)
+    _ops.need_cuda(("q", q), ("k", k), ("cos", cos), ("sin", sin), ("positions", positions), ("q_weight", q_weight),
+                   ("k_weight", k_weight))
     if q is None:
         raise TypeError("q must be a tensor, got None")
+    # (a token's step waits for these checks: each shape is asked for once)
+    dtype, shape = q.dtype, q.shape
     _ops.need_type("q", q, _ops.TYPES)
-    if q.dim() != 3 or q.shape[1] < 1 or not 1 <= q.shape[2] <= 256:
-        raise ValueError(f"q must be [T, H, D] with D up to 256, got shape {tuple(q.shape)}")
-    T, _, D = q.shape
+    if len(shape) != 3 or shape[1] < 1 or not 1 <= shape[2] <= 256:
+        raise ValueError(f"q must be [T, H, D] with D up to 256, got shape {tuple(shape)}")
+    T, _, D = shape
     if k is not None:
-        if k.dtype != q.dtype:
-            raise TypeError(f"k must have q's type {q.dtype}, got {k.dtype}")
-        if k.dim() != 3 or k.shape[0] != T or k.shape[1] < 1 or k.shape[2] != D:
-            raise ValueError(f"k must be [T, Hk, D] beside q {tuple(q.shape)}, got {tuple(k.shape)}")
+        if k.dtype != dtype:
+            raise TypeError(f"k must have q's type {dtype}, got {k.dtype}")
+        ks = k.shape
+        if len(ks) != 3 or ks[0] != T or ks[1] < 1 or ks[2] != D:
+            raise ValueError(f"k must be [T, Hk, D] beside q {tuple(shape)}, got {tuple(ks)}")
+    elif k_weight is not None:
+        raise ValueError("k_weight without k")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is None:
             continue
         if not norm:
             raise ValueError(f"{name} belongs to the norm: pass norm=True")
-        if name == "k_weight" and k is None:
-            raise ValueError("k_weight without k")
-        if tuple(w.shape) != (D,):
+        if w.shape != (D,):
             raise ValueError(f"{name} must have shape ({D},), got {tuple(w.shape)}")
         _ops.need_type(name, w, _ops.TYPES)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            _ops.need_type(name, t, _ops.TYPES)
-            if t.dim() != 2 or t.shape != cos.shape or t.shape[0] < 1 or not 1 <= t.shape[1] <= D // 2:
-                raise ValueError(f"cos and sin must be [P, R / 2] with R up to {D}, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+        _ops.need_type("cos", cos, _ops.TYPES)
+        _ops.need_type("sin", sin, _ops.TYPES)
+        cs = cos.shape
+        if len(cs) != 2 or sin.shape != cs or cs[0] < 1 or not 1 <= cs[1] <= D // 2:
+            raise ValueError(f"cos and sin must be [P, R / 2] with R up to {D}, got {tuple(cs)}, {tuple(sin.shape)}")
         if positions is not None:
             _ops.need_type("positions", positions, _INTS)
-            if tuple(positions.shape) != (T,):
+            if positions.shape != (T,):
                 raise ValueError(f"positions must have shape ({T},), got {tuple(positions.shape)}")
             positions = positions.contiguous()
         cos, sin = _floats(cos), _floats(sin)

@@ -224,6 +224,26 @@ def test_packed_layer_of_whole_numbers():
     assert torch.equal(eight.packed_w, plain.packed_w) and torch.equal(eight._bf16_weight_buf, plain._bf16_weight_buf)
 
 
+def test_packed_layer_with_gradient_noise():
+    """The noise's statistics come from the kept values: whole numbers, the same as without."""
+    from concord_b200 import packed_b
+    torch.manual_seed(9)
+    x, dy = (torch.randint(-n, n + 1, (200, k), device=DEV).bfloat16() for n, k in ((30, 256), (4, 128)))
+    packed_b.set_sigmag_noise(True)
+    try:
+        words = []
+        for eight in (False, True):
+            lay = _layer()
+            lay.save8 = eight
+            y = lay(x.clone().requires_grad_())
+            torch.manual_seed(10)
+            y.backward(dy)
+            words.append(lay.packed_w.clone())
+        assert torch.equal(words[0], words[1])
+    finally:
+        packed_b.set_sigmag_noise(False)
+
+
 def test_packed_layer_keeps_8_bits():
     """What a forward holds until its backward: the codes, not x."""
     from concord_b200 import save8
@@ -251,6 +271,10 @@ def test_packed_layer_bias_fp32_input_and_refusals():
     assert torch.equal(lay.bias.grad, torch.full_like(lay.bias.grad, 30)) and x.grad.shape == x.shape
     with pytest.raises(TypeError, match="saved must be a Saved8"):
         lay(x, saved=x)
+    other = save8(x.detach())
+    other.data = other.data.cpu()
+    with pytest.raises(RuntimeError, match="saved is on cpu"):
+        lay(x, saved=other)
     with pytest.raises(ValueError, match="saved is of shape"):
         lay(x, saved=save8(x[:3].detach()))
 
