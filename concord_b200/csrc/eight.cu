@@ -20,6 +20,8 @@ constexpr int THREADS = 128;
 // bytes want two features at least; the unit's forward holds two tiles and keeps more warps on
 // an SM with two features of 16 bits (16384 x 5504 bf16: 123 us, with four 152), the
 // others do better with four (save 17, with two the same; the unit's backward 121, with two 132).
+// (a row of the elementwise kernels by single elements: so many tokens a thread, to keep as much on its way)
+constexpr int TALL = 8;
 constexpr int SAVE_BYTES = 8, FWD_BYTES = 4, BWD_BYTES = 8;
 
 
@@ -68,6 +70,7 @@ __global__ void __launch_bounds__(THREADS)
         T* p = out + (t0 + i) * ldo + k;
         if constexpr (EL * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(v);
         else if constexpr (EL * sizeof(T) == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(v);
+        else if constexpr (EL * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(v);
         else p[0] = v[0];
     }
 }
@@ -262,51 +265,54 @@ int check_shape(const char* name, int32_t type, int64_t M, int64_t K, int64_t ld
         return fail(CONCORD_ETOOBIG, std::string(name) + ": more than 2^20 features or 2^31 tokens");
     return CONCORD_OK;
 }
-// rows of whole pieces of so many bytes
-bool rows_fit(const void* p, int64_t ld, int64_t K, int32_t type, int bytes) {
-    const int64_t el = bytes / (int64_t)esize(type);
-    return K % el == 0 && ld % el == 0 && aligned(p, bytes);
+// the widest piece of a row, in elements, up to `most` bytes, that the given rows are made of (K, their strides and
+// addresses in turn: `same` is all of these or-ed together)
+template <typename T> int piece(uint64_t same, int most) {
+    int el = most / (int)sizeof(T);
+    while (el > 1 && same % (el * sizeof(T))) el /= 2;
+    return el;
 }
+uint64_t bytes_of(const void* p, int64_t ld, int32_t type) { return reinterpret_cast<uintptr_t>(p) | (uint64_t)ld * esize(type); }
 
 template <typename T> int save(const void* x, int64_t ldx, int32_t type, uint8_t* saved, int64_t M, int64_t K, cudaStream_t st) {
-    constexpr int EL = SAVE_BYTES / sizeof(T);
-    const bool vec = rows_fit(x, ldx, K, type, SAVE_BYTES);
+    constexpr int MOST = SAVE_BYTES / sizeof(T);
+    const int el = piece<T>(bytes_of(x, ldx, type) | (uint64_t)K * sizeof(T), SAVE_BYTES);
     int threads, blocks_k;
-    across(K, vec ? EL : 1, &threads, &blocks_k);
-    auto k = vec ? save_kernel<T, EL> : save_kernel<T, 1>;
+    across(K, el, &threads, &blocks_k);
+    auto k = el == MOST ? save_kernel<T, MOST> : el == 2 ? save_kernel<T, 2> : save_kernel<T, 1>;
     k<<<dim3((unsigned)blocks(M), blocks_k), threads, 0, st>>>(static_cast<const T*>(x), ldx, saved, M, (int)K);
     return check_launch("concord_save8");
 }
 
 template <typename T> int dense(const uint8_t* saved, void* out, int64_t ldo, int32_t type, int64_t M, int64_t K, cudaStream_t st) {
-    constexpr int EL = SAVE_BYTES / sizeof(T);
-    const bool vec = rows_fit(out, ldo, K, type, SAVE_BYTES);
+    constexpr int MOST = SAVE_BYTES / sizeof(T);
+    const int el = piece<T>(bytes_of(out, ldo, type) | (uint64_t)K * sizeof(T), SAVE_BYTES);
     int threads, blocks_k;
-    across(K, vec ? EL : 1, &threads, &blocks_k);
-    auto k = vec ? dense_kernel<T, EL> : dense_kernel<T, 1>;
+    across(K, el, &threads, &blocks_k);
+    auto k = el == MOST ? dense_kernel<T, MOST> : el == 2 ? dense_kernel<T, 2> : dense_kernel<T, 1>;
     k<<<dim3((unsigned)(2 * blocks(M)), blocks_k), threads, 0, st>>>(saved, static_cast<T*>(out), ldo, M, (int)K);
     return check_launch("concord_dense8");
 }
 
 template <typename T, int ACT> int forward(const Unit& U, void* h, int32_t type, cudaStream_t st) {
     T* out = static_cast<T*>(h);
+    const uint64_t rows = bytes_of(U.gate, U.ldg, type) | bytes_of(U.up, U.ldu, type) | (uint64_t)U.K * sizeof(T);
     if (U.g8 || U.u8 || U.h8) {
-        constexpr int EL = FWD_BYTES / sizeof(T);
-        const bool vec = rows_fit(U.gate, U.ldg, U.K, type, FWD_BYTES) && rows_fit(U.up, U.ldu, U.K, type, FWD_BYTES) &&
-                         aligned(h, FWD_BYTES);
+        constexpr int MOST = FWD_BYTES / sizeof(T);
+        const int el = piece<T>(rows | reinterpret_cast<uintptr_t>(h), FWD_BYTES);
         int threads, blocks_k;
-        across(U.K, vec ? EL : 1, &threads, &blocks_k);
-        auto k = vec ? fwd8_kernel<T, EL, ACT> : fwd8_kernel<T, 1, ACT>;
+        across(U.K, el, &threads, &blocks_k);
+        auto k = el == MOST ? fwd8_kernel<T, MOST, ACT> : fwd8_kernel<T, 1, ACT>;
         k<<<dim3((unsigned)blocks(U.M), blocks_k), threads, 0, st>>>(U, out);
         return check_launch("concord_gated_fwd");
     }
-    const bool vec = U.K % 8 == 0 && rows_fit(U.gate, U.ldg, U.K, type, 16) && rows_fit(U.up, U.ldu, U.K, type, 16) && aligned(h, 16);
+    const bool vec = (rows | reinterpret_cast<uintptr_t>(h)) % 16 == 0 && U.K % 8 == 0;
     dim3 threads;
     int blocks_k;
     tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
-    const int64_t rows = (vec ? 2 : 1) * threads.y;
-    auto k = vec ? fwd_kernel<T, 8, 2, ACT> : fwd_kernel<T, 1, 1, ACT>;
-    k<<<dim3((unsigned)((U.M + rows - 1) / rows), blocks_k), threads, 0, st>>>(U, out);
+    const int64_t each = (vec ? 2 : TALL) * (int64_t)threads.y;
+    auto k = vec ? fwd_kernel<T, 8, 2, ACT> : fwd_kernel<T, 1, TALL, ACT>;
+    k<<<dim3((unsigned)((U.M + each - 1) / each), blocks_k), threads, 0, st>>>(U, out);
     return check_launch("concord_gated_fwd");
 }
 
@@ -315,24 +321,24 @@ int backward(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg
              cudaStream_t st) {
     const T* up = static_cast<const T*>(dh);
     T *og = static_cast<T*>(dg), *ou = static_cast<T*>(du);
+    uint64_t rows = bytes_of(dh, lddh, type) | bytes_of(dg, lddg, type) | bytes_of(du, lddu, type) | (uint64_t)U.K * sizeof(T);
     if (U.g8) {
-        constexpr int EL = BWD_BYTES / sizeof(T);
-        const bool vec = rows_fit(dh, lddh, U.K, type, BWD_BYTES) && rows_fit(dg, lddg, U.K, type, BWD_BYTES) &&
-                         rows_fit(du, lddu, U.K, type, BWD_BYTES);
+        constexpr int MOST = BWD_BYTES / sizeof(T);
+        const int el = piece<T>(rows, BWD_BYTES);
         int threads, blocks_k;
-        across(U.K, vec ? EL : 1, &threads, &blocks_k);
-        auto k = vec ? bwd8_kernel<T, EL, ACT> : bwd8_kernel<T, 1, ACT>;
+        across(U.K, el, &threads, &blocks_k);
+        auto k = el == MOST ? bwd8_kernel<T, MOST, ACT> : el == 2 ? bwd8_kernel<T, 2, ACT> : bwd8_kernel<T, 1, ACT>;
         k<<<dim3((unsigned)(2 * blocks(U.M)), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
         return check_launch("concord_gated_bwd");
     }
-    const bool vec = U.K % 8 == 0 && rows_fit(U.gate, U.ldg, U.K, type, 16) && rows_fit(U.up, U.ldu, U.K, type, 16) &&
-                     rows_fit(dh, lddh, U.K, type, 16) && rows_fit(dg, lddg, U.K, type, 16) && rows_fit(du, lddu, U.K, type, 16);
+    rows |= bytes_of(U.gate, U.ldg, type) | bytes_of(U.up, U.ldu, type);
+    const bool vec = rows % 16 == 0 && U.K % 8 == 0;
     dim3 threads;
     int blocks_k;
     tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
-    const int64_t rows = threads.y;
-    auto k = vec ? bwd_kernel<T, 8, 1, ACT> : bwd_kernel<T, 1, 1, ACT>;
-    k<<<dim3((unsigned)((U.M + rows - 1) / rows), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
+    const int64_t each = (vec ? 1 : TALL) * (int64_t)threads.y;
+    auto k = vec ? bwd_kernel<T, 8, 1, ACT> : bwd_kernel<T, 1, TALL, ACT>;
+    k<<<dim3((unsigned)((U.M + each - 1) / each), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
     return check_launch("concord_gated_bwd");
 }
 

@@ -28,14 +28,68 @@ constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32;
 constexpr int64_t SORT_CHUNK = 4096;       // tokens of a sorting block, and more where blocks would pass
 constexpr int64_t SORT_BLOCKS = 512;       // this number: each of them reads all blocks' counts
 
+// The columns that a thread holds: 8 neighbours (VEC), or 4 that are `step` apart,
+// for rows that do not start on 16 bytes (a column that is not there reads the last one).
+template <bool VEC> struct Cols {
+    static constexpr int N = VEC ? 8 : 4;
+    int at[VEC ? 1 : N];
+    int count;                            // that are there
+    __device__ __forceinline__ Cols(int block, int thread, int step, int D) {
+        if constexpr (VEC) {
+            at[0] = (block * step + thread) * 8;
+            count = at[0] < D ? 8 : 0;
+        } else {
+            const int first = block * step * N + thread;
+            count = 0;
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                at[c] = min(first + c * step, D - 1);
+                count += first + c * step < D;
+            }
+        }
+    }
+};
+// a row's columns as they come from memory
+template <typename T, bool VEC> struct Raw {
+    static constexpr int N = Cols<VEC>::N, W = VEC ? 8 * (int)sizeof(T) / 4 : N;
+    uint32_t v[W];
+    __device__ __forceinline__ void load(const T* row, const Cols<VEC>& C) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(row + C.at[0])[i];
+                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c) v[c] = __float_as_uint(to_f32(row[C.at[c]]));
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (!VEC || sizeof(T) == 4) return __uint_as_float(v[i]);
+        else {
+            const float2 f = unpack2(v[i / 2], T());
+            return i & 1 ? f.y : f.x;
+        }
+    }
+};
+template <typename T, bool VEC> __device__ __forceinline__ void store_cols(T* row, const Cols<VEC>& C, const float* v) {
+    if constexpr (VEC) store_vec<8>(row + C.at[0], v);
+    else {
+#pragma unroll
+        for (int c = 0; c < Cols<VEC>::N; ++c)
+            if (c < C.count) row[C.at[c]] = from_f32<T>(v[c]);
+    }
+}
+
 // ---------------------------------------------------------------- forward
-// A thread holds VEC columns of ROWS rows.
-template <typename TW, typename TY, int VEC, int ROWS>
+// A thread holds its columns of ROWS rows.
+template <typename TW, typename TY, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256)
     fwd_kernel(const void* ids, int ids64, const TW* w, int64_t ldw, TY* y, int64_t T, int64_t V, int D, float scale) {
-    const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    const Cols<VEC> C(blockIdx.y, threadIdx.x, blockDim.x, D);
     const int64_t t0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
-    if (col >= D || t0 >= T) return;
+    if (C.count == 0 || t0 >= T) return;
     int64_t id[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -43,21 +97,18 @@ __global__ void __launch_bounds__(256)
         if (t0 + r < T)
             id[r] = ids64 ? static_cast<const int64_t*>(ids)[t0 + r] : (int64_t)static_cast<const int32_t*>(ids)[t0 + r];
     }
-    float v[ROWS][VEC];
+    Raw<TW, VEC> raw[ROWS];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        if (id[r] >= 0 && id[r] < V) load_vec<VEC>(w + id[r] * ldw + col, v[r]);
-        else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[r][j] = 0.f;
-        }
-    }
+    for (int r = 0; r < ROWS; ++r)
+        if (id[r] >= 0 && id[r] < V) raw[r].load(w + id[r] * ldw, C);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         if (t0 + r >= T) continue;
+        const bool there = id[r] >= 0 && id[r] < V;
+        float v[Cols<VEC>::N];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[r][j] *= scale;
-        store_vec<VEC>(y + (t0 + r) * D + col, v[r]);
+        for (int j = 0; j < Cols<VEC>::N; ++j) v[j] = there ? raw[r].get(j) * scale : 0.f;
+        store_cols<TY, VEC>(y + (t0 + r) * D, C, v);
     }
 }
 
@@ -291,45 +342,17 @@ struct Sums {
     float scale;
 };
 
-// VEC columns of a row as they come from memory
-template <typename T, int VEC> struct RawVec {
-    static constexpr int W = VEC * (int)sizeof(T) / 4 > 0 ? VEC * (int)sizeof(T) / 4 : 1;
-    uint32_t v[W];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (VEC == 1) v[0] = __float_as_uint(to_f32(*p));
-        else {
-#pragma unroll
-            for (int i = 0; i < W / 4; ++i) {
-                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
-            }
-        }
-    }
-    __device__ __forceinline__ void add_to(float* acc) const {
-        if constexpr (VEC == 1) acc[0] += __uint_as_float(v[0]);
-        else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if constexpr (sizeof(T) == 4) acc[i] += __uint_as_float(v[i]);
-                else {
-                    const float2 f = unpack2(v[i / 2], T());
-                    acc[i] += i & 1 ? f.y : f.x;
-                }
-            }
-        }
-    }
-};
-
 // Blocks of two kinds, spread evenly: chunks, one a row of threads (their
 // loads run AHEAD tokens before their sums), and rows of no token to clear.
 constexpr int CLEAR = 64;             // rows of the table that a clearing block looks at
-template <typename TY, typename TW, int VEC>
+template <typename TY, typename TW, bool VEC>
 __global__ void __launch_bounds__(256, 3)
     sum_kernel(const TY* dy, TW* dw, const __grid_constant__ Sums P, int chunk_blocks, int clear_blocks) {
-    const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    float acc[VEC];
+    constexpr int N = Cols<VEC>::N;
+    const Cols<VEC> C(blockIdx.y, threadIdx.x, blockDim.x, P.D);
+    float acc[N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
     const int64_t both = chunk_blocks + clear_blocks;
     const int64_t nth = blockIdx.x * (int64_t)chunk_blocks / both;
     if (nth == (blockIdx.x + 1) * (int64_t)chunk_blocks / both) {          // the (blockIdx.x - nth)-th to clear
@@ -346,26 +369,25 @@ __global__ void __launch_bounds__(256, 3)
             }
         }
         __syncthreads();
-        if (col >= P.D) return;
+        if (C.count == 0) return;
         for (int r = threadIdx.y; r < CLEAR && v0 + r < P.V; r += blockDim.y)
-            if (!(some[r / 32] >> (r % 32) & 1)) store_vec<VEC>(dw + (v0 + r) * P.D + col, acc);
+            if (!(some[r / 32] >> (r % 32) & 1)) store_cols<TW, VEC>(dw + (v0 + r) * P.D, C, acc);
         return;
     }
-    if (col >= P.D) return;
-    constexpr int AHEAD = VEC == 1 || sizeof(TY) == 2 ? 8 : 4;
+    if (C.count == 0) return;
+    constexpr int AHEAD = !VEC || sizeof(TY) == 2 ? 8 : 4;
     const int64_t i = nth * blockDim.y + threadIdx.y;
     const uint32_t end = *P.end;
     if (i >= P.chunks || (uint32_t)i * SEG >= end) return;
     const uint32_t p0 = (uint32_t)i * SEG, p1 = min(p0 + SEG, end);
     const uint2* at = P.sorted;
-    const TY* src = dy + col;
-    RawVec<TY, VEC> ring[AHEAD];
+    Raw<TY, VEC> ring[AHEAD];
     uint32_t key[AHEAD];                                  // their rows
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
         const uint2 it = at[min(p0 + k, p1 - 1)];
         key[k] = it.x;
-        ring[k].load(src + it.y * P.lddy);
+        ring[k].load(dy + it.y * P.lddy, C);
     }
     bool before = p0 > 0 && at[p0 - 1].x == key[0];       // the row goes on from the chunk before
     const uint32_t after = p1 < end ? at[p1].x : (uint32_t)P.V;
@@ -373,23 +395,24 @@ __global__ void __launch_bounds__(256, 3)
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             if (p + k >= p1) break;
-            ring[k].add_to(acc);
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] += ring[k].get(j);
             const uint32_t v = key[k];
             const uint2 it = at[min(p + k + AHEAD, p1 - 1)];      // (the last one again where there are no more)
             key[k] = it.x;
-            ring[k].load(src + it.y * P.lddy);
+            ring[k].load(dy + it.y * P.lddy, C);
             const bool last = p + k + 1 == p1;
             const uint32_t next = last ? after : key[(k + 1) % AHEAD];
             if (next == v && !last) continue;
             if (!before && next != v) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] *= P.scale;
-                store_vec<VEC>(dw + (int64_t)v * P.D + col, acc);
+                for (int j = 0; j < N; ++j) acc[j] *= P.scale;
+                store_cols<TW, VEC>(dw + (int64_t)v * P.D, C, acc);
             } else {
-                store_vec<VEC>(P.part + (2 * i + !before) * P.D + col, acc);
+                store_cols<float, VEC>(P.part + (2 * i + !before) * P.D, C, acc);
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+            for (int j = 0; j < N; ++j) acc[j] = 0.f;
             before = false;
         }
     }
@@ -398,9 +421,10 @@ __global__ void __launch_bounds__(256, 3)
 // One row at most begins in a chunk and goes on: its pieces in order, eight runs of
 // them side by side, the runs' sums in order again.
 constexpr int JOIN = 8;
-template <typename TW, int VEC>
+template <typename TW, bool VEC>
 __global__ void __launch_bounds__(256) join_kernel(TW* dw, const __grid_constant__ Sums P) {
-    __shared__ float runs[JOIN][32][VEC];
+    constexpr int N = Cols<VEC>::N;
+    __shared__ float runs[JOIN][32][N];
     const int64_t i = blockIdx.x;
     const uint32_t end = *P.end, p0 = (uint32_t)i * SEG, p1 = p0 + SEG;
     if (p1 >= end) return;                                // (the last chunk: nothing goes on)
@@ -409,38 +433,43 @@ __global__ void __launch_bounds__(256) join_kernel(TW* dw, const __grid_constant
     if (p0 > 0 && P.sorted[p0 - 1].x == v) return;        // it began before
     const uint32_t b = p1 + lower_bound(P.sorted + p1, end - p1, (int64_t)v + 1);
     const int64_t pieces = (b - 1) / SEG - i;             // besides the first
-    const int col = (blockIdx.y * 32 + threadIdx.x) * VEC;
-    float acc[VEC];
+    const Cols<VEC> C(blockIdx.y, threadIdx.x, 32, P.D);
+    float acc[N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    if (col < P.D) {
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    if (C.count > 0) {
         const int64_t c0 = i + 1 + pieces * threadIdx.y / JOIN, c1 = i + 1 + pieces * (threadIdx.y + 1) / JOIN;
-        if (threadIdx.y == 0) load_vec<VEC>(P.part + (2 * i + 1) * P.D + col, acc);
+        if (threadIdx.y == 0) {
+            Raw<float, VEC> x;
+            x.load(P.part + (2 * i + 1) * P.D, C);
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] = x.get(j);
+        }
 #pragma unroll 4
         for (int64_t c = c0; c < c1; ++c) {
-            float x[VEC];
-            load_vec<VEC>(P.part + 2 * c * P.D + col, x);
+            Raw<float, VEC> x;
+            x.load(P.part + 2 * c * P.D, C);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+            for (int j = 0; j < N; ++j) acc[j] += x.get(j);
         }
     }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) runs[threadIdx.y][threadIdx.x][j] = acc[j];
+    for (int j = 0; j < N; ++j) runs[threadIdx.y][threadIdx.x][j] = acc[j];
     __syncthreads();
-    if (threadIdx.y == 0 && col < P.D) {
+    if (threadIdx.y == 0 && C.count > 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
+        for (int j = 0; j < N; ++j) {
             for (int k = 1; k < JOIN; ++k) acc[j] += runs[k][threadIdx.x][j];
             acc[j] *= P.scale;
         }
-        store_vec<VEC>(dw + (int64_t)v * P.D + col, acc);
+        store_cols<TW, VEC>(dw + (int64_t)v * P.D, C, acc);
     }
 }
 
 // ---------------------------------------------------------------- host side
-// threads of a block along the columns (any number: no kernel here shares within a warp), and blocks along them
-void shape(int64_t D, int vec, dim3* threads, int* across) {
-    const int64_t pieces = (D + vec - 1) / vec, x = pieces < 256 ? pieces : 256;
+// threads of a block along the columns (any number: only whole warps of the clearing blocks share), and blocks along them
+void shape(int64_t D, int each, dim3* threads, int* across) {
+    const int64_t pieces = (D + each - 1) / each, x = pieces < 256 ? pieces : 256;
     *threads = dim3((unsigned)x, (unsigned)(256 / x), 1);
     *across = (int)((pieces + x - 1) / x);
 }
@@ -450,12 +479,13 @@ int forward(const void* ids, int ids64, const void* w, int64_t ldw, void* y, int
             float scale, bool vec, cudaStream_t st) {
     dim3 threads;
     int across;
-    shape(D, vec ? 8 : 1, &threads, &across);
+    shape(D, vec ? 8 : 4, &threads, &across);
     // four rows a thread once that still fills the GPU twice over
-    const bool many = vec && T * D / 8 / 4 >= 2 * 148 * 2048;
+    const bool many = T * D / (vec ? 8 : 4) / 4 >= 2 * 148 * 2048;
     const int64_t rows = (many ? 4 : 1) * (int64_t)threads.y, blocks = (T + rows - 1) / rows;
     const dim3 grid((unsigned)blocks, across, 1);
-    auto k = !vec ? fwd_kernel<TW, TY, 1, 1> : many ? fwd_kernel<TW, TY, 8, 4> : fwd_kernel<TW, TY, 8, 1>;
+    auto k = vec ? (many ? fwd_kernel<TW, TY, true, 4> : fwd_kernel<TW, TY, true, 1>)
+                 : (many ? fwd_kernel<TW, TY, false, 4> : fwd_kernel<TW, TY, false, 1>);
     k<<<grid, threads, 0, st>>>(ids, ids64, static_cast<const TW*>(w), ldw, static_cast<TY*>(y), T, V, (int)D, scale);
     return check_launch("concord_embedding_fwd");
 }
@@ -517,15 +547,15 @@ int backward(const void* ids, int ids64, const void* dy, int64_t lddy, void* dw,
     const Sums S{sorted, end, reinterpret_cast<float*>(ws + L.part), T, V, lddy, L.chunks, (int)D, scale};
     dim3 threads;
     int across;
-    shape(D, vec ? 8 : 1, &threads, &across);
+    shape(D, vec ? 8 : 4, &threads, &across);
     const int chunk_blocks = (int)((L.chunks + threads.y - 1) / threads.y);
     const int clear_blocks = (int)((V + CLEAR - 1) / CLEAR);
-    auto k = vec ? sum_kernel<TY, TW, 8> : sum_kernel<TY, TW, 1>;
+    auto k = vec ? sum_kernel<TY, TW, true> : sum_kernel<TY, TW, false>;
     k<<<dim3((unsigned)(chunk_blocks + clear_blocks), across, 1), threads, 0, st>>>(
         static_cast<const TY*>(dy), static_cast<TW*>(dw), S, chunk_blocks, clear_blocks);
     if (L.chunks > 1) {
-        auto j = vec ? join_kernel<TW, 8> : join_kernel<TW, 1>;
-        const int wide = 32 * (vec ? 8 : 1);
+        auto j = vec ? join_kernel<TW, true> : join_kernel<TW, false>;
+        const int wide = 32 * (vec ? 8 : 4);
         j<<<dim3((unsigned)(L.chunks - 1), (unsigned)((D + wide - 1) / wide), 1), dim3(32, JOIN, 1), 0, st>>>(
             static_cast<TW*>(dw), S);
     }

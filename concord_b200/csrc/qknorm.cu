@@ -54,32 +54,34 @@ struct Params {
 enum Kind { ANY, HALVES, PAIRED };
 template <int N, Kind KIND> struct Lane {
     static constexpr bool VEC = KIND != ANY;
-    int at[VEC ? 2 : 1];          // VEC: the runs' first columns; else the first pair
+    // VEC: the runs' first columns; else the first pair, and the columns of all (not there: column 0, as loads
+    // need no condition, and `have` without their bits)
+    int at[VEC ? 2 : 1 + 2 * N];
+    uint32_t have;
     bool live, turns;             // VEC: any columns, rotated ones
-    int D, rot, interleaved;
-    __device__ __forceinline__ Lane(const Params& P, int lane) : D(P.D), rot(P.rot), interleaved(P.interleaved) {
+    int rot;
+    __device__ __forceinline__ Lane(const Params& P, int lane) : have(0), rot(P.rot) {
         if constexpr (VEC) {
-            live = lane * 2 * N < D;
+            live = lane * 2 * N < P.D;
             turns = lane * 2 * N < rot;
             at[0] = !live ? 0 : turns && KIND == HALVES ? lane * N : lane * 2 * N;
             at[1] = !live ? N : turns && KIND == HALVES ? rot / 2 + lane * N : lane * 2 * N + N;    // (not live: loads need no condition)
         } else {
             live = turns = true;
             at[0] = lane;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int p = lane + 32 * j, half = rot / 2;
+                int a = rot + 2 * (p - half), b = a + 1;
+                if (p < half) {
+                    a = P.interleaved ? 2 * p : p;
+                    b = P.interleaved ? 2 * p + 1 : half + p;
+                }
+                have |= (a < P.D ? 1u : 0u) << (2 * j) | (b < P.D ? 2u : 0u) << (2 * j);
+                at[1 + 2 * j] = a < P.D ? a : 0;
+                at[2 + 2 * j] = b < P.D ? b : 0;
+            }
         }
-    }
-    // pair j's columns (not VEC); -1: none
-    __device__ __forceinline__ void columns(int j, int* a, int* b) const {
-        const int p = at[0] + 32 * j, half = rot / 2;
-        if (p < half) {
-            *a = interleaved ? 2 * p : p;
-            *b = interleaved ? 2 * p + 1 : half + p;
-        } else {
-            *a = rot + 2 * (p - half);
-            *b = *a + 1;
-        }
-        if (*a >= D) *a = -1;
-        if (*b >= D) *b = -1;
     }
     __device__ __forceinline__ bool rotated(int j) const { return VEC ? turns : at[0] + 32 * j < rot / 2; }
 };
@@ -113,17 +115,11 @@ template <typename T, int N, Kind KIND> struct Raw {
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                int ca, cb;
-                L.columns(j, &ca, &cb);
-                v[2 * j] = ca >= 0 ? __float_as_uint(to_f32(row[ca])) : 0u;
-                v[2 * j + 1] = cb >= 0 ? __float_as_uint(to_f32(row[cb])) : 0u;
-            }
-        }
-    }
-    __device__ __forceinline__ void clear() {
+            for (int j = 0; j < 2 * N; ++j) v[j] = __float_as_uint(to_f32(row[L.at[1 + j]]));
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) v[i] = 0;
+            for (int j = 0; j < 2 * N; ++j)
+                if (!(L.have >> j & 1)) v[j] = 0;
+        }
     }
     __device__ __forceinline__ float element(int i) const {       // VEC: the i-th of both runs
         if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
@@ -185,10 +181,8 @@ __device__ __forceinline__ void store_pairs(const Lane<N, KIND>& L, T* row, cons
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            int ca, cb;
-            L.columns(j, &ca, &cb);
-            if (ca >= 0) row[ca] = from_f32<T>(a[j]);
-            if (cb >= 0) row[cb] = from_f32<T>(b[j]);
+            if (L.have >> (2 * j) & 1) row[L.at[1 + 2 * j]] = from_f32<T>(a[j]);
+            if (L.have >> (2 * j + 1) & 1) row[L.at[2 + 2 * j]] = from_f32<T>(b[j]);
         }
     }
 }
