@@ -20,8 +20,9 @@ constexpr int THREADS = 128;
 // bytes want two features at least; the unit's forward holds two tiles and keeps more warps on
 // an SM with two features of 16 bits (16384 x 5504 bf16: 123 us, with four 152), the
 // others do better with four (save 17, with two the same; the unit's backward 121, with two 132).
-// (a row of the elementwise kernels by single elements: so many tokens a thread, to keep as much on its way)
-constexpr int TALL = 8;
+// (a row of the elementwise kernels by single elements: so many tokens a thread,
+// to keep enough on its way; 16384 x 5503 bf16: 200 and 247 us, with one 322 and 374)
+constexpr int TALL = 4;
 constexpr int SAVE_BYTES = 8, FWD_BYTES = 4, BWD_BYTES = 8;
 
 
