@@ -568,7 +568,7 @@ def bench_sdxl(args, rank, world, steps=None, warmup=None, ret=False):
     warmup = args.warmup if warmup is None else warmup
     batch = args.batch if args.batch != 8 else 4
     r = workloads.train_sdxl_dp(steps=steps, warmup=warmup, batch_per_gpu=batch, gate=not args.nogate,
-                                ckpt=args.ckpt, graph=args.graph, channels_last=not args.nchw)
+                                ckpt=args.ckpt, graph=args.graph, channels_last=not args.nchw, save8=args.save8)
     ms = statistics.mean(r["ms"])
     mem = torch.tensor([r["peak_gb"], r["state_gb"]], device="cuda")
     if world > 1:
@@ -583,7 +583,8 @@ def bench_sdxl(args, rank, world, steps=None, warmup=None, ret=False):
                                  f"latents [{batch},4,128,128] per GPU, Concord on all {r['n_layers']} Linear and conv "
                                  f"layers ({r['concord_params'] / 1e9:.3f} B params), coh_pre gate "
                                  f"{'off' if args.nogate else 'on'}, activation checkpointing "
-                                 f"{'on' if args.ckpt else 'off'}, lr 5e-5, "
+                                 f"{'on' if args.ckpt else 'off'}, "
+                                 f"{'layer inputs kept in 8 bits, ' if args.save8 else ''}lr 5e-5, "
                                  f"{'NCHW' if args.nchw else 'channels-last'} activations, conv backend "
                                  f"{__import__('concord_b200').get_conv_backend()}",
                      "global_batch": batch * world, "parallelism": f"dp{world}"},
@@ -805,6 +806,7 @@ def main():
     ap.add_argument("--layers", type=int, default=24, help="llama: decoder layers")
     ap.add_argument("--nogate", action="store_true", help="sdxl: disable_cohpre on every layer")
     ap.add_argument("--ckpt", action="store_true", help="sdxl: activation checkpointing per block")
+    ap.add_argument("--save8", action="store_true", help="sdxl: the packed layers keep their inputs in 8 bits")
     ap.add_argument("--workload", default="c2", choices=["c2", "chargpt", "chardistill", "llama", "packedllama", "sdxl", "conv", "gemm"],
                     help="c2: the packed-step path on config 2's largest layer (default); "
                          "chargpt: config 3's char-level GPT trained end to end; "

@@ -18,9 +18,9 @@ def concordify(model, lr, convs=False, finetune=False, skip=None, device=None, s
 
     `finetune` loads with load_weights_finetune (pretrained weights at the
     steady state) instead of load_weights (the whole weight in the fast
-    accumulator, the from-scratch recipe).  `save8` makes the linear layers keep
-    their inputs in 8 bits for the backward (a copy each: where several layers
-    read one input, passing them one `save8(x)` is less).  `skip(name, module)` may return
+    accumulator, the from-scratch recipe).  `save8` makes the layers keep
+    their inputs in 8 bits for the backward (a copy each: where several linear
+    layers read one input, passing them one `save8(x)` is less).  `skip(name, module)` may return
     True to leave a module alone."""
     made = []
     for parent_name, parent in list(model.named_modules()):
@@ -32,7 +32,6 @@ def concordify(model, lr, convs=False, finetune=False, skip=None, device=None, s
             if isinstance(child, nn.Linear):
                 new = ConcordLinearPackedB(child.in_features, child.out_features,
                                            bias=child.bias is not None, device=dev, lr=lr)
-                new.save8 = save8
                 W = child.weight.float()
             elif convs and isinstance(child, nn.Conv2d) and child.groups == 1 and \
                     child.dilation == (1, 1) and child.padding_mode == "zeros" and \
@@ -44,6 +43,7 @@ def concordify(model, lr, convs=False, finetune=False, skip=None, device=None, s
                 W = child.weight.float().reshape(child.out_channels, -1)
             else:
                 continue
+            new.save8 = save8
             (new.load_weights_finetune if finetune else new.load_weights)(W)
             if child.bias is not None:
                 new.bias.copy_(child.bias.float())

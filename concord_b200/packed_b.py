@@ -1043,7 +1043,7 @@ class FusedConcordConv2dPackedB(torch.autograd.Function):
                 eps, step_cap, v_scale, precond_p, gf_consol, drift_cancel_C, alpha_v_fast, wd_sv,
                 wd_sf, mass_preserve, apply_chase, track_rebalance, weight_buf, row_max_buf,
                 col_max_buf, v_row, v_col, sum_v_inv, adafactor_beta2, track_adafactor_v,
-                gf_trust_delta_sq, coh_pre, coh_stats=None):
+                gf_trust_delta_sq, coh_pre, coh_stats=None, save8=False):
         weight_4d = weight_buf.view(out_channels, in_channels, kh, kw)
         x_bf16 = x.to(torch.bfloat16) if x.dtype != torch.bfloat16 else x
         bias_bf16 = (bias.to(torch.bfloat16)
@@ -1056,7 +1056,8 @@ class FusedConcordConv2dPackedB(torch.autograd.Function):
             w_krsc = _gemm.filter_krsc(weight_buf, in_channels, kh, kw)
             ctx.gemm = False
             y = _gemm.conv2d_forward_nhwc(x_bf16, w_krsc, bias_bf16, kh, kw, stride, padding)
-            ctx.save_for_backward(x_bf16, w_krsc)
+            ctx.saved8 = x_bf16.permute(0, 2, 3, 1).shape if save8 else None
+            ctx.save_for_backward(_saved8.save8(x_bf16.permute(0, 2, 3, 1)).data if save8 else x_bf16, w_krsc)
         else:
             # a channels-last input on the implicit backend whose convolution the
             # implicit GEMM does not run (odd channel counts, strides) goes to cuDNN
@@ -1091,6 +1092,8 @@ class FusedConcordConv2dPackedB(torch.autograd.Function):
         if grad_y.dtype != torch.bfloat16:
             grad_y = grad_y.to(torch.bfloat16)
         if ctx.implicit:                 # weight_4d holds the [O, kh, kw, C] filter here
+            if ctx.saved8 is not None:   # and x_bf16 the input in 8 bits, pixels as tokens
+                x_bf16 = _saved8.Saved8(x_bf16, ctx.saved8, torch.bfloat16).dense().permute(0, 3, 1, 2)
             grad_x, grad_W = _gemm.conv2d_backward_nhwc(x_bf16, weight_4d, grad_y, kh, kw, stride, padding)
         elif ctx.gemm:
             grad_y = grad_y.contiguous()
@@ -1105,7 +1108,7 @@ class FusedConcordConv2dPackedB(torch.autograd.Function):
             grad_W = grad_W.reshape(out_c, -1).to(torch.bfloat16).contiguous()
         _optimizer_half(ctx, grad_W)
         grad_bias = grad_y.sum(dim=(0, 2, 3)) if ctx.has_bias else None
-        return (grad_x, None, None, None, grad_bias) + (None,) * 35
+        return (grad_x, None, None, None, grad_bias) + (None,) * 36
 
 
 class ConcordConv2dPackedB(ConcordLinearPackedB):
@@ -1126,14 +1129,17 @@ class ConcordConv2dPackedB(ConcordLinearPackedB):
                          device=device, alpha=alpha, beta1=beta1, lr=lr)
 
     def forward(self, x):
-        if self.save8:
-            raise NotImplementedError("save8 is for linear layers: a convolution keeps its input as it is")
+        """conv2d(x, W) + bias.  With the attribute `save8` set, a convolution that runs as an implicit GEMM
+        (channels-last input, see set_conv_backend) keeps its input in 8 bits for the
+        backward, pixels as tokens; others keep it as it is."""
         in_dtype = x.dtype
         wbuf, rmbuf, cmbuf = self._ensure_buffers()
+        save8 = self.save8 and torch.is_grad_enabled() and (
+            x.requires_grad or (self.bias is not None and self.bias.requires_grad))
         y = FusedConcordConv2dPackedB.apply(
             x, self.packed_w, self.row_exp, self.col_exp, self.bias, self.in_channels,
             self.out_channels, self.kh, self.kw, self.stride, self.padding,
-            *self._apply_args(wbuf, rmbuf, cmbuf))
+            *self._apply_args(wbuf, rmbuf, cmbuf), save8)
         return y.to(in_dtype)
 
 

@@ -295,12 +295,72 @@ def test_refusals():
             call()
 
 
-def test_convolutions_refuse_the_switch():
+def _conv(C=16, O=24, k=3, stride=1):
     from concord_b200 import ConcordConv2dPackedB
-    conv = ConcordConv2dPackedB(8, 8, 3, padding=1, device=DEV)
-    conv.load_weights(torch.randn(8, 72, device=DEV) * 0.1)
-    x = torch.randn(1, 8, 8, 8, device=DEV).bfloat16()
-    conv(x)
-    conv.save8 = True
-    with pytest.raises(NotImplementedError, match="linear layers"):
-        conv(x)
+    from concord_b200.checkpoint import set_step_salt
+    torch.manual_seed(0)
+    set_step_salt(torch.device(DEV, torch.cuda.current_device()), 0)
+    lay = ConcordConv2dPackedB(C, O, k, stride=stride, padding=k // 2, bias=False, device=DEV, lr=1e-2)
+    lay.load_weights(torch.randn(O, C * k * k, device=DEV) * 0.1)
+    return lay
+
+
+@pytest.mark.parametrize("k", [1, 3])
+def test_convolution(k):
+    """Channels-last inputs in 8 bits, pixels as tokens: forward and the input's gradient as without; the step is the one
+    of the kept values' dW, and that of x itself where x is kept exactly."""
+    from concord_b200 import gemm, save8
+    torch.manual_seed(3)
+    for whole in (False, True):
+        x = torch.randint(-30, 31, (2, 16, 9, 7), device=DEV) if whole else torch.randn(2, 16, 9, 7, device=DEV)
+        x = x.bfloat16().contiguous(memory_format=torch.channels_last)
+        dy = torch.randint(-4, 5, (2, 24, 9, 7), device=DEV).bfloat16().contiguous(memory_format=torch.channels_last)
+        plain, eight = _conv(k=k), _conv(k=k)
+        _conv(k=k)                                           # (the salt at its start)
+        a = x.clone(memory_format=torch.preserve_format).requires_grad_()
+        ya = plain(a)
+        ya.backward(dy)
+        eight.save8 = True
+        _conv(k=k)
+        b = x.clone(memory_format=torch.preserve_format).requires_grad_()
+        yb = eight(b)
+        yb.backward(dy)
+        assert torch.equal(ya, yb) and torch.equal(a.grad, b.grad)
+        if whole:
+            assert torch.equal(plain.packed_w, eight.packed_w)
+            continue
+        given = _conv(k=k)
+        given(x)
+        kept = save8(x.permute(0, 2, 3, 1)).dense().permute(0, 3, 1, 2)
+        w = gemm.filter_krsc(given._bf16_weight_buf, 16, k, k)
+        given.optimizer_step(gemm.conv2d_backward_nhwc(kept, w, dy, k, k, 1, k // 2)[1])
+        assert torch.equal(eight.packed_w, given.packed_w) and not torch.equal(eight.packed_w, plain.packed_w)
+
+
+def test_other_convolutions_keep_their_input():
+    """A stride that the implicit kernels do not run: the switch changes nothing."""
+    x = torch.randn(2, 16, 8, 8, device=DEV).bfloat16().contiguous(memory_format=torch.channels_last)
+    words = []
+    for eight in (False, True):
+        lay = _conv(stride=2)
+        lay.save8 = eight
+        y = lay(x.clone(memory_format=torch.preserve_format).requires_grad_())
+        y.backward(torch.ones_like(y))
+        words.append(lay.packed_w.clone())
+    assert torch.equal(words[0], words[1])
+
+
+def test_a_whole_model_of_layers():
+    """concordify(save8=True): linear layers and convolutions; the ordinary ones beside them train as ever."""
+    from concord_b200.convert import concordify
+    torch.manual_seed(4)
+    m = torch.nn.Sequential(torch.nn.Conv2d(8, 16, 3, padding=1), torch.nn.SiLU(), torch.nn.Flatten(), torch.nn.Linear(16 * 36, 40),
+                            torch.nn.LayerNorm(40), torch.nn.Linear(40, 8)).to(DEV)
+    layers = concordify(m, lr=1e-3, convs=True, save8=True)
+    assert len(layers) == 3 and all(lay.save8 for lay in layers)
+    x = torch.randn(5, 8, 6, 6, device=DEV).contiguous(memory_format=torch.channels_last).requires_grad_()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = m(x)
+    before = [lay.packed_w.clone() for lay in layers]
+    out.float().square().sum().backward()
+    assert all(not torch.equal(a, lay.packed_w) for a, lay in zip(before, layers)) and bool(x.grad.isfinite().all())

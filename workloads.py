@@ -821,7 +821,7 @@ def sdxl_batch(B, gen, device, res=128):
 
 
 def train_sdxl_dp(steps, warmup, batch_per_gpu=4, res=128, lr=5e-5, aux_lr=1e-4, seed=0, group=None,
-                  gate=True, ckpt=False, graph=True, channels_last=True):
+                  gate=True, ckpt=False, graph=True, channels_last=True, save8=False):
     """Config 4: epsilon-prediction MSE fine-tune steps of the SDXL-architecture
     UNet (~2.6 B parameters, random init), bf16 autocast, Concord on every
     Linear and every convolution (3x3 ones as their reshaped [O, I*9] weight),
@@ -830,7 +830,8 @@ def train_sdxl_dp(steps, warmup, batch_per_gpu=4, res=128, lr=5e-5, aux_lr=1e-4,
     loss.backward()) and the other parameters' gradients are all-reduced.
     Weak scaling: `batch_per_gpu` samples per GPU.  lr 5e-5 is the
     reference's SDXL setting (notebook/src/sdxl_train.py:154); `ckpt` recomputes
-    every block in the backward (activation checkpointing).  `channels_last`
+    every block in the backward (activation checkpointing); `save8` keeps the
+    packed layers' inputs in 8 bits for it.  `channels_last`
     keeps the activations NHWC end to end (the latents and every conv output),
     the layout the implicit-GEMM convolutions read and write without copies."""
     import torch.distributed as dist
@@ -844,7 +845,7 @@ def train_sdxl_dp(steps, warmup, batch_per_gpu=4, res=128, lr=5e-5, aux_lr=1e-4,
         model = model.to(memory_format=torch.channels_last)
     model.ckpt = ckpt
     n_total = sum(p.numel() for p in model.parameters())
-    layers = concordify(model, lr=lr, convs=True)
+    layers = concordify(model, lr=lr, convs=True, save8=save8)
     if not gate:
         for l in layers:
             l.disable_cohpre()
