@@ -1,5 +1,6 @@
 """What the training operators (layer norm, packed attention, distillation
-loss) share: checks of arguments, and the extension that runs them."""
+loss, embedding, head norm and rotation, gated unit, activations in 8 bits)
+share: checks of arguments, and the extension that runs them."""
 import importlib.machinery
 import importlib.util
 import os

@@ -104,7 +104,7 @@ struct Pieces {
         tile = P.full + j;
         s0 = P.cut + (int)(at % len);
         s1 = (int)min((int64_t)P.stages, s0 + (end - at));
-        slot = P.rest + j + pair - P.rest;        // (j + helper grows from piece to piece along the line)
+        slot = pair + j;                          // (grows from piece to piece along the line)
         at += s1 - s0;
         return true;
     }

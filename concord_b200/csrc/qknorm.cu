@@ -92,13 +92,14 @@ template <typename T, int N, Kind KIND> struct Raw {
     static constexpr int RUN = N * (int)sizeof(T), WORDS = VEC ? 2 * RUN / 4 : 2 * N;
     uint32_t v[WORDS];
     __device__ __forceinline__ void fetch(const Lane<N, KIND>& L, const T* row) {
-        if constexpr (KIND == PAIRED && RUN == 8) {           // both runs side by side
+        if constexpr (KIND == PAIRED && N == 4 && RUN == 8) {           // both runs side by side
             const uint4 u = *reinterpret_cast<const uint4*>(row + L.at[0]);
             v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
         } else if constexpr (VEC) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if constexpr (RUN == 8) {
+                if constexpr (RUN == 4) v[r] = *reinterpret_cast<const uint32_t*>(row + L.at[r]);
+                else if constexpr (RUN == 8) {
                     const uint2 u = *reinterpret_cast<const uint2*>(row + L.at[r]);
                     v[2 * r] = u.x;
                     v[2 * r + 1] = u.y;
@@ -163,14 +164,16 @@ __device__ __forceinline__ void store_pairs(const Lane<N, KIND>& L, T* row, cons
 #pragma unroll
             for (int j = 0; j < N; ++j) { r[j] = a[j]; r[N + j] = b[j]; }
         }
-        if constexpr (KIND == PAIRED && N * sizeof(T) == 8) {
+        if constexpr (KIND == PAIRED && N == 4 && sizeof(T) == 2) {
             *reinterpret_cast<uint4*>(row + L.at[0]) = Pack16<T>::pack(r);
             return;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             T* p = row + L.at[k];
-            if constexpr (N * sizeof(T) == 8)
+            if constexpr (N * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = pack2(r[k * N], r[k * N + 1], T());
+            else if constexpr (N == 2) *reinterpret_cast<float2*>(p) = make_float2(r[k * N], r[k * N + 1]);
+            else if constexpr (N * sizeof(T) == 8)
                 *reinterpret_cast<uint2*>(p) = make_uint2(pack2(r[k * N], r[k * N + 1], T()), pack2(r[k * N + 2], r[k * N + 3], T()));
             else {
                 uint4* q = reinterpret_cast<uint4*>(p);
@@ -199,8 +202,12 @@ __device__ __forceinline__ void angles(const Params& P, const Lane<N, KIND>& L, 
     if constexpr (KIND != ANY) {
         if (L.live && L.turns && there) {
             const int64_t at = row + (KIND == PAIRED ? L.at[0] / 2 : L.at[0]);
+            if constexpr (N == 2) {
+                const float2 u = *reinterpret_cast<const float2*>(P.cos + at), v = *reinterpret_cast<const float2*>(P.sin + at);
+                c[0] = u.x; c[1] = u.y; s[0] = v.x; s[1] = v.y;
+            }
 #pragma unroll
-            for (int j = 0; j < N; j += 4) {
+            for (int j = 0; j + 4 <= N; j += 4) {
                 const float4 u = *reinterpret_cast<const float4*>(P.cos + at + j), v = *reinterpret_cast<const float4*>(P.sin + at + j);
                 c[j] = u.x; c[j + 1] = u.y; c[j + 2] = u.z; c[j + 3] = u.w;
                 s[j] = v.x; s[j + 1] = v.y; s[j + 2] = v.z; s[j + 3] = v.w;
@@ -499,17 +506,18 @@ int share_of(int64_t T, int heads, int groups) {
     return share;
 }
 
-// whether rows are whole runs of 4 columns that loads of 16 bits' worth of them may take (8 pairs a lane
-// instead, for sizes of 16 columns, measured 60 us beside 56 and 124 beside 122, 16384 x 32 heads of 128)
-bool rows_fit(const Params& P, int32_t type, bool bwd) {
-    const int per = type == CONCORD_F32 ? 4 : 8;
-    bool ok = P.D % 8 == 0 && P.rot % 8 == 0 && aligned(P.cos, 16) && aligned(P.sin, 16);
+// whether rows can be read in runs of n columns: sizes of whole pairs of runs, addresses and strides of whole
+// accesses (8 pairs a lane, of 16 columns, measured 60 us beside 56 and 124 beside 122, 16384 x 32 heads of 128)
+bool rows_fit(const Params& P, int32_t type, bool bwd, int n) {
+    const uintptr_t size = type == CONCORD_F32 ? 4 : 2, access = n * size * (n == 4 && P.interleaved && size == 2 ? 2 : 1);
+    uintptr_t all = 0;
     for (const Side& S : P.side) {
         if (S.heads == 0) continue;
-        ok = ok && aligned(S.x, 16) && S.ts % per == 0 && S.hs % per == 0 && aligned(S.out, 16) && aligned(S.w, 16);
-        if (bwd) ok = ok && aligned(S.dy, 16) && S.dts % per == 0 && S.dhs % per == 0;
+        all |= reinterpret_cast<uintptr_t>(S.x) | (uintptr_t)S.ts * size | (uintptr_t)S.hs * size | reinterpret_cast<uintptr_t>(S.out);
+        if (bwd) all |= reinterpret_cast<uintptr_t>(S.dy) | (uintptr_t)S.dts * size | (uintptr_t)S.dhs * size;
+        if (!aligned(S.w, 4 * n)) return false;
     }
-    return ok;
+    return P.D % (2 * n) == 0 && P.rot % (2 * n) == 0 && all % access == 0 && aligned(P.cos, 4 * n) && aligned(P.sin, 4 * n);
 }
 
 template <typename K> int resident_blocks(K k, size_t smem) {
@@ -559,25 +567,29 @@ template <typename T, int N, int LANES, Kind KIND, bool NORM> int launch(Params 
     return CONCORD_OK;
 }
 
-template <typename T, bool NORM> int run(const Params& P, bool vec, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
-    // (a lane 8 columns; rows of up to 32 columns leave half of the 8 lanes idle)
-#define QK_LAUNCH(LANES)                                                                                \
-    return P.interleaved ? launch<T, 4, LANES, PAIRED, NORM>(P, bwd, dqw, dkw, st)                     \
-                         : launch<T, 4, LANES, HALVES, NORM>(P, bwd, dqw, dkw, st)
-    if (vec && P.D <= 64) QK_LAUNCH(8);
-    if (vec && P.D <= 128) QK_LAUNCH(16);
-    if (vec) QK_LAUNCH(32);
+template <typename T, bool NORM> int run(const Params& P, int32_t type, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
+#define QK_LAUNCH(N, LANES)                                                                         \
+    return P.interleaved ? launch<T, N, LANES, PAIRED, NORM>(P, bwd, dqw, dkw, st)                 \
+                         : launch<T, N, LANES, HALVES, NORM>(P, bwd, dqw, dkw, st)
+    if (rows_fit(P, type, bwd, 4)) {              // a lane 8 columns (rows of up to 32 leave half of 8 lanes idle)
+        if (P.D <= 64) QK_LAUNCH(4, 8);
+        if (P.D <= 128) QK_LAUNCH(4, 16);
+        QK_LAUNCH(4, 32);
+    }
+    if (P.D <= 128 && rows_fit(P, type, bwd, 2)) {        // a lane 4 (heads of 72, 36 of them turned: 68 and 117 us, by
+        if (P.D <= 64) QK_LAUNCH(2, 16);                  // single columns 138 and 199, 16384 x 32 heads)
+        QK_LAUNCH(2, 32);
+    }
     return P.D <= 128 ? launch<T, 2, 32, ANY, NORM>(P, bwd, dqw, dkw, st) : launch<T, 4, 32, ANY, NORM>(P, bwd, dqw, dkw, st);
+#undef QK_LAUNCH
 }
 
 int dispatch(const Params& P, const concord_qk_params* p, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
-    const bool vec = rows_fit(P, p->type, bwd);
-    if (p->type == CONCORD_F32)
-        return p->norm ? run<float, true>(P, vec, bwd, dqw, dkw, st) : run<float, false>(P, vec, bwd, dqw, dkw, st);
-    if (p->type == CONCORD_BF16)
-        return p->norm ? run<__nv_bfloat16, true>(P, vec, bwd, dqw, dkw, st)
-                       : run<__nv_bfloat16, false>(P, vec, bwd, dqw, dkw, st);
-    return p->norm ? run<__half, true>(P, vec, bwd, dqw, dkw, st) : run<__half, false>(P, vec, bwd, dqw, dkw, st);
+    const int32_t t = p->type;
+    if (t == CONCORD_F32) return p->norm ? run<float, true>(P, t, bwd, dqw, dkw, st) : run<float, false>(P, t, bwd, dqw, dkw, st);
+    if (t == CONCORD_BF16)
+        return p->norm ? run<__nv_bfloat16, true>(P, t, bwd, dqw, dkw, st) : run<__nv_bfloat16, false>(P, t, bwd, dqw, dkw, st);
+    return p->norm ? run<__half, true>(P, t, bwd, dqw, dkw, st) : run<__half, false>(P, t, bwd, dqw, dkw, st);
 }
 
 int check_params(const char* name, const concord_qk_params* p) {

@@ -90,7 +90,8 @@ def _check(args, inter, norm, eps=1e-6):
 
 SHAPES = [(1, 1, 1, 128, 128), (5, 16, 4, 128, 128), (37, 6, 6, 64, 64), (130, 20, 5, 80, 40), (33, 10, 2, 72, 72),
           (64, 3, 1, 96, 96), (19, 4, 4, 256, 256), (1000, 8, 2, 32, 16), (7, 5, 5, 8, 8), (21, 2, 2, 72, 36),
-          (11, 3, 3, 10, 4), (9, 2, 1, 255, 254), (400, 12, 12, 64, 0), (3, 7, 7, 1, 0), (20, 32, 8, 128, 64)]
+          (11, 3, 3, 10, 4), (9, 2, 1, 255, 254), (400, 12, 12, 64, 0), (3, 7, 7, 1, 0), (20, 32, 8, 128, 64), (40, 6, 3, 36, 36),
+          (90, 4, 2, 60, 12), (33, 8, 4, 124, 124), (17, 3, 1, 132, 68), (70, 5, 5, 68, 0)]
 
 
 @pytest.mark.parametrize("inter", [False, True])
@@ -102,7 +103,7 @@ def test_sizes(T, H, Hk, D, rot, inter):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("norm,weights", [(True, True), (True, False), (False, False)])
 @pytest.mark.parametrize("inter", [False, True])
-@pytest.mark.parametrize("D,rot", [(128, 128), (80, 40), (18, 6)])
+@pytest.mark.parametrize("D,rot", [(128, 128), (80, 40), (72, 36), (60, 60), (18, 6)])
 def test_types(dtype, norm, weights, inter, D, rot):
     _check(_case(70, 8, 2, D, rot, dtype, inter, norm, weights), inter, norm)
 
@@ -157,6 +158,20 @@ def test_columns_that_do_not_turn_stay():
         q[..., 16:] = float("inf")
         y, _ = qk_norm_rope(q, None, cos, sin, norm=False)
         assert bool((y[..., 16:] == float("inf")).all()) and bool(y[..., :16].isfinite().all())
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("shift", [1, 2, 4, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_addresses(dtype, shift, inter):
+    """q and k that begin 1 to 8 elements behind an aligned address, with token strides to match: 2 to 32 bytes."""
+    T, H, D = 40, 4, 64
+    args = list(_case(T, H, H, D, D, dtype, inter, True, packed=False))
+    for i in (0, 1):
+        room = torch.zeros(T, H * D + 8 + shift, dtype=dtype, device=DEV)
+        room[:, shift:shift + H * D] = args[i].reshape(T, H * D)
+        args[i] = room[:, shift:shift + H * D].view(T, H, D)
+    _check(args, inter, True)
 
 
 @pytest.mark.parametrize("layout", ["heads_first", "unaligned", "every_second_column", "expanded", "transposed_gradient"])
