@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(co
                     gx = fma2(mul2(b[j], wb[j]), xb[j], fma2(mul2(a[j], wa[j]), xa[j], gx));
                 }
                 const float sq = lane_sum<LANES>(L.live ? sum2(ss) : 0.f), gs = lane_sum<LANES>(L.live ? sum2(gx) : 0.f);
-                const float r = rsqrtf(sq * inv_d + eps), q = -r * r * r * gs * inv_d;
+                const float r = rsqrtf(sq * inv_d + eps), q = -(r * gs) * inv_d * r * r;          // (r^3 alone leaves fp32 beyond 2^+-42)
                 const float rg = keep ? r : 0.f;           // (a row that is not there is another's copy)
                 const uint64_t r2 = f2(r, r), q2 = f2(q, q), rg2 = f2(rg, rg);
 #pragma unroll
@@ -538,7 +538,7 @@ template <typename T, int N, int LANES, Kind KIND, bool NORM> int launch(Params 
     static std::atomic<int> known[2];
     int most = known[bwd].load();
     if (most == 0) {
-        most = bwd ? resident_blocks(bwd_kernel<T, N, LANES, KIND, NORM>, 40 * 1024) : resident_blocks(fwd_kernel<T, N, LANES, KIND, NORM>, 0);
+        most = bwd ? resident_blocks(bwd_kernel<T, N, LANES, KIND, NORM>, THREADS * 2 * N * sizeof(float)) : resident_blocks(fwd_kernel<T, N, LANES, KIND, NORM>, 0);
         if (most > MAX_BLOCKS) most = MAX_BLOCKS;
         known[bwd].store(most);
     }

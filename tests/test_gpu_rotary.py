@@ -113,6 +113,15 @@ def test_lengths(T):
     _check(_case(T, 8, 2, 64, 64, torch.bfloat16, False, True), False, True)
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [2.0 ** -50, 2.0 ** 50])
+def test_heads_of_any_size(scale, dtype, inter):
+    """r^3 leaves fp32's range long before r x and the gradients do."""
+    q, k, *rest = _case(23, 4, 2, 64, 64, dtype, inter, True)
+    _check((q * scale, k * scale, *rest), inter, True, eps=0.0)
+
+
 def test_far_positions():
     """Positions up to 1,000,000, whose angles fp32 products would have lost: the tables come from 64 bits, so the
     definition's own angles serve; cos and sin held in fp32 add half a unit each."""
