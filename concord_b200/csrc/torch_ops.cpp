@@ -591,8 +591,17 @@ Tensor save8(const Tensor& x) {
     return out;
 }
 
+// a Saved8's bytes are the caller's to make: whole ones, as many as its shape has
+void check_saved(const Tensor& saved, int64_t M, int64_t K) {
+    TORCH_CHECK(saved.scalar_type() == at::kByte && saved.is_cuda() && saved.is_contiguous() &&
+                    saved.numel() == (int64_t)concord_saved8_bytes(M, K),
+                "saved must hold ", concord_saved8_bytes(M, K), " bytes for ", M, " x ", K, " values, got ", saved.sizes(), " of ",
+                saved.scalar_type());
+}
+
 Tensor dense8(const Tensor& saved, int64_t M, int64_t K, int64_t code) {
     at::NoGradGuard no_grad;
+    check_saved(saved, M, K);
     c10::cuda::CUDAGuard guard(saved.device());
     const Tensor out = at::empty({M, K}, saved.options().dtype(type_of(code)));
     check(concord_dense8(ptr(saved), ptr(out), (int32_t)code, K, M, K, current_stream()), "concord_dense8");
@@ -602,6 +611,7 @@ Tensor dense8(const Tensor& saved, int64_t M, int64_t K, int64_t code) {
 Tensor grad_weight8(const Tensor& dy0, const Tensor& saved, int64_t M, int64_t K) {
     refuse_transforms({dy0}, "grad_weight8");
     at::NoGradGuard no_grad;
+    check_saved(saved, M, K);
     c10::cuda::CUDAGuard guard(saved.device());
     const int64_t N = dy0.size(-1);
     Tensor dy = rows(dy0, N);

@@ -280,7 +280,7 @@ def test_packed_layer_bias_fp32_input_and_refusals():
 
 
 def test_refusals():
-    from concord_b200 import grad_weight8, save8
+    from concord_b200 import Saved8, grad_weight8, save8
     x = torch.zeros(4, 8, device=DEV)
     s = save8(x)
     for error, match, call in (
@@ -290,7 +290,12 @@ def test_refusals():
             (TypeError, "must be a Saved8", lambda: grad_weight8(x.bfloat16(), x)),
             (TypeError, "grad_y must be one of", lambda: grad_weight8(x, s)),
             (ValueError, "grad_y must be", lambda: grad_weight8(x[:3].bfloat16(), s)),
-            (TypeError, "dtype must be one of", lambda: s.dense(torch.float64))):
+            (TypeError, "dtype must be one of", lambda: s.dense(torch.float64)),
+            (RuntimeError, "saved must hold", lambda: Saved8(s.data, (65, 8), torch.float32).dense()),
+            (RuntimeError, "saved must hold", lambda: Saved8(s.data[1:], (4, 8), torch.float32).dense()),
+            (RuntimeError, "saved must hold", lambda: Saved8(s.data.float(), (4, 8), torch.float32).dense()),
+            (RuntimeError, "saved must hold", lambda: grad_weight8(torch.zeros(65, 8, device=DEV).bfloat16(),
+                                                                   Saved8(s.data, (65, 8), torch.float32)))):
         with pytest.raises(error, match=match):
             call()
 
