@@ -48,5 +48,14 @@ class Embedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale, self.out_dtype = scale, out_dtype
 
+    @classmethod
+    def from_pretrained(cls, embeddings, freeze=True, padding_idx=None, scale=1.0, out_dtype=None):
+        """The module around a table [V, D], which is not copied."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"embeddings must be [V, D], got shape {tuple(embeddings.shape)}")
+        module = cls(*embeddings.shape, padding_idx, scale, out_dtype, device="meta")
+        module.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return module
+
     def forward(self, ids):
         return embedding(ids, self.weight, self.scale, self.padding_idx, self.out_dtype)

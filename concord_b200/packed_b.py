@@ -736,6 +736,9 @@ class ConcordLinearPackedB(nn.Module):
     EXP_MIN = -8
     EXP_MAX = 7
     MAX_M = 24000
+    # keep the input in 8 bits for the backward (dW is computed from these); see save8.  A
+    # layer sets its own; the class's is for layers that were pickled before there was one
+    save8 = False
 
     def __init__(self, in_features, out_features, bias=True, device='cuda', alpha=0.1,
                  beta1=0.0, lr=0.01):
@@ -767,8 +770,6 @@ class ConcordLinearPackedB(nn.Module):
         self.track_rebalance = True
         # fused coherence meter: (sum of coh, count) accumulated by the step kernel
         self.coh_stats = None
-        # keep the input in 8 bits for the backward (dW is computed from these); see save8
-        self.save8 = False
         self.register_buffer('_reb_seed', torch.zeros(1, dtype=torch.int32, device=device))
         self.register_buffer('packed_w', torch.zeros(out_features, in_features,
                                                      dtype=torch.int32, device=device))

@@ -98,7 +98,7 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
 
 class QKNormRope(nn.Module):
     """`qk_norm_rope` with its weights (q_weight, k_weight [head_dim], ones at the start)
-    and its tables for `positions` positions (not in the state dict)."""
+    and its tables for `positions` positions (not in the state dict; fp32 whatever type the module is cast to)."""
 
     def __init__(self, head_dim, positions, rot=None, base=10000.0, eps=1e-6, interleaved=False, device=None):
         super().__init__()
@@ -107,6 +107,13 @@ class QKNormRope(nn.Module):
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
         self.eps, self.interleaved = eps, interleaved
+
+    def _apply(self, fn, recurse=True):
+        cos, sin = self.cos, self.sin
+        super()._apply(fn, recurse)
+        if self.cos.dtype != torch.float32:               # the tables stay in fp32 where the module is cast
+            self.cos, self.sin = cos.to(self.cos.device), sin.to(self.sin.device)
+        return self
 
     def forward(self, q, k, positions=None):
         return qk_norm_rope(q, k, self.cos, self.sin, positions, self.q_weight, self.k_weight, eps=self.eps,

@@ -35,6 +35,36 @@ def test_cpu_tensors_are_refused(lib):
         c.grad_weight8(x, x)
 
 
+def test_tables_stay_in_fp32():
+    from concord_b200 import QKNormRope, rope_tables
+    m = torch.nn.Sequential(QKNormRope(64, 100, rot=32))
+    want = rope_tables(100, 32, device="cpu")
+    for cast in (lambda: m.bfloat16(), lambda: m.half(), lambda: m.to(torch.float64), lambda: m.float()):
+        cast()
+        assert torch.equal(m[0].cos, want[0]) and torch.equal(m[0].sin, want[1]) and m[0].cos.dtype == torch.float32
+    assert m.half()[0].q_weight.dtype == torch.float16 and sorted(m.state_dict()) == ["0.k_weight", "0.q_weight"]
+
+
+def test_embedding_from_a_table():
+    from concord_b200 import Embedding
+    w = torch.randn(7, 5)
+    m = Embedding.from_pretrained(w, padding_idx=-1, scale=2.0)
+    assert m.weight.data_ptr() == w.data_ptr() and torch.equal(m.weight, w) and not m.weight.requires_grad
+    assert (m.num_embeddings, m.embedding_dim, m.padding_idx, m.scale) == (7, 5, 6, 2.0)
+    assert Embedding.from_pretrained(w, freeze=False).weight.requires_grad
+    with pytest.raises(ValueError, match=r"must be \[V, D\]"):
+        Embedding.from_pretrained(w[0])
+
+
+def test_layers_pickled_before_there_was_save8():
+    from concord_b200 import ConcordLinearPackedB
+    lay = ConcordLinearPackedB.__new__(ConcordLinearPackedB)          # (as unpickling makes them)
+    torch.nn.Module.__init__(lay)
+    assert lay.save8 is False
+    lay.save8 = True
+    assert lay.save8 and not ConcordLinearPackedB.save8
+
+
 def test_embedding_entries_refuse(lib):
     def forward(ids=ONE, w=ONE, wt=0, ldw=8, yt=0, T=4, V=5, D=8):
         return lib.concord_embedding_fwd(ids, 1, w, wt, ldw, ONE, yt, T, V, D, 1.0, None)
