@@ -307,12 +307,13 @@ template <typename T, int ACT> int forward(const Unit& U, void* h, int32_t type,
         k<<<dim3((unsigned)blocks(U.M), blocks_k), threads, 0, st>>>(U, out);
         return check_launch("concord_gated_fwd");
     }
-    const bool vec = (rows | reinterpret_cast<uintptr_t>(h)) % 16 == 0 && U.K % 8 == 0;
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = (rows | reinterpret_cast<uintptr_t>(h)) % 16 == 0;
     dim3 threads;
     int blocks_k;
-    tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
+    tall(U.K, vec ? VEC : 1, &threads, &blocks_k);
     const int64_t each = (vec ? 2 : TALL) * (int64_t)threads.y;
-    auto k = vec ? fwd_kernel<T, 8, 2, ACT> : fwd_kernel<T, 1, TALL, ACT>;
+    auto k = vec ? fwd_kernel<T, VEC, 2, ACT> : fwd_kernel<T, 1, TALL, ACT>;
     k<<<dim3((unsigned)((U.M + each - 1) / each), blocks_k), threads, 0, st>>>(U, out);
     return check_launch("concord_gated_fwd");
 }
@@ -333,12 +334,13 @@ int backward(const Unit& U, const void* dh, int64_t lddh, void* dg, int64_t lddg
         return check_launch("concord_gated_bwd");
     }
     rows |= bytes_of(U.gate, U.ldg, type) | bytes_of(U.up, U.ldu, type);
-    const bool vec = rows % 16 == 0 && U.K % 8 == 0;
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = rows % 16 == 0;
     dim3 threads;
     int blocks_k;
-    tall(U.K, vec ? 8 : 1, &threads, &blocks_k);
+    tall(U.K, vec ? VEC : 1, &threads, &blocks_k);
     const int64_t each = (vec ? 1 : TALL) * (int64_t)threads.y;
-    auto k = vec ? bwd_kernel<T, 8, 1, ACT> : bwd_kernel<T, 1, TALL, ACT>;
+    auto k = vec ? bwd_kernel<T, VEC, 1, ACT> : bwd_kernel<T, 1, TALL, ACT>;
     k<<<dim3((unsigned)((U.M + each - 1) / each), blocks_k), threads, 0, st>>>(U, up, lddh, og, lddg, ou, lddu);
     return check_launch("concord_gated_bwd");
 }

@@ -71,18 +71,6 @@ __device__ __forceinline__ float value(uint32_t flipped, int j, float scale) {
     return (__uint_as_float(__byte_perm(flipped, 0x4b000000u, 0x7650 + j)) - 8388736.f) * scale;
 }
 
-// 32 bytes at once
-__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
-                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
-                 : "memory");
-}
-__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
-    asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
-        : "l"(p));
-}
-
 // EL features of 32 tokens in registers, as loaded
 template <typename T, int EL> struct Tile {
     static constexpr int W = EL * (int)sizeof(T) / 4 > 0 ? EL * (int)sizeof(T) / 4 : 1;

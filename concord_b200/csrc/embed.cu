@@ -13,7 +13,7 @@
 // more go through memory, two launches a digit.  The sorted tokens are cut into
 // chunks of 32, summed side by side, each chunk's rows in order; a row that begins and
 // ends in one is finished there, the pieces of the others are joined in order
-// by a second kernel.  Rows of no token are cleared by other blocks meanwhile.
+// by a second kernel.  Rows of no token, which the sort's bit of each row tells, are cleared by the same launch's other blocks.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -55,11 +55,11 @@ template <typename T, bool VEC> struct Raw {
     uint32_t v[W];
     __device__ __forceinline__ void load(const T* row, const Cols<VEC>& C) {
         if constexpr (VEC) {
-#pragma unroll
-            for (int i = 0; i < W / 4; ++i) {
-                const uint4 u = reinterpret_cast<const uint4*>(row + C.at[0])[i];
-                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
-            }
+            uint4 a, b;
+            if constexpr (sizeof(T) == 4) load32(row + C.at[0], a, b);
+            else a = *reinterpret_cast<const uint4*>(row + C.at[0]);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            if constexpr (sizeof(T) == 4) { v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
         } else {
 #pragma unroll
             for (int c = 0; c < N; ++c) v[c] = __float_as_uint(to_f32(row[C.at[c]]));
@@ -74,7 +74,8 @@ template <typename T, bool VEC> struct Raw {
     }
 };
 template <typename T, bool VEC> __device__ __forceinline__ void store_cols(T* row, const Cols<VEC>& C, const float* v) {
-    if constexpr (VEC) store_vec<8>(row + C.at[0], v);
+    if constexpr (VEC && sizeof(T) == 4) store32(row + C.at[0], Pack16<T>::pack(v), Pack16<T>::pack(v + 4));
+    else if constexpr (VEC) store_vec<8>(row + C.at[0], v);
     else {
 #pragma unroll
         for (int c = 0; c < Cols<VEC>::N; ++c)
@@ -199,27 +200,6 @@ __global__ void __launch_bounds__(SORT_THREADS) place_kernel(const __grid_consta
     }
 }
 
-// The first of `n` sorted places whose key is v or more, by a whole warp: 32 places looked at at once.
-__device__ __forceinline__ uint32_t lower_bound(const uint2* sorted, uint32_t n, int64_t v) {
-    uint32_t lo = 0, len = n;                     // it is in [lo, lo + len]
-    uint32_t lane;                                // (blocks have two dimensions)
-    asm("mov.u32 %0, %%laneid;" : "=r"(lane));
-    while (len > 0) {
-        const uint32_t step = (len + 31) / 32, at = lane * step;
-        const bool below = at < len && (int64_t)sorted[lo + at].x < v;
-        const uint32_t k = __popc(__ballot_sync(0xffffffffu, below));      // lanes 0 .. k - 1
-        if (k == 0) return lo;
-        const uint32_t from = (k - 1) * step + 1;
-        len = min(step - 1, len - from);
-        lo += from;
-    }
-    return lo;
-}
-__global__ void __launch_bounds__(32) end_kernel(const uint2* sorted, uint32_t* end, int64_t T, int64_t V) {
-    const uint32_t e = lower_bound(sorted, (uint32_t)T, V);
-    if (threadIdx.x == 0) *end = e;
-}
-
 // The whole sort by one cluster: block r holds places [r n, (r + 1) n)
 // of the list, n a power of two.  A digit takes two exchanges: the blocks' counts,
 // and the items, stored straight into the shared memory of the block that owns their place.
@@ -232,7 +212,21 @@ struct ClusterSort {
     int T, n, log_n, passes, digit;       // digit: bits of a pass, up to 9
     uint2* sorted;
     uint32_t* end;                                // places of rows; behind them what counts for none
+    uint32_t* some;                               // a bit a row: it has tokens
 };
+// One place of the sorted list, its neighbours' keys beside it: the row's bit, and where rows end.
+__device__ __forceinline__ void mark(uint32_t* some, uint32_t* end, int64_t V, int64_t T, int64_t i, uint32_t before, uint32_t key, uint32_t after) {
+    if (key >= V) {
+        if (i == 0) *end = 0;
+        return;
+    }
+    if (before != key) atomicOr(&some[key / 32], 1u << (key % 32));
+    if (i + 1 == T || after >= V) *end = (uint32_t)(i + 1);
+}
+__global__ void __launch_bounds__(256) mark_kernel(const uint2* sorted, uint32_t* some, uint32_t* end, int64_t T, int64_t V) {
+    const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+    if (i < T) mark(some, end, V, T, i, i ? sorted[i - 1].x : ~0u, sorted[i].x, i + 1 < T ? sorted[i + 1].x : ~0u);
+}
 size_t cluster_smem(int n) { return (size_t)2 * n * sizeof(uint2) + CW * BINS * sizeof(uint16_t) + 2 * BINS * sizeof(uint32_t); }
 
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CT) cluster_sort_kernel(const __grid_constant__ ClusterSort P) {
@@ -249,6 +243,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CT) cluster_so
     const int run = max(32, P.n / CW), r0 = min(warp * run, have), r1 = min(r0 + run, have);
     for (int i = threadIdx.x; i < have; i += CT)
         list[0][i] = make_uint2(key_of(P.ids, P.ids64, begin + i, P.V, P.padding), (uint32_t)(begin + i));
+    for (int64_t i = rank * CT + threadIdx.x; i < (P.V + 31) / 32; i += CLUSTER * CT) P.some[i] = 0;
     const int bins = 1 << P.digit;
     for (int pass = 0; pass < P.passes; ++pass) {
         const uint2* from = list[pass & 1];
@@ -320,13 +315,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CT) cluster_so
     for (int i = threadIdx.x; i < have; i += CT) {
         const uint2 it = done[i];
         P.sorted[begin + i] = it;
-        const bool none = it.x >= P.V;
-        if (none && begin + i == 0) *P.end = 0;
-        if (!none && begin + i + 1 == P.T) *P.end = (uint32_t)P.T;
-        if (!none && begin + i + 1 < P.T) {
-            const uint32_t next = i + 1 < have ? done[i + 1].x : cluster.map_shared_rank(const_cast<uint2*>(done), rank + 1)[0].x;
-            if (next >= P.V) *P.end = (uint32_t)(begin + i + 1);
-        }
+        const int n = begin + i + 1;
+        const uint32_t after = n == P.T ? ~0u : i + 1 < have ? done[i + 1].x : cluster.map_shared_rank(const_cast<uint2*>(done), rank + 1)[0].x;
+        mark(P.some, P.end, P.V, P.T, begin + i, i > 0 ? done[i - 1].x : ~0u, it.x, after);
     }
     cluster.sync();                               // nobody leaves while its list is read
 }
@@ -334,7 +325,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CT) cluster_so
 // ---------------------------------------------------------------- sums
 struct Sums {
     const uint2* sorted;
-    const uint32_t* end;
+    const uint32_t *end, *some;
     float* part;              // [chunks][2][D]: a row's piece that goes on from the chunk before, one that begins here and goes on
     int64_t T, V, lddy;
     int64_t chunks;
@@ -342,41 +333,35 @@ struct Sums {
     float scale;
 };
 
-// Blocks of two kinds, spread evenly: chunks, one a row of threads (their
-// loads run AHEAD tokens before their sums), and rows of no token to clear.
-constexpr int CLEAR = 64;             // rows of the table that a clearing block looks at
+// Blocks of two kinds: chunks, one a row of threads (their loads run AHEAD
+// tokens before their sums), then rows of no token to clear, CLEAR a thread.  Chunks
+// first, as they wait for memory and the others only fill it (16384 tokens, 32000 x 2048
+// fp32: 49 us, 6.7 TB/s; both kinds mixed 56; with 16 bytes a store, which leave half a sector
+// of 8 columns of fp32 to the next one, 67).
+constexpr int CLEAR = 8;
 template <typename TY, typename TW, bool VEC>
-__global__ void __launch_bounds__(256, 3)
-    sum_kernel(const TY* dy, TW* dw, const __grid_constant__ Sums P, int chunk_blocks, int clear_blocks) {
+__global__ void __launch_bounds__(256, 3) sum_kernel(const TY* dy, TW* dw, const __grid_constant__ Sums P, int chunk_blocks) {
     constexpr int N = Cols<VEC>::N;
     const Cols<VEC> C(blockIdx.y, threadIdx.x, blockDim.x, P.D);
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
-    const int64_t both = chunk_blocks + clear_blocks;
-    const int64_t nth = blockIdx.x * (int64_t)chunk_blocks / both;
-    if (nth == (blockIdx.x + 1) * (int64_t)chunk_blocks / both) {          // the (blockIdx.x - nth)-th to clear
-        __shared__ uint32_t some[CLEAR / 32];
-        const int64_t v0 = (blockIdx.x - nth) * CLEAR;
-        const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
-        if (thread < CLEAR / 32) some[thread] = 0;
-        __syncthreads();
-        if (thread < (threads & ~31)) {           // (whole warps)
-            const uint32_t a = lower_bound(P.sorted, *P.end, v0), b = lower_bound(P.sorted, *P.end, v0 + CLEAR);
-            for (uint32_t p = a + thread; p < b; p += threads & ~31) {
-                const uint32_t r = P.sorted[p].x - (uint32_t)v0;
-                atomicOr(&some[r / 32], 1u << (r % 32));
-            }
+    if (C.count == 0) return;
+    if (blockIdx.x >= chunk_blocks) {
+        const int64_t v0 = (blockIdx.x - chunk_blocks) * (int64_t)(CLEAR * blockDim.y) + threadIdx.y;
+        bool none[CLEAR];
+#pragma unroll
+        for (int r = 0; r < CLEAR; ++r) {
+            const int64_t v = v0 + r * blockDim.y;
+            none[r] = v < P.V && !(P.some[v / 32] >> (v % 32) & 1);
         }
-        __syncthreads();
-        if (C.count == 0) return;
-        for (int r = threadIdx.y; r < CLEAR && v0 + r < P.V; r += blockDim.y)
-            if (!(some[r / 32] >> (r % 32) & 1)) store_cols<TW, VEC>(dw + (v0 + r) * P.D, C, acc);
+#pragma unroll
+        for (int r = 0; r < CLEAR; ++r)
+            if (none[r]) store_cols<TW, VEC>(dw + (v0 + r * blockDim.y) * P.D, C, acc);
         return;
     }
-    if (C.count == 0) return;
     constexpr int AHEAD = !VEC || sizeof(TY) == 2 ? 8 : 4;
-    const int64_t i = nth * blockDim.y + threadIdx.y;
+    const int64_t i = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
     const uint32_t end = *P.end;
     if (i >= P.chunks || (uint32_t)i * SEG >= end) return;
     const uint32_t p0 = (uint32_t)i * SEG, p1 = min(p0 + SEG, end);
@@ -418,6 +403,25 @@ __global__ void __launch_bounds__(256, 3)
     }
 }
 
+// How many of the chunks behind i, below `chunks`, begin with row v, by a whole warp: the next
+// 32, then 32 places of what is left at once.
+__device__ __forceinline__ int64_t going_on(const uint2* sorted, int64_t i, int64_t chunks, uint32_t v) {
+    int64_t known = 0, len = chunks - i - 1, step = 1;          // the answer is in [known, known + len]
+    uint32_t lane;                                              // (blocks have two dimensions)
+    asm("mov.u32 %0, %%laneid;" : "=r"(lane));
+    while (len > 0) {
+        const int64_t at = lane * step;
+        const bool on = at < len && sorted[(i + 1 + known + at) * SEG].x == v;
+        const int64_t k = __popc(__ballot_sync(0xffffffffu, on));          // lanes 0 .. k - 1
+        if (k == 0) break;
+        const int64_t from = (k - 1) * step + 1;
+        len = k < 32 ? min(step - 1, len - from) : len - from;
+        known += from;
+        step = (len + 31) / 32;
+    }
+    return known;
+}
+
 // One row at most begins in a chunk and goes on: its pieces in order, eight runs of
 // them side by side, the runs' sums in order again.
 constexpr int JOIN = 8;
@@ -426,13 +430,10 @@ __global__ void __launch_bounds__(256) join_kernel(TW* dw, const __grid_constant
     constexpr int N = Cols<VEC>::N;
     __shared__ float runs[JOIN][32][N];
     const int64_t i = blockIdx.x;
-    const uint32_t end = *P.end, p0 = (uint32_t)i * SEG, p1 = p0 + SEG;
-    if (p1 >= end) return;                                // (the last chunk: nothing goes on)
-    const uint32_t v = P.sorted[p1 - 1].x;
-    if (P.sorted[p1].x != v) return;
-    if (p0 > 0 && P.sorted[p0 - 1].x == v) return;        // it began before
-    const uint32_t b = p1 + lower_bound(P.sorted + p1, end - p1, (int64_t)v + 1);
-    const int64_t pieces = (b - 1) / SEG - i;             // besides the first
+    const uint32_t end = *P.end, p0 = (uint32_t)i * SEG, p1 = p0 + SEG;       // (p1 is below T: the last chunk has no block)
+    const uint32_t v = P.sorted[p1 - 1].x, next = P.sorted[p1].x, before = P.sorted[max(p0, 1u) - 1].x;
+    if (p1 >= end || next != v || (p0 > 0 && before == v)) return;            // nothing goes on, or it began before
+    const int64_t pieces = going_on(P.sorted, i, min(P.chunks, ((int64_t)end + SEG - 1) / SEG), v);
     const Cols<VEC> C(blockIdx.y, threadIdx.x, 32, P.D);
     float acc[N];
 #pragma unroll
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(256) join_kernel(TW* dw, const __grid_constant
 }
 
 // ---------------------------------------------------------------- host side
-// threads of a block along the columns (any number: only whole warps of the clearing blocks share), and blocks along them
+// threads of a block along the columns, and blocks along them
 void shape(int64_t D, int each, dim3* threads, int* across) {
     const int64_t pieces = (D + each - 1) / each, x = pieces < 256 ? pieces : 256;
     *threads = dim3((unsigned)x, (unsigned)(256 / x), 1);
@@ -492,9 +493,9 @@ int forward(const void* ids, int ids64, const void* w, int64_t ldw, void* y, int
 
 struct Layout {
     int64_t chunk, blocks, chunks;
-    size_t second, counts, end, part, total;        // offsets (the first list stands at 0)
+    size_t second, counts, end, some, part, total;        // offsets (the first list stands at 0)
 };
-Layout layout(int64_t T, int64_t D) {
+Layout layout(int64_t T, int64_t V, int64_t D) {
     Layout L;
     L.chunk = SORT_CHUNK;
     while ((T + L.chunk - 1) / L.chunk > SORT_BLOCKS) L.chunk *= 2;
@@ -504,7 +505,8 @@ Layout layout(int64_t T, int64_t D) {
     L.second = up(T * sizeof(uint2));
     L.counts = L.second + up(T * sizeof(uint2));
     L.end = L.counts + up(L.blocks * BINS * sizeof(uint32_t));
-    L.part = L.end + up(sizeof(uint32_t));
+    L.some = L.end + up(sizeof(uint32_t));
+    L.part = L.some + up((V + 31) / 32 * sizeof(uint32_t));
     L.total = L.part + up((size_t)L.chunks * 2 * D * sizeof(float));
     return L;
 }
@@ -512,16 +514,16 @@ Layout layout(int64_t T, int64_t D) {
 template <typename TY, typename TW>
 int backward(const void* ids, int ids64, const void* dy, int64_t lddy, void* dw, int64_t T, int64_t V, int64_t D,
              float scale, int64_t padding, char* ws, bool vec, cudaStream_t st) {
-    const Layout L = layout(T, D);
+    const Layout L = layout(T, V, D);
     uint2 *list[2] = {reinterpret_cast<uint2*>(ws), reinterpret_cast<uint2*>(ws + L.second)};
-    uint32_t* end = reinterpret_cast<uint32_t*>(ws + L.end);
+    uint32_t *end = reinterpret_cast<uint32_t*>(ws + L.end), *some = reinterpret_cast<uint32_t*>(ws + L.some);
     const uint2* sorted = list[0];
     int passes = 1;
     while (V >> (passes * DIGIT)) ++passes;
     if (T <= CLUSTER * CLUSTER_MOST) {
         int bits = 1;
         while (V >> bits) ++bits;
-        ClusterSort C{ids, ids64, V, padding, (int)T, 32, 5, passes, (bits + passes - 1) / passes, list[0], end};
+        ClusterSort C{ids, ids64, V, padding, (int)T, 32, 5, passes, (bits + passes - 1) / passes, list[0], end, some};
         if (C.digit < 3) C.digit = 3;             // (whole 16-byte pieces of counts)
         while ((int64_t)C.n * CLUSTER < T) {
             C.n *= 2;
@@ -542,17 +544,18 @@ int backward(const void* ids, int ids64, const void* dy, int64_t lddy, void* dw,
             P.from = P.to;
         }
         sorted = P.from;
-        end_kernel<<<1, 32, 0, st>>>(sorted, end, T, V);
+        cudaMemsetAsync(some, 0, (V + 31) / 32 * sizeof(uint32_t), st);
+        mark_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(sorted, some, end, T, V);
     }
-    const Sums S{sorted, end, reinterpret_cast<float*>(ws + L.part), T, V, lddy, L.chunks, (int)D, scale};
+    const Sums S{sorted, end, some, reinterpret_cast<float*>(ws + L.part), T, V, lddy, L.chunks, (int)D, scale};
     dim3 threads;
     int across;
     shape(D, vec ? 8 : 4, &threads, &across);
     const int chunk_blocks = (int)((L.chunks + threads.y - 1) / threads.y);
-    const int clear_blocks = (int)((V + CLEAR - 1) / CLEAR);
+    const int clear_blocks = (int)((V + CLEAR * threads.y - 1) / (CLEAR * threads.y));
     auto k = vec ? sum_kernel<TY, TW, true> : sum_kernel<TY, TW, false>;
     k<<<dim3((unsigned)(chunk_blocks + clear_blocks), across, 1), threads, 0, st>>>(
-        static_cast<const TY*>(dy), static_cast<TW*>(dw), S, chunk_blocks, clear_blocks);
+        static_cast<const TY*>(dy), static_cast<TW*>(dw), S, chunk_blocks);
     if (L.chunks > 1) {
         auto j = vec ? join_kernel<TW, true> : join_kernel<TW, false>;
         const int wide = 32 * (vec ? 8 : 4);
@@ -571,6 +574,8 @@ int check_shape(const char* name, int32_t ta, int32_t tb, int64_t T, int64_t V, 
 }
 
 size_t esize(int32_t t) { return t == CONCORD_F32 ? 4 : 2; }
+// whether rows are runs of 8 columns, each a whole access
+bool runs(const void* p, int32_t t, int64_t ld) { return ld % 8 == 0 && aligned(p, 8 * esize(t)); }
 
 // calls F<A, B> for the two type codes
 #define EMBED_TYPES(ta, tb, F, ...)                                                             \
@@ -597,13 +602,13 @@ extern "C" int concord_embedding_fwd(const void* ids, int32_t ids64, const void*
     if (int rc = embed::check_shape("concord_embedding_fwd", w_type, y_type, T, V, D, ldw)) return rc;
     if (T == 0) return CONCORD_OK;
     if (!ids || !w || !y) return fail(CONCORD_EINVAL, "concord_embedding_fwd: null pointer");
-    const bool vec = D % 8 == 0 && ldw * embed::esize(w_type) % 16 == 0 && aligned(w, 16) && aligned(y, 16);
+    const bool vec = embed::runs(w, w_type, ldw) && embed::runs(y, y_type, D);
     EMBED_TYPES(w_type, y_type, embed::forward, ids, ids64, w, ldw, y, T, V, D, scale, vec, as_stream(stream))
 }
 
 extern "C" size_t concord_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) {
     if (T <= 0 || V <= 0 || D <= 0 || T > (1 << 30) || V > (1 << 30) || D > (1 << 20)) return 0;
-    return embed::layout(T, D).total;
+    return embed::layout(T, V, D).total;
 }
 
 extern "C" int concord_embedding_bwd(const void* ids, int32_t ids64, const void* dy, int32_t dy_type, int64_t lddy,
@@ -619,7 +624,7 @@ extern "C" int concord_embedding_bwd(const void* ids, int32_t ids64, const void*
     if (!ids || !dy) return fail(CONCORD_EINVAL, "concord_embedding_bwd: null pointer");
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < concord_embedding_bwd_workspace_bytes(T, V, D))
         return fail(CONCORD_EWORKSPACE, "concord_embedding_bwd: workspace too small, or not 16-byte aligned");
-    const bool vec = D % 8 == 0 && lddy * embed::esize(dy_type) % 16 == 0 && aligned(dy, 16) && aligned(dw, 16);
+    const bool vec = embed::runs(dy, dy_type, lddy) && embed::runs(dw, dw_type, D) && aligned(workspace, 32);
     EMBED_TYPES(dy_type, dw_type, embed::backward, ids, ids64, dy, lddy, dw, T, V, D, scale, padding,
                 static_cast<char*>(workspace), vec, st)
 }

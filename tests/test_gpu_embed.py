@@ -113,6 +113,22 @@ def test_strides_and_padding():
     m.load_state_dict(torch.nn.Embedding(40, 64).state_dict())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset,stride", [(0, 72), (1, 72), (2, 72), (4, 72), (8, 72), (0, 68), (0, 66), (4, 68), (8, 70)])
+def test_addresses(dtype, offset, stride):
+    """Tables and upstream gradients whose rows begin on 2 to 32 bytes."""
+    from concord_b200 import embedding
+    g = torch.Generator(device=DEV).manual_seed(offset + stride)
+    ids = torch.randint(-1, 30, (200,), generator=g, device=DEV)
+    part = lambda rows: torch.randint(-8, 9, (rows * stride + offset,), generator=g, device=DEV).to(dtype)[offset:].view(rows, stride)[:, :56]  # noqa: E731
+    w, dy = part(30), part(200)
+    assert torch.equal(embedding(ids, w), torch.where(ids[:, None] < 0, 0, w[ids]))
+    leaf = w.detach().clone().requires_grad_()
+    (got,) = torch.autograd.grad(embedding(ids, leaf), leaf, dy)
+    want = torch.zeros(31, 56, device=DEV).index_add_(0, ids % 31, dy.float())[:30]       # (whole numbers: exact)
+    assert torch.equal(got, want.to(dtype))
+
+
 def test_empty_and_nan():
     from concord_b200 import embedding
     w = torch.randn(10, 16, device=DEV, requires_grad=True)
