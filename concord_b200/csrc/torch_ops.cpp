@@ -535,17 +535,23 @@ struct QKNormRopeBackward : public torch::autograd::Node {
 std::tuple<Tensor, MaybeTensor> qk_norm_rope(const Tensor& q, const MaybeTensor& k_in, const MaybeTensor& cos,
                                              const MaybeTensor& sin, const MaybeTensor& pos, const MaybeTensor& q_weight,
                                              const MaybeTensor& k_weight, bool norm, double eps, bool interleaved) {
-    const Tensor k = get(k_in), qw = get(q_weight), kw = get(k_weight);
+    const Tensor k = get(k_in);
+    refuse_transforms({q, k, get(q_weight), get(k_weight), get(cos), get(sin)}, "qk_norm_rope");
+    // (converted where a gradient passes through; most weights and tables are fp32 already)
+    auto floats = [](const MaybeTensor& m) {
+        const Tensor t = get(m);
+        return !t.defined() || (t.scalar_type() == at::kFloat && t.is_contiguous()) ? t : t.to(at::kFloat).contiguous();
+    };
+    c10::cuda::CUDAGuard guard(q.device());
+    const Tensor qw = floats(q_weight), kw = floats(k_weight);
     QKArgs A;
-    A.cos = get(cos);
-    A.sin = get(sin);
-    A.pos = get(pos);
+    A.cos = floats(cos);
+    A.sin = floats(sin);
+    A.pos = pos.has_value() ? pos->contiguous() : Tensor();
     A.norm = norm;
     A.interleaved = interleaved;
     A.eps = eps;
-    refuse_transforms({q, k, qw, kw, A.cos, A.sin}, "qk_norm_rope");
     const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw));
-    c10::cuda::CUDAGuard guard(q.device());
     Tensor q_out, k_out;
     const Heads hq(q.detach()), hk(k.defined() ? k.detach() : k);
     {

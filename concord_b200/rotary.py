@@ -9,11 +9,6 @@ from . import _ops
 _INTS = (torch.int64, torch.int32)
 
 
-def _floats(t):
-    """t (or None) in fp32, contiguous; most are already, and the two calls cost a single token's step 3 us for four of them."""
-    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.float().contiguous()
-
-
 def rope_tables(positions, rot, base=10000.0, device="cuda"):
     """(cos, sin), fp32 [positions, rot / 2], of position * base ** (-2 i / rot):
     angles and functions in 64 bits, so that far positions lose nothing."""
@@ -83,15 +78,12 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
             _ops.need_type("positions", positions, _INTS)
             if positions.shape != (T,):
                 raise ValueError(f"positions must have shape ({T},), got {tuple(positions.shape)}")
-            positions = positions.contiguous()
-        cos, sin = _floats(cos), _floats(sin)
     elif positions is not None:
         raise ValueError("positions without cos and sin")
     elif not norm:
         raise ValueError("neither norm nor rotation: nothing to do")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    q_weight, k_weight = _floats(q_weight), _floats(k_weight)
     return _ops.native().qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, bool(norm), float(eps),
                                       bool(interleaved))
 
