@@ -8,7 +8,7 @@
 //
 // Bound by memory: the forward reads and writes q and k once, the backward reads
 // dy and x and writes dx.  A row (one head of one token) stays in the
-// registers of a group of lanes, 8 or 4 pairs each, a pair's two halves in one lane
+// registers of a group of lanes, 4 or 2 pairs each, a pair's two halves in one lane
 // whichever way pairs are laid out, so that the rotation needs no exchange; the
 // group's lanes share sums by shuffles (both sums of the backward in one go:
 // neither needs r).  Blocks belong to q or to k; a thread walks its tokens' heads
@@ -17,6 +17,7 @@
 // them.  The weights' gradients are added per thread, then per block,
 // then over blocks in a fixed order: no atomics, the same bits on every run of
 // one device.
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -26,6 +27,12 @@ namespace concord {
 namespace qkn {
 
 constexpr int MAX_DIM = 256, THREADS = 256;
+// Rows that a thread has on their way or in hand where its part of them goes through shared memory: asynchronous
+// copies into its own place there, which it reads back itself, so that nothing waits but the
+// thread.  (16384 tokens, 2 x 16 heads of 128 bf16, neighbours and halves: forward 45 and 46 us, backward 67 and
+// 69; the rows in registers, two or three ahead, 51 and 55, 76 and 85.  fp32 does better in registers:
+// halves 93 and 150, through shared memory 161 and 239; so do pieces of 4 bytes, below.)
+constexpr int RING = 6;
 
 // q or k
 struct Side {
@@ -45,6 +52,7 @@ struct Params {
     float eps, inv_d;
     Side side[2];
     int blocks0;                  // blocks of q; the others are k's
+    int lanes;                    // of a row, where the kernel does not say
     float* part;                  // backward: [blocks][D]
 };
 
@@ -121,6 +129,20 @@ template <typename T, int N, Kind KIND> struct Raw {
             for (int j = 0; j < 2 * N; ++j)
                 if (!(L.have >> j & 1)) v[j] = 0;
         }
+    }
+    static constexpr bool ASYNC = VEC && RUN == 8 && N == 4;
+    static constexpr int SLOT = 4 * WORDS;                        // bytes of a thread's place in the ring
+    __device__ __forceinline__ static void start(const Lane<N, KIND>& L, const T* row, uint32_t slot) {
+        if constexpr (KIND == PAIRED) copy16(slot, row + L.at[0]);
+        else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(slot + r * RUN), "l"(row + L.at[r]), "n"(RUN) : "memory");
+        }
+    }
+    __device__ __forceinline__ void take(uint32_t slot) {
+        const uint4 u = read16(slot);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
     }
     __device__ __forceinline__ float element(int i) const {       // VEC: the i-th of both runs
         if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
@@ -261,12 +283,38 @@ __device__ __forceinline__ int64_t position(const Params& P, int64_t t) {
     return P.pos64 ? static_cast<const int64_t*>(P.pos)[t] : (int64_t)static_cast<const int32_t*>(P.pos)[t];
 }
 
-// the sum over a row's lanes (a power of two of them; every lane of the warp calls it)
-template <int LANES> __device__ __forceinline__ float lane_sum(float v) {
+// A thread's row group and its lane there: LANES of them in a row, or (LANES 0) `lanes`, as many groups of these as a warp
+// has room for (what is left over has lane 32, which has no columns).
+template <int LANES> struct Group {
+    int lane, group, groups, lanes;
+    __device__ __forceinline__ explicit Group(int of) : lanes(LANES ? LANES : of) {
+        if constexpr (LANES != 0) {
+            lane = threadIdx.x % LANES;
+            group = threadIdx.x / LANES;
+            groups = THREADS / LANES;
+        } else {
+            const int per = 32 / lanes, at = threadIdx.x % 32, in = at / lanes;
+            lane = in < per ? at % lanes : 32;
+            group = threadIdx.x / 32 * per + min(in, per - 1);
+            groups = THREADS / 32 * per;
+        }
+    }
+    // the sum over a row's lanes; every lane of the warp calls it
+    __device__ __forceinline__ float sum(float v) const {
+        if constexpr (LANES != 0) {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
+            for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            return v;
+        } else {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {             // (up to 16 lanes)
+                const float u = __shfl_down_sync(0xffffffffu, v, o);
+                if (lane + o < lanes) v += u;
+            }
+            return __shfl_sync(0xffffffffu, v, max((int)(threadIdx.x % 32) - lane, 0));
+        }
+    }
+};
 
 __device__ __forceinline__ float sum2(uint64_t v) {
     float a, b;
@@ -305,20 +353,29 @@ template <typename T> __device__ __forceinline__ const T* row_at(const void* p, 
 }
 
 template <typename T, int N, int LANES, Kind KIND, bool NORM>
-__global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const __grid_constant__ Params P) {
-    constexpr int DEPTH = 3;                      // rows of a thread, the present one included
+__global__ void __launch_bounds__(THREADS, Raw<T, N, KIND>::ASYNC ? 3 : KIND == ANY ? 2 : 4) fwd_kernel(const __grid_constant__ Params P) {
+    using Row = Raw<T, N, KIND>;
+    // rows on their way, the present one included, and those of them in registers
+    constexpr bool ASYNC = Row::ASYNC;
+    constexpr int DEPTH = ASYNC ? RING : 3, HELD = ASYNC ? 1 : DEPTH, STAGE = THREADS * Row::SLOT;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * Row::SLOT;
     const int which = blockIdx.x >= P.blocks0, block = blockIdx.x - (which ? P.blocks0 : 0);
     const Side& S = P.side[which];
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, h0 = group % S.share;
-    const Lane<N, KIND> L(P, lane);
-    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, group, THREADS / LANES), far = now;
+    const Group<LANES> G(P.lanes);
+    const int h0 = G.group % S.share;
+    const Lane<N, KIND> L(P, G.lane);
+    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, G.group, G.groups), far = now;
     const int64_t steps = now.steps(), ts = S.ts, hs = S.hs, in_step = hs * S.share, ld = (int64_t)S.heads * P.D;
     const int out_step = S.share * P.D;
     const T* in = row_at<T>(S.x, ts, hs, far.token(), h0);
     T* out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
-    Raw<T, N, KIND> raw[DEPTH];
+    Row raw[HELD];
     auto fetch = [&](int k) {
-        raw[k].fetch(L, in);
+        if constexpr (ASYNC) {
+            Row::start(L, in, ring + k * STAGE);
+            copy_commit();
+        } else raw[k].fetch(L, in);
         in += in_step;
         if (far.next()) in = row_at<T>(S.x, ts, hs, far.token(), h0);
     };
@@ -337,10 +394,14 @@ __global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const
     const bool turns = P.rot > 0;
     bool fresh = turns, keep = now.here() && L.live;
     int64_t pos = turns ? position(P, now.token()) : 0;                 // of the next token, once this one's is used
-    for (int64_t n = 0; n < steps; n += DEPTH) {
+    int stage = 0;
+    for (int64_t n = 0; n < steps; n += HELD) {
 #pragma unroll
-        for (int k = 0; k < DEPTH; ++k) {
-            fetch((k + DEPTH - 1) % DEPTH);
+        for (int k = 0; k < HELD; ++k) {
+            if constexpr (ASYNC) {
+                copy_wait<DEPTH - 2>();
+                raw[0].take(ring + stage * STAGE);
+            } else fetch((k + DEPTH - 1) % DEPTH);
             if (fresh) {
                 angles<N, KIND>(P, L, pos, c, s, m);
                 pos = position(P, min(now.base + now.mine + now.step, now.T - 1));
@@ -352,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const
                 ss = fma2(b[0], b[0], ss);
 #pragma unroll
                 for (int j = 1; j < N / 2; ++j) ss = fma2(b[j], b[j], fma2(a[j], a[j], ss));
-                const float r = rsqrtf(lane_sum<LANES>(L.live ? sum2(ss) : 0.f) * inv_d + eps);
+                const float r = rsqrtf(G.sum(L.live ? sum2(ss) : 0.f) * inv_d + eps);
                 const uint64_t r2 = f2(r, r);
 #pragma unroll
                 for (int j = 0; j < N / 2; ++j) {
@@ -369,35 +430,45 @@ __global__ void __launch_bounds__(THREADS, KIND == ANY ? 2 : 4) fwd_kernel(const
                 fresh = turns;
                 keep = now.here() && L.live;
             }
+            if constexpr (ASYNC) {
+                fetch(stage == 0 ? DEPTH - 1 : stage - 1);
+                stage = stage + 1 == DEPTH ? 0 : stage + 1;
+            }
         }
     }
+    if constexpr (ASYNC) copy_wait<0>();          // (the last rows again, which nobody reads)
 }
 
 template <typename T, int N, int LANES, Kind KIND, bool NORM>
-__global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(const __grid_constant__ Params P) {
-    // (16384 tokens, 2 x 16 heads of 128: neighbours' rows, one load each, 76 us with three rows ahead and 84 with
-    // one and more blocks, halves' rows 99 and 85)
-    constexpr int DEPTH = KIND == PAIRED ? 4 : 2;
-    extern __shared__ float sums[];               // [row groups][D]
+__global__ void __launch_bounds__(THREADS, Raw<T, N, KIND>::ASYNC || KIND != HALVES ? 2 : 3) bwd_kernel(const __grid_constant__ Params P) {
+    using Row = Raw<T, N, KIND>;
+    constexpr bool ASYNC = Row::ASYNC;            // (fp32: neighbours' rows three ahead 130 us, halves' one ahead and more blocks 150)
+    constexpr int DEPTH = ASYNC ? RING : KIND == PAIRED ? 4 : 2, HELD = ASYNC ? 1 : DEPTH;
+    constexpr int X = THREADS * Row::SLOT, STAGE = NORM ? 2 * X : X;              // dy's places, then x's
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* sums = reinterpret_cast<float*>(smem + (ASYNC ? DEPTH * STAGE : 0));   // [row groups][D]
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * Row::SLOT;
     const int which = blockIdx.x >= P.blocks0, block = blockIdx.x - (which ? P.blocks0 : 0);
     const Side& S = P.side[which];
-    constexpr int groups = THREADS / LANES;
-    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    const int h0 = group % S.share;
-    const Lane<N, KIND> L(P, lane);
-    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, group, groups), far = now;
+    const Group<LANES> G(P.lanes);
+    const int h0 = G.group % S.share;
+    const Lane<N, KIND> L(P, G.lane);
+    Rows now(P, S, block, which ? gridDim.x - P.blocks0 : P.blocks0, G.group, G.groups), far = now;
     const int64_t steps = now.steps(), ts = S.ts, hs = S.hs, dts = S.dts, dhs = S.dhs, ld = (int64_t)S.heads * P.D;
     const int out_step = S.share * P.D, share = S.share;
     const T *in = row_at<T>(S.dy, dts, dhs, far.token(), h0), *inx = row_at<T>(S.x, ts, hs, far.token(), h0);
     T* out = const_cast<T*>(row_at<T>(S.out, ld, P.D, now.token(), h0));
-    Raw<T, N, KIND> raw[DEPTH], rawx[DEPTH];
+    Row raw[HELD], rawx[HELD];
     auto fetch = [&](int k) {
-        raw[k].fetch(L, in);
+        if constexpr (ASYNC) Row::start(L, in, ring + k * STAGE);
+        else raw[k].fetch(L, in);
         in += dhs * share;
         if (NORM) {
-            rawx[k].fetch(L, inx);
+            if constexpr (ASYNC) Row::start(L, inx, ring + k * STAGE + X);
+            else rawx[k].fetch(L, inx);
             inx += hs * share;
         }
+        if constexpr (ASYNC) copy_commit();
         if (far.next()) {
             in = row_at<T>(S.dy, dts, dhs, far.token(), h0);
             if (NORM) inx = row_at<T>(S.x, ts, hs, far.token(), h0);
@@ -420,10 +491,15 @@ __global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(co
     const bool turns = P.rot > 0;
     bool fresh = turns, keep = now.here() && L.live;
     int64_t pos = turns ? position(P, now.token()) : 0;
-    for (int64_t n = 0; n < steps; n += DEPTH) {
+    int stage = 0;
+    for (int64_t n = 0; n < steps; n += HELD) {
 #pragma unroll
-        for (int k = 0; k < DEPTH; ++k) {
-            fetch((k + DEPTH - 1) % DEPTH);
+        for (int k = 0; k < HELD; ++k) {
+            if constexpr (ASYNC) {
+                copy_wait<DEPTH - 2>();
+                raw[0].take(ring + stage * STAGE);
+                if (NORM) rawx[0].take(ring + stage * STAGE + X);
+            } else fetch((k + DEPTH - 1) % DEPTH);
             if (fresh) {
                 angles<N, KIND>(P, L, pos, c, s, m);
                 pos = position(P, min(now.base + now.mine + now.step, now.T - 1));
@@ -439,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(co
                     ss = fma2(xb[j], xb[j], fma2(xa[j], xa[j], ss));
                     gx = fma2(mul2(b[j], wb[j]), xb[j], fma2(mul2(a[j], wa[j]), xa[j], gx));
                 }
-                const float sq = lane_sum<LANES>(L.live ? sum2(ss) : 0.f), gs = lane_sum<LANES>(L.live ? sum2(gx) : 0.f);
+                const float sq = G.sum(L.live ? sum2(ss) : 0.f), gs = G.sum(L.live ? sum2(gx) : 0.f);
                 const float r = rsqrtf(sq * inv_d + eps), q = -(r * gs) * inv_d * r * r;          // (r^3 alone leaves fp32 beyond 2^+-42)
                 const float rg = keep ? r : 0.f;           // (a row that is not there is another's copy)
                 const uint64_t r2 = f2(r, r), q2 = f2(q, q), rg2 = f2(rg, rg);
@@ -459,14 +535,19 @@ __global__ void __launch_bounds__(THREADS, KIND == HALVES ? 3 : 2) bwd_kernel(co
                 fresh = turns;
                 keep = now.here() && L.live;
             }
+            if constexpr (ASYNC) {
+                fetch(stage == 0 ? DEPTH - 1 : stage - 1);
+                stage = stage + 1 == DEPTH ? 0 : stage + 1;
+            }
         }
     }
+    if constexpr (ASYNC) copy_wait<0>();          // (the last rows again, which nobody reads)
     if (NORM && P.part) {
-        if (L.live) store_pairs<float, N, KIND>(L, sums + group * P.D, ga, gb);
+        if (L.live) store_pairs<float, N, KIND>(L, sums + G.group * P.D, ga, gb);
         __syncthreads();
         for (int i = threadIdx.x; i < P.D; i += THREADS) {
             float v = sums[i];
-            for (int g = 1; g < groups; ++g) v += sums[g * P.D + i];
+            for (int g = 1; g < G.groups; ++g) v += sums[g * P.D + i];
             P.part[(int64_t)blockIdx.x * P.D + i] = v;
         }
     }
@@ -496,14 +577,25 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int blocks0
 }
 
 // ---------------------------------------------------------------- host side
+constexpr int MAX_DEVICES = 64;
 constexpr int MAX_BLOCKS = 148 * 8;       // of the backward, whose blocks each leave a row of sums
 
-// Groups of a block that share a token's heads: one where tokens are many (cos and sin are
-// waited for once for all heads), more where the tokens alone would not fill the GPU twice.
-int share_of(int64_t T, int heads, int groups) {
-    int share = 1;
-    while (share < groups && heads % (2 * share) == 0 && heads > 0 && T * share < (int64_t)groups * 148 * 2) share *= 2;
-    return share;
+// Groups of a block that share a token's heads, a divisor of both, and the blocks: so that the group with
+// the most to do has least, a token's cos and sin counted as TOKEN_ROWS rows (16384 tokens, 2 x 32 heads of 64: 55
+// and 84 us, with a group a token 59 and 103; counted as 4 rows 59 and 85).
+constexpr int TOKEN_ROWS = 1;
+int share_of(int64_t T, int heads, int groups, int64_t most, int* blocks) {
+    int64_t least = INT64_MAX;
+    int best = 1;
+    for (int share = 1; groups % share == 0 && heads % share == 0; share *= 2) {
+        const int64_t tokens = groups / share, n = std::min((T + tokens - 1) / tokens, most);
+        const int64_t rows = (T + n * tokens - 1) / (n * tokens) * (heads / share + TOKEN_ROWS);
+        if (rows >= least) continue;
+        least = rows;
+        best = share;
+        *blocks = (int)n;
+    }
+    return best;
 }
 
 // whether rows can be read in runs of n columns: sizes of whole pairs of runs, addresses and strides of whole
@@ -522,6 +614,7 @@ bool rows_fit(const Params& P, int32_t type, bool bwd, int n) {
 
 template <typename K> int resident_blocks(K k, size_t smem) {
     int per_sm = 0;
+    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, THREADS, smem) != cudaSuccess || per_sm < 1) {
         cudaGetLastError();
         per_sm = 1;
@@ -532,30 +625,34 @@ template <typename K> int resident_blocks(K k, size_t smem) {
 }
 
 template <typename T, int N, int LANES, Kind KIND, bool NORM> int launch(Params P, bool bwd, float* dqw, float* dkw, cudaStream_t st) {
-    constexpr int groups = THREADS / LANES;
-    const size_t smem = bwd && NORM && P.part ? (size_t)groups * P.D * sizeof(float) : 0;
-    // one wave of blocks, q's and k's by their heads
-    static std::atomic<int> known[2];
-    int most = known[bwd].load();
+    using Row = Raw<T, N, KIND>;
+    P.lanes = (P.D + 2 * N - 1) / (2 * N);
+    const int groups = LANES ? THREADS / (LANES ? LANES : 1) : THREADS / 32 * (32 / P.lanes);
+    constexpr size_t ring = Row::ASYNC ? (size_t)RING * THREADS * Row::SLOT : 0, both = NORM ? 2 * ring : ring;
+    const size_t smem = !bwd ? ring : both + (NORM && P.part ? (size_t)groups * P.D * sizeof(float) : 0);
+    // one wave of blocks, q's and k's by their heads; asked for once a device
+    static std::atomic<int> known[2][MAX_DEVICES];
+    int d = 0;
+    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= MAX_DEVICES) return fail(CONCORD_ELAUNCH, "concord_qk_norm_rope: no device");
+    int most = known[bwd][d].load();
     if (most == 0) {
-        most = bwd ? resident_blocks(bwd_kernel<T, N, LANES, KIND, NORM>, THREADS * 2 * N * sizeof(float)) : resident_blocks(fwd_kernel<T, N, LANES, KIND, NORM>, 0);
+        most = bwd ? resident_blocks(bwd_kernel<T, N, LANES, KIND, NORM>, both + THREADS * 2 * N * sizeof(float))
+                   : resident_blocks(fwd_kernel<T, N, LANES, KIND, NORM>, ring);
         if (most > MAX_BLOCKS) most = MAX_BLOCKS;
-        known[bwd].store(most);
+        known[bwd][d].store(most);
     }
     int blocks[2];
     const int heads = P.side[0].heads + P.side[1].heads;
     for (int k = 0; k < 2; ++k) {
         Side& S = P.side[k];
-        S.share = share_of(P.T, S.heads, groups);
-        const int64_t tokens = groups / S.share, need = (P.T + tokens - 1) / tokens;
-        int64_t part = k ? most - most * (int64_t)P.side[0].heads / heads : most * (int64_t)P.side[0].heads / heads;
-        if (part < 1) part = 1;
-        blocks[k] = S.heads == 0 ? 0 : (int)(need < part ? need : part);
+        const int64_t part = most * (int64_t)P.side[0].heads / heads;
+        blocks[k] = 0;
+        S.share = S.heads == 0 ? 1 : share_of(P.T, S.heads, groups, std::max<int64_t>(k ? most - part : part, 1), &blocks[k]);
     }
     P.blocks0 = blocks[0];
     const int all = blocks[0] + blocks[1];
     if (!bwd) {
-        fwd_kernel<T, N, LANES, KIND, NORM><<<all, THREADS, 0, st>>>(P);
+        fwd_kernel<T, N, LANES, KIND, NORM><<<all, THREADS, smem, st>>>(P);
         return check_launch("concord_qk_norm_rope_fwd");
     }
     bwd_kernel<T, N, LANES, KIND, NORM><<<all, THREADS, smem, st>>>(P);
@@ -571,12 +668,15 @@ template <typename T, bool NORM> int run(const Params& P, int32_t type, bool bwd
 #define QK_LAUNCH(N, LANES)                                                                         \
     return P.interleaved ? launch<T, N, LANES, PAIRED, NORM>(P, bwd, dqw, dkw, st)                 \
                          : launch<T, N, LANES, HALVES, NORM>(P, bwd, dqw, dkw, st)
-    if (rows_fit(P, type, bwd, 4)) {              // a lane 8 columns (rows of up to 32 leave half of 8 lanes idle)
+    if (rows_fit(P, type, bwd, 4)) {              // a lane 8 columns
+        // where that makes room for more rows in a warp (64 heads of 32: 25 and 37 us, by 8 lanes 47 and 110; 25 heads of 80, 20011
+        // tokens: 36 and 56, by 16 lanes 54 and 98)
+        if (P.D <= 48 || (P.D > 64 && P.D <= 80)) QK_LAUNCH(4, 0);
         if (P.D <= 64) QK_LAUNCH(4, 8);
         if (P.D <= 128) QK_LAUNCH(4, 16);
         QK_LAUNCH(4, 32);
     }
-    if (P.D <= 128 && rows_fit(P, type, bwd, 2)) {        // a lane 4 (heads of 72, 36 of them turned: 68 and 117 us, by
+    if (P.D <= 128 && rows_fit(P, type, bwd, 2)) {        // a lane 4 (heads of 72, 36 of them turned: 68 and 117 us; through the ring 100 and 174; by
         if (P.D <= 64) QK_LAUNCH(2, 16);                  // single columns 138 and 199, 16384 x 32 heads)
         QK_LAUNCH(2, 32);
     }
