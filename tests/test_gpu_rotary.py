@@ -91,7 +91,9 @@ def _check(args, inter, norm, eps=1e-6):
 SHAPES = [(1, 1, 1, 128, 128), (5, 16, 4, 128, 128), (37, 6, 6, 64, 64), (130, 20, 5, 80, 40), (33, 10, 2, 72, 72),
           (64, 3, 1, 96, 96), (19, 4, 4, 256, 256), (1000, 8, 2, 32, 16), (7, 5, 5, 8, 8), (21, 2, 2, 72, 36),
           (11, 3, 3, 10, 4), (9, 2, 1, 255, 254), (400, 12, 12, 64, 0), (3, 7, 7, 1, 0), (20, 32, 8, 128, 64), (40, 6, 3, 36, 36),
-          (90, 4, 2, 60, 12), (33, 8, 4, 124, 124), (17, 3, 1, 132, 68), (70, 5, 5, 68, 0)]
+          (90, 4, 2, 60, 12), (33, 8, 4, 124, 124), (17, 3, 1, 132, 68), (70, 5, 5, 68, 0), (65, 3, 3, 24, 24),
+          (50, 6, 2, 40, 40), (77, 12, 4, 48, 24), (300, 7, 7, 16, 16), (2100, 24, 8, 80, 80), (20011, 5, 5, 80, 40),
+          (9001, 16, 4, 128, 128), (6000, 32, 32, 64, 32)]
 
 
 @pytest.mark.parametrize("inter", [False, True])
