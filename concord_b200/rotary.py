@@ -90,21 +90,28 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
 
 class QKNormRope(nn.Module):
     """`qk_norm_rope` with its weights (q_weight, k_weight [head_dim], ones at the start)
-    and its tables for `positions` positions (not in the state dict; fp32 whatever type the module is cast to)."""
+    and its tables for `positions` positions (not in the state dict; fp32 whatever type the module is cast to, and
+    made anew where it is given memory: built on the meta device, then to_empty)."""
+
+    base = 10000.0                  # (for modules that were pickled before they kept it)
 
     def __init__(self, head_dim, positions, rot=None, base=10000.0, eps=1e-6, interleaved=False, device=None):
         super().__init__()
         self.q_weight, self.k_weight = (nn.Parameter(torch.ones(head_dim, device=device)) for _ in range(2))
-        cos, sin = rope_tables(positions, head_dim if rot is None else rot, base, device=device or "cpu")
+        cos, sin = rope_tables(positions, head_dim if rot is None else rot, base, device=self.q_weight.device)
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
-        self.eps, self.interleaved = eps, interleaved
+        self.base, self.eps, self.interleaved = base, eps, interleaved
 
     def _apply(self, fn, recurse=True):
+        # fn says where the tables go; what it makes of them (another type, to_empty's bare memory) is not theirs
         cos, sin = self.cos, self.sin
         super()._apply(fn, recurse)
-        if self.cos.dtype != torch.float32:               # the tables stay in fp32 where the module is cast
-            self.cos, self.sin = cos.to(self.cos.device), sin.to(self.sin.device)
+        device = self.cos.device
+        if cos.is_meta and device.type != "meta":
+            self.cos, self.sin = rope_tables(cos.shape[0], 2 * cos.shape[1], self.base, device=device)
+        else:
+            self.cos, self.sin = cos.to(device), sin.to(device)
         return self
 
     def forward(self, q, k, positions=None):
