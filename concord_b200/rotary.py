@@ -115,5 +115,5 @@ class QKNormRope(nn.Module):
         return self
 
     def forward(self, q, k, positions=None):
-        return qk_norm_rope(q, k, self.cos, self.sin, positions, self.q_weight, self.k_weight, eps=self.eps,
-                            interleaved=self.interleaved)
+        return qk_norm_rope(q, k, self.cos, self.sin, positions, self.q_weight, None if k is None else self.k_weight,
+                            eps=self.eps, interleaved=self.interleaved)

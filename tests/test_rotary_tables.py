@@ -102,3 +102,15 @@ def test_on_the_gpu():
     for m in (a, b, c):
         with torch.no_grad():
             assert bool(((m(x, x)[0].double() - want).abs() <= 2.0 ** -18 * (p.abs() + q.abs()).repeat(1, 1, 2)).all())
+
+
+@pytest.mark.gpu
+def test_queries_alone():
+    """The module takes no keys, as the function does: k' is None, and k_weight gets no gradient."""
+    from concord_b200 import QKNormRope
+    m = QKNormRope(64, 100, device="cuda")
+    q = torch.randn(50, 2, 64, device="cuda")
+    out, none = m(q, None)
+    assert none is None and torch.equal(out, m(q, q)[0])
+    out.sum().backward()
+    assert m.q_weight.grad is not None and m.k_weight.grad is None
