@@ -306,6 +306,8 @@ _SIGS = [
     ("concord_gemm_dw8_workspace_bytes", ctypes.c_size_t, [_I64, _I64, _I64]),
     ("concord_gemm_dw8", ctypes.c_int, [_P, _I64, _P, _P, _I64, _I64, _I64, _P, ctypes.c_size_t, _P]),
     ("concord_gemm_dw8_error", ctypes.c_int, [_I32]),
+    ("concord_gemm_dw8_error_word", ctypes.POINTER(_I32), []),
+    ("concord_gemm_dw8_wait_check", ctypes.c_int, [_P]),
     ("concord_gated_fwd", ctypes.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _P, _P, _I64, _I64, _P]),
     ("concord_gated_bwd", ctypes.c_int,
      [_P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "errwords.cuh"
 #include "tc.cuh"
 #include "vec.cuh"
 
@@ -1357,48 +1358,7 @@ int device_index() {
     return cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < MAX_DEVICES ? d : -1;
 }
 
-// the host's error words, one a device, in memory that the kernels write to
-volatile int* host_word() {
-    static std::atomic<int*> words;
-    static std::mutex mu;
-    const int d = device_index();
-    if (d < 0) return nullptr;
-    int* w = words.load();
-    if (!w) {
-        std::lock_guard<std::mutex> g(mu);
-        w = words.load();
-        if (!w) {
-            // (an allocation is no work on a stream: it may come first in a capture)
-            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-            cudaThreadExchangeStreamCaptureMode(&mode);
-            void* p = nullptr;
-            const cudaError_t e = cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-            cudaThreadExchangeStreamCaptureMode(&mode);
-            if (e != cudaSuccess) {
-                cudaGetLastError();
-                return nullptr;
-            }
-            memset(p, 0, MAX_DEVICES * sizeof(int));
-            words.store(w = static_cast<int*>(p));
-        }
-    }
-    return w + d;
-}
-
-// where this device's kernels tell a wait that ran out; refuses while one is told
-int error_words(int** err, int** err_host, const char* name) {
-    volatile int* host = host_word();
-    void* p = nullptr;
-    if (!host || cudaGetSymbolAddress(&p, g_err) != cudaSuccess) return fail(CONCORD_ELAUNCH, std::string(name) + ": device set-up failed");
-    if (*host)
-        return fail(CONCORD_ETIMEOUT, std::string(name) + ": a wait inside an earlier attention kernel ran out (code " +
-                                          std::to_string(*host) + "), its results hold NaN; concord_attention_error(1) clears this");
-    *err = static_cast<int*>(p);
-    if (cudaHostGetDevicePointer(&p, const_cast<int*>(host), 0) != cudaSuccess)
-        return fail(CONCORD_ELAUNCH, std::string(name) + ": device set-up failed");
-    *err_host = static_cast<int*>(p);
-    return CONCORD_OK;
-}
+ErrorWords g_words(&g_err, "attention kernel", "concord_attention_error");
 
 // a wait on a barrier that nobody arrives on, by a warp and by a thread of another
 __global__ void __launch_bounds__(64) wait_check_kernel(int* err, int* err_host) {
@@ -1568,7 +1528,7 @@ extern "C" int concord_attention_fwd(const concord_attention_params* p, const vo
         !attn::make_map(&mv, v, bf, p->tokens_k, p->kv_heads, p->head_dim, v_ts, v_hs))
         return fail(CONCORD_ELAUNCH, "concord_attention_fwd: TMA descriptor encoding failed");
     int *err, *err_host;
-    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    if (int rc = attn::g_words.take(&err, &err_host, name)) return rc;
     if (!attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_fwd: device set-up failed");
     attn::Params P = attn::make_params(p, err, err_host);
     P.o = o;
@@ -1617,7 +1577,7 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
         !attn::make_map(&md, dout, bf, p->tokens_q, p->heads, p->head_dim, do_ts, do_hs))
         return fail(CONCORD_ELAUNCH, "concord_attention_bwd: TMA descriptor encoding failed");
     int *err, *err_host;
-    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    if (int rc = attn::g_words.take(&err, &err_host, name)) return rc;
     if (!attn::device_ready()) return fail(CONCORD_ELAUNCH, "concord_attention_bwd: device set-up failed");
     attn::Params P = attn::make_params(p, err, err_host);
     P.o = const_cast<void*>(o);
@@ -1652,27 +1612,14 @@ extern "C" int concord_attention_bwd(const concord_attention_params* p, const vo
 }
 
 // the attention kernels' error word on the current device (0: no wait ran out)
-extern "C" int concord_attention_error(int32_t reset) {
-    volatile int* host = attn::host_word();
-    void* p = nullptr;
-    int v = 0;
-    if (!host || cudaGetSymbolAddress(&p, attn::g_err) != cudaSuccess ||
-        cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
-        return -1;
-    if (!v) v = *host;
-    if (reset) {
-        if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return -1;
-        *host = 0;
-    }
-    return v;
-}
+extern "C" int concord_attention_error(int32_t reset) { return attn::g_words.read(reset); }
 
-extern "C" int32_t* concord_attention_error_word(void) { return const_cast<int32_t*>(attn::host_word()); }
+extern "C" int32_t* concord_attention_error_word(void) { return const_cast<int32_t*>(attn::g_words.host()); }
 
 extern "C" int concord_attention_wait_check(void* stream) {
     const char* name = "concord_attention_wait_check";
     int *err, *err_host;
-    if (int rc = attn::error_words(&err, &err_host, name)) return rc;
+    if (int rc = attn::g_words.take(&err, &err_host, name)) return rc;
     attn::wait_check_kernel<<<1, 64, 0, as_stream(stream)>>>(err, err_host);
     return check_launch(name);
 }

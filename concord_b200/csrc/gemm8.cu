@@ -26,7 +26,7 @@
 //
 // Every wait is bounded (tc.cuh): where one runs out, loads and products stop,
 // what is in flight lands (bounded again), the pair's remaining outputs become NaN and
-// the device's error word is set (concord_gemm_dw8_error).
+// the device's error word is set, and its copy in host memory, by which later calls refuse (concord_gemm_dw8_error).
 #include <cuda.h>
 
 #include <algorithm>
@@ -35,6 +35,7 @@
 
 #include "common.cuh"
 #include "eight.cuh"
+#include "errwords.cuh"
 #include "tc.cuh"
 
 namespace concord {
@@ -64,7 +65,7 @@ struct Params {
     const uint8_t* saved;
     __nv_bfloat16* dw;
     float* part;                                  // pieces of the rest: [2 pairs][256 outputs][256 features]
-    int* err;
+    int *err, *err_host;
 };
 
 // The rest's ends, tile after tile, are one line of stages.  Where helper h of them begins:
@@ -196,6 +197,11 @@ __device__ __forceinline__ uint32_t two(uint32_t word, uint32_t pick, uint32_t s
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(c));
     asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(scale2));
     return v;
+}
+
+__device__ __forceinline__ void tell_host(const int* err, int* err_host) {
+    *reinterpret_cast<volatile int*>(err_host) = *reinterpret_cast<const volatile int*>(err);
+    __threadfence_system();
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -367,10 +373,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     fence_before();
     __syncthreads();
     cluster_sync();
+    if (threadIdx.x == 0 && gave_up(bar0)) tell_host(P.err, P.err_host);
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
     }
+}
+
+// a wait on a barrier that nobody arrives on
+__global__ void __launch_bounds__(32) wait_check_kernel(int* err, int* err_host) {
+    __shared__ __align__(BARRIERS) uint8_t bars[BARRIERS];
+    const uint32_t b = smem_u32(bars);
+    if (threadIdx.x == 0) {
+        mbar_init(b, 1);
+        set_gave_up(b, 0);
+    }
+    __syncwarp();
+    warp_wait(b, 0, err, 99);
+    if (threadIdx.x == 0 && gave_up(b)) tell_host(err, err_host);
 }
 
 // The pieces of every tile that was cut, in token order: a block four rows of 256
@@ -424,11 +444,8 @@ bool make_map(CUtensorMap* m, const void* dy, int64_t M, int64_t N, int64_t ld) 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-__device__ int g_err;
-int* error_word() {
-    int* p = nullptr;
-    return cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_err) == cudaSuccess ? p : nullptr;
-}
+__device__ int g_err;      // first wait that ran out (0: none), per device
+ErrorWords g_words(&g_err, "weight gradient's kernel", "concord_gemm_dw8_error");
 
 // CTA pairs that are resident together, asked for once per device with the
 // kernel's shared memory; 0: refused
@@ -514,15 +531,15 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
     if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return fail(CONCORD_EWORKSPACE, std::string(name) + ": workspace too small, or not 16-byte aligned");
     if (int rc = bind_current_context(name)) return rc;
+    Params P{};
+    if (int rc = g_words.take(&P.err, &P.err_host, name)) return rc;
     CUtensorMap map;
     if (!make_map(&map, dy, M, N, lddy)) return fail(CONCORD_ELAUNCH, std::string(name) + ": TMA descriptor encoding failed");
-    Params P{};
     P.saved = static_cast<const uint8_t*>(saved);
     P.dw = reinterpret_cast<__nv_bfloat16*>(dw);
     P.part = static_cast<float*>(workspace);
-    P.err = error_word();
     const int resident = resident_pairs();
-    if (!P.err || resident <= 0) return fail(CONCORD_ELAUNCH, std::string(name) + ": no error word, or shared memory refused");
+    if (resident <= 0) return fail(CONCORD_ELAUNCH, std::string(name) + ": shared memory refused");
     const int pairs = share_out(P, M, N, K, resident);
     dw8_kernel<<<2 * pairs, THREADS, SMEM, st>>>(map, P);
     if (int rc = check_launch(name)) return rc;
@@ -533,11 +550,14 @@ extern "C" int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* sa
     return CONCORD_OK;
 }
 
-extern "C" int concord_gemm_dw8_error(int32_t reset) {
-    int* err = g8::error_word();
-    if (!err) return -1;
-    int v = 0;
-    cudaMemcpy(&v, err, sizeof(int), cudaMemcpyDeviceToHost);
-    if (reset) cudaMemset(err, 0, sizeof(int));
-    return v;
+extern "C" int concord_gemm_dw8_error(int32_t reset) { return g8::g_words.read(reset); }
+
+extern "C" int32_t* concord_gemm_dw8_error_word(void) { return const_cast<int32_t*>(g8::g_words.host()); }
+
+extern "C" int concord_gemm_dw8_wait_check(void* stream) {
+    const char* name = "concord_gemm_dw8_wait_check";
+    int *err, *err_host;
+    if (int rc = g8::g_words.take(&err, &err_host, name)) return rc;
+    g8::wait_check_kernel<<<1, 32, 0, as_stream(stream)>>>(err, err_host);
+    return check_launch(name);
 }

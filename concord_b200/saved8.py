@@ -106,5 +106,6 @@ def gated_unit(gate, up, act="silu", save8=False, out8=False):
 
 def gemm_dw8_error(reset=False):
     """Code of the first wait inside grad_weight8's kernel that ran out on the
-    current device, 0 if none did (its outputs are NaN then).  Synchronises."""
+    current device, 0 if none did (its outputs are NaN then, and later calls raise).
+    Synchronises; `reset` clears it, after which calls are taken again."""
     return _abi.load().concord_gemm_dw8_error(int(reset))

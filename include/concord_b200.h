@@ -725,8 +725,15 @@ int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t 
  * stride lddy) and x in 8 bits: the values it keeps are exact in bf16, sums are fp32,
  * rounded once.  N and lddy multiples of 8, dy 16-byte aligned; any M and K.
  * Workspace: 16-byte aligned, sums of tiles that are cut (up to 37 MB; as many bytes
- * as the current device asks for, 0 where no tile is cut).  Its waits are bounded as
- * concord_gemm2sm's are: concord_gemm_dw8_error reads and clears its error word.
+ * as the current device asks for, 0 where no tile is cut).  Its waits are bounded (2 s of running).
+ * Where one runs out, the tiles concerned hold NaN and every later concord_gemm_dw8 on the device
+ * gives CONCORD_ETIMEOUT (the word is in host memory: no call synchronises to look) until
+ * concord_gemm_dw8_error(1).
+ * concord_gemm_dw8_error: the code of the first such wait, 0 if there was none
+ * (synchronises; clears it with `reset`).  concord_gemm_dw8_error_word: the
+ * host's word of the current device, for a program that polls it.
+ * concord_gemm_dw8_wait_check: launches a wait that nothing ends, for programs
+ * (and tests) that rehearse the failure: 2 s later the error is set.
  */
 size_t concord_saved8_bytes(int64_t M, int64_t K);
 int concord_save8(const void* x, int32_t type, int64_t ldx, void* saved, int64_t M, int64_t K, void* stream);
@@ -735,6 +742,8 @@ size_t concord_gemm_dw8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int concord_gemm_dw8(const uint16_t* dy, int64_t lddy, const void* saved, uint16_t* dw, int64_t M, int64_t N, int64_t K,
                      void* workspace, size_t workspace_bytes, void* stream);
 int concord_gemm_dw8_error(int32_t reset);
+int32_t* concord_gemm_dw8_error_word(void);
+int concord_gemm_dw8_wait_check(void* stream);
 
 /*
  * Gated unit: h [M, K] = act(gate) * up, act CONCORD_SILU or CONCORD_GELU (of the error

@@ -1,0 +1,58 @@
+"""Activations in 8 bits at their edges: waits that run out, the border of a type's range, the shares of the weight gradient."""
+import pytest
+import torch
+
+DEV = "cuda"
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_is_reported():
+    """A rehearsal: a wait that nothing ends sets the error 2 s later, without a synchronisation of the caller's; then
+    grad_weight8 and a packed layer's backward refuse, and the layer keeps its words, until the error is cleared."""
+    import concord_b200
+    from concord_b200 import ConcordLinearPackedB, _abi, grad_weight8, save8
+    lib = _abi.load()
+    torch.manual_seed(0)
+    x, dy = (torch.randint(-9, 10, (200, n), device=DEV).bfloat16() for n in (96, 64))
+    s = save8(x)
+    want = grad_weight8(dy, s)
+    lay = ConcordLinearPackedB(96, 64, bias=False, device=DEV, lr=1e-2)
+    lay.load_weights(torch.randn(64, 96, device=DEV) * 0.05)
+    lay.save8 = True
+    y = lay(x.clone().requires_grad_())
+    words = lay.packed_w.clone()
+    word = lib.concord_gemm_dw8_error_word()
+    assert word[0] == 0 and concord_b200.gemm_dw8_error() == 0
+    try:
+        assert lib.concord_gemm_dw8_wait_check(torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert word[0] == 99 and concord_b200.gemm_dw8_error() == 99
+        with pytest.raises(RuntimeError, match="a wait inside an earlier weight gradient's kernel ran out .code 99."):
+            grad_weight8(dy, s)
+        with pytest.raises(RuntimeError, match="ran out"):
+            y.backward(dy)
+        assert torch.equal(lay.packed_w, words)
+        assert lib.concord_gemm_dw8_wait_check(None) == -8
+        assert concord_b200.attention_error() == 0           # (its word is its own)
+    finally:
+        assert concord_b200.gemm_dw8_error(reset=True) == 99
+    assert word[0] == 0 and concord_b200.gemm_dw8_error() == 0
+    assert torch.equal(grad_weight8(dy, s), want)
+    word[0] = 5                          # another program's handler, or a kernel, wrote the host's word alone
+    try:
+        with pytest.raises(RuntimeError, match="code 5"):
+            grad_weight8(dy, s)
+    finally:
+        assert concord_b200.gemm_dw8_error(reset=True) == 5
+    assert torch.equal(grad_weight8(dy, s), want)
+
+
+def test_error_word_without_a_device():
+    """No device: no word, and nothing that crashes."""
+    from concord_b200 import _abi, build
+    build.build()
+    lib = _abi.load()
+    if torch.cuda.is_available():
+        pytest.skip("a device is there")
+    assert lib.concord_gemm_dw8_error(0) == -1 and not lib.concord_gemm_dw8_error_word()
+    assert lib.concord_gemm_dw8_wait_check(None) < 0
