@@ -25,7 +25,7 @@
 // the workspace, which a second kernel adds in token order: the same bits on every run of one device.
 //
 // Every wait is bounded (tc.cuh): where one runs out, loads and products stop,
-// what is in flight lands (bounded again), the pair's remaining outputs become NaN and
+// what both CTAs have in flight lands (bounded again), the pair's remaining outputs become NaN and
 // the device's error word is set, and its copy in host memory, by which later calls refuse (concord_gemm_dw8_error).
 #include <cuda.h>
 
@@ -53,7 +53,7 @@ constexpr int DY_BYTES = TOKENS * OUTS * 2, X_BYTES = eight::TILE_BYTES;
 static_assert(FEATS == eight::FEATS && TOKENS == eight::TOKENS, "a stage reads one tile of codes");
 constexpr int CODES = STAGES * DY_BYTES, BARS = CODES + STAGES * X_BYTES;
 constexpr int NBARS = 4 * STAGES + 3;
-static_assert(BARS % BARRIERS == 0 && NBARS * 8 + 4 <= (int)BARRIERS - 4, "barriers, the tensor memory's address, the word");
+static_assert(BARS % BARRIERS == 0 && NBARS * 8 + 8 <= (int)BARRIERS - 4, "barriers, the tensor memory's address, tiles sent, the word");
 constexpr size_t SMEM = BARS + BARRIERS + 1024;
 constexpr int ACC = 256;                          // columns of the accumulator; stage s of A stands at ACC + 32 s
 constexpr int TILE = 256;
@@ -119,11 +119,20 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// this address in the leader's shared memory
-__device__ __forceinline__ uint32_t leaders(uint32_t addr) {
+// this address in the shared memory of a CTA of the pair; 0 is the leader
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+__device__ __forceinline__ uint32_t leaders(uint32_t addr) { return in_cta(addr, 0); }
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
 }
 // What the arrival says is ordered is in tensor memory alone (tcgen05.wait::st or ::ld
 // and the fence before it), so it need not release memory to the cluster: that
@@ -157,6 +166,23 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes, uint32_t on
         "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
         "r"(bytes), "r"(one)
         : "memory");
+}
+// What a CTA of a pair in which a wait has run out sent lands, or that wait too runs out (false): one thread of each CTA,
+// between two barriers of the cluster.  `sent`: the word in which each CTA left its number of stages.  Its codes count on its
+// own barriers; both halves of dy on the leader's, which expects them as far as it sent stages itself: for those that the
+// other CTA alone sent it now expects that half, and a half that was not sent is taken off.  (Neither is a whole
+// ring ahead: it waits for products that need both.)
+__device__ __noinline__ bool pair_landed(uint32_t cfull, uint32_t bfull, uint32_t sent, uint32_t half, uint32_t rank, int* err) {
+    const int mine = (int)load_cluster(in_cta(sent, rank));
+    bool ok = ring_landed(cfull, STAGES, mine, err);
+    if (rank == 0) {
+        const int theirs = (int)load_cluster(in_cta(sent, 1));
+        for (int x = mine; x < theirs; ++x) mbar_expect(bfull + 8u * (x % STAGES), half);
+        for (int x = theirs; x < mine; ++x)
+            asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bfull + 8u * (x % STAGES)), "r"(half) : "memory");
+        ok = ring_landed(bfull, STAGES, max(mine, theirs), err) && ok;
+    }
+    return ok;
 }
 // accumulator (both CTAs' tensor memory) = A (tensor memory) B (both CTAs' shared memory) [+ itself]
 __device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t one) {
@@ -210,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + BARS);
     uint32_t* slot = reinterpret_cast<uint32_t*>(bars + NBARS);
-    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
+    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars), sent_word = bar0 + NBARS * 8 + 4;
     auto cfull = [&](int s) { return bar0 + 8u * s; };                       // this CTA's codes and scales have landed
     auto bfull = [&](int s) { return bar0 + 8u * (STAGES + s); };            // leader: both halves of dy have
     auto afull = [&](int s) { return bar0 + 8u * (2 * STAGES + s); };        // leader: both CTAs' A is in tensor memory
@@ -265,10 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (++s == STAGES) { s = 0; ph ^= 1; }
             }
         }
-        if (!ok && lane == 0) {
-            ring_landed(cfull(0), STAGES, sent, P.err);
-            if (rank == 0) ring_landed(bfull(0), STAGES, sent, P.err);
-        }
+        if (lane == 0) store_cluster(in_cta(sent_word, rank), sent);
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
@@ -293,11 +316,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
                 if (ok) commit_pair(tfull, one);
-            }
-            if (!ok) {
-                commit_pair(drained, one);
-                Patience patience;
-                while (!__all_sync(0xffffffffu, mbar_try(drained, 0)) && !__any_sync(0xffffffffu, patience.over(P.err))) {}
             }
         }
     } else if (warp >= 4) {
@@ -372,25 +390,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && gave_up(bar0)) store_cluster(in_cta(gave_up_word(bar0), rank ^ 1), 1);
     cluster_sync();
-    if (threadIdx.x == 0 && gave_up(bar0)) tell_host(P.err, P.err_host);
+    if (gave_up(bar0)) {                          // here or in the other CTA: copies and products in flight end first
+        if (threadIdx.x == 0) {
+            tell_host(P.err, P.err_host);
+            pair_landed(cfull(0), bfull(0), sent_word, DY_BYTES, rank, P.err);
+        }
+        if (warp == 1) {
+            if (rank == 0) commit_pair(drained, elect_one());
+            Patience patience;
+            while (!__all_sync(0xffffffffu, mbar_try(drained, 0)) && !__any_sync(0xffffffffu, patience.over(P.err))) {}
+        }
+        __syncthreads();
+        cluster_sync();
+    }
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
     }
 }
 
-// a wait on a barrier that nobody arrives on
-__global__ void __launch_bounds__(32) wait_check_kernel(int* err, int* err_host) {
-    __shared__ __align__(BARRIERS) uint8_t bars[BARRIERS];
-    const uint32_t b = smem_u32(bars);
+// A rehearsal of a wait that runs out.  First pair_landed where the CTAs have sent as many stages, or one of them more: code
+// 98 where it does not see them land; then a wait on a barrier that nobody arrives on: code 99.  dy: 64 x 64.
+constexpr int CHECKS = 3, CHECK_CODES = CODES / 2, CHECK_BARS = CHECK_CODES + STAGES * 1024;
+constexpr size_t CHECK_SMEM = CHECK_BARS + BARRIERS + 1024;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(32)
+    wait_check_kernel(const __grid_constant__ CUtensorMap map_dy, const void* codes, int* err, int* err_host) {
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, bar0 = base + CHECK_BARS, one = elect_one(), rank = cluster_rank();
+    const uint32_t alone = bar0 + CHECKS * 2 * STAGES * 8, sent_word = alone + 8;
+    static_assert((CHECKS * 2 * STAGES + 1) * 8 + 4 <= (int)BARRIERS - 4, "barriers, tiles sent, the word");
     if (threadIdx.x == 0) {
-        mbar_init(b, 1);
-        set_gave_up(b, 0);
+        for (int i = 0; i <= CHECKS * 2 * STAGES; ++i) mbar_init(bar0 + 8u * i, 1);
+        set_gave_up(bar0, 0);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    warp_wait(b, 0, err, 99);
-    if (threadIdx.x == 0 && gave_up(b)) tell_host(err, err_host);
+    cluster_sync();
+    for (int i = 0; i < CHECKS; ++i) {
+        const int first = i == 1 ? 7 : 3, second = i == 2 ? 8 : 3, mine = rank ? second : first;
+        const uint32_t cfull = bar0 + i * 2 * STAGES * 8, bfull = cfull + STAGES * 8;
+        for (int s = 0; s < mine; ++s) {
+            if (rank == 0) expect(bfull + 8u * s, DY_BYTES, one);
+            expect(cfull + 8u * s, 1024, one);
+            load_dy(base + s * (DY_BYTES / 2), &map_dy, leaders(bfull + 8u * s), 0, 0, one);
+            load_bytes(base + CHECK_CODES + s * 1024, codes, 1024, cfull + 8u * s, one);
+        }
+        if (threadIdx.x == 0) store_cluster(in_cta(sent_word, rank), mine);
+        __syncwarp();
+        cluster_sync();
+        if (threadIdx.x == 0 && !pair_landed(cfull, bfull, sent_word, DY_BYTES / 2, rank, err)) atomicCAS(err, 0, 98);
+        __syncwarp();
+        cluster_sync();
+    }
+    if (rank == 0) {
+        warp_wait(alone, 0, err, 99);
+        if (threadIdx.x == 0 && gave_up(alone)) tell_host(err, err_host);
+    }
 }
 
 // The pieces of every tile that was cut, in token order: a block four rows of 256
@@ -445,6 +502,7 @@ bool make_map(CUtensorMap* m, const void* dy, int64_t M, int64_t N, int64_t ld) 
 }
 
 __device__ int g_err;      // first wait that ran out (0: none), per device
+__device__ __align__(128) uint8_t g_check[8192];           // what the rehearsal copies
 ErrorWords g_words(&g_err, "weight gradient's kernel", "concord_gemm_dw8_error");
 
 // CTA pairs that are resident together, asked for once per device with the
@@ -556,8 +614,14 @@ extern "C" int32_t* concord_gemm_dw8_error_word(void) { return const_cast<int32_
 
 extern "C" int concord_gemm_dw8_wait_check(void* stream) {
     const char* name = "concord_gemm_dw8_wait_check";
+    if (int rc = bind_current_context(name)) return rc;
     int *err, *err_host;
     if (int rc = g8::g_words.take(&err, &err_host, name)) return rc;
-    g8::wait_check_kernel<<<1, 32, 0, as_stream(stream)>>>(err, err_host);
+    void* src = nullptr;
+    CUtensorMap map;
+    if (cudaGetSymbolAddress(&src, g8::g_check) != cudaSuccess || !g8::make_map(&map, src, 64, 64, 64) ||
+        cudaFuncSetAttribute(g8::wait_check_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g8::CHECK_SMEM) != cudaSuccess)
+        return fail(CONCORD_ELAUNCH, std::string(name) + ": device set-up failed");
+    g8::wait_check_kernel<<<2, 32, g8::CHECK_SMEM, as_stream(stream)>>>(map, src, err, err_host);
     return check_launch(name);
 }

@@ -47,6 +47,19 @@ def test_a_wait_that_ran_out_is_reported():
     assert torch.equal(grad_weight8(dy, s), want)
 
 
+@pytest.mark.gpu
+def test_copies_of_a_pair_land():
+    """The rehearsal's CTAs stop after 3 and 3 stages, 7 and 3, 3 and 8: what each has sent lands, or the code is 98."""
+    import concord_b200
+    from concord_b200 import _abi
+    lib = _abi.load()
+    torch.zeros(1, device=DEV)
+    try:
+        assert lib.concord_gemm_dw8_wait_check(torch.cuda.current_stream().cuda_stream) == 0
+    finally:
+        assert concord_b200.gemm_dw8_error(reset=True) == 99
+
+
 def test_error_word_without_a_device():
     """No device: no word, and nothing that crashes."""
     from concord_b200 import _abi, build
