@@ -79,16 +79,22 @@ __global__ void __launch_bounds__(THREADS)
 // ---------------------------------------------------------------- the gated unit
 constexpr int SILU = 0, GELU = 1;
 
+// The functions for results of 16 bits, whose roundings are 2^-11 and 2^-8: the hardware's exponential and reciprocal, and
+// for gelu Hastings' rational form of Phi.  Results of fp32 (EXACT) take expf, erfcf and a division: relative errors of a few
+// 2^-24 far out too (an argument's rounding counts g^2 times there).  By the functions below 16384 x 5504 fp32 took, forward and
+// backward, silu 170 and 283 us, gelu 170 and 281, in 8 bits 240 and 211, 252 and 215; so silu takes
+// 170 and 283, gelu 190 and 283, in 8 bits 233 and 211, 299 and 293.
 __device__ __forceinline__ float sigmoid(float g) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2f(-1.4426950408889634f * g)));
     return r;
 }
 
-// Phi(g), and exp(-g^2 / 2): erfc(x) = e^(-x^2) (a1 t + .. + a5 t^5), t = 1 / (1 + p x), x = |g| / sqrt(2), off by at
-// most 1.5e-7 (Hastings, Approximations for Digital Computers, 1955; Abramowitz and
-// Stegun 7.1.26).  The derivative needs the exponential anyway; with erff the UNet's
-// unit (4096 x 5120 fp16) took 53 and 47 us, forward and backward, in place of 37 and 35.
+// Phi(g), and exp(-g^2 / 2): erfc(x) = e^(-x^2) (a1 t + .. + a5 t^5), t = 1 / (1 + p x), x = |g| / sqrt(2) (Hastings,
+// Approximations for Digital Computers, 1955; Abramowitz and Stegun 7.1.26): erfc off by 1.5e-7 at most in exact
+// arithmetic, Phi as evaluated here by 2.9e-7; relative to Phi 5e-5 down to g = -3, 5e-4 to -4, 1.6e-3 to -5 (fp16's
+// rounding is 4.9e-4, and g Phi there below its normal numbers).  The derivative needs the exponential anyway; with
+// erff the UNet's unit (4096 x 5120 fp16) took 53 and 47 us, forward and backward, in place of 37 and 35.
 __device__ __forceinline__ float2 normal(float g) {
     const float e = ex2f(-0.7213475204444817f * g * g);
     float t;
@@ -101,17 +107,23 @@ __device__ __forceinline__ float2 normal(float g) {
     return make_float2(g < 0.f ? q : 1.f - q, e);
 }
 
-template <int ACT> __device__ __forceinline__ float act(float g) {
-    if constexpr (ACT == SILU) return g * sigmoid(g);
+// Phi(g) for results of fp32, and as a call: the forward that keeps 8 bits holds 32 of them a feature (446 us inline, 299 as
+// a call, the elementwise forward 190 and 203; 16384 x 5504)
+__device__ __forceinline__ float exact_phi(float g) { return 0.5f * erfcf(-0.7071067811865476f * g); }
+__device__ __noinline__ float exact_phi_call(float g) { return exact_phi(g); }
+
+template <int ACT, bool EXACT, bool CALL = false> __device__ __forceinline__ float act(float g) {
+    if constexpr (ACT == SILU) return g * (EXACT ? 1.f / (1.f + expf(-g)) : sigmoid(g));
+    else if constexpr (EXACT) return g * (CALL ? exact_phi_call(g) : exact_phi(g));
     else return g * normal(g).x;
 }
 // act(g) and its derivative
-template <int ACT> __device__ __forceinline__ float2 act2(float g) {
+template <int ACT, bool EXACT> __device__ __forceinline__ float2 act2(float g) {
     if constexpr (ACT == SILU) {
-        const float q = sigmoid(g), a = g * q;
+        const float q = EXACT ? 1.f / (1.f + expf(-g)) : sigmoid(g), a = g * q;
         return make_float2(a, q + a * (1.f - q));
     } else {
-        const float2 n = normal(g);
+        const float2 n = EXACT ? make_float2(exact_phi(g), expf(-0.5f * g * g)) : normal(g);
         return make_float2(g * n.x, n.x + 0.3989422804014327f * g * n.y);
     }
 }
@@ -143,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 5 : 1) fwd8_kernel(c
     for (int i = 0; i < BLOCK; ++i) {
         float v[EL];
 #pragma unroll
-        for (int j = 0; j < EL; ++j) v[j] = act<ACT>(G.get(i, j)) * P.get(i, j);
+        for (int j = 0; j < EL; ++j) v[j] = act<ACT, sizeof(T) == 4, true>(G.get(i, j)) * P.get(i, j);
         G.set_row(i, v);
         if (t0 + i < U.M) G.store_row(i, out + (int64_t)i * U.K);
     }
@@ -178,7 +190,7 @@ __global__ void __launch_bounds__(THREADS)
             const uint32_t wg = (i < 4 ? cg[j].x : i < 8 ? cg[j].y : i < 12 ? cg[j].z : cg[j].w) ^ 0x80808080u;
             const uint32_t wu = (i < 4 ? cu[j].x : i < 8 ? cu[j].y : i < 12 ? cu[j].z : cu[j].w) ^ 0x80808080u;
             const float g = value(wg, i & 3, sg[j]), u = value(wu, i & 3, su[j]);
-            const float2 f = act2<ACT>(g);
+            const float2 f = act2<ACT, sizeof(T) == 4>(g);
             const float d = D.get(i, j);
             a[j] = d * u * f.y;
             b[j] = d * f.x;
@@ -210,7 +222,7 @@ __global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Unit U
     for (int r = 0; r < ROWS; ++r) {
         if (t0 + r >= U.M) break;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) g[r][j] = act<ACT>(g[r][j]) * u[r][j];
+        for (int j = 0; j < VEC; ++j) g[r][j] = act<ACT, sizeof(T) == 4>(g[r][j]) * u[r][j];
         store_vec<VEC>(h + (t0 + r) * U.K + k, g[r]);
     }
 }
@@ -234,7 +246,7 @@ __global__ void __launch_bounds__(256)
         if (t0 + r >= U.M) break;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float2 f = act2<ACT>(g[r][j]);
+            const float2 f = act2<ACT, sizeof(T) == 4>(g[r][j]);
             g[r][j] = d[r][j] * u[r][j] * f.y;
             u[r][j] = d[r][j] * f.x;
         }

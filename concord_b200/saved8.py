@@ -87,6 +87,8 @@ def gated_unit(gate, up, act="silu", save8=False, out8=False):
 
     gate and up may have strides of their own (halves of one projection are
     read in place).  Arithmetic is fp32, the result (contiguous, of their type) rounded once.
+    (For 16-bit types the functions are approximations, gelu's normal distribution function off by 2.9e-7, relative to it by
+    1.6e-3 at -5, where gelu is 1.4e-6.)
     save8: a call that is differentiated keeps gate and up in 8 bits (see
     `save8`) in place of the tensors themselves, and their gradients are computed from these.
     out8: returns (h, Saved8 of h) in the same pass, for the packed layer that
