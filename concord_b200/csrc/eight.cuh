@@ -1,8 +1,10 @@
 // eight.cuh — values kept in 8 bits.
 //
 // 32 tokens of one feature share a power of two 2^e, the least with |x| <= 127
-// 2^e; each value is the whole number nearest to x / 2^e (ties to even), so it is
-// off by at most half a step, 2^(e - 1) < max|x| / 127.  Powers of two make both
+// 2^e, -126 at least; each value is the whole number nearest to x / 2^e (ties to even), so it is
+// off by at most half a step, 2^(e - 1), which is below max|x| / 127 (where max|x| is above 2^-120).  In the block of
+// a type's largest values (fp16: above 127 2^9, else above 127 2^121) codes end at 63, as 64 steps
+// are more than the type holds: values there are off by less than one step.  Powers of two make both
 // directions exact: x / 2^e before its one rounding, and what is read back has at
 // most 7 significant bits, so it is the same in fp32, bf16 and fp16.  A block
 // is one feature's because features differ in size far more than a feature does from token to token.

@@ -53,8 +53,10 @@ def save8(x):
     """x [..., K] (fp32, bf16 or fp16; columns that are not contiguous are copied) as a Saved8.
 
     32 tokens (rows, in order) of one feature share a power of two 2^e, the
-    least with |x| <= 127 2^e; a value is the whole number nearest to x / 2^e, off by
-    at most 2^(e - 1), which is less than the 32 values' largest magnitude / 127.
+    least with |x| <= 127 2^e, -126 at least; a value is the whole number nearest to x / 2^e, off by
+    at most 2^(e - 1), which is less than the 32 values' largest magnitude / 127 (where that is above
+    2^-120).  At the top of a type's range, where 64 steps are more than it holds, it ends at 63 steps: fp16's 65504 is
+    kept as 64512.
     One NaN or infinity makes its 32 values NaN.  Not differentiable: the result stands for
     x in a backward pass.
     """

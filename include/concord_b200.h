@@ -712,9 +712,10 @@ int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t 
 
 /*
  * Activations x [M, K] kept in 8 bits for the backward pass: 32 tokens of one
- * feature share a power of two 2^e, the least with |x| <= 127 2^e, and a value is
+ * feature share a power of two 2^e, the least with |x| <= 127 2^e, -126 at least, and a value is
  * the whole number nearest to x / 2^e (ties to even; in the block of a type's largest
- * values at most 63, which it can still hold).  A block with a NaN or an infinity
+ * values, above 127 2^9 in fp16 and 127 2^121 elsewhere, at most 63, which it can still hold:
+ * off by less than 2^e there, by half of it elsewhere).  A block with a NaN or an infinity
  * reads back as NaN.  `saved`: concord_saved8_bytes(M, K) bytes, 32-byte aligned,
  * tiles of 64 tokens x 128 features in order of tokens, then features, each
  *   int8 codes [4][features][16], 16 tokens of a feature side by side, and
@@ -724,7 +725,7 @@ int concord_qk_norm_rope_bwd(const concord_qk_params* p, const void* q, int64_t 
  * concord_gemm_dw8: dw [N, K] (bf16, contiguous) = dy^T x for dy [M, N] (bf16, row
  * stride lddy) and x in 8 bits: the values it keeps are exact in bf16, sums are fp32,
  * rounded once.  N and lddy multiples of 8, dy 16-byte aligned; any M and K.
- * Workspace: 16-byte aligned, sums of tiles that are cut (up to 37 MB; as many bytes
+ * Workspace: 16-byte aligned, sums of tiles that are cut (up to 146 of 256 KiB, 38.3 MB; as many bytes
  * as the current device asks for, 0 where no tile is cut).  Its waits are bounded (2 s of running).
  * Where one runs out, the tiles concerned hold NaN and every later concord_gemm_dw8 on the device
  * gives CONCORD_ETIMEOUT (the word is in host memory: no call synchronises to look) until

@@ -60,6 +60,36 @@ def test_copies_of_a_pair_land():
         assert concord_b200.gemm_dw8_error(reset=True) == 99
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_top_and_bottom_of_the_range(dtype):
+    """Exactly the documented values: above 127 steps of the last block that is whole, codes end at 63 (less than one step
+    off); steps are 2^-126 at least."""
+    from concord_b200 import save8
+    top = 9 if dtype == torch.float16 else 121
+    info = torch.finfo(dtype)
+    border = torch.tensor(127.0 * 2.0 ** top, dtype=dtype, device=DEV)           # (exact in each type)
+    assert float(border) == 127 * 2.0 ** top
+    above = torch.nextafter(border, torch.tensor(float("inf"), device=DEV, dtype=dtype))
+    x = torch.zeros(64, 4, dtype=dtype, device=DEV)
+    x[:32, 0], x[:32, 1], x[:32, 2] = border, above, -info.max
+    x[1:32] *= torch.linspace(0.01, 1, 31, device=DEV)[:, None].to(dtype)
+    x[32:, 3] = info.max
+    kept = save8(x).dense().double()
+    step = torch.tensor([2.0 ** top] + 3 * [2.0 ** (top + 1)], dtype=torch.float64, device=DEV)
+    ends = torch.tensor([127.0, 63.0, 63.0, 63.0], dtype=torch.float64, device=DEV)
+    want = (x.double() / step).round().clamp(-ends, ends) * step
+    assert torch.equal(kept, want)
+    off = (kept - x.double()).abs()
+    assert bool((off[:, 1:] < step[1:]).all()) and bool((off[:, 0] <= step[0] / 2).all())
+    if dtype == torch.float16:
+        assert float(kept[0, 2]) == -64512 and float(off[0, 2]) == 992
+        return
+    small = torch.tensor([126.0, 2.5, 0.75, 0.5, 2.0 ** -7, 0.0], device=DEV).repeat(32, 1) * 2.0 ** -126     # a step is 2^-126
+    got = save8(small.to(dtype)).dense(torch.float32)[0] * 2.0 ** 126
+    assert got.tolist() == [126.0, 2.0, 1.0, 0.0, 0.0, 0.0]
+
+
 def test_error_word_without_a_device():
     """No device: no word, and nothing that crashes."""
     from concord_b200 import _abi, build
