@@ -74,7 +74,8 @@ extern "C" {
 #define CONCORD_ENODEVICE    -6  /* no usable CUDA device                      */
 #define CONCORD_ETOOBIG      -7  /* size above a fixed maximum                */
 #define CONCORD_ETIMEOUT     -8  /* a wait ran out: between GPUs (peer transport),
-                                    or in an earlier attention kernel          */
+                                    or in an earlier kernel of the same kind
+                                    (attention, weight gradient from 8 bits)   */
 
 /* step-kernel flag bits (the reference's Triton constexprs, packed_b.py:451-458) */
 #define CONCORD_F_MASS_PRESERVE   (1u << 0)
