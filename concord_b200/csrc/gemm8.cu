@@ -391,6 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && gave_up(bar0)) store_cluster(in_cta(gave_up_word(bar0), rank ^ 1), 1);
+    __syncwarp();                                 // (the cluster's barrier wants whole warps)
     cluster_sync();
     if (gave_up(bar0)) {                          // here or in the other CTA: copies and products in flight end first
         if (threadIdx.x == 0) {
@@ -403,6 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             while (!__all_sync(0xffffffffu, mbar_try(drained, 0)) && !__any_sync(0xffffffffu, patience.over(P.err))) {}
         }
         __syncthreads();
+        __syncwarp();
         cluster_sync();
     }
     if (warp == 1) {
