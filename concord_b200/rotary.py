@@ -14,6 +14,8 @@ def rope_tables(positions, rot, base=10000.0, device="cuda"):
     angles and functions in 64 bits, so that far positions lose nothing."""
     if rot < 2 or rot % 2 or positions < 1:
         raise ValueError(f"an even number of rotated columns and at least one position, got {rot} and {positions}")
+    if not 0 < base < float("inf"):
+        raise ValueError(f"base must be positive, got {base}")
     at = torch.arange(positions, dtype=torch.float64, device=device)
     freq = float(base) ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
     angle = at[:, None] * freq

@@ -114,3 +114,14 @@ def test_queries_alone():
     assert none is None and torch.equal(out, m(q, q)[0])
     out.sum().backward()
     assert m.q_weight.grad is not None and m.k_weight.grad is None
+
+
+def test_bases():
+    """A base that is no positive number has no angles: refused, in place of tables of NaN."""
+    from concord_b200 import QKNormRope, rope_tables
+    for base in (0.0, -10000.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="base must be positive"):
+            rope_tables(10, 8, base, device="cpu")
+        with pytest.raises(ValueError, match="base must be positive"):
+            QKNormRope(8, 10, base=base, device="cpu")
+    assert bool(rope_tables(10, 8, 0.5, device="cpu")[0].isfinite().all())
